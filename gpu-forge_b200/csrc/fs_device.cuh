@@ -123,6 +123,7 @@ struct FinalDesc {
 // Device error codes (ctl->err).
 constexpr int DEV_ERR_TIMEOUT = 1;  // a bounded wait (bulk-copy barrier) ran out
 constexpr int DEV_ERR_BOUNDS = 2;  // a scatter position fell outside [0, n)
+constexpr int DEV_ERR_PAGES = 3;   // a token of a step got no slot in the paged cache
 
 // Histogram-fill stage of a keys-only 32-bit sort (plan with `h16`): where
 // the keys grouped by their top 16 bits are, and how to read them.

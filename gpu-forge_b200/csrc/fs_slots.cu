@@ -1,0 +1,246 @@
+// fs_slots.cu -- block tables and slot maps of a batch's step over a paged
+// cache, from the requests' lengths (fs_plan_slots).
+//
+// With ctx_r tokens of request r in the cache, new_r to come and pages of P
+// tokens, request r holds have_r = ceil(ctx_r / P) pages and needs
+// need_r = ceil((ctx_r + new_r) / P).  Two exclusive sums over the requests
+// -- of new_r (where its tokens start in the step) and of need_r - have_r
+// (where its pages start in the list of free pages) -- decide everything
+// else token by token: token i belongs to the request whose range holds i,
+// its position is ctx_r + i - start_r, and its page is an entry of the
+// request's row of the block table if it is one of the have_r, else the next
+// free page, which the page's first token also writes into the table.
+#include "forgesort.h"
+#include "fs_device.cuh"
+#include "fs_internal.h"
+
+using namespace fs;
+
+namespace {
+
+#define FS_SLOTS_CUDA(s, call)                                       \
+  do {                                                               \
+    cudaError_t e_ = (call);                                         \
+    if (e_ != cudaSuccess) return sorter_cuda_fail((s), e_, #call);  \
+  } while (0)
+
+struct SlotArgs {
+  const void* ctx;
+  const void* neu;
+  uint32_t requests;
+  uint32_t page;
+  int32_t* table;
+  uint32_t width;
+  int64_t table_stride;
+  const int32_t* free_pages;
+  uint64_t n_free;
+  const int32_t* cursor;
+  int32_t* query_start;
+  void* seq_lens;
+  void* positions;
+  int32_t* request_of;
+  int64_t* slots;
+  uint64_t capacity;
+  int32_t* cursor_out;
+  int* host_err;
+};
+
+template <typename I> __device__ __forceinline__ int64_t length_of(const void* p, uint32_t r) {
+  const int64_t v = static_cast<const I*>(p)[r];
+  return v > 0 ? v : 0;
+}
+__device__ __forceinline__ int64_t pages_of(int64_t tokens, uint32_t page, uint32_t width) {
+  const int64_t n = tokens / page + (tokens % page != 0);
+  return n < width ? n : width;
+}
+
+constexpr int SLOT_THREADS = 512;
+constexpr int SLOT_CHUNK = 4 * SLOT_THREADS;  // requests scanned at a time
+constexpr int64_t MOST_TOKENS = 0x7fffffff;   // query_start is of 32 bits
+
+// Exclusive sums of two numbers over the block.
+__device__ __forceinline__ void block_scan(int64_t& x, int64_t& y, int64_t (*warp)[2], int64_t& all_x, int64_t& all_y) {
+  constexpr int WARPS = SLOT_THREADS / 32;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t x0 = x, y0 = y;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t ox = __shfl_up_sync(~0u, x, d), oy = __shfl_up_sync(~0u, y, d);
+    if (lane >= d) x += ox, y += oy;
+  }
+  if (lane == 31) warp[wid][0] = x, warp[wid][1] = y;
+  __syncthreads();
+  all_x = all_y = 0;
+  int64_t bx = 0, by = 0;
+  for (int w = 0; w < WARPS; ++w) {
+    if (w == wid) bx = all_x, by = all_y;
+    all_x += warp[w][0], all_y += warp[w][1];
+  }
+  x += bx - x0, y += by - y0;
+}
+
+// Every CTA takes both sums over all requests, SLOT_CHUNK of them at a time,
+// and plans the tokens of its own tiles of SLOT_THREADS tokens that belong to
+// the chunk; the first CTA writes what is one per request.  The sums are taken
+// again by each CTA (two numbers per request from L2) instead of handed on:
+// one launch, no scratch, nobody waits.
+template <typename I> __global__ void __launch_bounds__(SLOT_THREADS) k_plan_slots(const SlotArgs a) {
+  __shared__ int64_t warp[SLOT_THREADS / 32][2];
+  __shared__ int32_t start[SLOT_CHUNK + 1];  // of the chunk's requests
+  __shared__ int64_t took[SLOT_CHUNK];
+  const int tid = threadIdx.x;
+  const int64_t cursor = a.cursor[0] > 0 ? a.cursor[0] : 0;
+  int64_t tokens = 0, pages = 0;  // of the chunks before
+  bool missed = false;
+  for (uint32_t r0 = 0; r0 < a.requests; r0 += SLOT_CHUNK) {
+    const int n = (int)min((uint32_t)SLOT_CHUNK, a.requests - r0);
+    constexpr int PER = SLOT_CHUNK / SLOT_THREADS;
+    int64_t t = 0, p = 0, neu[PER], more[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int l = tid * PER + k;
+      neu[k] = more[k] = 0;
+      if (l < n) {
+        const int64_t ctx = length_of<I>(a.ctx, r0 + l);
+        neu[k] = length_of<I>(a.neu, r0 + l);
+        more[k] = pages_of(ctx + neu[k], a.page, a.width) - pages_of(ctx, a.page, a.width);
+        if (blockIdx.x == 0) static_cast<I*>(a.seq_lens)[r0 + l] = (I)(ctx + neu[k]);
+      }
+      t += neu[k], p += more[k];
+    }
+    int64_t all_t, all_p;
+    block_scan(t, p, warp, all_t, all_p);
+    t += tokens, p += pages;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int l = tid * PER + k;
+      if (l < n) {
+        start[l] = (int32_t)min(t, MOST_TOKENS);
+        took[l] = p;
+        if (blockIdx.x == 0) a.query_start[r0 + l] = start[l];
+      }
+      t += neu[k], p += more[k];
+    }
+    const int64_t from = min(tokens, MOST_TOKENS), to = min(tokens + all_t, MOST_TOKENS);
+    tokens += all_t, pages += all_p;
+    __syncthreads();
+    // the first of this CTA's tiles that reaches into [from, to)
+    int64_t tile = from / SLOT_THREADS;
+    tile += ((int64_t)blockIdx.x - tile % gridDim.x + gridDim.x) % gridDim.x;
+    for (int64_t i = tile * SLOT_THREADS + tid; i - tid < to; i += (int64_t)gridDim.x * SLOT_THREADS) {
+      if (i < from || i >= to) continue;
+      int lo = 0, hi = n;  // the chunk's last request that starts at or before i
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (start[mid] <= i)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const int64_t ctx = length_of<I>(a.ctx, r0 + lo);
+      const int64_t pos = ctx + i - start[lo];
+      const int64_t nth = pos / a.page, off = pos - nth * a.page;
+      int32_t id = -1;
+      if (nth < (int64_t)a.width) {
+        int32_t* entry = a.table + (int64_t)(r0 + lo) * a.table_stride + nth;
+        const int64_t have = pages_of(ctx, a.page, a.width);
+        if (nth < have) {
+          id = *entry;
+        } else {
+          const uint64_t f = (uint64_t)(cursor + took[lo] + nth - have);
+          if (f < a.n_free) id = a.free_pages[f];
+          if (off == 0) *entry = id;
+        }
+      }
+      if (id < 0) missed = true;
+      if (i < (int64_t)a.capacity) {
+        a.request_of[i] = (int32_t)(r0 + lo);
+        static_cast<I*>(a.positions)[i] = (I)pos;
+        a.slots[i] = id < 0 ? -1 : (int64_t)id * a.page + off;
+      } else {
+        missed = true;
+      }
+    }
+    __syncthreads();
+  }
+  const int64_t end = min(tokens, MOST_TOKENS);
+  for (int64_t i = end + (int64_t)blockIdx.x * SLOT_THREADS + tid; i < (int64_t)a.capacity;
+       i += (int64_t)gridDim.x * SLOT_THREADS) {
+    a.request_of[i] = -1;
+    static_cast<I*>(a.positions)[i] = 0;
+    a.slots[i] = -1;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    a.query_start[a.requests] = (int32_t)end;
+    a.cursor_out[0] = (int32_t)min(cursor + pages, (int64_t)a.n_free);
+    if (tokens > end) missed = true;
+  }
+  if (missed) *a.host_err = DEV_ERR_PAGES;
+}
+
+template <typename I> int launch_slots(fs_sorter* s, const SorterView& v, const SlotArgs& a) {
+  const uint64_t tiles = (a.capacity + SLOT_THREADS - 1) / SLOT_THREADS, cap = (uint64_t)v.sm_count * 2;
+  k_plan_slots<I><<<(unsigned)(tiles < 1 ? 1 : tiles < cap ? tiles : cap), SLOT_THREADS, 0, v.stream>>>(a);
+  FS_SLOTS_CUDA(s, cudaGetLastError());
+  return FS_OK;
+}
+
+}  // namespace
+
+extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_lens, const void* new_lens,
+                             uint64_t requests, uint32_t page_size, int32_t* block_table, uint64_t table_width,
+                             int64_t table_stride, const int32_t* free_pages, uint64_t n_free, const int32_t* cursor,
+                             int32_t* query_start, void* seq_lens, void* positions, int32_t* request_of,
+                             int64_t* slots, uint64_t capacity, int32_t* cursor_out, int sync, void* stream) {
+  if (!s) return FS_E_INVALID;
+  if (index_bytes != 4 && index_bytes != 8)
+    return sorter_fail(s, FS_E_INVALID, "lengths must be of 4 or 8 bytes, got %d", index_bytes);
+  if (requests == 0) return FS_OK;
+  if (requests > (1u << 24)) return sorter_fail(s, FS_E_INVALID, "requests = %llu exceeds 2^24", (unsigned long long)requests);
+  if (page_size == 0 || page_size > (1u << 20)) return sorter_fail(s, FS_E_INVALID, "page size %u outside [1, 2^20]", page_size);
+  if (table_width == 0 || table_width > 0x7fffffffull)
+    return sorter_fail(s, FS_E_INVALID, "block table width %llu outside [1, 2^31)", (unsigned long long)table_width);
+  if (requests > 1 && table_stride < (int64_t)table_width)
+    return sorter_fail(s, FS_E_INVALID, "block table rows overlap: stride %lld, width %llu", (long long)table_stride,
+                       (unsigned long long)table_width);
+  if (n_free > 0x7fffffffull) return sorter_fail(s, FS_E_INVALID, "more than 2^31 - 1 free pages");
+  if (capacity > 0x7fffffffull) return sorter_fail(s, FS_E_INVALID, "more than 2^31 - 1 tokens");
+  if (!context_lens || !new_lens || !block_table || !cursor || !query_start || !seq_lens || !cursor_out ||
+      (n_free && !free_pages) || (capacity && (!positions || !request_of || !slots)))
+    return sorter_fail(s, FS_E_INVALID, "a required pointer is NULL");
+  if (cursor == cursor_out) return sorter_fail(s, FS_E_INVALID, "cursor and cursor_out are the same memory");
+  SorterView v;
+  int rc = sorter_view(s, stream, &v);
+  if (rc) return rc;
+  const struct { const void* p; size_t bytes; const char* what; } ptrs[] = {
+      {context_lens, requests * index_bytes, "context_lens"}, {new_lens, requests * index_bytes, "new_lens"},
+      {block_table, ((size_t)(requests - 1) * table_stride + table_width) * 4, "block_table"},
+      {n_free ? free_pages : nullptr, n_free * 4, "free_pages"}, {cursor, 4, "cursor"},
+      {query_start, (requests + 1) * 4, "query_start"}, {seq_lens, requests * index_bytes, "seq_lens"},
+      {capacity ? positions : nullptr, capacity * index_bytes, "positions"},
+      {capacity ? request_of : nullptr, capacity * 4, "request_of"}, {capacity ? slots : nullptr, capacity * 8, "slots"},
+      {cursor_out, 4, "cursor_out"}};
+  for (const auto& q : ptrs)
+    if (q.p && (rc = sorter_check(s, q.p, q.bytes, q.what))) return rc;
+  SlotArgs a{};
+  a.ctx = context_lens;
+  a.neu = new_lens;
+  a.requests = (uint32_t)requests;
+  a.page = page_size;
+  a.table = block_table;
+  a.width = (uint32_t)table_width;
+  a.table_stride = table_stride;
+  a.free_pages = free_pages;
+  a.n_free = n_free;
+  a.cursor = cursor;
+  a.query_start = query_start;
+  a.seq_lens = seq_lens;
+  a.positions = positions;
+  a.request_of = request_of;
+  a.slots = slots;
+  a.capacity = capacity;
+  a.cursor_out = cursor_out;
+  a.host_err = v.host_err;
+  rc = index_bytes == 4 ? launch_slots<int32_t>(s, v, a) : launch_slots<int64_t>(s, v, a);
+  return rc ? rc : sorter_finish(s, v, 1, sync);
+}

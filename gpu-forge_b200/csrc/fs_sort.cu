@@ -6,6 +6,7 @@
 // on that stream (P = key bytes), with no host round trip in between.
 #include "forgesort.h"
 #include "forgesort_bench.h"
+#include "fs_internal.h"
 #include "fs_resident.cuh"
 #include "fs_hoststage.h"
 #include "fs_kernels.cuh"
@@ -239,7 +240,7 @@ constexpr int HIST_BLOCK = 512;  // histogram / count kernels: more loads in fli
 int key_bytes_of(int dtype) { return dtype >= FS_U64 ? 8 : 4; }
 
 // Device ordinals the per-device caches below cover (fs_create refuses more).
-constexpr int MAX_DEVICES = 64;
+constexpr int MAX_DEVICES = SORTER_MAX_DEVICES;
 
 // Bound on every device-side wait: FORGESORT_WAIT_TIMEOUT_MS, default 2 s.
 uint64_t wait_timeout_ns_env() {
@@ -1095,13 +1096,16 @@ int enqueue_partition_dispatch(fs_sorter* s, const void* keys, const uint32_t* v
 #undef FS_DISPATCH_NB
 }
 
-int finish(fs_sorter* s, int sync) {
+int finish_on(fs_sorter* s, cudaStream_t stream, int sync) {
   FS_CUDA(s, cudaGetLastError());
   if (!sync) return FS_OK;
-  FS_CUDA(s, cudaStreamSynchronize(s->stream));
+  FS_CUDA(s, cudaStreamSynchronize(stream));
   const int he = *(volatile int*)s->host_err;
   if (he != 0) {
     *(volatile int*)s->host_err = 0;
+    if (he == DEV_ERR_PAGES)
+      return fail(s, FS_E_GPU_EXECUTION,
+                  "a token has no slot: the free pages, a request's row of the block table or the token arrays ran out");
     if (he == DEV_ERR_BOUNDS)
       return fail(s, FS_E_GPU_EXECUTION, "a device position fell out of range (scatter offset or gather index)");
     return fail(s, FS_E_TIMEOUT, "device wait timeout: a bulk copy or grid barrier did not complete within %llu ms",
@@ -1109,6 +1113,8 @@ int finish(fs_sorter* s, int sync) {
   }
   return FS_OK;
 }
+
+int finish(fs_sorter* s, int sync) { return finish_on(s, s->stream, sync); }
 
 int check_common(fs_sorter* s, int dtype, uint64_t n) {
   if (!s) return FS_E_INVALID;
@@ -1162,6 +1168,38 @@ int noalloc_base(int device, unsigned char** out) {
 // ============================================================================
 // C ABI
 // ============================================================================
+// ---- the serving operators' view of a sorter (fs_internal.h) ------------------
+namespace fs {
+
+int sorter_view(fs_sorter* s, void* stream, SorterView* v) {
+  const int rc = set_device(s);
+  if (rc) return rc;
+  *v = SorterView{s->device, s->sm_count, stream ? static_cast<cudaStream_t>(stream) : s->stream, s->host_err_dev};
+  return FS_OK;
+}
+
+int sorter_fail(fs_sorter* s, int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return fail(s, code, "%s", buf);
+}
+
+int sorter_cuda_fail(fs_sorter* s, cudaError_t e, const char* what) { return cuda_fail(s, e, what); }
+
+int sorter_check(fs_sorter* s, const void* p, size_t bytes, const char* what) {
+  return prepare_ptr(s, p, bytes, what);
+}
+
+int sorter_finish(fs_sorter* s, const SorterView& v, int launches, int sync) {
+  s->last_launches = launches;
+  return finish_on(s, v.stream, sync);
+}
+
+}  // namespace fs
+
 extern "C" {
 
 int fs_abi_version(void) { return FS_ABI_VERSION; }

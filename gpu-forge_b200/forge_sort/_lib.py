@@ -16,6 +16,9 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 # fs_dtype (include/forgesort.h)
 U32, I32, F32, U64, I64, F64 = range(6)
 
+# fs_logits_dtype
+LOGITS_F32, LOGITS_F16, LOGITS_BF16 = range(3)
+
 IPC_HANDLE_BYTES = 64  # FS_IPC_HANDLE_BYTES
 
 # fs_status
@@ -31,6 +34,7 @@ E_INVALID = 8
 
 # Every symbol include/forgesort.h declares, with (restype, argtypes).
 _vp, _u64, _i32 = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int
+_i64, _u32 = ctypes.c_int64, ctypes.c_uint32
 _pp = ctypes.POINTER(ctypes.c_void_p)
 SIGNATURES = {
     "fs_create": (_i32, [_i32, _vp, _pp]),
@@ -53,6 +57,10 @@ SIGNATURES = {
     "fs_partition": (_i32, [_vp, _i32, _vp, _u64, _u64, _vp, _vp, _i32, _vp, _vp, _i32]),
     "fs_host_sort_keys_copy_async": (_i32, [_vp, _i32, _vp, _vp, _u64]),
     "fs_gather": (_i32, [_vp, _i32, _vp, _u64, _vp, _vp, _u64, _i32]),
+    "fs_sample_rows": (_i32, [_vp, _i32, _vp, _u64, _u64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp]),
+    "fs_top_logprobs": (_i32, [_vp, _i32, _vp, _u64, _u64, _i64, _i32, _vp, _vp, _vp, _i32, _vp]),
+    "fs_plan_slots": (_i32, [_vp, _i32, _vp, _vp, _u64, _u32, _vp, _u64, _i64, _vp, _u64, _vp, _vp, _vp, _vp, _vp,
+                             _vp, _u64, _vp, _i32, _vp]),
     "fs_sort_pairs_copy": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _u64, _i32]),
     "fs_partition_dispatch_pairs": (_i32, [_vp, _i32, _vp, _vp, _u64, _u64, _vp, _vp, _i32, _vp, _vp, _i32]),
     "fs_stream_create": (_i32, [_i32, _vp]),

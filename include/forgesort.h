@@ -247,6 +247,88 @@ int fs_host_sort_keys_copy_async(fs_sorter* s, int dtype, const void* host_in,
 int fs_gather(fs_sorter* s, int width, const void* src, uint64_t src_n,
               const uint32_t* idx, void* dst, uint64_t n, int sync);
 
+/* ---- serving: a batch's step over the sorter's stream --------------------- */
+
+/* The three calls of a decode step.  No counterpart in the reference: each is
+ * an ordering or a running sum per row or per request, which callers of the
+ * whole-array sorts had to arrange by hand.  Device or managed pointers of the
+ * sorter's device, ready on `stream` (a cudaStream_t, or NULL for the
+ * sorter's own), on which the work is enqueued; they keep no scratch, so calls
+ * on several streams may overlap and a call may be captured into a graph
+ * (with sync == 0).  sync != 0 waits for `stream` and reports device failures,
+ * as fs_synchronize does later for sync == 0. */
+
+/* Types of logits. */
+typedef enum fs_logits_dtype {
+  FS_LOGITS_F32 = 0,
+  FS_LOGITS_F16 = 1,
+  FS_LOGITS_BF16 = 2
+} fs_logits_dtype;
+
+/* One token for each of `rows` rows of `cols` logits (cols <= 2^19; row r
+ * begins row_stride elements after row r-1, any alignment of the element
+ * type).  NaN reads as -inf (a masked entry), +inf as the type's largest
+ * finite value.  Per-row parameters, each of `rows` entries or NULL (off):
+ *   temperature  softmax(x / t); t <= 0 (or NaN) takes the first maximum
+ *                instead.  NULL: 1
+ *   top_k        keep the k largest (ties: lowest index first); k <= 0: all
+ *   top_p        then the shortest prefix of descending order that holds at
+ *                least p of the mass of those; p >= 1: all; p <= 0: the best
+ *   min_p        then the entries of at least min_p times the largest weight
+ * uniform holds one number u of [0, 1) for each row (clamped to it): the
+ * token is the first index at which the running mass of the kept entries, in
+ * index order, exceeds u times their sum.  Weights are 32-bit 2^-y with
+ * y = (max - x) * (log2(e) / t), each rounded to a whole multiple of 2^-40,
+ * and all sums are of whole numbers: equal inputs give equal tokens, whatever
+ * the batch around them.  logprobs (or NULL) gets log softmax(x / t) of the
+ * token over the whole row (t <= 0: over softmax(x)).  A row without an entry
+ * above -inf gets token -1 and log-probability -inf. */
+int fs_sample_rows(fs_sorter* s, int dtype, const void* logits, uint64_t rows,
+                   uint64_t cols, int64_t row_stride, const float* temperature,
+                   const int32_t* top_k, const float* top_p, const float* min_p,
+                   const float* uniform, int32_t* tokens, float* logprobs,
+                   int sync, void* stream);
+
+/* The n (1..1024) largest logits of each row in descending order (ties:
+ * lowest index first): their indices (rows x n), their log softmax(x)
+ * (rows x n) and the row's log-sum-exp (lse, or NULL).  Rows as in
+ * fs_sample_rows; places beyond the row's entries above -inf get index -1 and
+ * log-probability -inf. */
+int fs_top_logprobs(fs_sorter* s, int dtype, const void* logits, uint64_t rows,
+                    uint64_t cols, int64_t row_stride, int n, int32_t* indices,
+                    float* logprobs, float* lse, int sync, void* stream);
+
+/* Plans a step of `requests` requests over a paged cache: request r has
+ * context_lens[r] tokens in it and gets new_lens[r] more (integers of
+ * index_bytes = 4 or 8 bytes; below 0 reads as 0).  Pages of page_size tokens
+ * that they need beyond the ceil(context / page_size) they hold are taken from
+ * free_pages[cursor[0] ..] in request order and entered into block_table (one
+ * row of table_width entries per request, table_stride entries apart; the
+ * entries of pages held are read, the new ones written, no other touched).
+ * Writes:
+ *   query_start  requests + 1 entries: where each request's tokens start
+ *   seq_lens     context + new of each request (index_bytes each)
+ *   positions    of each token in its request (index_bytes each), 0 beyond
+ *                the last token
+ *   request_of   the token's request, -1 beyond the last token
+ *   slots        page * page_size + position % page_size, -1 beyond the last
+ *                token and where a token has no page
+ *   cursor_out   cursor[0] + pages needed, at most n_free (not the same
+ *                memory as cursor: a call may be repeated)
+ * positions, request_of and slots hold `capacity` entries.  A token without a
+ * page (free pages used up, a row of the block table full, a negative entry
+ * where a held page should be) or tokens beyond `capacity` are reported as
+ * FS_E_GPU_EXECUTION at the next synchronisation; what has a page is still
+ * planned. */
+int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_lens,
+                  const void* new_lens, uint64_t requests, uint32_t page_size,
+                  int32_t* block_table, uint64_t table_width,
+                  int64_t table_stride, const int32_t* free_pages,
+                  uint64_t n_free, const int32_t* cursor, int32_t* query_start,
+                  void* seq_lens, void* positions, int32_t* request_of,
+                  int64_t* slots, uint64_t capacity, int32_t* cursor_out,
+                  int sync, void* stream);
+
 /* ---- streams --------------------------------------------------------------- */
 
 /* A non-blocking CUDA stream on `device`, for callers that have no CUDA
