@@ -10,6 +10,9 @@ using namespace fs;
 
 namespace {
 
+// Shared-memory bytes of row data a CTA may hold: a row of 2^19 32-bit logits over 16 CTAs.
+constexpr uint32_t ROW_PART_MAX = 132u << 10;
+
 #define FS_ROWS_CUDA(s, call)                                        \
   do {                                                               \
     cudaError_t e_ = (call);                                         \
@@ -18,37 +21,39 @@ namespace {
 
 size_t elem_bytes(int dtype) { return dtype == FS_LOGITS_F32 ? 4 : 2; }
 
-// CTAs per row.  A row is cut until a part fits PART bytes of shared memory,
-// and further while the batch has fewer CTAs than the GPU has SMs and a part
+// CTAs per row.  A row is cut until three CTAs of its parts fit an SM, and
+// further while the batch has fewer CTAs than the GPU has SMs and a part
 // keeps PART_MIN bytes.
 constexpr uint32_t PART = 64u << 10;
-constexpr uint32_t PART_MIN = 8u << 10;
+constexpr uint32_t PART_MIN = 16u << 10;
 
 uint32_t row_ctas(uint32_t vecs, uint64_t rows, int sm_count) {
   uint32_t c = 1;
   while (c < ROW_MAX_CLUSTER && (uint64_t)((vecs + c - 1) / c) * 16 > PART) c <<= 1;
-  while (c < ROW_MAX_CLUSTER && rows * c * 2 <= (uint64_t)sm_count && (uint64_t)((vecs + 2 * c - 1) / (2 * c)) * 16 >= PART_MIN)
+  while (c < 8 && rows * c * 2 <= (uint64_t)sm_count && (uint64_t)((vecs + 2 * c - 1) / (2 * c)) * 16 >= PART_MIN)
     c <<= 1;
   return c;
 }
-
-constexpr size_t SHARED_BYTES = (sizeof(RowShared) + 15) / 16 * 16;
 
 template <typename Kern>
 int launch(fs_sorter* s, const SorterView& v, Kern kern, std::atomic<bool>* configured, RowArgs& a, int lanes) {
   if (!configured[v.device].load()) {  // idempotent: two threads may both get here
     FS_ROWS_CUDA(s, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(SHARED_BYTES + ROW_PART_MAX)));
+                                         (int)(ROW_SHARED_BYTES + ROW_PART_MAX)));
     FS_ROWS_CUDA(s, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured[v.device].store(true);
   }
-  const uint32_t vecs = (a.cols + 2 * lanes - 2) / lanes;  // with the worst lead of lanes - 1
+  // vectors of a row: with the worst lead of lanes - 1 elements, unless every row begins at a vector
+  const int64_t step = a.rows > 1 ? a.stride : 0;
+  const bool aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && step % lanes == 0;
+  const uint32_t vecs = (a.cols + (aligned ? lanes - 1 : 2 * lanes - 2)) / lanes;
   const uint32_t ctas = row_ctas(vecs, a.rows, v.sm_count);
   a.part_vecs = (vecs + ctas - 1) / ctas;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.rows * ctas);
   cfg.blockDim = dim3(ROW_THREADS);
-  cfg.dynamicSmemBytes = SHARED_BYTES + (size_t)a.part_vecs * 16;
+  const size_t part = (size_t)a.part_vecs * 16;
+  cfg.dynamicSmemBytes = ROW_SHARED_BYTES + (part > sizeof(RowFinish) ? part : sizeof(RowFinish));
   cfg.stream = v.stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -27,21 +27,30 @@ namespace fs {
 
 namespace cg = cooperative_groups;
 
-constexpr int ROW_THREADS = 512;
+constexpr int ROW_THREADS = 256;
 constexpr int ROW_WARPS = ROW_THREADS / 32;
 constexpr int ROW_MAX_CLUSTER = 16;
-constexpr uint32_t ROW_MAX_COLS = 1u << 19;
-constexpr int ROW_BINS = 2048;
+constexpr int ROW_IDX_BITS = 19;
+constexpr uint32_t ROW_MAX_COLS = 1u << ROW_IDX_BITS;
+constexpr int ROW_LIST = 640;   // candidates of a row above its edge
+constexpr int ROW_POOL = 1024;  // undecided entries of a row that narrowing leaves
+constexpr int ROW_FEW = 256;    // ... where they are ranked in place
 constexpr int ROW_BEST_MAX = 1024;
-// Level-0 bins of a selection: linear in y, 1/48 of an octave of weight each,
-// so that the bins 0..2046 cover every entry with q > 0 (y < 41) and the last
-// one the rest.
-constexpr float ROW_BIN_SCALE = 48.0f;
-// Shared-memory bytes of row data a CTA may hold.
-constexpr uint32_t ROW_PART_MAX = 160u << 10;
+constexpr int ROW_TOPS = 512;   // thread maxima that a cluster's warps publish
+// A nucleus is first looked for among about this many entries.
+constexpr uint32_t ROW_NUCLEUS_GUESS = 128;
+// Bins linear in y: of the published maxima (1/6 octave of weight each, 42 in
+// all; entries with q > 0 have y < 41), and of all entries (1/42 octave).
+constexpr int ROW_EDGE_BINS = 256;  // one a thread
+constexpr float ROW_EDGE_SCALE = 6.0f;
+constexpr int ROW_BINS = 1792;
+constexpr float ROW_BIN_SCALE = 42.0f;
+constexpr float ROW_MASS_END = 42.0f;  // octaves: no mass beyond
+constexpr int ROW_SORT_BINS = 1024;
 
 constexpr float ROW_LOG2E = 1.4426950408889634f;
 constexpr float ROW_LN2 = 0.6931471805599453f;
+constexpr float ROW_F32_MAX = 3.402823466e+38f;
 
 struct RowArgs {
   const void* x;        // rows x cols logits
@@ -64,46 +73,94 @@ struct RowArgs {
 };
 
 // ---- elements -------------------------------------------------------------------
-// A 16-byte vector of logits with NaN read as -inf and +inf as the type's
-// largest finite value: -inf is then the only value that is not finite.
+// 16-byte vectors of logits.  top() is the maximum with NaN passed on, so that
+// a thread whose running maximum is NaN or +inf knows that it has values to
+// clean: NaN becomes -inf and +inf the type's largest finite value, after
+// which -inf is the only value that is not finite.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <typename T> struct RowElem;
 template <> struct RowElem<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ uint32_t clean(uint32_t v) {
-    return __float_as_uint(fminf(fmaxf(__uint_as_float(v), -INFINITY), 3.402823466e+38f));
-  }
-  static __device__ __forceinline__ float get(const uint4& v, int e) {
-    return __uint_as_float(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w);
-  }
   static constexpr uint32_t NEG_INF = 0xff800000u;  // fills a 32-bit word
+  using Top = float;                                // running maximum
+  static __device__ __forceinline__ Top top0() { return -INFINITY; }
+  static __device__ __forceinline__ Top top(Top t, const uint4& v) {
+    return fmax_nan(fmax_nan(fmax_nan(t, __uint_as_float(v.x)), fmax_nan(__uint_as_float(v.y), __uint_as_float(v.z))),
+                    __uint_as_float(v.w));
+  }
+  static __device__ __forceinline__ float value(Top t) { return t; }
+  static __device__ __forceinline__ uint32_t clean(uint32_t v) {
+    return __float_as_uint(fminf(fmaxf(__uint_as_float(v), -INFINITY), ROW_F32_MAX));
+  }
+  static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+  }
 };
 template <> struct RowElem<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ uint32_t clean(uint32_t v) {
-    __nv_bfloat162 b = *reinterpret_cast<__nv_bfloat162*>(&v);
-    const uint32_t lo = 0xff80ff80u, hi = 0x7f7f7f7fu;
-    b = __hmin2(__hmax2(b, *reinterpret_cast<const __nv_bfloat162*>(&lo)), *reinterpret_cast<const __nv_bfloat162*>(&hi));
-    return *reinterpret_cast<uint32_t*>(&b);
-  }
-  static __device__ __forceinline__ float get(const uint4& v, int e) {
-    const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
-    return __uint_as_float((e & 1) ? (w & 0xffff0000u) : (w << 16));
-  }
   static constexpr uint32_t NEG_INF = 0xff80ff80u;
+  using Top = uint32_t;
+  static __device__ __forceinline__ Top top0() { return NEG_INF; }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ Top top(Top t, const uint4& v) {
+    return max2(max2(t, v.x), max2(max2(v.y, v.z), v.w));
+  }
+  static __device__ __forceinline__ float value(Top t) {
+    return fmax_nan(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t clean(uint32_t v) {
+    asm("max.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(NEG_INF));
+    asm("min.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7f7f7f7fu));
+    return v;
+  }
+  static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[2 * k] = __uint_as_float(w[k] << 16), x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+  }
 };
 template <> struct RowElem<__half> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ uint32_t clean(uint32_t v) {
-    __half2 b = *reinterpret_cast<__half2*>(&v);
-    const uint32_t lo = 0xfc00fc00u, hi = 0x7bff7bffu;
-    b = __hmin2(__hmax2(b, *reinterpret_cast<const __half2*>(&lo)), *reinterpret_cast<const __half2*>(&hi));
-    return *reinterpret_cast<uint32_t*>(&b);
-  }
-  static __device__ __forceinline__ float get(const uint4& v, int e) {
-    const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
-    return __half2float(__ushort_as_half((unsigned short)((e & 1) ? (w >> 16) : (w & 0xffffu))));
-  }
   static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+  using Top = uint32_t;
+  static __device__ __forceinline__ Top top0() { return NEG_INF; }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ Top top(Top t, const uint4& v) {
+    return max2(max2(t, v.x), max2(max2(v.y, v.z), v.w));
+  }
+  static __device__ __forceinline__ float2 both(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+  static __device__ __forceinline__ float value(Top t) {
+    const float2 f = both(t);
+    return fmax_nan(f.x, f.y);
+  }
+  static __device__ __forceinline__ uint32_t clean(uint32_t v) {
+    asm("max.f16x2 %0, %0, %1;" : "+r"(v) : "r"(NEG_INF));
+    asm("min.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7bff7bffu));
+    return v;
+  }
+  static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = both(w[k]);
+      x[2 * k] = f.x, x[2 * k + 1] = f.y;
+    }
+  }
 };
 
 __device__ __forceinline__ uint4 row_load(const uint4* p) {
@@ -128,30 +185,48 @@ __device__ __forceinline__ float row_exp2(float v) {
   return r;
 }
 
-// y = (m - x) c, each step rounded (no fused multiply-add).
-__device__ __forceinline__ float row_y(float x, float m, float c) { return __fmul_rn(__fsub_rn(m, x), c); }
+// -y = (x - m) c, each step rounded (no fused multiply-add).
+__device__ __forceinline__ float row_neg_y(float x, float m, float c) { return __fmul_rn(__fsub_rn(x, m), c); }
 
 // q = round(w 2^40) of 0 <= w <= 1 in two 32-bit parts, by two additions that
 // push the unwanted bits out of the mantissa: hi = w to a multiple of 2^-23
 // (the mantissa bits of w + 1), lo = the rest to a multiple of 2^-40 (the
 // mantissa bits of rest + 1.5 2^-17).  Each addition rounds half to even and
-// w - hi is exact.  (A conversion to a 64-bit integer would run at the rate
-// of the exponential; these are ordinary additions.)
-struct RowQ {
-  uint32_t hi;  // units of 2^-23
-  int lo;       // units of 2^-40
-};
-__device__ __forceinline__ RowQ row_quant(float w) {
-  constexpr float MAGIC = 1.5f / 131072.0f;
-  const float a = __fadd_rn(w, 1.0f);
-  const float r = __fsub_rn(w, __fsub_rn(a, 1.0f));
-  const float b = __fadd_rn(r, MAGIC);
-  return RowQ{__float_as_uint(a) - 0x3f800000u, __float_as_int(b) - __float_as_int(MAGIC)};
-}
-__device__ __forceinline__ uint64_t row_mass(uint64_t hi, int64_t lo) { return (hi << 17) + (uint64_t)lo; }
+// w - hi is exact.  (A conversion to an integer runs at the rate of the
+// exponential, an eighth of that of these additions.)
+constexpr float ROW_MAGIC = 1.5f / 131072.0f;
+constexpr uint32_t ROW_ONE_BITS = 0x3f800000u;    // 1.0f
+constexpr uint32_t ROW_MAGIC_BITS = 0x37400000u;  // 1.5 2^-17
+__device__ __forceinline__ uint64_t row_mass(uint32_t hi, int lo) { return ((uint64_t)hi << 17) + (int64_t)lo; }
 __device__ __forceinline__ uint64_t row_q(float w) {
-  const RowQ q = row_quant(w);
-  return row_mass(q.hi, q.lo);
+  const float a = __fadd_rn(w, 1.0f);
+  const float b = __fadd_rn(__fsub_rn(w, __fsub_rn(a, 1.0f)), ROW_MAGIC);
+  return row_mass(__float_as_uint(a) - ROW_ONE_BITS, __float_as_int(b) - (int)ROW_MAGIC_BITS);
+}
+
+// Two 32-bit numbers in one instruction.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
@@ -159,39 +234,44 @@ __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
   return v;
 }
-__device__ __forceinline__ uint64_t warp_scan_u64(uint64_t v, int lane) {  // inclusive
+template <typename V> __device__ __forceinline__ V warp_scan(V v, int lane) {  // inclusive
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const uint64_t o = __shfl_up_sync(~0u, v, d);
+    const V o = __shfl_up_sync(~0u, v, d);
     if (lane >= d) v += o;
   }
   return v;
 }
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // ---- shared state ---------------------------------------------------------------
-struct RowPick {     // what the cluster's first CTA found in a histogram
-  uint32_t bin;      // ROW_BINS: the target is beyond the last entry
-  uint32_t above_n;  // entries of the bins before it
-  uint32_t bin_n;
-  uint64_t above_q;  // mass of the bins before it
-  uint64_t bin_q;
-};
-struct RowCut {  // entries before or at (key, idx) in (key, index) order
-  uint32_t key;
-  uint32_t idx;
-  uint64_t mass;  // their mass
-};
-
 struct RowShared {
-  uint64_t q[ROW_BINS];  // bin masses; the list of the best
-  uint32_t n[ROW_BINS];  // bin counts
-  uint64_t warp_q[ROW_WARPS];
-  uint32_t warp_n[ROW_WARPS];
-  uint64_t cta_q[ROW_MAX_CLUSTER];
-  float cta_max[ROW_MAX_CLUSTER];
-  RowPick pick;
-  uint32_t found;
-  uint32_t count;
+  union {
+    struct {
+      uint64_t list[ROW_LIST];         // candidates: key << 19 | index
+      uint32_t tops[ROW_TOPS];         // keys of the largest thread maxima of each warp of the cluster
+      uint32_t edge_n[ROW_EDGE_BINS];  // those by bin
+    };
+    uint32_t bins[ROW_BINS];  // while a cut is narrowed down: weights or counts,
+    uint64_t pool[ROW_POOL];  // then the undecided entries
+  };
+  uint64_t mass[ROW_MAX_CLUSTER][ROW_WARPS];  // of each warp of the cluster
+  uint64_t part[ROW_MAX_CLUSTER][ROW_WARPS];  // of its candidates; of its kept entries
+  uint64_t scan_q[ROW_WARPS];
+  uint32_t scan_n[ROW_WARPS];
+  uint32_t n[ROW_MAX_CLUSTER];
+  uint64_t lo, hi, cut_q;
+  uint32_t cut_n, count, above, first, b1, b2;
+};
+constexpr size_t ROW_SHARED_BYTES = (sizeof(RowShared) + 15) / 16 * 16;
+static_assert(3 * (ROW_SHARED_BYTES + (64 << 10) + 1024) <= 228 << 10, "three CTAs on an SM");
+
+// What the first CTA lays over its part of the row when only the listed
+// entries (or the copy in memory) matter any more.
+struct RowFinish {
+  uint32_t start[ROW_SORT_BINS + 4];
+  uint64_t loose[ROW_POOL];
+  uint64_t sorted[ROW_POOL];
 };
 
 // ---- one row --------------------------------------------------------------------
@@ -204,11 +284,18 @@ template <typename T> struct Row {
   uint4* data;
   const int tid, lane, wid;
   const uint32_t rank, ctas;
+  // the row in memory, cut into 16-byte vectors at memory's boundaries
+  const T* x;
+  const uint4* vecs;
+  uint32_t cols, part_vecs;
+  int lead;             // elements of the first vector that are not the row's
+  uint32_t total_vecs;
   uint32_t seg0, seg1;  // this warp's vectors of the CTA's part
   int first;            // index of the part's element 0 (negative inside the row's leading fill)
+  float mine;           // this thread's maximum
   float m, c;
 
-  __device__ __forceinline__ Row(RowShared& s, uint4* d)
+  __device__ __forceinline__ Row(RowShared& s, uint4* d, const RowArgs& a, uint32_t row)
       : cluster(cg::this_cluster()),
         sh(s),
         data(d),
@@ -217,262 +304,650 @@ template <typename T> struct Row {
         wid(threadIdx.x >> 5),
         rank(cluster.block_rank()),
         ctas(cluster.num_blocks()) {
+    sh.edge_n[tid] = 0;
+    if (tid == 0) sh.count = 0, sh.first = ~0u;
     cluster.barrier_arrive();  // waited for in load(): no CTA writes into one that has not started
+    x = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
+    cols = a.cols;
+    part_vecs = a.part_vecs;
+    lead = (int)((uint32_t)(reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    total_vecs = ((uint32_t)lead + cols + N - 1) / N;
+    vecs = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x) & ~(uintptr_t)15);
   }
 
-  // Reads this CTA's part into shared memory and finds the row's maximum.  The
-  // part is cut at 16-byte boundaries of memory, wherever the row begins;
-  // slots outside the row hold -inf.
-  __device__ __forceinline__ void load(const RowArgs& a, uint32_t row) {
-    const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
-    const uint32_t lead = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T);
-    const uint32_t total = (lead + a.cols + N - 1) / N;
-    const uint32_t v0 = min(rank * a.part_vecs, total), v1 = min(v0 + a.part_vecs, total);
-    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x) & ~(uintptr_t)15) + v0;
-    first = (int)(v0 * N) - (int)lead;
-    const uint32_t nv = v1 - v0, sv = (nv + ROW_WARPS - 1) / ROW_WARPS;
-    seg0 = min(wid * sv, nv);
-    seg1 = min(seg0 + sv, nv);
-    float mx = -INFINITY;
+  static __device__ __forceinline__ uint4 nothing() {
+    return make_uint4(E::NEG_INF, E::NEG_INF, E::NEG_INF, E::NEG_INF);
+  }
+  static __device__ __forceinline__ uint4 cleaned(uint4 v) {
+    v.x = E::clean(v.x), v.y = E::clean(v.y), v.z = E::clean(v.z), v.w = E::clean(v.w);
+    return v;
+  }
+  __device__ __forceinline__ bool inside(uint32_t v) const {  // all of the row's vector v belongs to the row
+    const int j0 = (int)(v * N) - lead;
+    return j0 >= 0 && j0 + N <= (int)cols;
+  }
+  __device__ __forceinline__ uint4 ragged(uint32_t v) const {  // the row's first or last vector
+    const int j0 = (int)(v * N) - lead;
+    union { uint4 v; T e[N]; } u;
+    u.v = nothing();
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (j0 + e >= 0 && j0 + e < (int)cols) u.e[e] = x[j0 + e];
+    return u.v;
+  }
+  __device__ __forceinline__ uint4 from_memory(uint32_t v) const {
+    return cleaned(inside(v) ? __ldg(vecs + v) : ragged(v));
+  }
+  // vectors [v0, v1) of warp w's stretch of CTA r's part
+  __device__ __forceinline__ void stretch(uint32_t r, uint32_t w, uint32_t& v0, uint32_t& v1) const {
+    const uint32_t p0 = min(r * part_vecs, total_vecs), p1 = min(p0 + part_vecs, total_vecs);
+    const uint32_t sv = (p1 - p0 + ROW_WARPS - 1) / ROW_WARPS;
+    v0 = min(p0 + w * sv, p1);
+    v1 = min(v0 + sv, p1);
+  }
+
+  // Reads this CTA's part into shared memory and finds the row's maximum.
+  // Each warp has a stretch of its own, in index order; each thread copies the
+  // vectors that it will work on itself, all of them in flight at once, so
+  // nothing but its own copies has to be waited for.
+  // With `tops`, the warps also publish their threads' largest maxima.
+  __device__ __forceinline__ void load(bool tops) {
+    const uint32_t p0 = min(rank * part_vecs, total_vecs);
+    stretch(rank, wid, seg0, seg1);
+    seg0 -= p0, seg1 -= p0;
+    first = (int)(p0 * N) - lead;
     for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
-      const int j0 = first + (int)(i * N);
-      uint4 v;
-      if (j0 >= 0 && j0 + N <= (int)a.cols) {
-        v = row_load(src + i);
-      } else {  // the row's first or last vector
-        union { uint4 v; T e[N]; } u;
-        u.v = make_uint4(E::NEG_INF, E::NEG_INF, E::NEG_INF, E::NEG_INF);
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (j0 + e >= 0 && j0 + e < (int)a.cols) u.e[e] = x[j0 + e];
-        v = u.v;
-      }
-      v.x = E::clean(v.x), v.y = E::clean(v.y), v.z = E::clean(v.z), v.w = E::clean(v.w);
-      data[i] = v;
-#pragma unroll
-      for (int e = 0; e < N; ++e) mx = fmaxf(mx, E::get(v, e));
+      if (inside(p0 + i))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_of(data + i)), "l"(vecs + p0 + i) : "memory");
+      else
+        data[i] = ragged(p0 + i);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    typename E::Top top = E::top0();
+#pragma unroll 4
+    for (uint32_t i = seg0 + lane; i < seg1; i += 32) top = E::top(top, data[i]);
+    mine = E::value(top);
+    if (!(mine <= ROW_F32_MAX)) {  // NaN or +inf among this thread's entries
+      top = E::top0();
+      for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
+        const uint4 v = cleaned(data[i]);
+        data[i] = v;
+        top = E::top(top, v);
+      }
+      mine = E::value(top);
+    }
+    // the warp's maxima in ascending order of key: lane 0 has the largest entry
+    uint32_t k = row_key(mine);
+    if (tops) {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, d));
-    float* warp_max = reinterpret_cast<float*>(sh.warp_n);
-    if (lane == 0) warp_max[wid] = mx;
-    __syncthreads();
+      for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+        for (int d = n >> 1; d; d >>= 1) {
+          const uint32_t o = __shfl_xor_sync(~0u, k, d);
+          k = ((lane & d) == 0) == ((lane & n) == 0) ? min(k, o) : max(k, o);
+        }
+    } else {
+      k = __reduce_min_sync(~0u, k);
+    }
     cluster.barrier_wait();
-    if (tid < (int)ctas) {  // thread t tells CTA t
-      float b = -INFINITY;
-      for (int w = 0; w < ROW_WARPS; ++w) b = fmaxf(b, warp_max[w]);
-      *cluster.map_shared_rank(&sh.cta_max[rank], tid) = b;
+    const uint32_t per = top_count();
+    for (uint32_t i = lane; i < per * ctas; i += 32) {  // (32 or 64) entry e of CTA i / per's copy
+      const uint32_t e = i & (per - 1), v = __shfl_sync(~0u, k, e);
+      if (tops || e == 0) *cluster.map_shared_rank(&sh.tops[(rank * ROW_WARPS + wid) * per + e], i / per) = v;
     }
     cluster.sync();
-    m = -INFINITY;
-    for (uint32_t k = 0; k < ctas; ++k) m = fmaxf(m, sh.cta_max[k]);
+    uint32_t best = ~0u;
+    for (uint32_t i = lane; i < ctas * ROW_WARPS; i += 32) best = min(best, sh.tops[i * per]);
+    m = row_unkey(__reduce_min_sync(~0u, best));
   }
+  // How many of its 32 sorted thread maxima a warp publishes.
+  __device__ __forceinline__ uint32_t top_count() const { return min(32u, (uint32_t)ROW_TOPS / (ctas * ROW_WARPS)); }
 
   // f(x, index) for every entry of this thread
   template <typename F> __device__ __forceinline__ void each(F f) const {
     for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
-      const uint4 v = data[i];
+      float v[N];
+      E::get(data[i], v);
       const int j0 = first + (int)(i * N);
 #pragma unroll
-      for (int e = 0; e < N; ++e) f(E::get(v, e), j0 + e);
+      for (int e = 0; e < N; ++e) f(v[e], j0 + e);
     }
   }
 
-  // Sums `mine` over the cluster; leaves the warps' sums in sh.warp_q and the
-  // CTAs' in sh.cta_q.
-  __device__ __forceinline__ uint64_t sum(uint64_t mine) {
-    const uint64_t w = warp_sum_u64(mine);
-    if (lane == 0) sh.warp_q[wid] = w;
+  __device__ __forceinline__ float weight(float v) const { return row_exp2(row_neg_y(v, m, c)); }
+  __device__ __forceinline__ uint64_t mass(float v) const { return row_q(weight(v)); }
+  __device__ __forceinline__ uint32_t bin_of(float v, float scale, int bins) const {
+    return (uint32_t)fminf(__fmul_rn(-row_neg_y(v, m, c), scale), (float)(bins - 1));
+  }
+
+  // Exclusive sum over the block, and the block's sum.
+  template <typename V> __device__ __forceinline__ V block_scan(V v, V* scratch, V& all) const {
+    const V in = warp_scan(v, lane);
+    if (lane == 31) scratch[wid] = in;
     __syncthreads();
-    if (tid < (int)ctas) {
-      uint64_t t = 0;
-      for (int k = 0; k < ROW_WARPS; ++k) t += sh.warp_q[k];
-      *cluster.map_shared_rank(&sh.cta_q[rank], tid) = t;
+    V before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < ROW_WARPS; ++w) {
+      const V s = scratch[w];
+      if (w < wid) before += s;
+      all += s;
     }
-    cluster.sync();
-    uint64_t t = 0;
-    for (uint32_t k = 0; k < ctas; ++k) t += sh.cta_q[k];
-    return t;
+    return before + in - v;
   }
 
-  // After sum() of value(x, index): the entry at which the running sum in
-  // index order first exceeds t calls hit(x, index), on one thread of the cluster.
-  template <typename V, typename H> __device__ __forceinline__ void locate(uint64_t t, V value, H hit) {
-    uint64_t before = 0;
-    for (uint32_t k = 0; k < rank; ++k) before += sh.cta_q[k];
-    if (t < before || t - before >= sh.cta_q[rank]) return;
-    t -= before;
-    for (int k = 0; k < wid; ++k) {
-      if (t < sh.warp_q[k]) return;
-      t -= sh.warp_q[k];
+  // ---- the one pass over all weights ----
+  // The mass of this thread's entries (ABOVE: of those over `least`).  Per
+  // entry: a half of four packed additions, a half of one packed
+  // multiplication, the exponential and one integer addition.  A thread holds
+  // fewer than 2^9 entries, so that neither 32-bit sum of hi < 2^23 or
+  // |lo| <= 2^17 wraps.
+  template <bool ABOVE> __device__ __forceinline__ uint64_t weigh(float least) const {
+    const uint64_t m2 = f2_pack(-m, -m), c2 = f2_pack(c, c), one = f2_pack(1.0f, 1.0f), none = f2_pack(-1.0f, -1.0f),
+                   magic = f2_pack(ROW_MAGIC, ROW_MAGIC);
+    uint32_t hi = 0, lo = 0, n = 0;
+#pragma unroll 2
+    for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
+      float f[N];
+      E::get(data[i], f);
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        float w0, w1, a0, a1, b0, b1;
+        f2_unpack(f2_mul(f2_add(f2_pack(f[e], f[e + 1]), m2), c2), w0, w1);
+        w0 = row_exp2(w0), w1 = row_exp2(w1);
+        if (ABOVE) w0 = f[e] > least ? w0 : 0.0f, w1 = f[e + 1] > least ? w1 : 0.0f;
+        const uint64_t w = f2_pack(w0, w1);
+        const uint64_t a = f2_add(w, one);
+        const uint64_t b = f2_add(f2_fma(f2_add(a, none), none, w), magic);
+        f2_unpack(a, a0, a1);
+        f2_unpack(b, b0, b1);
+        hi += __float_as_uint(a0) + __float_as_uint(a1);
+        lo += __float_as_uint(b0) + __float_as_uint(b1);
+      }
+      n += N;
     }
-    if (t >= sh.warp_q[wid]) return;
-    for (uint32_t i0 = seg0; i0 < seg1; i0 += 32) {
-      const uint32_t i = i0 + lane;
-      uint64_t mine = 0;
-      uint4 v = make_uint4(E::NEG_INF, E::NEG_INF, E::NEG_INF, E::NEG_INF);
+    return row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
+  }
+
+  // Calls f(x, index) for this thread's entries in [low, high].
+  template <typename F> __device__ __forceinline__ void between(float low, float high, F f) const {
+    if (mine < low) return;
+    for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
+      const uint4 v = data[i];
+      if (E::value(E::top(E::top0(), v)) < low) continue;
+      float z[N];
+      E::get(v, z);
       const int j0 = first + (int)(i * N);
-      if (i < seg1) {
-        v = data[i];
 #pragma unroll
-        for (int e = 0; e < N; ++e) mine += value(E::get(v, e), j0 + e);
-      }
-      const uint64_t upto = warp_scan_u64(mine, lane);
-      const uint64_t all = __shfl_sync(~0u, upto, 31);
-      if (t >= all) {
-        t -= all;
-        continue;
-      }
-      if (t < upto && t >= upto - mine) {
-        uint64_t left = t - (upto - mine);
-        bool done = false;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float x = E::get(v, e);
-          const uint64_t q = value(x, j0 + e);
-          if (!done && left < q) {
-            hit(x, j0 + e);
-            done = true;
-          }
-          left -= q;
-        }
-      }
-      return;
+      for (int e = 0; e < N; ++e)
+        if (z[e] >= low && z[e] <= high) f(z[e], j0 + e);
     }
   }
 
-  __device__ __forceinline__ float weight(float x) const { return row_exp2(-row_y(x, m, c)); }
-  __device__ __forceinline__ uint64_t mass(float x) const { return row_q(weight(x)); }
-  __device__ __forceinline__ uint32_t bin0(float x) const {
-    return (uint32_t)fminf(__fmul_rn(row_y(x, m, c), ROW_BIN_SCALE), (float)(ROW_BINS - 1));
+  // A value with at least `k` of the row's entries at or above it: the k-th
+  // largest of the published thread maxima, rounded down to the bound of a bin
+  // of 1 / scale and by more than the bound's rounding.  Where fewer are within
+  // the bins: `last`.  Of entries in no particular order, and maxima of G
+  // groups, about G ln(G / (G - k)) lie above the k-th largest maximum: hardly
+  // more than k.  Every warp scans the histogram for itself, which spares a
+  // barrier.
+  __device__ __forceinline__ float edge_of(uint32_t k, float scale, float last) {
+    const uint32_t tops = top_count() * ctas * ROW_WARPS;
+    scale = fminf(scale, ROW_F32_MAX);
+    for (uint32_t i = tid; i < tops; i += ROW_THREADS) {
+      const float z = row_unkey(sh.tops[i]);
+      if (z > -INFINITY)
+        atomicAdd(&sh.edge_n[(uint32_t)fminf(__fmul_rn(__fsub_rn(m, z), scale), (float)(ROW_EDGE_BINS - 1))], 1u);
+    }
+    __syncthreads();
+    constexpr int PER = ROW_EDGE_BINS / 32;
+    uint32_t n[PER], t = 0;
+#pragma unroll
+    for (int b = 0; b < PER; ++b) n[b] = sh.edge_n[lane * PER + b], t += n[b];
+    const uint32_t upto = warp_scan(t, lane);
+    const uint32_t has = __ballot_sync(~0u, upto >= k);
+    if (!has) return last;
+    uint32_t bin = lane * PER, run = upto - t;
+#pragma unroll
+    for (int b = 0; b + 1 < PER; ++b) {
+      run += n[b];
+      bin += run < k;
+    }
+    bin = __shfl_sync(~0u, bin, __ffs((int)has) - 1);
+    if (bin >= (uint32_t)ROW_EDGE_BINS - 1) return last;
+    const float d = (float)(bin + 1) / scale;
+    return fmaxf(m - d * (1.0f + 0x1p-18f) - fabsf(m) * 0x1p-21f, last);
+  }
+  // Its scale where 42 octaves of weight are too short: up to the smallest
+  // maximum, or 512.  Empties the bins again.
+  __device__ __forceinline__ float far_scale() {
+    const uint32_t tops = top_count() * ctas * ROW_WARPS;
+    float low = m;
+    for (uint32_t i = lane; i < tops; i += 32) {
+      const float z = row_unkey(sh.tops[i]);
+      if (z > m - 512.0f) low = fminf(low, z);
+    }
+    low = row_unkey(__reduce_max_sync(~0u, row_key(low)));
+    __syncthreads();
+    sh.edge_n[tid] = 0;
+    __syncthreads();
+    return (ROW_EDGE_BINS - 2) / fmaxf(m - low, 0x1p-20f);
+  }
+  // Below this no entry has mass.
+  __device__ __forceinline__ float mass_end() const {
+    return fmaxf(m - ROW_MASS_END / c - fabsf(m) * 0x1p-21f, -ROW_F32_MAX);
   }
 
-  // Histogram of the entries for which digit(x, key) gives a bin, over the
-  // whole row; then the bin where the running count (BY_MASS: mass) reaches
-  // `target`.
-  template <bool BY_MASS, typename D> __device__ __forceinline__ RowPick pick(uint64_t target, D digit) {
-    for (int b = tid; b < ROW_BINS; b += ROW_THREADS) sh.n[b] = 0, sh.q[b] = 0;
-    cluster.sync();
-    each([&](float x, int) {
-      if (x == -INFINITY) return;
-      const uint32_t b = digit(x, row_key(x));
-      if (b >= (uint32_t)ROW_BINS) return;
-      atomicAdd(&sh.n[b], 1u);
-      const uint64_t q = mass(x);
-      if (q) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.q[b]), (unsigned long long)q);
+  // Hands this warp's masses to the first CTA (ALL: to every CTA).
+  template <bool ALL> __device__ __forceinline__ void hand(uint64_t own, uint64_t part) {
+    own = warp_sum_u64(own);
+    part = warp_sum_u64(part);
+    if (lane < (ALL ? (int)ctas : 1)) {
+      *cluster.map_shared_rank(&sh.mass[rank][wid], lane) = own;
+      *cluster.map_shared_rank(&sh.part[rank][wid], lane) = part;
+    }
+  }
+  // Sums of what was handed over.
+  __device__ __forceinline__ uint64_t handed(const uint64_t (&of)[ROW_MAX_CLUSTER][ROW_WARPS]) const {
+    uint64_t t = 0;
+    for (uint32_t i = lane; i < ctas * ROW_WARPS; i += 32) t += (&of[0][0])[i];
+    return warp_sum_u64(t);
+  }
+  // Collects this CTA's entries in [lo, hi] of (key, index) order at `to`, of
+  // room for `room`; sh.count is their number (sh.count = 0 before).
+  __device__ __forceinline__ void collect(uint64_t lo, uint64_t hi, uint64_t* to, uint32_t room) {
+    between(value_of(hi), value_of(lo), [&](float z, int j) {
+      const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+      if (e < lo || e > hi) return;
+      const uint32_t at = atomicAdd(&sh.count, 1u);
+      if (at < room) to[at] = e;
     });
     __syncthreads();
-    if (rank) {
-      uint32_t* n0 = cluster.map_shared_rank(sh.n, 0);
-      uint64_t* q0 = cluster.map_shared_rank(sh.q, 0);
-      for (int b = tid; b < ROW_BINS; b += ROW_THREADS)
-        if (sh.n[b]) {
-          atomicAdd(&n0[b], sh.n[b]);
-          atomicAdd(reinterpret_cast<unsigned long long*>(&q0[b]), (unsigned long long)sh.q[b]);
-        }
+    if (tid < (int)ctas) *cluster.map_shared_rank(&sh.n[rank], tid) = sh.count;
+  }
+  // After collect() on every CTA and a cluster barrier: their total, and
+  // where they fit, the other CTAs' entries go behind the first CTA's.
+  __device__ __forceinline__ uint32_t pooled(uint64_t* from, uint32_t room) {
+    uint32_t n = 0, base = 0;
+    for (uint32_t i = 0; i < ctas; ++i) {
+      if (i == rank) base = n;
+      n += sh.n[i];
     }
-    cluster.sync();
-    if (rank == 0) {
-      constexpr int PER = ROW_BINS / ROW_THREADS;
-      uint64_t tq = 0;
-      uint32_t tn = 0;
-      for (int k = 0; k < PER; ++k) tq += sh.q[tid * PER + k], tn += sh.n[tid * PER + k];
-      uint64_t iq = warp_scan_u64(tq, lane);
-      uint32_t in = tn;
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t o = __shfl_up_sync(~0u, in, d);
-        if (lane >= d) in += o;
-      }
-      if (lane == 31) sh.warp_q[wid] = iq, sh.warp_n[wid] = in;
-      if (tid == 0) sh.pick = RowPick{(uint32_t)ROW_BINS, 0, 0, 0, 0};
-      __syncthreads();
-      for (int k = 0; k < wid; ++k) iq += sh.warp_q[k], in += sh.warp_n[k];
-      uint64_t bq = iq - tq;
-      uint32_t bn = in - tn;
-      for (int k = 0; k < PER; ++k) {
-        const uint64_t q = sh.q[tid * PER + k];
-        const uint32_t n = sh.n[tid * PER + k];
-        const uint64_t lo = BY_MASS ? bq : bn, hi = BY_MASS ? bq + q : bn + n;
-        if (lo < target && target <= hi) sh.pick = RowPick{(uint32_t)(tid * PER + k), bn, n, bq, q};
-        bq += q, bn += n;
-      }
-      __syncthreads();
-      if (tid > 0 && tid < (int)ctas) *cluster.map_shared_rank(&sh.pick, tid) = sh.pick;
+    if (n <= room && rank) {
+      uint64_t* const to = cluster.map_shared_rank(from, 0) + base;
+      for (uint32_t i = tid; i < sh.n[rank]; i += ROW_THREADS) to[i] = from[i];
     }
-    cluster.sync();
-    return sh.pick;
+    return n;
+  }
+  // The end of the cluster's common work: true on the first CTA, once the
+  // others' writes into it are there; the others are done.
+  __device__ __forceinline__ bool last_part() {
+    cluster.barrier_arrive();
+    if (rank) return false;
+    cluster.barrier_wait();
+    return true;
   }
 
-  // The shortest prefix of (descending x, ascending index) order with at
-  // least `target` entries (BY_MASS: mass), target >= 1; where the row has
-  // less than that, all of it, with mass ~0.
-  template <bool BY_MASS> __device__ __noinline__ RowCut select(uint64_t target) {
-    RowPick p = pick<BY_MASS>(target, [&](float x, uint32_t) { return bin0(x); });
-    if (p.bin == (uint32_t)ROW_BINS) return RowCut{~0u, ~0u, ~0ull};
-    const uint32_t b0 = p.bin;
-    uint64_t left = target, above_q = 0;
-    left -= BY_MASS ? p.above_q : p.above_n;
-    above_q += p.above_q;
-    // Keys of the bin's entries, as far as its bounds tell; keys outside them
-    // fall into the first or the last digit, whose interval is then open.
-    const float step = 1.0f / (ROW_BIN_SCALE * c);
-    uint32_t lo = row_key(fminf(m, m - (float)b0 * step));
-    uint32_t hi = b0 == (uint32_t)ROW_BINS - 1 ? ~0u : row_key(fmaxf(m - (float)(b0 + 1) * step, -3.402823466e+38f));
-    hi = max(hi, lo);
-    bool open_lo = true, open_hi = true;
-    for (int level = 0; level < 8; ++level) {  // at most one open and three closed intervals
-      const int shift = max(0, 32 - __clz((int)((hi - lo) | 1)) - 11);
-      const uint32_t last = (hi - lo) >> shift;
-      p = pick<BY_MASS>(left, [&](float x, uint32_t k) -> uint32_t {
-        if (bin0(x) != b0) return ~0u;
-        if (k < lo) return open_lo ? 0u : ~0u;
-        if (k > hi) return open_hi ? last : ~0u;
-        return (k - lo) >> shift;
-      });
-      if (p.bin == (uint32_t)ROW_BINS) return RowCut{~0u, ~0u, ~0ull};
-      left -= BY_MASS ? p.above_q : p.above_n;
-      above_q += p.above_q;
-      const uint32_t base = lo;
-      const bool was_lo = open_lo, was_hi = open_hi;
-      open_lo = was_lo && p.bin == 0;
-      open_hi = was_hi && p.bin == last;
-      lo = open_lo ? 0u : base + (p.bin << shift);
-      const uint32_t top = base + (p.bin << shift) + ((1u << shift) - 1);
-      hi = open_hi ? ~0u : min(top, hi);
-      // an interval that was closed on both sides is now one key, or is cut again
-      if (open_lo || open_hi) {
-        open_lo = open_hi = false;
-        continue;
+  // ---- narrowing a cut down, by the whole cluster ----
+  // The smallest key from the maximum's on whose bin is b or later; one warp,
+  // 32 probes at a time.
+  __device__ __forceinline__ uint32_t first_key(uint32_t b) const {
+    uint32_t lo = row_key(m), hi = row_key(-ROW_F32_MAX) + 1;
+    while (lo < hi) {
+      const uint32_t step = max(1u, (hi - lo) / 32), at = lo + lane * step;
+      const bool past = at - lo >= hi - lo || bin_of(row_unkey(at), ROW_BIN_SCALE, ROW_BINS) >= b;
+      const uint32_t has = __ballot_sync(~0u, past);
+      if (has & 1) break;
+      const int f = has ? __ffs((int)has) - 1 : 32;
+      if (has) hi = min(hi, lo + f * step);
+      lo += (f - 1) * step + 1;
+    }
+    return lo;
+  }
+
+  // Finds an interval [sh.lo, sh.hi] of (key, index) order, with at most
+  // `most` <= ROW_POOL entries, in which the prefix of `target` entries
+  // (by_mass: mass) ends, and leaves
+  //   those entries in the first CTA's sh.pool, their number in n,
+  //   every warp's mass before the interval in sh.mass, and of that the mass
+  //   of entries with w >= least_w in sh.part, on all CTAs,
+  //   the number of entries before it in above_n.
+  // Each round counts the undecided entries by bin -- in the first round 1/42
+  // octave of weight, then a 2^-10th of the interval -- or sums their weights,
+  // each to 13 bits of its bin's, which tells the bin, or next to its bounds
+  // the two or three, that the prefix ends in; a second pass takes what comes
+  // before by its exact mass.  Ends: (key, index) has no ties.
+  // A weight as q holds it.
+  static __device__ __forceinline__ float held(float w) {
+    return w < 0x1p-17f ? __fsub_rn(__fadd_rn(w, ROW_MAGIC), ROW_MAGIC) : w;
+  }
+  __device__ __noinline__ void narrow(bool by_mass, uint64_t target, float least_w, uint32_t most, uint32_t& n,
+                                      uint32_t& above_n) {
+    uint64_t lo = (uint64_t)row_key(m) << ROW_IDX_BITS, hi = (uint64_t)row_key(-ROW_F32_MAX) << ROW_IDX_BITS | (ROW_MAX_COLS - 1);
+    uint64_t above_q = 0;
+    above_n = 0;
+    for (int round = 0;; ++round) {
+      cluster.sync();  // what the round before left has been read
+      for (int b = tid; b < ROW_BINS; b += ROW_THREADS) sh.bins[b] = 0;
+      if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ROW_BINS - 1;
+      __syncthreads();
+      cluster.barrier_arrive();  // the first CTA's bins are empty
+      const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
+      const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w;
+      if (round == 0) {
+        each([&](float z, int) {
+          const float y = __fmul_rn(-row_neg_y(z, m, c), ROW_BIN_SCALE);
+          if (by_mass) {
+            if (y < ROW_MASS_END * ROW_BIN_SCALE) {
+              const float b = truncf(y);
+              atomicAdd(&sh.bins[(int)b], (uint32_t)(held(weight(z)) * row_exp2(b * (1.0f / ROW_BIN_SCALE) + 12.0f) + 0.5f));
+            }
+          } else if (z > -INFINITY) {
+            atomicAdd(&sh.bins[(int)fminf(y, (float)(ROW_BINS - 1))], 1u);
+          }
+        });
+      } else {
+        between(value_of(hi), value_of(lo), [&](float z, int j) {
+          const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+          if (e < lo || e > hi) return;
+          atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], by_mass ? (uint32_t)(held(weight(z)) * scale + 0.5f) : 1u);
+        });
       }
-      if (shift == 0) break;
-    }
-    // p.bin_n entries share the key; the first `ties` of them in index order belong
-    const uint64_t each_q = p.bin_q / p.bin_n;
-    const uint64_t ties = BY_MASS ? (left + each_q - 1) / each_q : left;
-    RowCut cut{lo, ~0u, above_q + ties * each_q};
-    if (ties < p.bin_n) {
-      auto is = [&](float x, int) -> uint64_t { return x != -INFINITY && row_key(x) == cut.key; };
-      uint64_t mine = 0;
-      each([&](float x, int j) { mine += is(x, j); });
-      sum(mine);
-      locate(ties - 1, is, [&](float, int j) {
-        for (uint32_t k = 0; k < ctas; ++k) *cluster.map_shared_rank(&sh.found, k) = (uint32_t)j;
-      });
+      __syncthreads();
+      cluster.barrier_wait();
+      if (rank)
+        for (int b = tid; b < ROW_BINS; b += ROW_THREADS)
+          if (const uint32_t v = sh.bins[b]) atomicAdd(cluster.map_shared_rank(&sh.bins[b], 0), v);
       cluster.sync();
-      cut.idx = sh.found;
+      if (rank == 0) {
+        // the prefix ends in b1 or later, and in b2 or before: where a sum of estimates, 2^-12 of it added, and taken
+        // off, reaches the target (half a unit of at least 2730 is less than that; counts are exact)
+        constexpr int PER = ROW_BINS / ROW_THREADS;
+        float s[PER], own = 0, all;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int b = tid * PER + i;
+          s[i] = (float)sh.bins[b];
+          if (by_mass) s[i] *= round == 0 ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w;
+          own += s[i];
+        }
+        float run = block_scan(own, reinterpret_cast<float*>(sh.scan_n), all);
+        const float goal = by_mass ? (float)(target - above_q) * 0x1p-28f : (float)(target - above_n);
+        const float slack = by_mass ? 0x1p-12f : 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const bool last = tid * PER + i == ROW_BINS - 1;
+          if (run < goal && (run + s[i] >= goal || last)) sh.above = above_n + (uint32_t)run;  // read for counts alone
+          run += s[i];
+          if (run * (1.0f + slack) >= goal) atomicMin(&sh.b1, (uint32_t)(tid * PER + i));
+          if (run * (1.0f - slack) >= goal) atomicMin(&sh.b2, (uint32_t)(tid * PER + i));
+        }
+        __syncthreads();
+        if (wid < 2) {  // the interval's ends
+          const uint32_t b = wid ? sh.b2 + 1 : sh.b1;
+          uint64_t at;
+          if (round == 0)
+            at = b < (uint32_t)ROW_BINS ? (uint64_t)first_key(b) << ROW_IDX_BITS : hi + 1;
+          else
+            at = min(lo + ((uint64_t)b << shift), hi + 1);
+          if (lane < (int)ctas) {
+            *cluster.map_shared_rank(wid ? &sh.hi : &sh.lo, lane) = wid ? at - 1 : at;
+            if (wid && lane) *cluster.map_shared_rank(&sh.above, lane) = sh.above;
+          }
+        }
+      }
+      cluster.sync();
+      lo = sh.lo, hi = sh.hi;
+      // exact sums of what comes before, and the entries of the interval
+      above_n = by_mass ? 0 : sh.above;
+      uint64_t before = weigh<true>(value_of(lo)), kept;
+      if (lo & (ROW_MAX_COLS - 1))  // equal values on both sides of the bound
+        between(value_of(lo), value_of(lo), [&](float z, int j) {
+          if (((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) < lo) before += mass(z);
+        });
+      kept = before;
+      if (least_w > 0.0f) {
+        kept = 0;
+        each([&](float z, int j) {
+          const float w = weight(z);
+          if (w >= least_w && ((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) < lo) kept += row_q(w);
+        });
+      }
+      hand<true>(before, kept);
+      collect(lo, hi, sh.pool, ROW_POOL);
+      cluster.sync();
+      above_q = handed(sh.mass);
+      n = pooled(sh.pool, most);
+      if (n <= most) return;
     }
-    return cut;
+  }
+
+  // ---- ordering the candidates, on the first CTA alone ----
+  // Sorts the places c (all different) of up to ROW_POOL entries, entry i of
+  // thread tid + 256 i: in(i, c, bin) says whether there is one, its place and
+  // its bin, which grows with c.  A counting sort by bin; what shares a bin is
+  // then ranked by comparing.  Returns their number.
+  template <typename F> __device__ __forceinline__ uint32_t order(RowFinish& f, F in) {
+    constexpr int PER = ROW_POOL / ROW_THREADS;
+    uint64_t c[PER];
+    uint32_t bin[PER], at[PER];
+    static_assert(ROW_SORT_BINS == 4 * ROW_THREADS, "four bins a thread");
+    *reinterpret_cast<uint4*>(&f.start[4 * tid]) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      bin[i] = ~0u;
+      if (in(i, c[i], bin[i])) at[i] = atomicAdd(&f.start[bin[i]], 1u);
+    }
+    __syncthreads();
+    const uint4 n = *reinterpret_cast<uint4*>(&f.start[4 * tid]);
+    uint32_t all;
+    const uint32_t s = block_scan(n.x + n.y + n.z + n.w, sh.scan_n, all);
+    *reinterpret_cast<uint4*>(&f.start[4 * tid]) = make_uint4(s, s + n.x, s + n.x + n.y, s + n.x + n.y + n.z);
+    if (tid == 0) f.start[ROW_SORT_BINS] = all;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (bin[i] != ~0u) f.loose[f.start[bin[i]] + at[i]] = c[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (bin[i] != ~0u) {
+        const uint32_t b0 = f.start[bin[i]], b1 = f.start[bin[i] + 1];
+        uint32_t r = b0;
+        if (b1 - b0 > 1)
+          for (uint32_t k = b0; k < b1; ++k) r += f.loose[k] < c[i];
+        f.sorted[r] = c[i];
+      }
+    __syncthreads();
+    return all;
+  }
+
+  static __device__ __forceinline__ float value_of(uint64_t e) { return row_unkey((uint32_t)(e >> ROW_IDX_BITS)); }
+
+  // The n entries at `from` in descending order of x into f.sorted.  Bins
+  // linear in x over [low, m], or over 42 octaves where that is less.
+  __device__ __forceinline__ void order_by_value(RowFinish& f, const uint64_t* from, uint32_t n, float low) {
+    float scale = fmaxf((ROW_SORT_BINS - 1) / (m - low), (ROW_SORT_BINS - 1) / ROW_MASS_END * c);
+    if (!(scale <= ROW_F32_MAX)) scale = 0.0f;  // all equal
+    order(f, [&](int i, uint64_t& e, uint32_t& bin) {
+      if (tid + i * ROW_THREADS >= n) return false;
+      e = from[tid + i * ROW_THREADS];
+      bin = (uint32_t)fminf(__fmul_rn(__fsub_rn(m, value_of(e)), scale), (float)(ROW_SORT_BINS - 1));
+      return true;
+    });
+  }
+  // The same by bins linear in (key, index) over [lo, hi].
+  __device__ __forceinline__ void order_by_place(RowFinish& f, const uint64_t* from, uint32_t n, uint64_t lo, uint64_t hi) {
+    const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
+    order(f, [&](int i, uint64_t& e, uint32_t& bin) {
+      if (tid + i * ROW_THREADS >= n) return false;
+      e = from[tid + i * ROW_THREADS];
+      bin = (uint32_t)((e - lo) >> shift);
+      return true;
+    });
+  }
+  // Entry number `nth` (from 1) of the n <= ROW_FEW in sh.pool and the mass up
+  // to it, into sh.hi and sh.cut_q; both stay where there is no such entry.
+  __device__ __forceinline__ void nth_of_few(uint32_t n, uint32_t nth) {
+    uint64_t* const q = sh.pool + ROW_FEW;
+    const uint64_t e = tid < n ? sh.pool[tid] : 0;
+    if (tid < n) q[tid] = mass(value_of(e));
+    __syncthreads();
+    uint32_t rank_in = 0;
+    uint64_t upto = 0;
+    for (uint32_t i = 0; i < n; ++i)
+      if (sh.pool[i] <= e) ++rank_in, upto += q[i];
+    if (tid < n && rank_in == nth) sh.hi = e, sh.cut_q = upto;
+    __syncthreads();
+  }
+
+  // Draws among the first n of f.sorted, kept where w >= least_w, of together
+  // `mass`: the entry at which the running mass in index order exceeds t.
+  template <typename H> __device__ __forceinline__ void draw(RowFinish& f, uint32_t n, float least_w, uint64_t t, H hit) {
+    auto mass_of = [&](uint64_t e) {
+      const float w = weight(value_of(e));
+      return w >= least_w ? row_q(w) : 0;
+    };
+    if (n <= 32) {  // one warp sums, for each, those with lower indexes
+      if (wid) return;
+      const uint64_t e = f.sorted[min(lane, (int)n - 1)];
+      const uint64_t q = lane < (int)n ? mass_of(e) : 0;
+      const uint32_t j = (uint32_t)e & (ROW_MAX_COLS - 1);
+      uint64_t before = 0;
+      for (int k = 0; k < (int)n; ++k) {
+        const uint64_t qk = __shfl_sync(~0u, q, k);
+        if (__shfl_sync(~0u, j, k) < j) before += qk;
+      }
+      if (lane < (int)n && before <= t && t < before + q) hit(value_of(e), (int)j);
+      return;
+    }
+    const int shift = max(0, 32 - __clz((int)cols) - 10);
+    constexpr int PER = ROW_POOL / ROW_THREADS;
+    uint64_t e[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) e[i] = tid + i * ROW_THREADS < n ? f.sorted[tid + i * ROW_THREADS] : 0;
+    order(f, [&](int i, uint64_t& c, uint32_t& bin) {
+      if (tid + i * ROW_THREADS >= n) return false;
+      const uint32_t j = (uint32_t)e[i] & (ROW_MAX_COLS - 1);
+      c = (uint64_t)j << 32 | (uint32_t)(e[i] >> ROW_IDX_BITS);
+      bin = j >> shift;
+      return true;
+    });
+    const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    auto mass_at = [&](uint32_t i) {
+      const float w = weight(row_unkey((uint32_t)f.sorted[i]));
+      return w >= least_w ? row_q(w) : 0;
+    };
+    uint64_t own = 0, all;
+    for (uint32_t i = i0; i < i1; ++i) own += mass_at(i);
+    uint64_t run = block_scan(own, sh.scan_q, all);
+    if (t < run || t >= run + own) return;
+    for (uint32_t i = i0; i < i1; ++i) {
+      const uint64_t q = mass_at(i);
+      if (t >= run && t < run + q) hit(row_unkey((uint32_t)f.sorted[i]), (int)(f.sorted[i] >> 32));
+      run += q;
+    }
+  }
+
+  // ---- over the row in memory, by one CTA ----
+  // The entry of vectors [v0, v1) at which the running sum of value(x, index)
+  // exceeds t calls hit(x, index), on one thread.
+  template <typename V, typename H>
+  __device__ __forceinline__ void scan_memory(uint32_t v0, uint32_t v1, uint64_t t, V value, H hit) {
+    for (uint32_t i0 = v0; i0 < v1; i0 += ROW_THREADS) {
+      const uint32_t i = i0 + tid;
+      const uint4 v = i < v1 ? from_memory(i) : nothing();
+      const int j0 = (int)(i * N) - lead;
+      float f[N];
+      E::get(v, f);
+      uint64_t own = 0, all;
+#pragma unroll
+      for (int e = 0; e < N; ++e) own += value(f[e], j0 + e);
+      uint64_t run = block_scan(own, sh.scan_q, all);
+      if (t < all) {
+        if (t >= run && t < run + own) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const uint64_t q = value(f[e], j0 + e);
+            if (t >= run && t < run + q) hit(f[e], j0 + e);
+            run += q;
+          }
+        }
+        return;
+      }
+      t -= all;
+      __syncthreads();
+    }
+  }
+  // The same over the cluster's parts, given the sum of each warp's stretch.
+  template <typename V, typename H>
+  __device__ __forceinline__ void scan_parts(const uint64_t (&of)[ROW_MAX_CLUSTER][ROW_WARPS], uint64_t t, V value, H hit) {
+    // each warp finds the stretch for itself: lanes hold up to four sums each, in order
+    constexpr int PER = ROW_MAX_CLUSTER * ROW_WARPS / 32;
+    const uint32_t count = ctas * ROW_WARPS;
+    uint64_t s[PER], own = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const uint32_t i = lane * PER + k;
+      s[k] = i < count ? (&of[0][0])[i] : 0;
+      own += s[k];
+    }
+    uint64_t run = warp_scan(own, lane) - own;
+    uint32_t which = 0;
+    uint64_t left = t;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if (t >= run && t < run + s[k]) which = lane * PER + k + 1, left = t - run;
+      run += s[k];
+    }
+    const uint32_t has = __ballot_sync(~0u, which != 0);
+    if (!has) return;
+    const int owner = __ffs((int)has) - 1;
+    which = __shfl_sync(~0u, which, owner) - 1;
+    left = __shfl_sync(~0u, left, owner);
+    uint32_t v0, v1;
+    stretch(which / ROW_WARPS, which % ROW_WARPS, v0, v1);
+    scan_memory(v0, v1, left, value, hit);
   }
 };
 
+__device__ __forceinline__ uint64_t row_target(float p, uint64_t mass) {  // ceil(p mass), at least 1
+  const double least = ceil((double)fmaxf(p, 0.0f) * (double)mass);
+  return least < 1.0 ? 1ull : (uint64_t)least;
+}
+__device__ __forceinline__ uint64_t row_draw(float u, uint64_t mass) {  // floor(u mass), below mass
+  const double at = floor((double)(u > 0.0f ? u : 0.0f) * (double)mass);
+  return at < (double)mass ? min((uint64_t)at, mass - 1) : mass - 1;
+}
+
 // ---- sampling ---------------------------------------------------------------------
-template <typename T> __global__ void __launch_bounds__(ROW_THREADS) k_row_sample(const RowArgs a) {
+// Every CTA of the cluster: the load with the maximum (HBM), then a pass over
+// shared memory that sums the weights.  Where a cut is asked for, the CTAs
+// collect its candidates -- the entries above a value that at least top_k of
+// them are known to reach, or, for a nucleus, above a guess -- and the first CTA
+// orders them, cuts, and draws among them.  Without a cut it draws from the
+// warps' sums and reads the stretch that holds the drawn entry again.
+//
+// A cut that does not end among the candidates (a nucleus beyond the guess,
+// a large top_k, many equal values) keeps the cluster to narrow it down.
+template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sample(const RowArgs a) {
   extern __shared__ __align__(16) unsigned char row_smem[];
   RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
-  Row<T> r(sh, reinterpret_cast<uint4*>(row_smem + (sizeof(RowShared) + 15) / 16 * 16));
-  const uint32_t row = blockIdx.x / r.ctas;
-  r.load(a, row);
-
+  uint4* const data = reinterpret_cast<uint4*>(row_smem + ROW_SHARED_BYTES);
+  RowFinish& f = *reinterpret_cast<RowFinish*>(data);
+  const uint32_t row = blockIdx.x / cg::this_cluster().num_blocks();
+  Row<T> r(sh, data, a, row);
+  const float t = a.temperature ? a.temperature[row] : 1.0f;
+  const int k_arg = a.top_k ? a.top_k[row] : 0;
+  const float p = a.top_p ? a.top_p[row] : 1.0f;
+  const float least_w = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
+  const float u = a.uniform[row];
+  const bool greedy = !(t > 0.0f);
+  const bool by_k = !greedy && k_arg > 0 && (uint32_t)k_arg < a.cols, by_p = !greedy && p < 1.0f;
+  const bool by_w = !greedy && least_w > 0.0f;
+  const uint32_t k = (uint32_t)k_arg;
+  r.load(by_k || by_p);
   if (r.m == -INFINITY) {
     if (r.rank == 0 && r.tid == 0) {
       a.tokens[row] = -1;
@@ -480,113 +955,233 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS) k_row_sampl
     }
     return;
   }
-  const float t = a.temperature ? a.temperature[row] : 1.0f;
-  const bool greedy = !(t > 0.0f);
   // within the finite numbers above 0: 0 * c and (max + inf) * c stay what they are for the smallest and infinite t
-  r.c = greedy ? ROW_LOG2E : fminf(fmaxf(__fdiv_rn(ROW_LOG2E, t), 1.175494351e-38f), 3.402823466e+38f);
-  uint64_t mine = 0;
-  r.each([&](float x, int) { mine += r.mass(x); });
-  const uint64_t total = r.sum(mine);
+  r.c = greedy ? ROW_LOG2E : fminf(fmaxf(__fdiv_rn(ROW_LOG2E, t), 1.175494351e-38f), ROW_F32_MAX);
 
-  auto store = [&](float x, int j) {
+  uint64_t total = 0;
+  auto store = [&](float z, int j) {
     a.tokens[row] = j;
-    if (a.logprobs) a.logprobs[row] = -(row_y(x, r.m, r.c) * ROW_LN2) - logf((float)total * 0x1p-40f);
+    if (a.logprobs) a.logprobs[row] = row_neg_y(z, r.m, r.c) * ROW_LN2 - logf((float)total * 0x1p-40f);
   };
-  if (greedy) {
-    auto top = [&](float x, int) -> uint64_t { return x == r.m; };
-    mine = 0;
-    r.cluster.sync();
-    r.each([&](float x, int j) { mine += top(x, j); });
-    r.sum(mine);
-    r.locate(0, top, store);
+  if (greedy && r.mine == r.m)
+    r.between(r.m, r.m, [&](float, int j) { atomicMin(r.cluster.map_shared_rank(&sh.first, 0), (uint32_t)j); });
+  const uint64_t own = r.template weigh<false>(0.0f);
+  if (!by_k && !by_p && !by_w) {
+    r.template hand<false>(own, 0);
+    if (!r.last_part()) return;
+    total = r.handed(sh.mass);
+    if (!greedy)
+      r.scan_parts(sh.mass, row_draw(u, total), [&](float z, int) { return r.mass(z); }, store);
+    else if (r.tid == 0)
+      store(r.m, (int)sh.first);
     return;
   }
-  RowCut cut{~0u, ~0u, total};
-  const int k = a.top_k ? a.top_k[row] : 0;
-  if (k > 0 && (uint32_t)k < a.cols) {
-    cut = r.template select<false>((uint64_t)k);
-    if (cut.mass == ~0ull) cut.mass = total;
-  }
-  const float p = a.top_p ? a.top_p[row] : 1.0f;
-  if (p < 1.0f) {
-    const double least = ceil((double)fmaxf(p, 0.0f) * (double)cut.mass);
-    cut = r.template select<true>(least < 1.0 ? 1ull : (uint64_t)least);
-  }
-  const float least_w = fminf(a.min_p ? a.min_p[row] : 0.0f, 1.0f);
-  auto kept = [&](float x, int j) -> uint64_t {
-    const float w = r.weight(x);
-    const uint32_t key = row_key(x);
-    if (w < least_w || key > cut.key || (key == cut.key && (uint32_t)j > cut.idx)) return 0;
-    return row_q(w);
-  };
-  mine = 0;
-  r.cluster.sync();
-  r.each([&](float x, int j) { mine += kept(x, j); });
-  const uint64_t mass = r.sum(mine);
-  const float u = a.uniform[row];
-  const double at = floor((double)(u > 0.0f ? u : 0.0f) * (double)mass);
-  const uint64_t draw = at < (double)mass ? min((uint64_t)at, mass - 1) : mass - 1;
-  r.locate(draw, kept, store);
-}
 
-// Ascending sort of n (a power of two) 64-bit numbers in shared memory.
-__device__ __forceinline__ void row_bitonic(uint64_t* v, int n) {
-  for (int k = 2; k <= n; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += ROW_THREADS) {
-        const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const uint64_t x = v[a], y = v[b];
-        if ((x > y) == ((a & k) == 0)) v[a] = y, v[b] = x;
+  // ---- candidates ----
+  float edge;
+  if (by_k || by_p) {
+    const uint32_t want = by_k ? k : ROW_NUCLEUS_GUESS;
+    edge = want <= r.top_count() * r.ctas * ROW_WARPS * 3 / 4 ? r.edge_of(want, ROW_EDGE_SCALE * r.c, r.mass_end()) : INFINITY;
+  } else {
+    edge = fmaxf(r.m + (log2f(least_w) - 0x1p-10f) / r.c - fabsf(r.m) * 0x1p-21f, r.mass_end());
+  }
+  uint64_t part = 0;
+  if (edge < INFINITY) {
+    r.collect((uint64_t)row_key(r.m) << ROW_IDX_BITS, (uint64_t)row_key(edge) << ROW_IDX_BITS | (ROW_MAX_COLS - 1), sh.list,
+              ROW_LIST);
+    if (by_p && !by_k)
+      for (uint32_t i = r.tid; i < min(sh.count, (uint32_t)ROW_LIST); i += ROW_THREADS) part += r.mass(r.value_of(sh.list[i]));
+  }
+  r.template hand<true>(own, part);
+  r.cluster.sync();
+  total = r.handed(sh.mass);
+  uint32_t n = 0;
+  bool enough = false;
+  if (edge < INFINITY) {
+    n = r.pooled(sh.list, ROW_LIST);
+    enough = n <= (uint32_t)ROW_LIST && (by_k || !by_p || r.handed(sh.part) >= row_target(p, total));
+  }
+  if (enough) {
+    if (!r.last_part()) return;
+    r.order_by_value(f, sh.list, n, edge);
+    // running masses in descending order, `per` entries a thread
+    const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(r.tid * per, n), i1 = min(i0 + per, n);
+    uint64_t sum = 0, all;
+    for (uint32_t i = i0; i < i1; ++i) sum += r.mass(r.value_of(f.sorted[i]));
+    const uint64_t before = r.block_scan(sum, sh.scan_q, all);
+    if (r.tid == 0) sh.cut_n = n, sh.cut_q = by_k ? all : total;
+    __syncthreads();
+    uint64_t run = before;
+    if (by_k && n > k) {
+      for (uint32_t i = i0; i < i1; ++i) {
+        run += r.mass(r.value_of(f.sorted[i]));
+        if (i == k - 1) sh.cut_n = k, sh.cut_q = run;
       }
+      __syncthreads();
     }
+    uint32_t cut = sh.cut_n;
+    if (by_p) {
+      const uint64_t target = row_target(p, sh.cut_q);
+      __syncthreads();
+      run = before;
+      for (uint32_t i = i0; i < i1 && i < cut; ++i) {
+        const uint64_t q = r.mass(r.value_of(f.sorted[i]));
+        if (run < target && target <= run + q) sh.cut_n = i + 1, sh.cut_q = run + q;
+        run += q;
+      }
+      __syncthreads();
+      cut = sh.cut_n;
+    }
+    uint64_t mass = sh.cut_q;
+    if (by_w) {
+      sum = 0;
+      for (uint32_t i = r.tid; i < cut; i += ROW_THREADS) {
+        const float w = r.weight(r.value_of(f.sorted[i]));
+        if (w >= least_w) sum += row_q(w);
+      }
+      __syncthreads();
+      r.block_scan(sum, sh.scan_q, mass);
+    }
+    r.draw(f, cut, least_w, row_draw(u, mass), store);
+    return;
+  }
+
+  // ---- a cut beyond the candidates ----
+  uint64_t last = ~0ull;  // the last entry of the cut
+  if (by_k || by_p) {
+    uint32_t above_n;
+    uint64_t target = k;
+    if (by_k) r.narrow(false, k, least_w, by_p ? ROW_FEW : ROW_POOL, n, above_n);
+    if (by_p) {
+      uint64_t mass = total;
+      if (by_k) {
+        if (!r.rank) {  // the mass of the top k
+          const uint64_t above = r.handed(sh.mass);
+          r.cluster.barrier_arrive();  // the others' entries
+          r.cluster.barrier_wait();
+          if (r.tid == 0) sh.cut_q = total - above;
+          __syncthreads();
+          r.nth_of_few(n, k - above_n);
+          if (r.tid < (int)r.ctas) *r.cluster.map_shared_rank(&sh.cut_q, r.tid) = above + sh.cut_q;
+        } else {
+          r.cluster.sync();
+        }
+        r.cluster.sync();
+        mass = sh.cut_q;
+      }
+      target = row_target(p, mass);
+      r.narrow(true, target, least_w, ROW_POOL, n, above_n);
+    }
+    if (!r.last_part()) return;
+    const uint64_t lo = sh.lo, hi = sh.hi, above = r.handed(sh.mass);
+    r.order_by_place(f, sh.pool, n, lo, hi);
+    uint32_t cut = n;
+    if (by_p) {
+      const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(r.tid * per, n), i1 = min(i0 + per, n);
+      uint64_t sum = 0, all;
+      for (uint32_t i = i0; i < i1; ++i) sum += r.mass(r.value_of(f.sorted[i]));
+      uint64_t run = above + r.block_scan(sum, sh.scan_q, all);
+      if (r.tid == 0) sh.cut_n = n;
+      __syncthreads();
+      for (uint32_t i = i0; i < i1; ++i) {
+        const uint64_t q = r.mass(r.value_of(f.sorted[i]));
+        if (run < target && target <= run + q) sh.cut_n = i + 1;
+        run += q;
+      }
+      __syncthreads();
+      cut = sh.cut_n;
+    } else {
+      cut = min(n, k - above_n);
+    }
+    last = cut ? f.sorted[cut - 1] : hi;
+    // the warps' kept masses: before the interval, and those of its entries
+    for (uint32_t i = r.tid; i < cut; i += ROW_THREADS) {
+      const uint64_t e = f.sorted[i];
+      const float w = r.weight(r.value_of(e));
+      const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + r.lead) / Row<T>::N;
+      const uint32_t cta = v / r.part_vecs, p0 = cta * r.part_vecs, p1 = min(p0 + r.part_vecs, r.total_vecs);
+      const uint32_t warp = (v - p0) / ((p1 - p0 + ROW_WARPS - 1) / ROW_WARPS);
+      if (w >= least_w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.part[cta][warp]), (unsigned long long)row_q(w));
+    }
+  } else {  // min_p alone
+    uint64_t kept = 0;
+    r.each([&](float z, int) {
+      const float w = r.weight(z);
+      if (w >= least_w) kept += row_q(w);
+    });
+    r.cluster.sync();  // every CTA has read the sums before the next ones
+    r.template hand<false>(own, kept);
+    if (!r.last_part()) return;
+  }
   __syncthreads();
+  r.scan_parts(sh.part, row_draw(u, r.handed(sh.part)),
+               [&](float z, int j) -> uint64_t {
+                 const float w = r.weight(z);
+                 return w >= least_w && ((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) <= last ? row_q(w) : 0;
+               },
+               store);
 }
 
 // ---- the n best ---------------------------------------------------------------------
-template <typename T> __global__ void __launch_bounds__(ROW_THREADS) k_row_best(const RowArgs a) {
+// As a sampling row with top_k = n, whose ordered candidates are the answer.
+template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_best(const RowArgs a) {
   extern __shared__ __align__(16) unsigned char row_smem[];
   RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
-  Row<T> r(sh, reinterpret_cast<uint4*>(row_smem + (sizeof(RowShared) + 15) / 16 * 16));
-  const uint32_t row = blockIdx.x / r.ctas;
-  if (r.tid == 0) sh.count = 0;
-  r.load(a, row);
+  uint4* const data = reinterpret_cast<uint4*>(row_smem + ROW_SHARED_BYTES);
+  RowFinish& f = *reinterpret_cast<RowFinish*>(data);
+  const uint32_t row = blockIdx.x / cg::this_cluster().num_blocks();
+  Row<T> r(sh, data, a, row);
+  r.load(true);
+  int* const out_idx = a.best_idx + (int64_t)row * a.n;
+  float* const out_lp = a.best_logprob + (int64_t)row * a.n;
   if (r.m == -INFINITY) {
     if (r.rank == 0) {
-      for (int i = r.tid; i < a.n; i += ROW_THREADS) {
-        a.best_idx[(int64_t)row * a.n + i] = -1;
-        a.best_logprob[(int64_t)row * a.n + i] = -INFINITY;
-      }
+      for (int i = r.tid; i < a.n; i += ROW_THREADS) out_idx[i] = -1, out_lp[i] = -INFINITY;
       if (a.lse && r.tid == 0) a.lse[row] = -INFINITY;
     }
     return;
   }
   r.c = ROW_LOG2E;
-  uint64_t mine = 0;
-  r.each([&](float x, int) { mine += r.mass(x); });
-  const float ln = logf((float)r.sum(mine) * 0x1p-40f);
-  if (a.lse && r.rank == 0 && r.tid == 0) a.lse[row] = r.m + ln;
-  const RowCut cut = r.template select<false>((uint64_t)a.n);
+  const uint32_t k = (uint32_t)a.n;
+  const uint64_t first = (uint64_t)row_key(r.m) << ROW_IDX_BITS;
+  float edge = INFINITY;
+  if (k <= r.top_count() * r.ctas * ROW_WARPS * 3 / 4) {
+    edge = r.edge_of(k, ROW_EDGE_SCALE * ROW_LOG2E, -ROW_F32_MAX);
+    if (edge == -ROW_F32_MAX) edge = r.edge_of(k, r.far_scale(), -ROW_F32_MAX);
+    r.collect(first, (uint64_t)row_key(edge) << ROW_IDX_BITS | (ROW_MAX_COLS - 1), sh.list, ROW_LIST);
+  }
+  r.template hand<true>(r.template weigh<false>(0.0f), 0);
   r.cluster.sync();
-  uint32_t* count = r.cluster.map_shared_rank(&sh.count, 0);
-  uint64_t* list = r.cluster.map_shared_rank(sh.q, 0);
-  r.each([&](float x, int j) {
-    const uint32_t key = row_key(x);
-    if (x == -INFINITY || key > cut.key || (key == cut.key && (uint32_t)j > cut.idx)) return;
-    list[atomicAdd(count, 1u)] = (uint64_t)key << 32 | (uint32_t)j;
-  });
-  r.cluster.sync();
-  if (r.rank) return;
-  int n2 = 1;
-  while (n2 < a.n) n2 <<= 1;
-  const int have = (int)sh.count;
-  for (int i = have + r.tid; i < n2; i += ROW_THREADS) sh.q[i] = ~0ull;
-  row_bitonic(sh.q, n2);
+  const float ln = logf((float)r.handed(sh.mass) * 0x1p-40f);
+  uint32_t n = ~0u;
+  uint64_t* from = sh.list;
+  if (edge < INFINITY) n = r.pooled(sh.list, ROW_LIST);
+  if (n > (uint32_t)ROW_LIST) {
+    // the n-th entry, then the entries up to it
+    uint32_t above_n;
+    r.narrow(false, k, 0.0f, ROW_FEW, n, above_n);
+    r.cluster.sync();
+    if (r.rank == 0) {
+      r.nth_of_few(n, k - above_n);
+      if (r.tid > 0 && r.tid < (int)r.ctas) *r.cluster.map_shared_rank(&sh.hi, r.tid) = sh.hi;
+    }
+    if (r.tid == 0) sh.count = 0;
+    r.cluster.sync();
+    r.collect(first, sh.hi, sh.pool, ROW_POOL);
+    edge = r.value_of(sh.hi);
+    r.cluster.sync();
+    n = r.pooled(sh.pool, ROW_POOL);
+    from = sh.pool;
+  }
+  if (!r.last_part()) return;
+  if (a.lse && r.tid == 0) a.lse[row] = r.m + ln;
+  r.order_by_value(f, from, n, edge);
+  const uint32_t have = min(n, k);
   for (int i = r.tid; i < a.n; i += ROW_THREADS) {
-    const uint64_t e = sh.q[i];
-    const bool in = i < have;
-    a.best_idx[(int64_t)row * a.n + i] = in ? (int)(uint32_t)e : -1;
-    a.best_logprob[(int64_t)row * a.n + i] = in ? (row_unkey((uint32_t)(e >> 32)) - r.m) - ln : -INFINITY;
+    const bool in = i < (int)have;
+    const uint64_t e = in ? f.sorted[i] : 0;
+    out_idx[i] = in ? (int)(e & (ROW_MAX_COLS - 1)) : -1;
+    out_lp[i] = in ? (r.value_of(e) - r.m) - ln : -INFINITY;
   }
 }
 
