@@ -97,6 +97,7 @@ template <> struct RowElem<float> {
   static __device__ __forceinline__ uint32_t clean(uint32_t v) {
     return __float_as_uint(fminf(fmaxf(__uint_as_float(v), -INFINITY), ROW_F32_MAX));
   }
+  static __device__ __forceinline__ float one(const uint4* v, uint32_t i) { return reinterpret_cast<const float*>(v)[i]; }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
@@ -121,6 +122,9 @@ template <> struct RowElem<__nv_bfloat16> {
     asm("max.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(NEG_INF));
     asm("min.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7f7f7f7fu));
     return v;
+  }
+  static __device__ __forceinline__ float one(const uint4* v, uint32_t i) {
+    return __uint_as_float((uint32_t) reinterpret_cast<const unsigned short*>(v)[i] << 16);
   }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -152,6 +156,9 @@ template <> struct RowElem<__half> {
     asm("max.f16x2 %0, %0, %1;" : "+r"(v) : "r"(NEG_INF));
     asm("min.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7bff7bffu));
     return v;
+  }
+  static __device__ __forceinline__ float one(const uint4* v, uint32_t i) {
+    return __half2float(__ushort_as_half(reinterpret_cast<const unsigned short*>(v)[i]));
   }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -261,7 +268,7 @@ struct RowShared {
   uint32_t scan_n[ROW_WARPS];
   uint32_t n[ROW_MAX_CLUSTER];
   uint64_t lo, hi, cut_q;
-  uint32_t cut_n, count, above, first, b1, b2;
+  uint32_t cut_n, count, above, first, b1, b2, last;
 };
 constexpr size_t ROW_SHARED_BYTES = (sizeof(RowShared) + 15) / 16 * 16;
 static_assert(3 * (ROW_SHARED_BYTES + (64 << 10) + 1024) <= 228 << 10, "three CTAs on an SM");
@@ -469,18 +476,42 @@ template <typename T> struct Row {
     return row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
   }
 
-  // Calls f(x, index) for this thread's entries in [low, high].
-  template <typename F> __device__ __forceinline__ void between(float low, float high, F f) const {
-    if (mine < low) return;
-    for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
-      const uint4 v = data[i];
-      if (E::value(E::top(E::top0(), v)) < low) continue;
-      float z[N];
-      E::get(v, z);
-      const int j0 = first + (int)(i * N);
+  // Bits of the entries of a vector in [low, high].
+  static __device__ __forceinline__ uint32_t hits(const uint4& v, float low, float high) {
+    float z[N];
+    E::get(v, z);
+    uint32_t mask = 0;
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (z[e] >= low && z[e] <= high) f(z[e], j0 + e);
+    for (int e = 0; e < N; ++e) mask |= (uint32_t)(z[e] >= low && z[e] <= high) << e;
+    return mask;
+  }
+  // f(x, index) for the entries of vector i of this CTA's part that mask names
+  template <typename F> __device__ __forceinline__ void each_of(uint32_t mask, uint32_t i, F f) const {
+    while (mask) {
+      const int e = __ffs((int)mask) - 1;
+      mask &= mask - 1;
+      f(E::one(data, i * N + e), first + (int)(i * N) + e);
+    }
+  }
+  // Calls f(x, index) for the warp's entries in [low, high], many of them.
+  template <typename F> __device__ __forceinline__ void between(float low, float high, F f) const {
+    constexpr int U = 4;
+    for (uint32_t i = seg0 + lane; i < seg1; i += 32 * U) {
+      uint32_t mask[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) mask[u] = i + 32 * u < seg1 ? hits(data[i + 32 * u], low, high) : 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) each_of(mask[u], i + 32 * u, f);
+    }
+  }
+  // The same, where few of the warp's threads have any above low: the warp
+  // looks through the vectors of one such thread at a time.
+  template <typename F> __device__ __forceinline__ void above(float low, F f) const {
+    uint32_t threads = __ballot_sync(~0u, mine >= low);
+    while (threads) {
+      const uint32_t owner = __ffs((int)threads) - 1;
+      threads &= threads - 1;
+      for (uint32_t i = seg0 + owner + 32 * lane; i < seg1; i += 32 * 32) each_of(hits(data[i], low, INFINITY), i, f);
     }
   }
 
@@ -553,8 +584,17 @@ template <typename T> struct Row {
     for (uint32_t i = lane; i < ctas * ROW_WARPS; i += 32) t += (&of[0][0])[i];
     return warp_sum_u64(t);
   }
-  // Collects this CTA's entries in [lo, hi] of (key, index) order at `to`, of
-  // room for `room`; sh.count is their number (sh.count = 0 before).
+  // Collects this CTA's entries from the maximum to `edge`, or in [lo, hi] of
+  // (key, index) order, at `to`, of room for `room`; sh.count is their number
+  // (sh.count = 0 before).
+  __device__ __forceinline__ void collect_above(float edge, uint64_t* to, uint32_t room) {
+    above(edge, [&](float z, int j) {
+      const uint32_t at = atomicAdd(&sh.count, 1u);
+      if (at < room) to[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+    });
+    __syncthreads();
+    if (tid < (int)ctas) *cluster.map_shared_rank(&sh.n[rank], tid) = sh.count;
+  }
   __device__ __forceinline__ void collect(uint64_t lo, uint64_t hi, uint64_t* to, uint32_t room) {
     between(value_of(hi), value_of(lo), [&](float z, int j) {
       const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
@@ -589,13 +629,19 @@ template <typename T> struct Row {
   }
 
   // ---- narrowing a cut down, by the whole cluster ----
+  // Bins of 1/42 octave: y c 42 to the nearest whole number, by an addition
+  // that pushes the fraction out of the mantissa.
+  __device__ __forceinline__ float place_of(float v, float c42) const { return __fmul_rn(__fsub_rn(m, v), c42); }
+  static __device__ __forceinline__ uint32_t bin_at(float place) {
+    return __float_as_uint(__fadd_rn(fminf(place, (float)(ROW_BINS - 1)), 0x1p23f)) & 0x7fffffu;
+  }
   // The smallest key from the maximum's on whose bin is b or later; one warp,
   // 32 probes at a time.
-  __device__ __forceinline__ uint32_t first_key(uint32_t b) const {
+  __device__ __forceinline__ uint32_t first_key(uint32_t b, float c42) const {
     uint32_t lo = row_key(m), hi = row_key(-ROW_F32_MAX) + 1;
     while (lo < hi) {
       const uint32_t step = max(1u, (hi - lo) / 32), at = lo + lane * step;
-      const bool past = at - lo >= hi - lo || bin_of(row_unkey(at), ROW_BIN_SCALE, ROW_BINS) >= b;
+      const bool past = at - lo >= hi - lo || bin_at(place_of(row_unkey(at), c42)) >= b;
       const uint32_t has = __ballot_sync(~0u, past);
       if (has & 1) break;
       const int f = has ? __ffs((int)has) - 1 : 32;
@@ -611,12 +657,16 @@ template <typename T> struct Row {
   //   those entries in the first CTA's sh.pool, their number in n,
   //   every warp's mass before the interval in sh.mass, and of that the mass
   //   of entries with w >= least_w in sh.part, on all CTAs,
-  //   the number of entries before it in above_n.
-  // Each round counts the undecided entries by bin -- in the first round 1/42
-  // octave of weight, then a 2^-10th of the interval -- or sums their weights,
-  // each to 13 bits of its bin's, which tells the bin, or next to its bounds
-  // the two or three, that the prefix ends in; a second pass takes what comes
-  // before by its exact mass.  Ends: (key, index) has no ties.
+  //   the number of entries before it in above_n (counts alone).
+  // Each round counts the undecided entries by bin, or sums their weights, each
+  // to 13 bits of its bin's, which tells the bin, or next to its bounds the two
+  // or three, that the prefix ends in; a second pass takes what comes before by
+  // its exact mass, so that the estimates of the next round err by a part of
+  // the rest alone.  Bins are of 1/42 octave of weight, and of a 2^-10th of the
+  // interval once it is shorter than three of those (for counts: after the
+  // first round).  (key, index) has no ties: an interval can always be cut.
+  // `rounds` bounds them all the same; it takes two or three, and far in the
+  // tail, where the rest shrinks by 2^-12 a round, up to eight.
   // A weight as q holds it.
   static __device__ __forceinline__ float held(float w) {
     return w < 0x1p-17f ? __fsub_rn(__fadd_rn(w, ROW_MAGIC), ROW_MAGIC) : w;
@@ -626,70 +676,93 @@ template <typename T> struct Row {
     uint64_t lo = (uint64_t)row_key(m) << ROW_IDX_BITS, hi = (uint64_t)row_key(-ROW_F32_MAX) << ROW_IDX_BITS | (ROW_MAX_COLS - 1);
     uint64_t above_q = 0;
     above_n = 0;
-    for (int round = 0;; ++round) {
-      cluster.sync();  // what the round before left has been read
+    constexpr int ROUNDS = 16;
+    for (int round = 0; round < ROUNDS; ++round) {
+      cluster.sync();  // what was there has been read
       for (int b = tid; b < ROW_BINS; b += ROW_THREADS) sh.bins[b] = 0;
-      if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ROW_BINS - 1;
+      if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ~0u, sh.last = 0;
       __syncthreads();
-      cluster.barrier_arrive();  // the first CTA's bins are empty
       const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
-      const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w;
+      const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w, c42 = fminf(c * ROW_BIN_SCALE, ROW_F32_MAX);
+      const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), c42)) >= bin_at(place_of(value_of(lo), c42)) + 3);
       if (round == 0) {
         each([&](float z, int) {
-          const float y = __fmul_rn(-row_neg_y(z, m, c), ROW_BIN_SCALE);
+          const float y = place_of(z, c42);
           if (by_mass) {
             if (y < ROW_MASS_END * ROW_BIN_SCALE) {
-              const float b = truncf(y);
-              atomicAdd(&sh.bins[(int)b], (uint32_t)(held(weight(z)) * row_exp2(b * (1.0f / ROW_BIN_SCALE) + 12.0f) + 0.5f));
+              const float b = __fadd_rn(y, 0x1p23f);  // 2^-(y - b) / 42 by its tangent, as a whole number by another such addition
+              const float v = __fmaf_rn(__fsub_rn(y, __fsub_rn(b, 0x1p23f)), -4096.0f * ROW_LN2 / ROW_BIN_SCALE, 0x1p23f + 4096.0f);
+              atomicAdd(&sh.bins[__float_as_uint(b) & 0x7fffffu], __float_as_uint(v) & 0x7fffffu);
             }
           } else if (z > -INFINITY) {
-            atomicAdd(&sh.bins[(int)fminf(y, (float)(ROW_BINS - 1))], 1u);
+            atomicAdd(&sh.bins[bin_at(y)], 1u);
           }
         });
       } else {
         between(value_of(hi), value_of(lo), [&](float z, int j) {
           const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
           if (e < lo || e > hi) return;
-          atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], by_mass ? (uint32_t)(held(weight(z)) * scale + 0.5f) : 1u);
+          if (!by_mass) {
+            atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], 1u);
+          } else if (by_weight) {
+            const uint32_t b = bin_at(place_of(z, c42));
+            atomicAdd(&sh.bins[b], (uint32_t)(held(weight(z)) * row_exp2((float)b * (1.0f / ROW_BIN_SCALE) + 12.0f) + 0.5f));
+          } else {
+            atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], (uint32_t)(held(weight(z)) * scale + 0.5f));
+          }
         });
       }
-      __syncthreads();
-      cluster.barrier_wait();
-      if (rank)
-        for (int b = tid; b < ROW_BINS; b += ROW_THREADS)
-          if (const uint32_t v = sh.bins[b]) atomicAdd(cluster.map_shared_rank(&sh.bins[b], 0), v);
       cluster.sync();
       if (rank == 0) {
-        // the prefix ends in b1 or later, and in b2 or before: where a sum of estimates, 2^-12 of it added, and taken
-        // off, reaches the target (half a unit of at least 2730 is less than that; counts are exact)
+        // the prefix ends in b1 or later, and in b2 or before: where a sum of estimates, 2^-12 of it and 2^-20 of the
+        // largest weight added, and taken off, reaches the target.  (An estimate is off by half a unit of 4060 and less
+        // than 2^-14; the weights' rounding to q by at most 2^-22 together, and the target is no less than the largest
+        // weight; from the second round on they follow q.  Counts are exact.)  Else it ends in the last bin with
+        // anything; a count that is not reached, beyond all of them.
         constexpr int PER = ROW_BINS / ROW_THREADS;
         float s[PER], own = 0, all;
+        uint32_t filled = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {  // bins tid * PER + i, read side by side and handed over in shared memory
+          uint32_t n = sh.bins[i * ROW_THREADS + tid];
+          for (uint32_t k = 1; k < ctas; ++k) n += cluster.map_shared_rank(sh.bins, k)[i * ROW_THREADS + tid];
+          s[i] = (float)n;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; ++i) reinterpret_cast<float*>(sh.bins)[i * ROW_THREADS + tid] = s[i];
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int b = tid * PER + i;
-          s[i] = (float)sh.bins[b];
-          if (by_mass) s[i] *= round == 0 ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w;
+          s[i] = reinterpret_cast<float*>(sh.bins)[b];
+          if (s[i] > 0.0f) filled = b;
+          if (by_mass) s[i] *= by_weight ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w;
           own += s[i];
         }
+        filled = __reduce_max_sync(~0u, filled);
+        if (lane == 0) atomicMax(&sh.last, filled);
         float run = block_scan(own, reinterpret_cast<float*>(sh.scan_n), all);
         const float goal = by_mass ? (float)(target - above_q) * 0x1p-28f : (float)(target - above_n);
-        const float slack = by_mass ? 0x1p-12f : 0.0f;
+        const float slack = by_mass ? 0x1p-12f : 0.0f, more = by_mass && round == 0 ? 0x1p-8f : 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const bool last = tid * PER + i == ROW_BINS - 1;
           if (run < goal && (run + s[i] >= goal || last)) sh.above = above_n + (uint32_t)run;  // read for counts alone
           run += s[i];
-          if (run * (1.0f + slack) >= goal) atomicMin(&sh.b1, (uint32_t)(tid * PER + i));
-          if (run * (1.0f - slack) >= goal) atomicMin(&sh.b2, (uint32_t)(tid * PER + i));
+          if (run * (1.0f + slack) + more >= goal) atomicMin(&sh.b1, (uint32_t)(tid * PER + i));
+          if (run * (1.0f - slack) - more >= goal) atomicMin(&sh.b2, (uint32_t)(tid * PER + i));
         }
         __syncthreads();
         if (wid < 2) {  // the interval's ends
-          const uint32_t b = wid ? sh.b2 + 1 : sh.b1;
+          const uint32_t end = by_mass ? sh.last : (uint32_t)ROW_BINS - 1;
+          const uint32_t b = wid ? min(sh.b2, end) + 1 : min(sh.b1, end);
           uint64_t at;
-          if (round == 0)
-            at = b < (uint32_t)ROW_BINS ? (uint64_t)first_key(b) << ROW_IDX_BITS : hi + 1;
+          if (by_weight)
+            at = b < (uint32_t)ROW_BINS ? max(lo, (uint64_t)first_key(b, c42) << ROW_IDX_BITS) : hi + 1;
           else
-            at = min(lo + ((uint64_t)b << shift), hi + 1);
+            at = lo + ((uint64_t)b << shift);
+          at = min(at, hi + 1);
           if (lane < (int)ctas) {
             *cluster.map_shared_rank(wid ? &sh.hi : &sh.lo, lane) = wid ? at - 1 : at;
             if (wid && lane) *cluster.map_shared_rank(&sh.above, lane) = sh.above;
@@ -720,6 +793,7 @@ template <typename T> struct Row {
       n = pooled(sh.pool, most);
       if (n <= most) return;
     }
+    n = 0;  // never: what the last round left undecided is cut off
   }
 
   // ---- ordering the candidates, on the first CTA alone ----
@@ -963,8 +1037,8 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sa
     a.tokens[row] = j;
     if (a.logprobs) a.logprobs[row] = row_neg_y(z, r.m, r.c) * ROW_LN2 - logf((float)total * 0x1p-40f);
   };
-  if (greedy && r.mine == r.m)
-    r.between(r.m, r.m, [&](float, int j) { atomicMin(r.cluster.map_shared_rank(&sh.first, 0), (uint32_t)j); });
+  if (greedy)
+    r.above(r.m, [&](float, int j) { atomicMin(r.cluster.map_shared_rank(&sh.first, 0), (uint32_t)j); });
   const uint64_t own = r.template weigh<false>(0.0f);
   if (!by_k && !by_p && !by_w) {
     r.template hand<false>(own, 0);
@@ -987,8 +1061,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sa
   }
   uint64_t part = 0;
   if (edge < INFINITY) {
-    r.collect((uint64_t)row_key(r.m) << ROW_IDX_BITS, (uint64_t)row_key(edge) << ROW_IDX_BITS | (ROW_MAX_COLS - 1), sh.list,
-              ROW_LIST);
+    r.collect_above(edge, sh.list, ROW_LIST);
     if (by_p && !by_k)
       for (uint32_t i = r.tid; i < min(sh.count, (uint32_t)ROW_LIST); i += ROW_THREADS) part += r.mass(r.value_of(sh.list[i]));
   }
@@ -1148,7 +1221,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_be
   if (k <= r.top_count() * r.ctas * ROW_WARPS * 3 / 4) {
     edge = r.edge_of(k, ROW_EDGE_SCALE * ROW_LOG2E, -ROW_F32_MAX);
     if (edge == -ROW_F32_MAX) edge = r.edge_of(k, r.far_scale(), -ROW_F32_MAX);
-    r.collect(first, (uint64_t)row_key(edge) << ROW_IDX_BITS | (ROW_MAX_COLS - 1), sh.list, ROW_LIST);
+    r.collect_above(edge, sh.list, ROW_LIST);
   }
   r.template hand<true>(r.template weigh<false>(0.0f), 0);
   r.cluster.sync();
