@@ -21,18 +21,20 @@ constexpr uint32_t ROW_PART_MAX = 132u << 10;
 
 size_t elem_bytes(int dtype) { return dtype == FS_LOGITS_F32 ? 4 : 2; }
 
-// CTAs per row.  A row is cut until three CTAs of its parts fit an SM, and
-// further while the batch has fewer CTAs than the GPU has SMs and a part
-// keeps PART_MIN bytes.
-constexpr uint32_t PART = 64u << 10;
+// CTAs per row: as many as cut it into parts of PART bytes, of which three fit
+// an SM, and more while the batch has fewer CTAs than the GPU has SMs and a
+// part keeps PART_MIN bytes.
+#ifndef VPART
+#define VPART 64
+#endif
+constexpr uint32_t PART = VPART << 10;
 constexpr uint32_t PART_MIN = 16u << 10;
 
 uint32_t row_ctas(uint32_t vecs, uint64_t rows, int sm_count) {
-  uint32_t c = 1;
-  while (c < ROW_MAX_CLUSTER && (uint64_t)((vecs + c - 1) / c) * 16 > PART) c <<= 1;
-  while (c < 8 && rows * c * 2 <= (uint64_t)sm_count && (uint64_t)((vecs + 2 * c - 1) / (2 * c)) * 16 >= PART_MIN)
-    c <<= 1;
-  return c;
+  const uint32_t bytes = vecs * 16;
+  uint32_t c = (bytes + PART - 1) / PART;
+  while (c < 8 && rows * c * 2 <= (uint64_t)sm_count && bytes / (2 * c) >= PART_MIN) c *= 2;
+  return c < ROW_MAX_CLUSTER ? c : ROW_MAX_CLUSTER;
 }
 
 template <typename Kern>

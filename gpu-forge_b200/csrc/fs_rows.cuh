@@ -28,6 +28,9 @@ namespace fs {
 namespace cg = cooperative_groups;
 
 constexpr int ROW_THREADS = 256;
+#ifndef ROW_MINB
+#define ROW_MINB 3
+#endif
 constexpr int ROW_WARPS = ROW_THREADS / 32;
 constexpr int ROW_MAX_CLUSTER = 16;
 constexpr int ROW_IDX_BITS = 19;
@@ -249,7 +252,23 @@ template <typename V> __device__ __forceinline__ V warp_scan(V v, int lane) {  /
   }
   return v;
 }
+// *p += v in shared memory where yes, without a branch.
+__device__ __forceinline__ void smem_add_if(bool yes, uint32_t* p, uint32_t v) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n @q red.shared.add.u32 [%0], %1;\n}" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(p)),
+               "r"(v), "r"((uint32_t)yes)
+               : "memory");
+}
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ uint64_t row_target(float p, uint64_t mass) {  // ceil(p mass), at least 1
+  const double least = ceil((double)fmaxf(p, 0.0f) * (double)mass);
+  return least < 1.0 ? 1ull : (uint64_t)least;
+}
+__device__ __forceinline__ uint64_t row_draw(float u, uint64_t mass) {  // floor(u mass), below mass
+  const double at = floor((double)(u > 0.0f ? u : 0.0f) * (double)mass);
+  return at < (double)mass ? min((uint64_t)at, mass - 1) : mass - 1;
+}
 
 // ---- shared state ---------------------------------------------------------------
 struct RowShared {
@@ -267,7 +286,7 @@ struct RowShared {
   uint64_t scan_q[ROW_WARPS];
   uint32_t scan_n[ROW_WARPS];
   uint32_t n[ROW_MAX_CLUSTER];
-  uint64_t lo, hi, cut_q;
+  uint64_t lo, hi, cut_q, cut_c;
   uint32_t cut_n, count, above, first, b1, b2, last;
 };
 constexpr size_t ROW_SHARED_BYTES = (sizeof(RowShared) + 15) / 16 * 16;
@@ -279,6 +298,8 @@ struct RowFinish {
   uint32_t start[ROW_SORT_BINS + 4];
   uint64_t loose[ROW_POOL];
   uint64_t sorted[ROW_POOL];
+  uint64_t input[ROW_LIST];
+  uint32_t part[ROW_MAX_CLUSTER * ROW_WARPS][2];  // masses of a stretch's entries in the interval: their low 20 bits, the rest
 };
 
 // ---- one row --------------------------------------------------------------------
@@ -398,9 +419,9 @@ template <typename T> struct Row {
     }
     cluster.barrier_wait();
     const uint32_t per = top_count();
-    for (uint32_t i = lane; i < per * ctas; i += 32) {  // (32 or 64) entry e of CTA i / per's copy
-      const uint32_t e = i & (per - 1), v = __shfl_sync(~0u, k, e);
-      if (tops || e == 0) *cluster.map_shared_rank(&sh.tops[(rank * ROW_WARPS + wid) * per + e], i / per) = v;
+    for (uint32_t i0 = 0; i0 < per * ctas; i0 += 32) {
+      const uint32_t to = (i0 + lane) / per, e = i0 + lane - to * per, v = __shfl_sync(~0u, k, e);
+      if (to < ctas && (tops || e == 0)) *cluster.map_shared_rank(&sh.tops[(rank * ROW_WARPS + wid) * per + e], to) = v;
     }
     cluster.sync();
     uint32_t best = ~0u;
@@ -444,25 +465,26 @@ template <typename T> struct Row {
   }
 
   // ---- the one pass over all weights ----
-  // The mass of this thread's entries (ABOVE: of those over `least`).  Per
-  // entry: a half of four packed additions, a half of one packed
-  // multiplication, the exponential and one integer addition.  A thread holds
-  // fewer than 2^9 entries, so that neither 32-bit sum of hi < 2^23 or
-  // |lo| <= 2^17 wraps.
-  template <bool ABOVE> __device__ __forceinline__ uint64_t weigh(float least) const {
+  // The mass of this thread's entries (ABOVE: of those over `over`, and
+  // f(x, index) for those from `low` to `over`).  Per entry: a half of four
+  // packed additions, a half of one packed multiplication, the exponential and
+  // one integer addition.  A thread holds fewer than 2^9 entries, so that
+  // neither 32-bit sum of hi < 2^23 or |lo| <= 2^17 wraps.
+  template <bool ABOVE, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, F f) const {
     const uint64_t m2 = f2_pack(-m, -m), c2 = f2_pack(c, c), one = f2_pack(1.0f, 1.0f), none = f2_pack(-1.0f, -1.0f),
                    magic = f2_pack(ROW_MAGIC, ROW_MAGIC);
     uint32_t hi = 0, lo = 0, n = 0;
 #pragma unroll 2
     for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
-      float f[N];
-      E::get(data[i], f);
+      float z[N];
+      const uint4 v = data[i];
+      E::get(v, z);
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
         float w0, w1, a0, a1, b0, b1;
-        f2_unpack(f2_mul(f2_add(f2_pack(f[e], f[e + 1]), m2), c2), w0, w1);
+        f2_unpack(f2_mul(f2_add(f2_pack(z[e], z[e + 1]), m2), c2), w0, w1);
         w0 = row_exp2(w0), w1 = row_exp2(w1);
-        if (ABOVE) w0 = f[e] > least ? w0 : 0.0f, w1 = f[e + 1] > least ? w1 : 0.0f;
+        if (ABOVE) w0 = z[e] > over ? w0 : 0.0f, w1 = z[e + 1] > over ? w1 : 0.0f;
         const uint64_t w = f2_pack(w0, w1);
         const uint64_t a = f2_add(w, one);
         const uint64_t b = f2_add(f2_fma(f2_add(a, none), none, w), magic);
@@ -472,8 +494,12 @@ template <typename T> struct Row {
         lo += __float_as_uint(b0) + __float_as_uint(b1);
       }
       n += N;
+      if (ABOVE) each_of(hits(v, low, over), i, f);
     }
     return row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
+  }
+  __device__ __forceinline__ uint64_t weigh() const {
+    return weigh<false>(0.0f, 0.0f, [](float, int) {});
   }
 
   // Bits of the entries of a vector in [low, high].
@@ -570,13 +596,9 @@ template <typename T> struct Row {
   }
 
   // Hands this warp's masses to the first CTA (ALL: to every CTA).
-  template <bool ALL> __device__ __forceinline__ void hand(uint64_t own, uint64_t part) {
+  template <bool ALL> __device__ __forceinline__ void hand(uint64_t (&to)[ROW_MAX_CLUSTER][ROW_WARPS], uint64_t own) {
     own = warp_sum_u64(own);
-    part = warp_sum_u64(part);
-    if (lane < (ALL ? (int)ctas : 1)) {
-      *cluster.map_shared_rank(&sh.mass[rank][wid], lane) = own;
-      *cluster.map_shared_rank(&sh.part[rank][wid], lane) = part;
-    }
+    if (lane < (ALL ? (int)ctas : 1)) *cluster.map_shared_rank(&to[rank][wid], lane) = own;
   }
   // Sums of what was handed over.
   __device__ __forceinline__ uint64_t handed(const uint64_t (&of)[ROW_MAX_CLUSTER][ROW_WARPS]) const {
@@ -584,38 +606,60 @@ template <typename T> struct Row {
     for (uint32_t i = lane; i < ctas * ROW_WARPS; i += 32) t += (&of[0][0])[i];
     return warp_sum_u64(t);
   }
-  // Collects this CTA's entries from the maximum to `edge`, or in [lo, hi] of
-  // (key, index) order, at `to`, of room for `room`; sh.count is their number
-  // (sh.count = 0 before).
-  __device__ __forceinline__ void collect_above(float edge, uint64_t* to, uint32_t room) {
+  // The first CTA's list of candidates is divided among the CTAs.
+  __device__ __forceinline__ uint32_t share() const { return ROW_LIST / ctas; }
+  // Collects this CTA's entries of at least `edge` in its share of the first
+  // CTA's list, and tells every CTA their number (sh.count = 0 before).
+  __device__ __forceinline__ void collect_above(float edge) {
+    const uint32_t room = share();
     above(edge, [&](float z, int j) {
       const uint32_t at = atomicAdd(&sh.count, 1u);
-      if (at < room) to[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+      if (at < room) sh.list[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
     });
     __syncthreads();
     if (tid < (int)ctas) *cluster.map_shared_rank(&sh.n[rank], tid) = sh.count;
+    if (rank) {
+      uint64_t* const to = cluster.map_shared_rank(sh.list, 0) + rank * room;
+      for (uint32_t i = tid; i < min(sh.count, room); i += ROW_THREADS) to[i] = sh.list[i];
+    }
   }
-  __device__ __forceinline__ void collect(uint64_t lo, uint64_t hi, uint64_t* to, uint32_t room) {
-    between(value_of(hi), value_of(lo), [&](float z, int j) {
-      const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
-      if (e < lo || e > hi) return;
-      const uint32_t at = atomicAdd(&sh.count, 1u);
-      if (at < room) to[at] = e;
-    });
+  // Whether the candidates of all CTAs fit their shares; their total.
+  __device__ __forceinline__ bool all_listed(uint32_t& n) const {
+    bool fit = true;
+    n = 0;
+    for (uint32_t i = 0; i < ctas; ++i) n += sh.n[i], fit &= sh.n[i] <= share();
+    return fit;
+  }
+  // f(number, entry) for this thread's candidates, on the first CTA.
+  template <typename F> __device__ __forceinline__ void each_listed(F f) const {
+    const uint32_t room = share();
+    for (uint32_t s = tid; s < room * ctas; s += ROW_THREADS) {
+      uint32_t before = 0, mine_n = 0, at = s;
+      for (uint32_t i = 0; i < ctas; ++i) {
+        const bool in = s >= i * room;
+        if (in) at = s - i * room, mine_n = sh.n[i];
+        if (s >= (i + 1) * room) before += sh.n[i];
+      }
+      if (at < mine_n) f(before + at, sh.list[s]);
+    }
+  }
+  // Tells every CTA the number of entries that this one has put at the start
+  // of its pool.
+  __device__ __forceinline__ void tell_pool() {
     __syncthreads();
     if (tid < (int)ctas) *cluster.map_shared_rank(&sh.n[rank], tid) = sh.count;
   }
-  // After collect() on every CTA and a cluster barrier: their total, and
-  // where they fit, the other CTAs' entries go behind the first CTA's.
-  __device__ __forceinline__ uint32_t pooled(uint64_t* from, uint32_t room) {
+  // After tell_pool() on every CTA and a cluster barrier: their total, and
+  // where they are at most `room`, the others' go behind the first CTA's.
+  __device__ __forceinline__ uint32_t pooled(uint32_t room) {
     uint32_t n = 0, base = 0;
     for (uint32_t i = 0; i < ctas; ++i) {
       if (i == rank) base = n;
       n += sh.n[i];
     }
     if (n <= room && rank) {
-      uint64_t* const to = cluster.map_shared_rank(from, 0) + base;
-      for (uint32_t i = tid; i < sh.n[rank]; i += ROW_THREADS) to[i] = from[i];
+      uint64_t* const to = cluster.map_shared_rank(sh.pool, 0) + base;
+      for (uint32_t i = tid; i < sh.n[rank]; i += ROW_THREADS) to[i] = sh.pool[i];
     }
     return n;
   }
@@ -686,18 +730,20 @@ template <typename T> struct Row {
       const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w, c42 = fminf(c * ROW_BIN_SCALE, ROW_F32_MAX);
       const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), c42)) >= bin_at(place_of(value_of(lo), c42)) + 3);
       if (round == 0) {
-        each([&](float z, int) {
-          const float y = place_of(z, c42);
-          if (by_mass) {
-            if (y < ROW_MASS_END * ROW_BIN_SCALE) {
-              const float b = __fadd_rn(y, 0x1p23f);  // 2^-(y - b) / 42 by its tangent, as a whole number by another such addition
-              const float v = __fmaf_rn(__fsub_rn(y, __fsub_rn(b, 0x1p23f)), -4096.0f * ROW_LN2 / ROW_BIN_SCALE, 0x1p23f + 4096.0f);
-              atomicAdd(&sh.bins[__float_as_uint(b) & 0x7fffffu], __float_as_uint(v) & 0x7fffffu);
-            }
-          } else if (z > -INFINITY) {
-            atomicAdd(&sh.bins[bin_at(y)], 1u);
+#pragma unroll 2
+        for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
+          float z[N];
+          E::get(data[i], z);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float y = place_of(z[e], c42);
+            // 2^-(y - b) / 42 by its tangent, as a whole number by another such addition
+            const float b = __fadd_rn(fminf(y, (float)(ROW_BINS - 1)), 0x1p23f);
+            const float v = __fmaf_rn(__fsub_rn(y, __fsub_rn(b, 0x1p23f)), -4096.0f * ROW_LN2 / ROW_BIN_SCALE, 0x1p23f + 4096.0f);
+            smem_add_if(by_mass ? y < ROW_MASS_END * ROW_BIN_SCALE : z[e] > -INFINITY, &sh.bins[__float_as_uint(b) & 0x7fffffu],
+                        by_mass ? __float_as_uint(v) & 0x7fffffu : 1u);
           }
-        });
+        }
       } else {
         between(value_of(hi), value_of(lo), [&](float z, int j) {
           const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
@@ -713,6 +759,18 @@ template <typename T> struct Row {
         });
       }
       cluster.sync();
+      // each CTA sums a slice of the bins over the cluster, into the first CTA's
+      const uint32_t slice = (ROW_BINS + ctas - 1) / ctas;
+      for (uint32_t i = tid; i < slice; i += ROW_THREADS) {
+        const uint32_t b = rank * slice + i;
+        if (b < ROW_BINS) {
+          uint32_t v = 0;
+#pragma unroll 8
+          for (uint32_t k = 0; k < ctas; ++k) v += cluster.map_shared_rank(sh.bins, k)[b];
+          cluster.map_shared_rank(sh.bins, 0)[b] = v;
+        }
+      }
+      cluster.sync();
       if (rank == 0) {
         // the prefix ends in b1 or later, and in b2 or before: where a sum of estimates, 2^-12 of it and 2^-20 of the
         // largest weight added, and taken off, reaches the target.  (An estimate is off by half a unit of 4060 and less
@@ -723,19 +781,9 @@ template <typename T> struct Row {
         float s[PER], own = 0, all;
         uint32_t filled = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {  // bins tid * PER + i, read side by side and handed over in shared memory
-          uint32_t n = sh.bins[i * ROW_THREADS + tid];
-          for (uint32_t k = 1; k < ctas; ++k) n += cluster.map_shared_rank(sh.bins, k)[i * ROW_THREADS + tid];
-          s[i] = (float)n;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < PER; ++i) reinterpret_cast<float*>(sh.bins)[i * ROW_THREADS + tid] = s[i];
-        __syncthreads();
-#pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int b = tid * PER + i;
-          s[i] = reinterpret_cast<float*>(sh.bins)[b];
+          s[i] = (float)sh.bins[b];
           if (s[i] > 0.0f) filled = b;
           if (by_mass) s[i] *= by_weight ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w;
           own += s[i];
@@ -773,9 +821,17 @@ template <typename T> struct Row {
       lo = sh.lo, hi = sh.hi;
       // exact sums of what comes before, and the entries of the interval
       above_n = by_mass ? 0 : sh.above;
-      uint64_t before = weigh<true>(value_of(lo)), kept;
-      if (lo & (ROW_MAX_COLS - 1))  // equal values on both sides of the bound
-        between(value_of(lo), value_of(lo), [&](float z, int j) {
+      uint64_t before = 0, kept;
+      const float over = value_of(lo);
+      const bool cuts_equals = (lo & (ROW_MAX_COLS - 1)) != 0;  // equal values lie on both sides of lo
+      before = weigh<true>(over, value_of(hi), [&](float z, int j) {
+        const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+        if (e < lo || e > hi) return;
+        const uint32_t at = atomicAdd(&sh.count, 1u);
+        if (at < ROW_POOL) sh.pool[at] = e;
+      });
+      if (cuts_equals)
+        between(over, over, [&](float z, int j) {
           if (((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) < lo) before += mass(z);
         });
       kept = before;
@@ -786,11 +842,12 @@ template <typename T> struct Row {
           if (w >= least_w && ((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) < lo) kept += row_q(w);
         });
       }
-      hand<true>(before, kept);
-      collect(lo, hi, sh.pool, ROW_POOL);
+      hand<true>(sh.mass, before);
+      hand<true>(sh.part, kept);
+      tell_pool();
       cluster.sync();
       above_q = handed(sh.mass);
-      n = pooled(sh.pool, most);
+      n = pooled(most);
       if (n <= most) return;
     }
     n = 0;  // never: what the last round left undecided is cut off
@@ -876,26 +933,70 @@ template <typename T> struct Row {
     __syncthreads();
   }
 
+  // Cuts the n <= ROW_THREADS entries of f.loose to the first k (0: all),
+  // then to the shortest prefix of at least p of their mass (without k: of the
+  // row's, `total`), then to w >= least_w, and draws: each thread
+  // compares its entry with all others, once in descending order and once in
+  // index order.
+  template <typename H>
+  __device__ __forceinline__ void finish_few(RowFinish& f, uint32_t n, uint32_t k, float p, float least_w, float u, uint64_t total,
+                                             H hit) {
+    const bool in = tid < n;
+    const uint64_t e = in ? f.loose[tid] : ~0ull;
+    const float z = value_of(e), w = in ? weight(z) : 0.0f;
+    const uint64_t q = row_q(w);
+    f.sorted[tid] = q;
+    if (tid == 0) sh.cut_q = total, sh.cut_c = ~0ull;
+    __syncthreads();
+    uint32_t rank_of = 0;
+    uint64_t before = 0;
+    if (wid * 32 < (int)n) {
+#pragma unroll 4
+      for (uint32_t i = 0; i < n; ++i) {
+        const bool less = f.loose[i] < e;
+        const uint64_t qi = f.sorted[i];
+        rank_of += less;
+        before += less ? qi : 0;
+      }
+    }
+    if (k) {
+      if (in && rank_of == min(k, n) - 1) sh.cut_c = e, sh.cut_q = before + q;
+      __syncthreads();
+    }
+    uint64_t last = sh.cut_c, mass = sh.cut_q;
+    if (p < 1.0f) {
+      const uint64_t target = row_target(p, mass);
+      __syncthreads();
+      if (in && before < target && target <= before + q) sh.cut_c = e, sh.cut_q = before + q;
+      __syncthreads();
+      last = sh.cut_c, mass = sh.cut_q;
+    }
+    if (least_w > 0.0f) {
+      __syncthreads();
+      block_scan(in && e <= last && w >= least_w ? q : 0, sh.scan_q, mass);
+    }
+    const uint64_t t = row_draw(u, mass);
+    const uint64_t own = in && e <= last && w >= least_w ? q : 0;
+    if (__syncthreads_or(own && own == mass)) {  // one entry is left
+      if (own) hit(z, (int)(e & (ROW_MAX_COLS - 1)));
+      return;
+    }
+    f.sorted[tid] = own;  // kept masses
+    __syncthreads();
+    if (wid * 32 >= (int)n) return;
+    const uint32_t j = (uint32_t)e & (ROW_MAX_COLS - 1);
+    before = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < n; ++i) {
+      const uint64_t qi = f.sorted[i];
+      before += ((uint32_t)f.loose[i] & (ROW_MAX_COLS - 1)) < j ? qi : 0;
+    }
+    if (own && before <= t && t < before + own) hit(z, (int)j);
+  }
+
   // Draws among the first n of f.sorted, kept where w >= least_w, of together
   // `mass`: the entry at which the running mass in index order exceeds t.
   template <typename H> __device__ __forceinline__ void draw(RowFinish& f, uint32_t n, float least_w, uint64_t t, H hit) {
-    auto mass_of = [&](uint64_t e) {
-      const float w = weight(value_of(e));
-      return w >= least_w ? row_q(w) : 0;
-    };
-    if (n <= 32) {  // one warp sums, for each, those with lower indexes
-      if (wid) return;
-      const uint64_t e = f.sorted[min(lane, (int)n - 1)];
-      const uint64_t q = lane < (int)n ? mass_of(e) : 0;
-      const uint32_t j = (uint32_t)e & (ROW_MAX_COLS - 1);
-      uint64_t before = 0;
-      for (int k = 0; k < (int)n; ++k) {
-        const uint64_t qk = __shfl_sync(~0u, q, k);
-        if (__shfl_sync(~0u, j, k) < j) before += qk;
-      }
-      if (lane < (int)n && before <= t && t < before + q) hit(value_of(e), (int)j);
-      return;
-    }
     const int shift = max(0, 32 - __clz((int)cols) - 10);
     constexpr int PER = ROW_POOL / ROW_THREADS;
     uint64_t e[PER];
@@ -986,15 +1087,6 @@ template <typename T> struct Row {
   }
 };
 
-__device__ __forceinline__ uint64_t row_target(float p, uint64_t mass) {  // ceil(p mass), at least 1
-  const double least = ceil((double)fmaxf(p, 0.0f) * (double)mass);
-  return least < 1.0 ? 1ull : (uint64_t)least;
-}
-__device__ __forceinline__ uint64_t row_draw(float u, uint64_t mass) {  // floor(u mass), below mass
-  const double at = floor((double)(u > 0.0f ? u : 0.0f) * (double)mass);
-  return at < (double)mass ? min((uint64_t)at, mass - 1) : mass - 1;
-}
-
 // ---- sampling ---------------------------------------------------------------------
 // Every CTA of the cluster: the load with the maximum (HBM), then a pass over
 // shared memory that sums the weights.  Where a cut is asked for, the CTAs
@@ -1005,7 +1097,7 @@ __device__ __forceinline__ uint64_t row_draw(float u, uint64_t mass) {  // floor
 //
 // A cut that does not end among the candidates (a nucleus beyond the guess,
 // a large top_k, many equal values) keeps the cluster to narrow it down.
-template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sample(const RowArgs a) {
+template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k_row_sample(const RowArgs a) {
   extern __shared__ __align__(16) unsigned char row_smem[];
   RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
   uint4* const data = reinterpret_cast<uint4*>(row_smem + ROW_SHARED_BYTES);
@@ -1039,9 +1131,9 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sa
   };
   if (greedy)
     r.above(r.m, [&](float, int j) { atomicMin(r.cluster.map_shared_rank(&sh.first, 0), (uint32_t)j); });
-  const uint64_t own = r.template weigh<false>(0.0f);
+  const uint64_t own = r.weigh();
   if (!by_k && !by_p && !by_w) {
-    r.template hand<false>(own, 0);
+    r.template hand<false>(sh.mass, own);
     if (!r.last_part()) return;
     total = r.handed(sh.mass);
     if (!greedy)
@@ -1059,24 +1151,35 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sa
   } else {
     edge = fmaxf(r.m + (log2f(least_w) - 0x1p-10f) / r.c - fabsf(r.m) * 0x1p-21f, r.mass_end());
   }
-  uint64_t part = 0;
+  r.template hand<true>(sh.mass, own);
   if (edge < INFINITY) {
-    r.collect_above(edge, sh.list, ROW_LIST);
-    if (by_p && !by_k)
-      for (uint32_t i = r.tid; i < min(sh.count, (uint32_t)ROW_LIST); i += ROW_THREADS) part += r.mass(r.value_of(sh.list[i]));
+    r.collect_above(edge);
+    if (by_p && !by_k) {
+      uint64_t part = 0;
+      for (uint32_t i = r.tid; i < min(sh.count, r.share()); i += ROW_THREADS) part += r.mass(r.value_of(sh.list[i]));
+      r.template hand<true>(sh.part, part);
+    }
   }
-  r.template hand<true>(own, part);
   r.cluster.sync();
-  total = r.handed(sh.mass);
   uint32_t n = 0;
   bool enough = false;
   if (edge < INFINITY) {
-    n = r.pooled(sh.list, ROW_LIST);
-    enough = n <= (uint32_t)ROW_LIST && (by_k || !by_p || r.handed(sh.part) >= row_target(p, total));
+    enough = r.all_listed(n);
+    if (by_k && enough && r.rank) return;
   }
+  total = r.handed(sh.mass);
+  if (enough && !by_k && by_p) enough = r.handed(sh.part) >= row_target(p, total);
   if (enough) {
-    if (!r.last_part()) return;
-    r.order_by_value(f, sh.list, n, edge);
+    if (r.rank) return;
+    if (n <= (uint32_t)ROW_THREADS) {
+      r.each_listed([&](uint32_t i, uint64_t e) { f.loose[i] = e; });
+      __syncthreads();
+      r.finish_few(f, n, by_k ? k : 0, p, least_w, u, total, store);
+      return;
+    }
+    r.each_listed([&](uint32_t i, uint64_t e) { f.input[i] = e; });
+    __syncthreads();
+    r.order_by_value(f, f.input, n, edge);
     // running masses in descending order, `per` entries a thread
     const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(r.tid * per, n), i1 = min(i0 + per, n);
     uint64_t sum = 0, all;
@@ -1168,14 +1271,22 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sa
     }
     last = cut ? f.sorted[cut - 1] : hi;
     // the warps' kept masses: before the interval, and those of its entries
+    if (r.tid < ROW_MAX_CLUSTER * ROW_WARPS) f.part[r.tid][0] = f.part[r.tid][1] = 0;
+    __syncthreads();
     for (uint32_t i = r.tid; i < cut; i += ROW_THREADS) {
       const uint64_t e = f.sorted[i];
       const float w = r.weight(r.value_of(e));
       const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + r.lead) / Row<T>::N;
       const uint32_t cta = v / r.part_vecs, p0 = cta * r.part_vecs, p1 = min(p0 + r.part_vecs, r.total_vecs);
       const uint32_t warp = (v - p0) / ((p1 - p0 + ROW_WARPS - 1) / ROW_WARPS);
-      if (w >= least_w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.part[cta][warp]), (unsigned long long)row_q(w));
+      if (w >= least_w) {
+        const uint64_t q = row_q(w);
+        atomicAdd(&f.part[cta * ROW_WARPS + warp][0], (uint32_t)q & 0xfffffu);
+        atomicAdd(&f.part[cta * ROW_WARPS + warp][1], (uint32_t)(q >> 20));
+      }
     }
+    __syncthreads();
+    if (r.tid < ROW_MAX_CLUSTER * ROW_WARPS) (&sh.part[0][0])[r.tid] += ((uint64_t)f.part[r.tid][1] << 20) + f.part[r.tid][0];
   } else {  // min_p alone
     uint64_t kept = 0;
     r.each([&](float z, int) {
@@ -1183,7 +1294,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sa
       if (w >= least_w) kept += row_q(w);
     });
     r.cluster.sync();  // every CTA has read the sums before the next ones
-    r.template hand<false>(own, kept);
+    r.template hand<false>(sh.part, kept);
     if (!r.last_part()) return;
   }
   __syncthreads();
@@ -1197,7 +1308,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_sa
 
 // ---- the n best ---------------------------------------------------------------------
 // As a sampling row with top_k = n, whose ordered candidates are the answer.
-template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_best(const RowArgs a) {
+template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k_row_best(const RowArgs a) {
   extern __shared__ __align__(16) unsigned char row_smem[];
   RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
   uint4* const data = reinterpret_cast<uint4*>(row_smem + ROW_SHARED_BYTES);
@@ -1216,20 +1327,23 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_be
   }
   r.c = ROW_LOG2E;
   const uint32_t k = (uint32_t)a.n;
-  const uint64_t first = (uint64_t)row_key(r.m) << ROW_IDX_BITS;
   float edge = INFINITY;
+  r.template hand<true>(sh.mass, r.weigh());
   if (k <= r.top_count() * r.ctas * ROW_WARPS * 3 / 4) {
     edge = r.edge_of(k, ROW_EDGE_SCALE * ROW_LOG2E, -ROW_F32_MAX);
     if (edge == -ROW_F32_MAX) edge = r.edge_of(k, r.far_scale(), -ROW_F32_MAX);
-    r.collect_above(edge, sh.list, ROW_LIST);
+    r.collect_above(edge);
   }
-  r.template hand<true>(r.template weigh<false>(0.0f), 0);
   r.cluster.sync();
+  uint32_t n = 0;
+  const bool listed = edge < INFINITY && r.all_listed(n);
+  if (listed && r.rank) return;
   const float ln = logf((float)r.handed(sh.mass) * 0x1p-40f);
-  uint32_t n = ~0u;
-  uint64_t* from = sh.list;
-  if (edge < INFINITY) n = r.pooled(sh.list, ROW_LIST);
-  if (n > (uint32_t)ROW_LIST) {
+  const uint64_t* from = f.input;
+  if (listed) {
+    r.each_listed([&](uint32_t i, uint64_t e) { f.input[i] = e; });
+    __syncthreads();
+  } else {
     // the n-th entry, then the entries up to it
     uint32_t above_n;
     r.narrow(false, k, 0.0f, ROW_FEW, n, above_n);
@@ -1240,13 +1354,19 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_row_be
     }
     if (r.tid == 0) sh.count = 0;
     r.cluster.sync();
-    r.collect(first, sh.hi, sh.pool, ROW_POOL);
+    r.between(r.value_of(sh.hi), r.m, [&](float z, int j) {
+      const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+      if (e > sh.hi) return;
+      const uint32_t at = atomicAdd(&sh.count, 1u);
+      if (at < ROW_POOL) sh.pool[at] = e;
+    });
+    r.tell_pool();
     edge = r.value_of(sh.hi);
     r.cluster.sync();
-    n = r.pooled(sh.pool, ROW_POOL);
+    n = r.pooled(ROW_POOL);
     from = sh.pool;
+    if (!r.last_part()) return;
   }
-  if (!r.last_part()) return;
   if (a.lse && r.tid == 0) a.lse[row] = r.m + ln;
   r.order_by_value(f, from, n, edge);
   const uint32_t have = min(n, k);
