@@ -16,6 +16,8 @@ struct SorterView {
   int sm_count;
   cudaStream_t stream;
   int* host_err;  // device alias of the mapped error word (DEV_ERR_*)
+  cudaMemPool_t pool;      // of stream-ordered scratch
+  uint64_t row_pass_min;   // row operators over at least this many bytes go in passes
 };
 
 // Makes the sorter's device current and fills *v; stream NULL: the sorter's.

@@ -3,6 +3,7 @@
 #include "forgesort.h"
 #include "fs_internal.h"
 #include "fs_rows.cuh"
+#include "fs_rows_stream.cuh"
 
 #include <atomic>
 
@@ -29,6 +30,13 @@ size_t elem_bytes(int dtype) { return dtype == FS_LOGITS_F32 ? 4 : 2; }
 #endif
 constexpr uint32_t PART = VPART << 10;
 constexpr uint32_t PART_MIN = 16u << 10;
+// Large batches go in passes over all rows, in groups of STREAM_ROWS rows
+// (of 25 KB of scratch each), cut into parts of STREAM_PART bytes.
+#ifndef VSPART
+#define VSPART 32
+#endif
+constexpr uint64_t STREAM_ROWS = 4096;
+constexpr uint32_t STREAM_PART = VSPART << 10;
 
 uint32_t row_ctas(uint32_t vecs, uint64_t rows, int sm_count) {
   const uint32_t bytes = vecs * 16;
@@ -37,44 +45,164 @@ uint32_t row_ctas(uint32_t vecs, uint64_t rows, int sm_count) {
   return c < ROW_MAX_CLUSTER ? c : ROW_MAX_CLUSTER;
 }
 
-template <typename Kern>
-int launch(fs_sorter* s, const SorterView& v, Kern kern, std::atomic<bool>* configured, RowArgs& a, int lanes) {
-  if (!configured[v.device].load()) {  // idempotent: two threads may both get here
-    FS_ROWS_CUDA(s, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(ROW_SHARED_BYTES + ROW_PART_MAX)));
-    FS_ROWS_CUDA(s, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    configured[v.device].store(true);
-  }
-  // vectors of a row: with the worst lead of lanes - 1 elements, unless every row begins at a vector
+// A launch behind the call's previous one (fs_rows_stream.cuh), scheduled
+// while that one drains; every such kernel waits for it first.
+template <typename Kern, typename... Args>
+cudaError_t chained(const SorterView& v, Kern kern, unsigned grid, size_t smem, uint32_t cluster, const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(ROW_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = v.stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// 16-byte vectors of a row: with the worst lead, unless every row begins at a
+// vector.
+uint32_t row_vecs(const RowArgs& a, int lanes) {
   const int64_t step = a.rows > 1 ? a.stride : 0;
   const bool aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && step % lanes == 0;
-  const uint32_t vecs = (a.cols + (aligned ? lanes - 1 : 2 * lanes - 2)) / lanes;
-  const uint32_t ctas = row_ctas(vecs, a.rows, v.sm_count);
+  return (a.cols + (aligned ? lanes - 1 : 2 * lanes - 2)) / lanes;
+}
+size_t cluster_smem(uint32_t part_vecs) {
+  const size_t part = (size_t)part_vecs * 16;
+  return ROW_SHARED_BYTES + (part > sizeof(RowFinish) ? part : sizeof(RowFinish));
+}
+constexpr size_t FINISH_SMEM = ROW_SHARED_BYTES + sizeof(RowFinish);
+
+// Small batches: one cluster a row.
+template <typename T, bool BEST> int launch_clusters(fs_sorter* s, const SorterView& v, RowArgs& a, int* launches) {
+  const uint32_t vecs = row_vecs(a, RowElem<T>::N), ctas = row_ctas(vecs, a.rows, v.sm_count);
   a.part_vecs = (vecs + ctas - 1) / ctas;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.rows * ctas);
   cfg.blockDim = dim3(ROW_THREADS);
-  const size_t part = (size_t)a.part_vecs * 16;
-  cfg.dynamicSmemBytes = ROW_SHARED_BYTES + (part > sizeof(RowFinish) ? part : sizeof(RowFinish));
+  cfg.dynamicSmemBytes = cluster_smem(a.part_vecs);
   cfg.stream = v.stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = ctas;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  FS_ROWS_CUDA(s, cudaLaunchKernelEx(&cfg, kern, static_cast<const RowArgs>(a)));
+  FS_ROWS_CUDA(s, cudaLaunchKernelEx(&cfg, k_rows<T, BEST>, static_cast<const RowArgs>(a)));
+  *launches += 1;
   return FS_OK;
 }
 
-template <typename T> int launch_sample(fs_sorter* s, const SorterView& v, RowArgs& a) {
-  static std::atomic<bool> configured[SORTER_MAX_DEVICES];
-  return launch(s, v, k_row_sample<T>, configured, a, RowElem<T>::N);
+// Large batches: passes over all rows, with scratch from the stream-ordered
+// allocator, so that a call keeps nothing and may be captured.
+template <typename T, bool BEST> int launch_passes(fs_sorter* s, const SorterView& v, RowArgs& a, int* launches) {
+  const uint32_t vecs = row_vecs(a, RowElem<T>::N);
+  RowStream st{};
+  st.parts = (vecs * 16 + STREAM_PART - 1) / STREAM_PART;
+  if (st.parts > ROW_MAX_CLUSTER) st.parts = ROW_MAX_CLUSTER;
+  a.part_vecs = (vecs + st.parts - 1) / st.parts;
+  const bool narrows = !BEST && a.top_p;  // rows may have wide nuclei
+  size_t bytes = 0;
+  auto take = [&](size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  const size_t R = a.rows;
+  const size_t o_rec = take(R * sizeof(RowRecord)), o_counts = take(8), zeroed = bytes;
+  const size_t o_tops = take(R * ROW_TOPS * 4), o_mass = take(R * ROW_SUMS * 8), o_list = take(R * ROW_LIST * 8), o_left = take(R * 4);
+  const size_t o_wide = take(narrows ? R * 4 : 0), o_part = take(narrows ? R * ROW_SUMS * 8 : 0);
+  const size_t o_bins = take(narrows ? R * ROW_BINS * 4 : 0), o_pool = take(narrows ? R * ROW_POOL * 8 : 0);
+  void* mem = nullptr;
+  FS_ROWS_CUDA(s, cudaMallocFromPoolAsync(&mem, bytes, v.pool, v.stream));
+  unsigned char* const b = static_cast<unsigned char*>(mem);
+  st.rec = reinterpret_cast<RowRecord*>(b + o_rec);
+  st.counts = reinterpret_cast<uint32_t*>(b + o_counts);
+  st.tops = reinterpret_cast<uint32_t*>(b + o_tops);
+  st.mass = reinterpret_cast<uint64_t*>(b + o_mass);
+  st.list = reinterpret_cast<uint64_t*>(b + o_list);
+  st.left = reinterpret_cast<uint32_t*>(b + o_left);
+  st.wide = reinterpret_cast<uint32_t*>(b + o_wide);
+  st.part = reinterpret_cast<uint64_t*>(b + o_part);
+  st.bins = reinterpret_cast<uint32_t*>(b + o_bins);
+  st.pool = reinterpret_cast<uint64_t*>(b + o_pool);
+  const RowArgs args = a;
+  const unsigned grid = a.rows * st.parts;
+  cudaError_t e = cudaMemsetAsync(mem, 0, zeroed, v.stream);
+  if (e == cudaSuccess) {
+    k_stream_max<T, BEST><<<grid, ROW_THREADS, 0, v.stream>>>(args, st);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = chained(v, k_stream_weigh<T, BEST>, grid, FINISH_SMEM, 0, args, st);
+  if constexpr (!BEST) {
+    if (narrows) {
+      const unsigned most = (unsigned)v.sm_count * 3, few = grid < most ? grid : most;
+      if (e == cudaSuccess) e = chained(v, k_stream_bins<T>, few, 0, 0, args, st);
+      if (e == cudaSuccess) e = chained(v, k_stream_cut<T>, few, FINISH_SMEM, 0, args, st);
+      *launches += 2;
+    }
+  }
+  if (e == cudaSuccess && (BEST || a.top_k || a.top_p || a.min_p)) {
+    RowArgs left = a;
+    left.only = st.left;
+    left.only_n = st.counts + 1;
+    const uint32_t ctas = row_ctas(vecs, 1, v.sm_count), most = (uint32_t)v.sm_count / ctas;
+    left.part_vecs = (vecs + ctas - 1) / ctas;
+    e = chained(v, k_rows<T, BEST>, (a.rows < most ? a.rows : most) * ctas, cluster_smem(left.part_vecs), ctas,
+                static_cast<const RowArgs>(left));
+    *launches += 1;
+  }
+  *launches += 2;
+  const cudaError_t freed = cudaFreeAsync(mem, v.stream);
+  FS_ROWS_CUDA(s, e);
+  FS_ROWS_CUDA(s, freed);
+  return FS_OK;
 }
-template <typename T> int launch_best(fs_sorter* s, const SorterView& v, RowArgs& a) {
+
+template <typename T, bool BEST> int launch(fs_sorter* s, const SorterView& v, RowArgs a, int* launches) {
   static std::atomic<bool> configured[SORTER_MAX_DEVICES];
-  return launch(s, v, k_row_best<T>, configured, a, RowElem<T>::N);
+  if (!configured[v.device].load()) {  // idempotent: two threads may both get here
+    FS_ROWS_CUDA(s, cudaFuncSetAttribute(k_rows<T, BEST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)(ROW_SHARED_BYTES + ROW_PART_MAX)));
+    FS_ROWS_CUDA(s, cudaFuncSetAttribute(k_rows<T, BEST>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    configured[v.device].store(true);
+  }
+  const uint64_t total = a.rows;
+  if (total * a.cols * sizeof(T) < v.row_pass_min) return launch_clusters<T, BEST>(s, v, a, launches);
+  for (uint64_t r = 0; r < total; r += STREAM_ROWS) {
+    RowArgs g = a;
+    g.rows = (uint32_t)(total - r < STREAM_ROWS ? total - r : STREAM_ROWS);
+    g.x = static_cast<const T*>(a.x) + (int64_t)r * a.stride;
+    if constexpr (BEST) {
+      g.best_idx = a.best_idx + r * a.n;
+      g.best_logprob = a.best_logprob + r * a.n;
+      g.lse = a.lse ? a.lse + r : nullptr;
+    } else {
+      g.temperature = a.temperature ? a.temperature + r : nullptr;
+      g.top_k = a.top_k ? a.top_k + r : nullptr;
+      g.top_p = a.top_p ? a.top_p + r : nullptr;
+      g.min_p = a.min_p ? a.min_p + r : nullptr;
+      g.uniform = a.uniform + r;
+      g.tokens = a.tokens + r;
+      g.logprobs = a.logprobs ? a.logprobs + r : nullptr;
+    }
+    const int rc = launch_passes<T, BEST>(s, v, g, launches);
+    if (rc) return rc;
+  }
+  return FS_OK;
+}
+
+template <bool BEST> int launch_rows(fs_sorter* s, const SorterView& v, int dtype, const RowArgs& a, int sync) {
+  int launches = 0;
+  const int rc = dtype == FS_LOGITS_F32   ? launch<float, BEST>(s, v, a, &launches)
+                 : dtype == FS_LOGITS_F16 ? launch<__half, BEST>(s, v, a, &launches)
+                                          : launch<__nv_bfloat16, BEST>(s, v, a, &launches);
+  return rc ? rc : sorter_finish(s, v, launches, sync);
 }
 
 int check_rows(fs_sorter* s, int dtype, const void* logits, uint64_t rows, uint64_t cols, int64_t stride) {
@@ -123,10 +251,7 @@ int fs_sample_rows(fs_sorter* s, int dtype, const void* logits, uint64_t rows, u
   a.uniform = uniform;
   a.tokens = tokens;
   a.logprobs = logprobs;
-  rc = dtype == FS_LOGITS_F32   ? launch_sample<float>(s, v, a)
-       : dtype == FS_LOGITS_F16 ? launch_sample<__half>(s, v, a)
-                                : launch_sample<__nv_bfloat16>(s, v, a);
-  return rc ? rc : sorter_finish(s, v, 1, sync);
+  return launch_rows<false>(s, v, dtype, a, sync);
 }
 
 int fs_top_logprobs(fs_sorter* s, int dtype, const void* logits, uint64_t rows, uint64_t cols, int64_t row_stride,
@@ -152,10 +277,7 @@ int fs_top_logprobs(fs_sorter* s, int dtype, const void* logits, uint64_t rows, 
   a.best_idx = indices;
   a.best_logprob = logprobs;
   a.lse = lse;
-  rc = dtype == FS_LOGITS_F32   ? launch_best<float>(s, v, a)
-       : dtype == FS_LOGITS_F16 ? launch_best<__half>(s, v, a)
-                                : launch_best<__nv_bfloat16>(s, v, a);
-  return rc ? rc : sorter_finish(s, v, 1, sync);
+  return launch_rows<true>(s, v, dtype, a, sync);
 }
 
 }  // extern "C"

@@ -60,6 +60,8 @@ struct RowArgs {
   int64_t stride;       // elements between rows
   uint32_t rows, cols;
   uint32_t part_vecs;   // 16-byte vectors of a row per CTA of its cluster
+  const uint32_t* only; // null, or the rows to work on, of number *only_n
+  const uint32_t* only_n;
   // sampling (null: off)
   const float* temperature;
   const int* top_k;
@@ -101,6 +103,9 @@ template <> struct RowElem<float> {
     return __float_as_uint(fminf(fmaxf(__uint_as_float(v), -INFINITY), ROW_F32_MAX));
   }
   static __device__ __forceinline__ float one(const uint4* v, uint32_t i) { return reinterpret_cast<const float*>(v)[i]; }
+  static __device__ __forceinline__ float at(const uint4& v, int e) {
+    return __uint_as_float(e < 2 ? (e ? v.y : v.x) : (e & 1 ? v.w : v.z));
+  }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
@@ -128,6 +133,10 @@ template <> struct RowElem<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float one(const uint4* v, uint32_t i) {
     return __uint_as_float((uint32_t) reinterpret_cast<const unsigned short*>(v)[i] << 16);
+  }
+  static __device__ __forceinline__ float at(const uint4& v, int e) {
+    const uint32_t w = e < 4 ? (e < 2 ? v.x : v.y) : (e < 6 ? v.z : v.w);
+    return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
   }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -162,6 +171,10 @@ template <> struct RowElem<__half> {
   }
   static __device__ __forceinline__ float one(const uint4* v, uint32_t i) {
     return __half2float(__ushort_as_half(reinterpret_cast<const unsigned short*>(v)[i]));
+  }
+  static __device__ __forceinline__ float at(const uint4& v, int e) {
+    const uint32_t w = e < 4 ? (e < 2 ? v.x : v.y) : (e < 6 ? v.z : v.w);
+    return __half2float(__ushort_as_half((unsigned short)(e & 1 ? w >> 16 : w)));
   }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -259,6 +272,11 @@ __device__ __forceinline__ void smem_add_if(bool yes, uint32_t* p, uint32_t v) {
                "r"(v), "r"((uint32_t)yes)
                : "memory");
 }
+// Where kernels of one call are launched one behind the other before the
+// first has ended: waits until it has, with all that it wrote.
+__device__ __forceinline__ void row_chain_wait() {
+  asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ uint64_t row_target(float p, uint64_t mass) {  // ceil(p mass), at least 1
@@ -269,6 +287,32 @@ __device__ __forceinline__ uint64_t row_draw(float u, uint64_t mass) {  // floor
   const double at = floor((double)(u > 0.0f ? u : 0.0f) * (double)mass);
   return at < (double)mass ? min((uint64_t)at, mass - 1) : mass - 1;
 }
+
+// A row's sampling parameters.
+struct RowParams {
+  float t, p, least_w, u;
+  uint32_t k;
+  bool greedy, by_k, by_p, by_w;
+
+  __device__ __forceinline__ RowParams(const RowArgs& a, uint32_t row) {
+    t = a.temperature ? a.temperature[row] : 1.0f;
+    const int k_arg = a.top_k ? a.top_k[row] : 0;
+    p = a.top_p ? a.top_p[row] : 1.0f;
+    least_w = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
+    u = a.uniform[row];
+    k = (uint32_t)k_arg;
+    greedy = !(t > 0.0f);
+    by_k = !greedy && k_arg > 0 && k < a.cols;
+    by_p = !greedy && p < 1.0f;
+    by_w = !greedy && least_w > 0.0f;
+  }
+  __device__ __forceinline__ bool cuts() const { return by_k || by_p || by_w; }
+  // log2(e) / t, within the finite numbers above 0: 0 * c and (max + inf) * c stay what they are for the smallest and
+  // infinite t
+  __device__ __forceinline__ float c() const {
+    return greedy ? ROW_LOG2E : fminf(fmaxf(__fdiv_rn(ROW_LOG2E, t), 1.175494351e-38f), ROW_F32_MAX);
+  }
+};
 
 // ---- shared state ---------------------------------------------------------------
 struct RowShared {
@@ -287,7 +331,7 @@ struct RowShared {
   uint32_t scan_n[ROW_WARPS];
   uint32_t n[ROW_MAX_CLUSTER];
   uint64_t lo, hi, cut_q, cut_c;
-  uint32_t cut_n, count, above, first, b1, b2, last;
+  uint32_t cut_n, count, above, first, b1, b2, last, found;
 };
 constexpr size_t ROW_SHARED_BYTES = (sizeof(RowShared) + 15) / 16 * 16;
 static_assert(3 * (ROW_SHARED_BYTES + (64 << 10) + 1024) <= 228 << 10, "three CTAs on an SM");
@@ -312,6 +356,7 @@ template <typename T> struct Row {
   uint4* data;
   const int tid, lane, wid;
   const uint32_t rank, ctas;
+  const bool again;  // the cluster works on one row after another
   // the row in memory, cut into 16-byte vectors at memory's boundaries
   const T* x;
   const uint4* vecs;
@@ -323,18 +368,19 @@ template <typename T> struct Row {
   float mine;           // this thread's maximum
   float m, c;
 
-  __device__ __forceinline__ Row(RowShared& s, uint4* d, const RowArgs& a, uint32_t row)
+  // CTA `part` of the `parts` of a row; d: where it keeps its part (null: nowhere).
+  __device__ __forceinline__ Row(RowShared& s, uint4* d, const RowArgs& a, uint32_t row, uint32_t part, uint32_t parts)
       : cluster(cg::this_cluster()),
         sh(s),
         data(d),
         tid(threadIdx.x),
         lane(threadIdx.x & 31),
         wid(threadIdx.x >> 5),
-        rank(cluster.block_rank()),
-        ctas(cluster.num_blocks()) {
+        rank(part),
+        ctas(parts),
+        again(a.only != nullptr) {
     sh.edge_n[tid] = 0;
     if (tid == 0) sh.count = 0, sh.first = ~0u;
-    cluster.barrier_arrive();  // waited for in load(): no CTA writes into one that has not started
     x = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
     cols = a.cols;
     part_vecs = a.part_vecs;
@@ -380,6 +426,7 @@ template <typename T> struct Row {
   // nothing but its own copies has to be waited for.
   // With `tops`, the warps also publish their threads' largest maxima.
   __device__ __forceinline__ void load(bool tops) {
+    cluster.barrier_arrive();  // waited for below: no CTA writes into one that has not started
     const uint32_t p0 = min(rank * part_vecs, total_vecs);
     stretch(rank, wid, seg0, seg1);
     seg0 -= p0, seg1 -= p0;
@@ -404,19 +451,7 @@ template <typename T> struct Row {
       }
       mine = E::value(top);
     }
-    // the warp's maxima in ascending order of key: lane 0 has the largest entry
-    uint32_t k = row_key(mine);
-    if (tops) {
-#pragma unroll
-      for (int n = 2; n <= 32; n <<= 1)
-#pragma unroll
-        for (int d = n >> 1; d; d >>= 1) {
-          const uint32_t o = __shfl_xor_sync(~0u, k, d);
-          k = ((lane & d) == 0) == ((lane & n) == 0) ? min(k, o) : max(k, o);
-        }
-    } else {
-      k = __reduce_min_sync(~0u, k);
-    }
+    const uint32_t k = tops ? sorted_tops() : __reduce_min_sync(~0u, row_key(mine));
     cluster.barrier_wait();
     const uint32_t per = top_count();
     for (uint32_t i0 = 0; i0 < per * ctas; i0 += 32) {
@@ -424,10 +459,41 @@ template <typename T> struct Row {
       if (to < ctas && (tops || e == 0)) *cluster.map_shared_rank(&sh.tops[(rank * ROW_WARPS + wid) * per + e], to) = v;
     }
     cluster.sync();
+    find_max();
+  }
+  // The keys of the warp's thread maxima in ascending order: lane 0 has the
+  // largest entry's.
+  __device__ __forceinline__ uint32_t sorted_tops() const {
+    uint32_t k = row_key(mine);
+#pragma unroll
+    for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+      for (int d = n >> 1; d; d >>= 1) {
+        const uint32_t o = __shfl_xor_sync(~0u, k, d);
+        k = ((lane & d) == 0) == ((lane & n) == 0) ? min(k, o) : max(k, o);
+      }
+    return k;
+  }
+  // The row's maximum from the published ones.
+  __device__ __forceinline__ void find_max() {
     uint32_t best = ~0u;
-    for (uint32_t i = lane; i < ctas * ROW_WARPS; i += 32) best = min(best, sh.tops[i * per]);
+    for (uint32_t i = lane; i < ctas * ROW_WARPS; i += 32) best = min(best, sh.tops[i * top_count()]);
     m = row_unkey(__reduce_min_sync(~0u, best));
   }
+  // The edge of the candidates of a cut; infinity where they are too many to list.
+  __device__ __forceinline__ float edge_for(const RowParams& q) {
+    if (q.by_k || q.by_p) {
+      const uint32_t want = q.by_k ? q.k : ROW_NUCLEUS_GUESS;
+      return want <= most_tops() ? edge_of(want, ROW_EDGE_SCALE * c, mass_end()) : INFINITY;
+    }
+    return fmaxf(m + (log2f(q.least_w) - 0x1p-10f) / c - fabsf(m) * 0x1p-21f, mass_end());
+  }
+  __device__ __forceinline__ float edge_for_best(uint32_t n) {
+    if (n > most_tops()) return INFINITY;
+    const float edge = edge_of(n, ROW_EDGE_SCALE * ROW_LOG2E, -ROW_F32_MAX);
+    return edge == -ROW_F32_MAX ? edge_of(n, far_scale(), -ROW_F32_MAX) : edge;
+  }
+  __device__ __forceinline__ uint32_t most_tops() const { return top_count() * ctas * ROW_WARPS * 3 / 4; }
   // How many of its 32 sorted thread maxima a warp publishes.
   __device__ __forceinline__ uint32_t top_count() const { return min(32u, (uint32_t)ROW_TOPS / (ctas * ROW_WARPS)); }
 
@@ -470,14 +536,13 @@ template <typename T> struct Row {
   // packed additions, a half of one packed multiplication, the exponential and
   // one integer addition.  A thread holds fewer than 2^9 entries, so that
   // neither 32-bit sum of hi < 2^23 or |lo| <= 2^17 wraps.
-  template <bool ABOVE, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, F f) const {
-    const uint64_t m2 = f2_pack(-m, -m), c2 = f2_pack(c, c), one = f2_pack(1.0f, 1.0f), none = f2_pack(-1.0f, -1.0f),
-                   magic = f2_pack(ROW_MAGIC, ROW_MAGIC);
+  struct Sum {
+    uint64_t m2, c2;
     uint32_t hi = 0, lo = 0, n = 0;
-#pragma unroll 2
-    for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
+    __device__ __forceinline__ Sum(float m, float c) : m2(f2_pack(-m, -m)), c2(f2_pack(c, c)) {}
+    template <bool ABOVE> __device__ __forceinline__ void add(const uint4& v, float over) {
+      const uint64_t one = f2_pack(1.0f, 1.0f), none = f2_pack(-1.0f, -1.0f), magic = f2_pack(ROW_MAGIC, ROW_MAGIC);
       float z[N];
-      const uint4 v = data[i];
       E::get(v, z);
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
@@ -494,9 +559,20 @@ template <typename T> struct Row {
         lo += __float_as_uint(b0) + __float_as_uint(b1);
       }
       n += N;
+    }
+    __device__ __forceinline__ uint64_t mass() const {
+      return row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
+    }
+  };
+  template <bool ABOVE, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, F f) const {
+    Sum sum(m, c);
+#pragma unroll 2
+    for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
+      const uint4 v = data[i];
+      sum.template add<ABOVE>(v, over);
       if (ABOVE) each_of(hits(v, low, over), i, f);
     }
-    return row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
+    return sum.mass();
   }
   __device__ __forceinline__ uint64_t weigh() const {
     return weigh<false>(0.0f, 0.0f, [](float, int) {});
@@ -666,6 +742,10 @@ template <typename T> struct Row {
   // The end of the cluster's common work: true on the first CTA, once the
   // others' writes into it are there; the others are done.
   __device__ __forceinline__ bool last_part() {
+    if (again) {  // another row follows
+      cluster.sync();
+      return rank == 0;
+    }
     cluster.barrier_arrive();
     if (rank) return false;
     cluster.barrier_wait();
@@ -693,6 +773,69 @@ template <typename T> struct Row {
       lo += (f - 1) * step + 1;
     }
     return lo;
+  }
+
+  // A vector's entries by bin of 1/42 octave: their number, or their weights as
+  // 4096 2^-(y - b) / 42 by the power's tangent, made a whole number by another
+  // addition of 2^23.
+  __device__ __forceinline__ void count_bins(const uint4& v, bool by_mass, float c42) const {
+    float z[N];
+    E::get(v, z);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float y = place_of(z[e], c42);
+      const float b = __fadd_rn(fminf(y, (float)(ROW_BINS - 1)), 0x1p23f);
+      const float w = __fmaf_rn(__fsub_rn(y, __fsub_rn(b, 0x1p23f)), -4096.0f * ROW_LN2 / ROW_BIN_SCALE, 0x1p23f + 4096.0f);
+      smem_add_if(by_mass ? y < ROW_MASS_END * ROW_BIN_SCALE : z[e] > -INFINITY, &sh.bins[__float_as_uint(b) & 0x7fffffu],
+                  by_mass ? __float_as_uint(w) & 0x7fffffu : 1u);
+    }
+  }
+  // From the bins' sums over the row, by one CTA: warp 0 gets the first entry
+  // of the interval that the prefix ends in, warp 1 its last.  sh.b1 = sh.b2 =
+  // ~0 and sh.last = 0 before; sh.above: entries before the interval (counts).
+  // The prefix ends in b1 or later, and in b2 or before: where a sum of
+  // estimates, 2^-12 of it and in the first round 2^-20 of the largest weight
+  // added, and taken off, reaches the goal.  (An estimate is off by half a unit
+  // of 4060 and less than 2^-14; the weights' rounding to q by at most 2^-22
+  // together; from the second round on estimates follow q.  Counts are exact.)
+  // Else it ends in the last bin with anything; a count that is not reached,
+  // beyond all of them.
+  __device__ __forceinline__ uint64_t end_of(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n,
+                                             float top_w, float c42, int shift, uint64_t lo, uint64_t hi) {
+    constexpr int PER = ROW_BINS / ROW_THREADS;
+    float s[PER], own = 0, all;
+    uint32_t filled = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int b = tid * PER + i;
+      s[i] = (float)sh.bins[b];
+      if (s[i] > 0.0f) filled = b;
+      if (by_mass) s[i] *= by_weight ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w;
+      own += s[i];
+    }
+    filled = __reduce_max_sync(~0u, filled);
+    if (lane == 0) atomicMax(&sh.last, filled);
+    float run = block_scan(own, reinterpret_cast<float*>(sh.scan_n), all);
+    const float slack = by_mass ? 0x1p-12f : 0.0f, more = by_mass && first_round ? 0x1p-8f : 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool last = tid * PER + i == ROW_BINS - 1;
+      if (run < goal && (run + s[i] >= goal || last)) sh.above = above_n + (uint32_t)run;  // read for counts alone
+      run += s[i];
+      if (run * (1.0f + slack) + more >= goal) atomicMin(&sh.b1, (uint32_t)(tid * PER + i));
+      if (run * (1.0f - slack) - more >= goal) atomicMin(&sh.b2, (uint32_t)(tid * PER + i));
+    }
+    __syncthreads();
+    if (wid >= 2) return 0;
+    const uint32_t end = by_mass ? sh.last : (uint32_t)ROW_BINS - 1;
+    const uint32_t b = wid ? min(sh.b2, end) + 1 : min(sh.b1, end);
+    uint64_t at;
+    if (by_weight)
+      at = b < (uint32_t)ROW_BINS ? max(lo, (uint64_t)first_key(b, c42) << ROW_IDX_BITS) : hi + 1;
+    else
+      at = lo + ((uint64_t)b << shift);
+    at = min(at, hi + 1);
+    return wid ? at - 1 : at;
   }
 
   // Finds an interval [sh.lo, sh.hi] of (key, index) order, with at most
@@ -731,19 +874,7 @@ template <typename T> struct Row {
       const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), c42)) >= bin_at(place_of(value_of(lo), c42)) + 3);
       if (round == 0) {
 #pragma unroll 2
-        for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
-          float z[N];
-          E::get(data[i], z);
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float y = place_of(z[e], c42);
-            // 2^-(y - b) / 42 by its tangent, as a whole number by another such addition
-            const float b = __fadd_rn(fminf(y, (float)(ROW_BINS - 1)), 0x1p23f);
-            const float v = __fmaf_rn(__fsub_rn(y, __fsub_rn(b, 0x1p23f)), -4096.0f * ROW_LN2 / ROW_BIN_SCALE, 0x1p23f + 4096.0f);
-            smem_add_if(by_mass ? y < ROW_MASS_END * ROW_BIN_SCALE : z[e] > -INFINITY, &sh.bins[__float_as_uint(b) & 0x7fffffu],
-                        by_mass ? __float_as_uint(v) & 0x7fffffu : 1u);
-          }
-        }
+        for (uint32_t i = seg0 + lane; i < seg1; i += 32) count_bins(data[i], by_mass, c42);
       } else {
         between(value_of(hi), value_of(lo), [&](float z, int j) {
           const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
@@ -772,47 +903,11 @@ template <typename T> struct Row {
       }
       cluster.sync();
       if (rank == 0) {
-        // the prefix ends in b1 or later, and in b2 or before: where a sum of estimates, 2^-12 of it and 2^-20 of the
-        // largest weight added, and taken off, reaches the target.  (An estimate is off by half a unit of 4060 and less
-        // than 2^-14; the weights' rounding to q by at most 2^-22 together, and the target is no less than the largest
-        // weight; from the second round on they follow q.  Counts are exact.)  Else it ends in the last bin with
-        // anything; a count that is not reached, beyond all of them.
-        constexpr int PER = ROW_BINS / ROW_THREADS;
-        float s[PER], own = 0, all;
-        uint32_t filled = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int b = tid * PER + i;
-          s[i] = (float)sh.bins[b];
-          if (s[i] > 0.0f) filled = b;
-          if (by_mass) s[i] *= by_weight ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w;
-          own += s[i];
-        }
-        filled = __reduce_max_sync(~0u, filled);
-        if (lane == 0) atomicMax(&sh.last, filled);
-        float run = block_scan(own, reinterpret_cast<float*>(sh.scan_n), all);
         const float goal = by_mass ? (float)(target - above_q) * 0x1p-28f : (float)(target - above_n);
-        const float slack = by_mass ? 0x1p-12f : 0.0f, more = by_mass && round == 0 ? 0x1p-8f : 0.0f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const bool last = tid * PER + i == ROW_BINS - 1;
-          if (run < goal && (run + s[i] >= goal || last)) sh.above = above_n + (uint32_t)run;  // read for counts alone
-          run += s[i];
-          if (run * (1.0f + slack) + more >= goal) atomicMin(&sh.b1, (uint32_t)(tid * PER + i));
-          if (run * (1.0f - slack) - more >= goal) atomicMin(&sh.b2, (uint32_t)(tid * PER + i));
-        }
-        __syncthreads();
-        if (wid < 2) {  // the interval's ends
-          const uint32_t end = by_mass ? sh.last : (uint32_t)ROW_BINS - 1;
-          const uint32_t b = wid ? min(sh.b2, end) + 1 : min(sh.b1, end);
-          uint64_t at;
-          if (by_weight)
-            at = b < (uint32_t)ROW_BINS ? max(lo, (uint64_t)first_key(b, c42) << ROW_IDX_BITS) : hi + 1;
-          else
-            at = lo + ((uint64_t)b << shift);
-          at = min(at, hi + 1);
+        const uint64_t at = end_of(by_mass, by_weight, round == 0, goal, above_n, top_w, c42, shift, lo, hi);
+        if (wid < 2) {
           if (lane < (int)ctas) {
-            *cluster.map_shared_rank(wid ? &sh.hi : &sh.lo, lane) = wid ? at - 1 : at;
+            *cluster.map_shared_rank(wid ? &sh.hi : &sh.lo, lane) = at;
             if (wid && lane) *cluster.map_shared_rank(&sh.above, lane) = sh.above;
           }
         }
@@ -1025,6 +1120,118 @@ template <typename T> struct Row {
     }
   }
 
+  // The same for n <= ROW_LIST entries, at f.loose where they are no more than
+  // the threads, else at f.input, above `edge`: by sorting.
+  template <typename H>
+  __device__ __forceinline__ void finish_listed(RowFinish& f, uint32_t n, float edge, const RowParams& q, uint64_t total, H hit) {
+    if (n <= (uint32_t)ROW_THREADS) {
+      finish_few(f, n, q.by_k ? q.k : 0, q.p, q.least_w, q.u, total, hit);
+      return;
+    }
+    order_by_value(f, f.input, n, edge);
+    // running masses in descending order, `per` entries a thread
+    const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    uint64_t sum = 0, all;
+    for (uint32_t i = i0; i < i1; ++i) sum += mass(value_of(f.sorted[i]));
+    const uint64_t before = block_scan(sum, sh.scan_q, all);
+    if (tid == 0) sh.cut_n = n, sh.cut_q = q.by_k ? all : total;
+    __syncthreads();
+    uint64_t run = before;
+    if (q.by_k && n > q.k) {
+      for (uint32_t i = i0; i < i1; ++i) {
+        run += mass(value_of(f.sorted[i]));
+        if (i == q.k - 1) sh.cut_n = q.k, sh.cut_q = run;
+      }
+      __syncthreads();
+    }
+    uint32_t cut = sh.cut_n;
+    if (q.by_p) {
+      const uint64_t target = row_target(q.p, sh.cut_q);
+      __syncthreads();
+      run = before;
+      for (uint32_t i = i0; i < i1 && i < cut; ++i) {
+        const uint64_t qi = mass(value_of(f.sorted[i]));
+        if (run < target && target <= run + qi) sh.cut_n = i + 1, sh.cut_q = run + qi;
+        run += qi;
+      }
+      __syncthreads();
+      cut = sh.cut_n;
+    }
+    uint64_t left = sh.cut_q;
+    if (q.by_w) {
+      sum = 0;
+      for (uint32_t i = tid; i < cut; i += ROW_THREADS) {
+        const float w = weight(value_of(f.sorted[i]));
+        if (w >= q.least_w) sum += row_q(w);
+      }
+      __syncthreads();
+      block_scan(sum, sh.scan_q, left);
+    }
+    draw(f, cut, q.least_w, row_draw(q.u, left), hit);
+  }
+
+  // Cuts the n entries in sh.pool, those of [sh.lo, sh.hi], where the prefix of
+  // `target` of them (by_p: of mass `target` with what sh.mass holds) ends, and
+  // adds the kept ones' masses to their stretches' in sh.part.  Returns the
+  // last entry of the cut.
+  __device__ __forceinline__ uint64_t finish_pool(RowFinish& f, uint32_t n, const RowParams& p, uint64_t target) {
+    const uint64_t lo = sh.lo, hi = sh.hi, above = handed(sh.mass);
+    order_by_place(f, sh.pool, n, lo, hi);
+    uint32_t cut = n;
+    if (p.by_p) {
+      const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+      uint64_t sum = 0, all;
+      for (uint32_t i = i0; i < i1; ++i) sum += mass(value_of(f.sorted[i]));
+      uint64_t run = above + block_scan(sum, sh.scan_q, all);
+      if (tid == 0) sh.cut_n = n;
+      __syncthreads();
+      for (uint32_t i = i0; i < i1; ++i) {
+        const uint64_t q = mass(value_of(f.sorted[i]));
+        if (run < target && target <= run + q) sh.cut_n = i + 1;
+        run += q;
+      }
+      __syncthreads();
+      cut = sh.cut_n;
+    } else {
+      cut = (uint32_t)min((uint64_t)n, target);
+    }
+    const uint64_t last = cut ? f.sorted[cut - 1] : hi;
+    // the warps' kept masses: before the interval, and those of its entries
+    if (tid < ROW_MAX_CLUSTER * ROW_WARPS) f.part[tid][0] = f.part[tid][1] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < cut; i += ROW_THREADS) {
+      const uint64_t e = f.sorted[i];
+      const float w = weight(value_of(e));
+      const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + lead) / N;
+      const uint32_t cta = v / part_vecs, p0 = cta * part_vecs, p1 = min(p0 + part_vecs, total_vecs);
+      const uint32_t warp = (v - p0) / ((p1 - p0 + ROW_WARPS - 1) / ROW_WARPS);
+      if (w >= p.least_w) {
+        const uint64_t q = row_q(w);
+        atomicAdd(&f.part[cta * ROW_WARPS + warp][0], (uint32_t)q & 0xfffffu);
+        atomicAdd(&f.part[cta * ROW_WARPS + warp][1], (uint32_t)(q >> 20));
+      }
+    }
+    __syncthreads();
+    if (tid < ROW_MAX_CLUSTER * ROW_WARPS) (&sh.part[0][0])[tid] += ((uint64_t)f.part[tid][1] << 20) + f.part[tid][0];
+    __syncthreads();
+    return last;
+  }
+
+  // Writes the first `have` of f.sorted as the row's best.
+  __device__ __forceinline__ void put_best(const RowArgs& a, uint32_t row, const RowFinish& f, uint32_t have, float ln) const {
+    for (int i = tid; i < a.n; i += ROW_THREADS) {
+      const bool in = i < (int)have;
+      const uint64_t e = in ? f.sorted[i] : 0;
+      a.best_idx[(int64_t)row * a.n + i] = in ? (int)(e & (ROW_MAX_COLS - 1)) : -1;
+      a.best_logprob[(int64_t)row * a.n + i] = in ? (value_of(e) - m) - ln : -INFINITY;
+    }
+  }
+  __device__ __forceinline__ void put_nothing(const RowArgs& a, uint32_t row) const {
+    for (int i = tid; i < a.n; i += ROW_THREADS)
+      a.best_idx[(int64_t)row * a.n + i] = -1, a.best_logprob[(int64_t)row * a.n + i] = -INFINITY;
+    if (a.lse && tid == 0) a.lse[row] = -INFINITY;
+  }
+
   // ---- over the row in memory, by one CTA ----
   // The entry of vectors [v0, v1) at which the running sum of value(x, index)
   // exceeds t calls hit(x, index), on one thread.
@@ -1097,23 +1304,11 @@ template <typename T> struct Row {
 //
 // A cut that does not end among the candidates (a nucleus beyond the guess,
 // a large top_k, many equal values) keeps the cluster to narrow it down.
-template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k_row_sample(const RowArgs a) {
-  extern __shared__ __align__(16) unsigned char row_smem[];
-  RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
-  uint4* const data = reinterpret_cast<uint4*>(row_smem + ROW_SHARED_BYTES);
+template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, RowShared& sh, uint4* data) {
   RowFinish& f = *reinterpret_cast<RowFinish*>(data);
-  const uint32_t row = blockIdx.x / cg::this_cluster().num_blocks();
-  Row<T> r(sh, data, a, row);
-  const float t = a.temperature ? a.temperature[row] : 1.0f;
-  const int k_arg = a.top_k ? a.top_k[row] : 0;
-  const float p = a.top_p ? a.top_p[row] : 1.0f;
-  const float least_w = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
-  const float u = a.uniform[row];
-  const bool greedy = !(t > 0.0f);
-  const bool by_k = !greedy && k_arg > 0 && (uint32_t)k_arg < a.cols, by_p = !greedy && p < 1.0f;
-  const bool by_w = !greedy && least_w > 0.0f;
-  const uint32_t k = (uint32_t)k_arg;
-  r.load(by_k || by_p);
+  Row<T> r(sh, data, a, row, cg::this_cluster().block_rank(), cg::this_cluster().num_blocks());
+  const RowParams q(a, row);
+  r.load(q.by_k || q.by_p);
   if (r.m == -INFINITY) {
     if (r.rank == 0 && r.tid == 0) {
       a.tokens[row] = -1;
@@ -1121,40 +1316,34 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k
     }
     return;
   }
-  // within the finite numbers above 0: 0 * c and (max + inf) * c stay what they are for the smallest and infinite t
-  r.c = greedy ? ROW_LOG2E : fminf(fmaxf(__fdiv_rn(ROW_LOG2E, t), 1.175494351e-38f), ROW_F32_MAX);
-
+  r.c = q.c();
+  const uint32_t k = q.k;
+  const float least_w = q.least_w;
   uint64_t total = 0;
   auto store = [&](float z, int j) {
     a.tokens[row] = j;
     if (a.logprobs) a.logprobs[row] = row_neg_y(z, r.m, r.c) * ROW_LN2 - logf((float)total * 0x1p-40f);
   };
-  if (greedy)
+  if (q.greedy)
     r.above(r.m, [&](float, int j) { atomicMin(r.cluster.map_shared_rank(&sh.first, 0), (uint32_t)j); });
   const uint64_t own = r.weigh();
-  if (!by_k && !by_p && !by_w) {
+  if (!q.cuts()) {
     r.template hand<false>(sh.mass, own);
     if (!r.last_part()) return;
     total = r.handed(sh.mass);
-    if (!greedy)
-      r.scan_parts(sh.mass, row_draw(u, total), [&](float z, int) { return r.mass(z); }, store);
+    if (!q.greedy)
+      r.scan_parts(sh.mass, row_draw(q.u, total), [&](float z, int) { return r.mass(z); }, store);
     else if (r.tid == 0)
       store(r.m, (int)sh.first);
     return;
   }
 
   // ---- candidates ----
-  float edge;
-  if (by_k || by_p) {
-    const uint32_t want = by_k ? k : ROW_NUCLEUS_GUESS;
-    edge = want <= r.top_count() * r.ctas * ROW_WARPS * 3 / 4 ? r.edge_of(want, ROW_EDGE_SCALE * r.c, r.mass_end()) : INFINITY;
-  } else {
-    edge = fmaxf(r.m + (log2f(least_w) - 0x1p-10f) / r.c - fabsf(r.m) * 0x1p-21f, r.mass_end());
-  }
+  const float edge = r.edge_for(q);
   r.template hand<true>(sh.mass, own);
   if (edge < INFINITY) {
     r.collect_above(edge);
-    if (by_p && !by_k) {
+    if (q.by_p && !q.by_k) {
       uint64_t part = 0;
       for (uint32_t i = r.tid; i < min(sh.count, r.share()); i += ROW_THREADS) part += r.mass(r.value_of(sh.list[i]));
       r.template hand<true>(sh.part, part);
@@ -1165,72 +1354,28 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k
   bool enough = false;
   if (edge < INFINITY) {
     enough = r.all_listed(n);
-    if (by_k && enough && r.rank) return;
+    if (q.by_k && enough && r.rank) return;
   }
   total = r.handed(sh.mass);
-  if (enough && !by_k && by_p) enough = r.handed(sh.part) >= row_target(p, total);
+  if (enough && !q.by_k && q.by_p) enough = r.handed(sh.part) >= row_target(q.p, total);
   if (enough) {
     if (r.rank) return;
-    if (n <= (uint32_t)ROW_THREADS) {
-      r.each_listed([&](uint32_t i, uint64_t e) { f.loose[i] = e; });
-      __syncthreads();
-      r.finish_few(f, n, by_k ? k : 0, p, least_w, u, total, store);
-      return;
-    }
-    r.each_listed([&](uint32_t i, uint64_t e) { f.input[i] = e; });
+    uint64_t* const to = n <= (uint32_t)ROW_THREADS ? f.loose : f.input;
+    r.each_listed([&](uint32_t i, uint64_t e) { to[i] = e; });
     __syncthreads();
-    r.order_by_value(f, f.input, n, edge);
-    // running masses in descending order, `per` entries a thread
-    const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(r.tid * per, n), i1 = min(i0 + per, n);
-    uint64_t sum = 0, all;
-    for (uint32_t i = i0; i < i1; ++i) sum += r.mass(r.value_of(f.sorted[i]));
-    const uint64_t before = r.block_scan(sum, sh.scan_q, all);
-    if (r.tid == 0) sh.cut_n = n, sh.cut_q = by_k ? all : total;
-    __syncthreads();
-    uint64_t run = before;
-    if (by_k && n > k) {
-      for (uint32_t i = i0; i < i1; ++i) {
-        run += r.mass(r.value_of(f.sorted[i]));
-        if (i == k - 1) sh.cut_n = k, sh.cut_q = run;
-      }
-      __syncthreads();
-    }
-    uint32_t cut = sh.cut_n;
-    if (by_p) {
-      const uint64_t target = row_target(p, sh.cut_q);
-      __syncthreads();
-      run = before;
-      for (uint32_t i = i0; i < i1 && i < cut; ++i) {
-        const uint64_t q = r.mass(r.value_of(f.sorted[i]));
-        if (run < target && target <= run + q) sh.cut_n = i + 1, sh.cut_q = run + q;
-        run += q;
-      }
-      __syncthreads();
-      cut = sh.cut_n;
-    }
-    uint64_t mass = sh.cut_q;
-    if (by_w) {
-      sum = 0;
-      for (uint32_t i = r.tid; i < cut; i += ROW_THREADS) {
-        const float w = r.weight(r.value_of(f.sorted[i]));
-        if (w >= least_w) sum += row_q(w);
-      }
-      __syncthreads();
-      r.block_scan(sum, sh.scan_q, mass);
-    }
-    r.draw(f, cut, least_w, row_draw(u, mass), store);
+    r.finish_listed(f, n, edge, q, total, store);
     return;
   }
 
   // ---- a cut beyond the candidates ----
   uint64_t last = ~0ull;  // the last entry of the cut
-  if (by_k || by_p) {
+  if (q.by_k || q.by_p) {
     uint32_t above_n;
     uint64_t target = k;
-    if (by_k) r.narrow(false, k, least_w, by_p ? ROW_FEW : ROW_POOL, n, above_n);
-    if (by_p) {
+    if (q.by_k) r.narrow(false, k, least_w, q.by_p ? ROW_FEW : ROW_POOL, n, above_n);
+    if (q.by_p) {
       uint64_t mass = total;
-      if (by_k) {
+      if (q.by_k) {
         if (!r.rank) {  // the mass of the top k
           const uint64_t above = r.handed(sh.mass);
           r.cluster.barrier_arrive();  // the others' entries
@@ -1245,48 +1390,11 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k
         r.cluster.sync();
         mass = sh.cut_q;
       }
-      target = row_target(p, mass);
+      target = row_target(q.p, mass);
       r.narrow(true, target, least_w, ROW_POOL, n, above_n);
     }
     if (!r.last_part()) return;
-    const uint64_t lo = sh.lo, hi = sh.hi, above = r.handed(sh.mass);
-    r.order_by_place(f, sh.pool, n, lo, hi);
-    uint32_t cut = n;
-    if (by_p) {
-      const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(r.tid * per, n), i1 = min(i0 + per, n);
-      uint64_t sum = 0, all;
-      for (uint32_t i = i0; i < i1; ++i) sum += r.mass(r.value_of(f.sorted[i]));
-      uint64_t run = above + r.block_scan(sum, sh.scan_q, all);
-      if (r.tid == 0) sh.cut_n = n;
-      __syncthreads();
-      for (uint32_t i = i0; i < i1; ++i) {
-        const uint64_t q = r.mass(r.value_of(f.sorted[i]));
-        if (run < target && target <= run + q) sh.cut_n = i + 1;
-        run += q;
-      }
-      __syncthreads();
-      cut = sh.cut_n;
-    } else {
-      cut = min(n, k - above_n);
-    }
-    last = cut ? f.sorted[cut - 1] : hi;
-    // the warps' kept masses: before the interval, and those of its entries
-    if (r.tid < ROW_MAX_CLUSTER * ROW_WARPS) f.part[r.tid][0] = f.part[r.tid][1] = 0;
-    __syncthreads();
-    for (uint32_t i = r.tid; i < cut; i += ROW_THREADS) {
-      const uint64_t e = f.sorted[i];
-      const float w = r.weight(r.value_of(e));
-      const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + r.lead) / Row<T>::N;
-      const uint32_t cta = v / r.part_vecs, p0 = cta * r.part_vecs, p1 = min(p0 + r.part_vecs, r.total_vecs);
-      const uint32_t warp = (v - p0) / ((p1 - p0 + ROW_WARPS - 1) / ROW_WARPS);
-      if (w >= least_w) {
-        const uint64_t q = row_q(w);
-        atomicAdd(&f.part[cta * ROW_WARPS + warp][0], (uint32_t)q & 0xfffffu);
-        atomicAdd(&f.part[cta * ROW_WARPS + warp][1], (uint32_t)(q >> 20));
-      }
-    }
-    __syncthreads();
-    if (r.tid < ROW_MAX_CLUSTER * ROW_WARPS) (&sh.part[0][0])[r.tid] += ((uint64_t)f.part[r.tid][1] << 20) + f.part[r.tid][0];
+    last = r.finish_pool(f, n, q, q.by_p ? target : k - above_n);
   } else {  // min_p alone
     uint64_t kept = 0;
     r.each([&](float z, int) {
@@ -1298,7 +1406,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k
     if (!r.last_part()) return;
   }
   __syncthreads();
-  r.scan_parts(sh.part, row_draw(u, r.handed(sh.part)),
+  r.scan_parts(sh.part, row_draw(q.u, r.handed(sh.part)),
                [&](float z, int j) -> uint64_t {
                  const float w = r.weight(z);
                  return w >= least_w && ((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) <= last ? row_q(w) : 0;
@@ -1308,32 +1416,20 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k
 
 // ---- the n best ---------------------------------------------------------------------
 // As a sampling row with top_k = n, whose ordered candidates are the answer.
-template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k_row_best(const RowArgs a) {
-  extern __shared__ __align__(16) unsigned char row_smem[];
-  RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
-  uint4* const data = reinterpret_cast<uint4*>(row_smem + ROW_SHARED_BYTES);
+template <typename T> __device__ __forceinline__ void row_best(const RowArgs& a, uint32_t row, RowShared& sh, uint4* data) {
   RowFinish& f = *reinterpret_cast<RowFinish*>(data);
-  const uint32_t row = blockIdx.x / cg::this_cluster().num_blocks();
-  Row<T> r(sh, data, a, row);
+  Row<T> r(sh, data, a, row, cg::this_cluster().block_rank(), cg::this_cluster().num_blocks());
   r.load(true);
-  int* const out_idx = a.best_idx + (int64_t)row * a.n;
-  float* const out_lp = a.best_logprob + (int64_t)row * a.n;
   if (r.m == -INFINITY) {
-    if (r.rank == 0) {
-      for (int i = r.tid; i < a.n; i += ROW_THREADS) out_idx[i] = -1, out_lp[i] = -INFINITY;
-      if (a.lse && r.tid == 0) a.lse[row] = -INFINITY;
-    }
+    if (r.rank == 0) r.put_nothing(a, row);
     return;
   }
   r.c = ROW_LOG2E;
   const uint32_t k = (uint32_t)a.n;
   float edge = INFINITY;
   r.template hand<true>(sh.mass, r.weigh());
-  if (k <= r.top_count() * r.ctas * ROW_WARPS * 3 / 4) {
-    edge = r.edge_of(k, ROW_EDGE_SCALE * ROW_LOG2E, -ROW_F32_MAX);
-    if (edge == -ROW_F32_MAX) edge = r.edge_of(k, r.far_scale(), -ROW_F32_MAX);
-    r.collect_above(edge);
-  }
+  edge = r.edge_for_best(k);
+  if (edge < INFINITY) r.collect_above(edge);
   r.cluster.sync();
   uint32_t n = 0;
   const bool listed = edge < INFINITY && r.all_listed(n);
@@ -1369,12 +1465,21 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k
   }
   if (a.lse && r.tid == 0) a.lse[row] = r.m + ln;
   r.order_by_value(f, from, n, edge);
-  const uint32_t have = min(n, k);
-  for (int i = r.tid; i < a.n; i += ROW_THREADS) {
-    const bool in = i < (int)have;
-    const uint64_t e = in ? f.sorted[i] : 0;
-    out_idx[i] = in ? (int)(e & (ROW_MAX_COLS - 1)) : -1;
-    out_lp[i] = in ? (r.value_of(e) - r.m) - ln : -INFINITY;
+  r.put_best(a, row, f, min(n, k), ln);
+}
+
+// One cluster a row, or the listed rows in turn.
+template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k_rows(const RowArgs a) {
+  extern __shared__ __align__(16) unsigned char row_smem[];
+  RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
+  uint4* const data = reinterpret_cast<uint4*>(row_smem + ROW_SHARED_BYTES);
+  const uint32_t ctas = cg::this_cluster().num_blocks(), id = blockIdx.x / ctas;
+  if (a.only) row_chain_wait();
+  const uint32_t n = a.only ? *a.only_n : a.rows, step = a.only ? gridDim.x / ctas : a.rows;
+  for (uint32_t i = id; i < n; i += step) {
+    const uint32_t row = a.only ? a.only[i] : i;
+    BEST ? row_best<T>(a, row, sh, data) : row_sample<T>(a, row, sh, data);
+    if (a.only) cg::this_cluster().sync();  // nobody's shared memory is written any more
   }
 }
 

@@ -1,0 +1,345 @@
+// fs_rows_stream.cuh -- the row operators over large batches: the same
+// definitions and the same whole numbers as fs_rows.cuh, as passes over the
+// whole batch instead of one cluster a row.
+//
+// A cluster that keeps its row in shared memory reads it from HBM once, but
+// holds that memory through the row's barriers and its ranking: three CTAs of
+// 64 KB on an SM for about 10 us each are 2 TB/s.  Passes hold nothing: any
+// number of CTAs stream the batch, and whichever CTA is the last to finish with
+// a row (an atomic counter tells) draws the conclusion for it.
+//   k_stream_max    the row's maximum and published thread maxima; the last
+//                   CTA of a row finds its candidates' edge
+//   k_stream_weigh  the sum of the weights, and the candidates; the last CTA
+//                   orders, cuts and draws.  Rows in reverse order, so that
+//                   what the first pass read last is still in L2
+//   k_stream_bins   for rows whose nucleus does not end among the candidates,
+//                   weights by bin; the last CTA finds the interval it ends in
+//   k_stream_cut    the exact mass before the interval and its entries; the
+//                   last CTA cuts and draws
+//   k_rows          (fs_rows.cuh) the rows that fit none of these
+// Reading twice costs HBM time beyond the size of L2 (126 MB), and is still
+// the faster from a few megabytes on.
+#pragma once
+
+#include "fs_rows.cuh"
+
+namespace fs {
+
+struct RowRecord {
+  float m, c, edge;
+  uint32_t dirty;       // the row has NaN or +inf
+  uint32_t done[4];     // CTAs that have finished with it, by pass
+  uint32_t list_n, pool_n, first, pad;
+  uint64_t total, lo, hi, target;
+};
+
+struct RowStream {
+  RowRecord* rec;       // a record a row, zero before the first pass
+  uint32_t* tops;       // ROW_TOPS a row
+  uint64_t* mass;       // ROW_SUMS a row: each warp's sum
+  uint64_t* part;       // ... of its kept entries
+  uint64_t* list;       // ROW_LIST a row
+  uint32_t* wide;       // rows whose nucleus is wide,
+  uint32_t* left;       // rows left to k_rows,
+  uint32_t* counts;     // and their numbers
+  uint32_t* bins;       // ROW_BINS for each wide row
+  uint64_t* pool;       // ROW_POOL for each wide row
+  uint32_t parts;       // CTAs a row
+};
+constexpr int ROW_SUMS = ROW_MAX_CLUSTER * ROW_WARPS;
+
+// Whether this CTA is the last of `parts` to get here; what the others wrote
+// is then visible.
+__device__ __forceinline__ bool row_last(uint32_t* done, uint32_t parts, uint32_t& flag) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) flag = atomicAdd(done, 1u) == parts - 1;
+  __syncthreads();
+  if (!flag) return false;
+  if (threadIdx.x == 0) *done = 0;
+  __threadfence();
+  return true;
+}
+
+// f(vector, number) for the vectors of warp r.wid's stretch of part r.rank,
+// U of them in flight.
+template <int U, typename T, typename F> __device__ __forceinline__ void row_stream(const Row<T>& r, bool dirty, F f) {
+  uint32_t v0, v1;
+  r.stretch(r.rank, r.wid, v0, v1);
+  uint32_t i = v0 + r.lane;
+  for (; i + 32 * (U - 1) < v1; i += 32 * U) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = r.inside(i + 32 * u) ? row_load(r.vecs + i + 32 * u) : r.ragged(i + 32 * u);
+#pragma unroll
+    for (int u = 0; u < U; ++u) f(dirty ? r.cleaned(v[u]) : v[u], i + 32 * u);
+  }
+  for (; i < v1; i += 32) {
+    const uint4 v = r.inside(i) ? row_load(r.vecs + i) : r.ragged(i);
+    f(dirty ? r.cleaned(v) : v, i);
+  }
+}
+// f(x, index) for the entries of a vector that mask names
+template <typename T, typename F> __device__ __forceinline__ void row_each(const Row<T>& r, uint32_t mask, const uint4& v, uint32_t i, F f) {
+  while (mask) {
+    const int e = __ffs((int)mask) - 1;
+    mask &= mask - 1;
+    f(RowElem<T>::at(v, e), (int)(i * Row<T>::N) - r.lead + e);
+  }
+}
+template <typename V> __device__ __forceinline__ V row_get(const V* p) { return __ldcg(p); }  // written by other CTAs
+
+template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream_max(const RowArgs a, const RowStream s) {
+  __shared__ RowShared sh;
+  asm volatile("griddepcontrol.launch_dependents;");
+  using E = RowElem<T>;
+  const uint32_t row = blockIdx.x / s.parts;
+  Row<T> r(sh, nullptr, a, row, blockIdx.x % s.parts, s.parts);
+  RowRecord& rec = s.rec[row];
+  bool tops = true;
+  if constexpr (!BEST) {
+    const RowParams q(a, row);
+    tops = q.by_k || q.by_p;
+  }
+  typename E::Top top = E::top0();
+  row_stream<8>(r, false, [&](const uint4& v, uint32_t) { top = E::top(top, v); });
+  r.mine = E::value(top);
+  if (!(r.mine <= ROW_F32_MAX)) {
+    rec.dirty = 1;
+    top = E::top0();
+    row_stream<1>(r, true, [&](const uint4& v, uint32_t) { top = E::top(top, v); });
+    r.mine = E::value(top);
+  }
+  __syncwarp();
+  const uint32_t key = tops ? r.sorted_tops() : __reduce_min_sync(~0u, row_key(r.mine));
+  const uint32_t per = r.top_count();
+  uint32_t* const all = s.tops + (size_t)row * ROW_TOPS;
+  if (r.lane < (int)(tops ? per : 1)) all[(r.rank * ROW_WARPS + r.wid) * per + r.lane] = key;
+  if (!row_last(&rec.done[0], s.parts, sh.found)) return;
+
+  for (uint32_t i = r.tid; i < per * s.parts * ROW_WARPS; i += ROW_THREADS) sh.tops[i] = row_get(all + i);
+  __syncthreads();
+  r.find_max();
+  float edge = INFINITY;
+  if (r.m == -INFINITY) {
+    if constexpr (BEST) {
+      r.put_nothing(a, row);
+    } else if (r.tid == 0) {
+      a.tokens[row] = -1;
+      if (a.logprobs) a.logprobs[row] = -INFINITY;
+    }
+  } else if constexpr (BEST) {
+    r.c = ROW_LOG2E;
+    edge = r.edge_for_best((uint32_t)a.n);
+  } else {
+    const RowParams q(a, row);
+    r.c = q.c();
+    if (q.greedy)
+      edge = r.m;
+    else if (q.cuts())
+      edge = r.edge_for(q);
+  }
+  if (r.tid == 0) rec.m = r.m, rec.c = r.c, rec.edge = edge, rec.first = ~0u;
+}
+
+template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream_weigh(const RowArgs a, const RowStream s) {
+  extern __shared__ __align__(16) unsigned char row_smem[];
+  RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
+  RowFinish& f = *reinterpret_cast<RowFinish*>(row_smem + ROW_SHARED_BYTES);
+  const uint32_t row = a.rows - 1 - blockIdx.x / s.parts;
+  Row<T> r(sh, nullptr, a, row, blockIdx.x % s.parts, s.parts);
+  RowRecord& rec = s.rec[row];
+  __syncthreads();
+  row_chain_wait();
+  r.m = row_get(&rec.m), r.c = row_get(&rec.c);
+  if (r.m == -INFINITY) return;
+  const float edge = row_get(&rec.edge);
+  bool greedy = false;
+  if constexpr (!BEST) greedy = a.temperature && !(a.temperature[row] > 0.0f);
+  typename Row<T>::Sum sum(r.m, r.c);
+  row_stream<4>(r, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t i) {
+    sum.template add<false>(v, 0.0f);
+    if (RowElem<T>::value(RowElem<T>::top(RowElem<T>::top0(), v)) >= edge)
+      row_each(r, r.hits(v, edge, INFINITY), v, i, [&](float z, int j) {
+        if (greedy) {
+          atomicMin(&rec.first, (uint32_t)j);
+        } else {
+          const uint32_t at = atomicAdd(&sh.count, 1u);
+          if (at < ROW_LIST) sh.list[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+        }
+      });
+  });
+  const uint64_t own = warp_sum_u64(sum.mass());
+  uint64_t* const masses = s.mass + (size_t)row * ROW_SUMS;
+  uint64_t* const list = s.list + (size_t)row * ROW_LIST;
+  if (r.lane == 0) masses[r.rank * ROW_WARPS + r.wid] = own;
+  __syncthreads();
+  uint32_t n = sh.count;
+  if (n) {
+    if (r.tid == 0) sh.found = atomicAdd(&rec.list_n, n);
+    __syncthreads();
+    const uint32_t base = sh.found;
+    for (uint32_t i = r.tid; i < min(n, (uint32_t)ROW_LIST) && base + i < ROW_LIST; i += ROW_THREADS) list[base + i] = sh.list[i];
+    __syncthreads();
+  }
+  if (!row_last(&rec.done[1], s.parts, sh.found)) return;
+
+  for (uint32_t i = r.tid; i < s.parts * ROW_WARPS; i += ROW_THREADS) (&sh.mass[0][0])[i] = row_get(masses + i);
+  __syncthreads();
+  const uint64_t total = r.handed(sh.mass);
+  n = row_get(&rec.list_n);
+  const bool listed = edge < INFINITY && n <= (uint32_t)ROW_LIST;
+  auto leave = [&] {
+    if (r.tid == 0) s.left[atomicAdd(&s.counts[1], 1u)] = row;
+  };
+  if constexpr (BEST) {
+    if (!listed) return leave();
+    const float ln = logf((float)total * 0x1p-40f);
+    if (a.lse && r.tid == 0) a.lse[row] = r.m + ln;
+    for (uint32_t i = r.tid; i < n; i += ROW_THREADS) f.input[i] = row_get(list + i);
+    __syncthreads();
+    r.order_by_value(f, f.input, n, edge);
+    r.put_best(a, row, f, min(n, (uint32_t)a.n), ln);
+  } else {
+    const RowParams q(a, row);
+    auto store = [&](float z, int j) {
+      a.tokens[row] = j;
+      if (a.logprobs) a.logprobs[row] = row_neg_y(z, r.m, r.c) * ROW_LN2 - logf((float)total * 0x1p-40f);
+    };
+    if (q.greedy) {
+      if (r.tid == 0) store(r.m, (int)row_get(&rec.first));
+      return;
+    }
+    if (!q.cuts()) {
+      r.scan_parts(sh.mass, row_draw(q.u, total), [&](float z, int) { return r.mass(z); }, store);
+      return;
+    }
+    uint64_t* const to = n <= (uint32_t)ROW_THREADS ? f.loose : f.input;
+    uint64_t part = 0, all = 0;
+    if (listed)
+      for (uint32_t i = r.tid; i < n; i += ROW_THREADS) {
+        to[i] = row_get(list + i);
+        part += r.mass(r.value_of(to[i]));
+      }
+    const uint64_t target = row_target(q.p, total);
+    if (q.by_p && !q.by_k) {
+      r.block_scan(part, sh.scan_q, all);
+      if (all < target || !listed) {  // narrow it down
+        if (r.tid == 0) sh.found = atomicAdd(&s.counts[0], 1u);
+        __syncthreads();
+        const uint32_t slot = sh.found;
+        for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS) s.bins[(size_t)slot * ROW_BINS + b] = 0;
+        if (r.tid == 0) s.wide[slot] = row, rec.total = total, rec.target = target;
+        return;
+      }
+    } else if (!listed) {
+      return leave();
+    }
+    __syncthreads();
+    r.finish_listed(f, n, edge, q, total, store);
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream_bins(const RowArgs a, const RowStream s) {
+  __shared__ RowShared sh;
+  row_chain_wait();
+  const uint32_t items = row_get(&s.counts[0]) * s.parts;
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const uint32_t slot = item / s.parts, row = row_get(&s.wide[slot]);
+    __syncthreads();
+    Row<T> r(sh, nullptr, a, row, item % s.parts, s.parts);
+    RowRecord& rec = s.rec[row];
+    r.m = row_get(&rec.m), r.c = row_get(&rec.c);
+    const float c42 = fminf(r.c * ROW_BIN_SCALE, ROW_F32_MAX);
+    for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS) sh.bins[b] = 0;
+    if (r.tid == 0) sh.b1 = sh.b2 = ~0u, sh.last = 0;
+    __syncthreads();
+    row_stream<4>(r, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t) { r.count_bins(v, true, c42); });
+    __syncthreads();
+    uint32_t* const bins = s.bins + (size_t)slot * ROW_BINS;
+    for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS)
+      if (const uint32_t v = sh.bins[b]) atomicAdd(&bins[b], v);
+    if (!row_last(&rec.done[2], s.parts, sh.found)) continue;
+    for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS) sh.bins[b] = row_get(bins + b);
+    __syncthreads();
+    const uint64_t lo = (uint64_t)row_key(r.m) << ROW_IDX_BITS,
+                   hi = (uint64_t)row_key(-ROW_F32_MAX) << ROW_IDX_BITS | (ROW_MAX_COLS - 1);
+    const uint64_t at = r.end_of(true, true, true, (float)row_get(&rec.target) * 0x1p-28f, 0, 1.0f, c42, 0, lo, hi);
+    if (r.wid < 2 && r.lane == 0) *(r.wid ? &rec.hi : &rec.lo) = at;
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_stream_cut(const RowArgs a, const RowStream s) {
+  extern __shared__ __align__(16) unsigned char row_smem[];
+  RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
+  RowFinish& f = *reinterpret_cast<RowFinish*>(row_smem + ROW_SHARED_BYTES);
+  row_chain_wait();
+  const uint32_t items = row_get(&s.counts[0]) * s.parts;
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const uint32_t slot = item / s.parts, row = row_get(&s.wide[slot]);
+    __syncthreads();
+    Row<T> r(sh, nullptr, a, row, item % s.parts, s.parts);
+    RowRecord& rec = s.rec[row];
+    const RowParams q(a, row);
+    r.m = row_get(&rec.m), r.c = row_get(&rec.c);
+    const uint64_t lo = row_get(&rec.lo), hi = row_get(&rec.hi);
+    const float over = r.value_of(lo), least = r.value_of(hi);
+    __syncthreads();
+    typename Row<T>::Sum sum(r.m, r.c);
+    uint64_t kept = 0;
+    row_stream<4>(r, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t i) {
+      sum.template add<true>(v, over);
+      row_each(r, r.hits(v, least, over), v, i, [&](float z, int j) {
+        const uint32_t at = atomicAdd(&sh.count, 1u);
+        if (at < ROW_POOL) sh.pool[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+      });
+      if (q.by_w) {
+        float z[Row<T>::N];
+        RowElem<T>::get(v, z);
+#pragma unroll
+        for (int e = 0; e < Row<T>::N; ++e) {
+          const float w = r.weight(z[e]);
+          if (z[e] > over && w >= q.least_w) kept += row_q(w);
+        }
+      }
+    });
+    const uint64_t own = warp_sum_u64(sum.mass());
+    kept = q.by_w ? warp_sum_u64(kept) : own;
+    uint64_t* const masses = s.mass + (size_t)row * ROW_SUMS;
+    uint64_t* const parts = s.part + (size_t)row * ROW_SUMS;
+    uint64_t* const pool = s.pool + (size_t)slot * ROW_POOL;
+    if (r.lane == 0) masses[r.rank * ROW_WARPS + r.wid] = own, parts[r.rank * ROW_WARPS + r.wid] = kept;
+    __syncthreads();
+    uint32_t n = sh.count;
+    if (r.tid == 0) sh.found = atomicAdd(&rec.pool_n, n);
+    __syncthreads();
+    const uint32_t base = sh.found;
+    for (uint32_t i = r.tid; i < min(n, (uint32_t)ROW_POOL) && base + i < ROW_POOL; i += ROW_THREADS) pool[base + i] = sh.pool[i];
+    __syncthreads();
+    if (!row_last(&rec.done[3], s.parts, sh.found)) continue;
+
+    n = row_get(&rec.pool_n);
+    if (n > (uint32_t)ROW_POOL) {
+      if (r.tid == 0) s.left[atomicAdd(&s.counts[1], 1u)] = row;
+      continue;
+    }
+    for (uint32_t i = r.tid; i < s.parts * ROW_WARPS; i += ROW_THREADS)
+      (&sh.mass[0][0])[i] = row_get(masses + i), (&sh.part[0][0])[i] = row_get(parts + i);
+    for (uint32_t i = r.tid; i < n; i += ROW_THREADS) sh.pool[i] = row_get(pool + i);
+    if (r.tid == 0) sh.lo = lo, sh.hi = hi;
+    __syncthreads();
+    const uint64_t total = row_get(&rec.total);
+    const uint64_t last = r.finish_pool(f, n, q, row_get(&rec.target));
+    r.scan_parts(sh.part, row_draw(q.u, r.handed(sh.part)),
+                 [&](float z, int j) -> uint64_t {
+                   const float w = r.weight(z);
+                   return w >= q.least_w && ((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) <= last ? row_q(w) : 0;
+                 },
+                 [&](float z, int j) {
+                   a.tokens[row] = j;
+                   if (a.logprobs) a.logprobs[row] = row_neg_y(z, r.m, r.c) * ROW_LN2 - logf((float)total * 0x1p-40f);
+                 });
+  }
+}
+
+}  // namespace fs

@@ -14,10 +14,13 @@ pytestmark = pytest.mark.gpu
 DT = ["f32", "f16", "bf16"]
 
 
-@pytest.fixture(scope="module")
-def gs():
+@pytest.fixture(scope="module", params=["clusters", "passes"])
+def gs(request):
+    """Both forms for every case: one cluster a row, and passes over the batch."""
     import forge_sort
-    s = forge_sort.GpuSampler.new()
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setenv("FORGESORT_ROW_PASS_MIN_BYTES", "0" if request.param == "passes" else str(1 << 40))
+        s = forge_sort.GpuSampler.new()
     yield s
     s.close()
 
