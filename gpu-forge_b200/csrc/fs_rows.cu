@@ -33,9 +33,9 @@ constexpr uint32_t PART_MIN = 16u << 10;
 // Large batches go in passes over all rows, in groups of STREAM_ROWS rows
 // (of 25 KB of scratch each), cut into parts of STREAM_PART bytes.
 #ifndef VSPART
-#define VSPART 32
+#define VSPART 16
 #endif
-constexpr uint64_t STREAM_ROWS = 4096;
+constexpr uint64_t STREAM_ROWS = 1024;
 constexpr uint32_t STREAM_PART = VSPART << 10;
 
 uint32_t row_ctas(uint32_t vecs, uint64_t rows, int sm_count) {
@@ -103,8 +103,11 @@ template <typename T, bool BEST> int launch_clusters(fs_sorter* s, const SorterV
 template <typename T, bool BEST> int launch_passes(fs_sorter* s, const SorterView& v, RowArgs& a, int* launches) {
   const uint32_t vecs = row_vecs(a, RowElem<T>::N);
   RowStream st{};
-  st.parts = (vecs * 16 + STREAM_PART - 1) / STREAM_PART;
+  // as many parts as fill the GPU once (four CTAs an SM), of at least STREAM_PART bytes
+  st.parts = (uint32_t)v.sm_count * 4 / a.rows;
+  if (st.parts > vecs * 16 / STREAM_PART) st.parts = vecs * 16 / STREAM_PART;
   if (st.parts > ROW_MAX_CLUSTER) st.parts = ROW_MAX_CLUSTER;
+  if (st.parts < 1) st.parts = 1;
   a.part_vecs = (vecs + st.parts - 1) / st.parts;
   const bool narrows = !BEST && a.top_p;  // rows may have wide nuclei
   size_t bytes = 0;
@@ -117,7 +120,7 @@ template <typename T, bool BEST> int launch_passes(fs_sorter* s, const SorterVie
   const size_t o_rec = take(R * sizeof(RowRecord)), o_counts = take(8), zeroed = bytes;
   const size_t o_tops = take(R * ROW_TOPS * 4), o_mass = take(R * ROW_SUMS * 8), o_list = take(R * ROW_LIST * 8), o_left = take(R * 4);
   const size_t o_wide = take(narrows ? R * 4 : 0), o_part = take(narrows ? R * ROW_SUMS * 8 : 0);
-  const size_t o_bins = take(narrows ? R * ROW_BINS * 4 : 0), o_pool = take(narrows ? R * ROW_POOL * 8 : 0);
+  const size_t o_bins = take(narrows ? R * ROW_BINS * 4 : 0), o_pool = take(narrows ? R * ROW_WIDE_POOL * 8 : 0);
   void* mem = nullptr;
   FS_ROWS_CUDA(s, cudaMallocFromPoolAsync(&mem, bytes, v.pool, v.stream));
   unsigned char* const b = static_cast<unsigned char*>(mem);
@@ -143,7 +146,7 @@ template <typename T, bool BEST> int launch_passes(fs_sorter* s, const SorterVie
     if (narrows) {
       const unsigned most = (unsigned)v.sm_count * 3, few = grid < most ? grid : most;
       if (e == cudaSuccess) e = chained(v, k_stream_bins<T>, few, 0, 0, args, st);
-      if (e == cudaSuccess) e = chained(v, k_stream_cut<T>, few, FINISH_SMEM, 0, args, st);
+      if (e == cudaSuccess) e = chained(v, k_stream_cut<T>, few, ROW_SHARED_BYTES + sizeof(RowWide), 0, args, st);
       *launches += 2;
     }
   }

@@ -534,10 +534,12 @@ template <typename T> struct Row {
   // The mass of this thread's entries (ABOVE: of those over `over`, and
   // f(x, index) for those from `low` to `over`).  Per entry: a half of four
   // packed additions, a half of one packed multiplication, the exponential and
-  // one integer addition.  A thread holds fewer than 2^9 entries, so that
-  // neither 32-bit sum of hi < 2^23 or |lo| <= 2^17 wraps.
+  // one integer addition.  At most 256 entries
+  // come between folds, so that neither 32-bit sum of hi < 2^23 or |lo| <= 2^17
+  // wraps.
   struct Sum {
     uint64_t m2, c2;
+    uint64_t folded = 0;
     uint32_t hi = 0, lo = 0, n = 0;
     __device__ __forceinline__ Sum(float m, float c) : m2(f2_pack(-m, -m)), c2(f2_pack(c, c)) {}
     template <bool ABOVE> __device__ __forceinline__ void add(const uint4& v, float over) {
@@ -559,9 +561,13 @@ template <typename T> struct Row {
         lo += __float_as_uint(b0) + __float_as_uint(b1);
       }
       n += N;
+      if (n == 256) {
+        folded = mass();
+        hi = lo = n = 0;
+      }
     }
     __device__ __forceinline__ uint64_t mass() const {
-      return row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
+      return folded + row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
     }
   };
   template <bool ABOVE, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, F f) const {

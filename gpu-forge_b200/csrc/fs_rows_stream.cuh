@@ -43,10 +43,18 @@ struct RowStream {
   uint32_t* left;       // rows left to k_rows,
   uint32_t* counts;     // and their numbers
   uint32_t* bins;       // ROW_BINS for each wide row
-  uint64_t* pool;       // ROW_POOL for each wide row
+  uint64_t* pool;       // ROW_WIDE_POOL for each wide row
   uint32_t parts;       // CTAs a row
 };
 constexpr int ROW_SUMS = ROW_MAX_CLUSTER * ROW_WARPS;
+constexpr int ROW_WIDE_POOL = 4095;  // entries of a wide nucleus's last interval: below 2^12, see RowWide
+
+// The last CTA's working memory for a wide row.
+struct RowWide {
+  uint32_t sums[1024][2];  // masses by bin of the interval: of their low 20 bits, of the rest (both below 2^32)
+  uint32_t part[ROW_SUMS][2];
+  uint64_t few[ROW_THREADS], few_q[ROW_THREADS];
+};
 
 // Whether this CTA is the last of `parts` to get here; what the others wrote
 // is then visible.
@@ -157,7 +165,7 @@ template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, 
   bool greedy = false;
   if constexpr (!BEST) greedy = a.temperature && !(a.temperature[row] > 0.0f);
   typename Row<T>::Sum sum(r.m, r.c);
-  row_stream<4>(r, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t i) {
+  row_stream<8>(r, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t i) {
     sum.template add<false>(v, 0.0f);
     if (RowElem<T>::value(RowElem<T>::top(RowElem<T>::top0(), v)) >= edge)
       row_each(r, r.hits(v, edge, INFINITY), v, i, [&](float z, int j) {
@@ -240,14 +248,22 @@ template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, 
   }
 }
 
-template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream_bins(const RowArgs a, const RowStream s) {
+// Wide rows are cut anew, into as many parts as give every CTA one.
+__device__ __forceinline__ uint32_t row_wide_parts(RowArgs& a, uint32_t n, uint32_t vecs) {
+  const uint32_t parts = max(1u, min(min(gridDim.x / max(n, 1u), (uint32_t)ROW_MAX_CLUSTER), vecs / (2 * ROW_THREADS)));
+  a.part_vecs = (vecs + parts - 1) / parts;
+  return parts;
+}
+
+template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream_bins(const RowArgs args, const RowStream s) {
   __shared__ RowShared sh;
   row_chain_wait();
-  const uint32_t items = row_get(&s.counts[0]) * s.parts;
-  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const uint32_t slot = item / s.parts, row = row_get(&s.wide[slot]);
+  RowArgs a = args;
+  const uint32_t wide = row_get(&s.counts[0]), parts = row_wide_parts(a, wide, s.parts * args.part_vecs);
+  for (uint32_t item = blockIdx.x; item < wide * parts; item += gridDim.x) {
+    const uint32_t slot = item / parts, row = row_get(&s.wide[slot]);
     __syncthreads();
-    Row<T> r(sh, nullptr, a, row, item % s.parts, s.parts);
+    Row<T> r(sh, nullptr, a, row, item % parts, parts);
     RowRecord& rec = s.rec[row];
     r.m = row_get(&rec.m), r.c = row_get(&rec.c);
     const float c42 = fminf(r.c * ROW_BIN_SCALE, ROW_F32_MAX);
@@ -259,7 +275,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream
     uint32_t* const bins = s.bins + (size_t)slot * ROW_BINS;
     for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS)
       if (const uint32_t v = sh.bins[b]) atomicAdd(&bins[b], v);
-    if (!row_last(&rec.done[2], s.parts, sh.found)) continue;
+    if (!row_last(&rec.done[2], parts, sh.found)) continue;
     for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS) sh.bins[b] = row_get(bins + b);
     __syncthreads();
     const uint64_t lo = (uint64_t)row_key(r.m) << ROW_IDX_BITS,
@@ -269,16 +285,17 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream
   }
 }
 
-template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_stream_cut(const RowArgs a, const RowStream s) {
+template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_stream_cut(const RowArgs args, const RowStream s) {
   extern __shared__ __align__(16) unsigned char row_smem[];
   RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
-  RowFinish& f = *reinterpret_cast<RowFinish*>(row_smem + ROW_SHARED_BYTES);
+  RowWide& f = *reinterpret_cast<RowWide*>(row_smem + ROW_SHARED_BYTES);
   row_chain_wait();
-  const uint32_t items = row_get(&s.counts[0]) * s.parts;
-  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const uint32_t slot = item / s.parts, row = row_get(&s.wide[slot]);
+  RowArgs a = args;
+  const uint32_t wide = row_get(&s.counts[0]), parts = row_wide_parts(a, wide, s.parts * args.part_vecs);
+  for (uint32_t item = blockIdx.x; item < wide * parts; item += gridDim.x) {
+    const uint32_t slot = item / parts, row = row_get(&s.wide[slot]);
     __syncthreads();
-    Row<T> r(sh, nullptr, a, row, item % s.parts, s.parts);
+    Row<T> r(sh, nullptr, a, row, item % parts, parts);
     RowRecord& rec = s.rec[row];
     const RowParams q(a, row);
     r.m = row_get(&rec.m), r.c = row_get(&rec.c);
@@ -306,30 +323,92 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_stream
     const uint64_t own = warp_sum_u64(sum.mass());
     kept = q.by_w ? warp_sum_u64(kept) : own;
     uint64_t* const masses = s.mass + (size_t)row * ROW_SUMS;
-    uint64_t* const parts = s.part + (size_t)row * ROW_SUMS;
-    uint64_t* const pool = s.pool + (size_t)slot * ROW_POOL;
-    if (r.lane == 0) masses[r.rank * ROW_WARPS + r.wid] = own, parts[r.rank * ROW_WARPS + r.wid] = kept;
+    uint64_t* const kepts = s.part + (size_t)row * ROW_SUMS;
+    uint64_t* const pool = s.pool + (size_t)slot * ROW_WIDE_POOL;
+    if (r.lane == 0) masses[r.rank * ROW_WARPS + r.wid] = own, kepts[r.rank * ROW_WARPS + r.wid] = kept;
     __syncthreads();
     uint32_t n = sh.count;
-    if (r.tid == 0) sh.found = atomicAdd(&rec.pool_n, n);
+    if (r.tid == 0) sh.found = atomicAdd(&rec.pool_n, n <= ROW_POOL ? n : ROW_WIDE_POOL + 1);  // more is too much
     __syncthreads();
     const uint32_t base = sh.found;
-    for (uint32_t i = r.tid; i < min(n, (uint32_t)ROW_POOL) && base + i < ROW_POOL; i += ROW_THREADS) pool[base + i] = sh.pool[i];
+    for (uint32_t i = r.tid; i < min(n, (uint32_t)ROW_POOL) && base + i < ROW_WIDE_POOL; i += ROW_THREADS) pool[base + i] = sh.pool[i];
     __syncthreads();
-    if (!row_last(&rec.done[3], s.parts, sh.found)) continue;
+    if (!row_last(&rec.done[3], parts, sh.found)) continue;
 
+    // the entry of the interval at which the mass reaches the target: by bins of the interval, then among a bin's entries
     n = row_get(&rec.pool_n);
-    if (n > (uint32_t)ROW_POOL) {
+    auto leave = [&] {
       if (r.tid == 0) s.left[atomicAdd(&s.counts[1], 1u)] = row;
+    };
+    if (n > (uint32_t)ROW_WIDE_POOL) {
+      leave();
       continue;
     }
-    for (uint32_t i = r.tid; i < s.parts * ROW_WARPS; i += ROW_THREADS)
-      (&sh.mass[0][0])[i] = row_get(masses + i), (&sh.part[0][0])[i] = row_get(parts + i);
-    for (uint32_t i = r.tid; i < n; i += ROW_THREADS) sh.pool[i] = row_get(pool + i);
-    if (r.tid == 0) sh.lo = lo, sh.hi = hi;
+    for (uint32_t i = r.tid; i < parts * ROW_WARPS; i += ROW_THREADS)
+      (&sh.mass[0][0])[i] = row_get(masses + i), (&sh.part[0][0])[i] = row_get(kepts + i);
+    for (int i = r.tid; i < 1024; i += ROW_THREADS) f.sums[i][0] = f.sums[i][1] = 0;
+    if (r.tid < ROW_SUMS) f.part[r.tid][0] = f.part[r.tid][1] = 0;
+    if (r.tid == 0) sh.count = 0, sh.cut_c = hi, sh.cut_n = 1024;
     __syncthreads();
-    const uint64_t total = row_get(&rec.total);
-    const uint64_t last = r.finish_pool(f, n, q, row_get(&rec.target));
+    const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
+    for (uint32_t i = r.tid; i < n; i += ROW_THREADS) {
+      const uint64_t e = row_get(pool + i), m = r.mass(r.value_of(e));
+      uint32_t* const to = f.sums[(e - lo) >> shift];
+      atomicAdd(&to[0], (uint32_t)m & 0xfffffu);
+      atomicAdd(&to[1], (uint32_t)(m >> 20));
+    }
+    __syncthreads();
+    uint64_t b[4], t = 0, all;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t* const p = f.sums[4 * r.tid + i];
+      b[i] = ((uint64_t)p[1] << 20) + p[0];
+      t += b[i];
+    }
+    const uint64_t target = row_get(&rec.target);
+    uint64_t run = r.handed(sh.mass) + r.block_scan(t, sh.scan_q, all);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (run < target && target <= run + b[i]) sh.cut_n = 4 * r.tid + i, sh.cut_q = run;
+      run += b[i];
+    }
+    __syncthreads();
+    const uint32_t bin = sh.cut_n;
+    auto keep = [&](uint64_t e, uint64_t m) {  // adds to its stretch's kept mass
+      if (r.weight(r.value_of(e)) < q.least_w) return;
+      const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + r.lead) / Row<T>::N;
+      const uint32_t part = v / r.part_vecs, p0 = part * r.part_vecs, p1 = min(p0 + r.part_vecs, r.total_vecs);
+      uint32_t* const to = f.part[part * ROW_WARPS + (v - p0) / ((p1 - p0 + ROW_WARPS - 1) / ROW_WARPS)];
+      atomicAdd(&to[0], (uint32_t)m & 0xfffffu);
+      atomicAdd(&to[1], (uint32_t)(m >> 20));
+    };
+    for (uint32_t i = r.tid; i < n; i += ROW_THREADS) {
+      const uint64_t e = row_get(pool + i), m = r.mass(r.value_of(e));
+      const uint32_t at_bin = (uint32_t)((e - lo) >> shift);
+      if (at_bin < bin) {
+        keep(e, m);
+      } else if (at_bin == bin) {
+        const uint32_t at = atomicAdd(&sh.count, 1u);
+        if (at < ROW_THREADS) f.few[at] = e, f.few_q[at] = m;
+      }
+    }
+    __syncthreads();
+    const uint32_t few = sh.count;
+    if (few > ROW_THREADS || bin == 1024) {  // the estimate of the interval is never that far off
+      leave();
+      continue;
+    }
+    if (r.tid < few) {
+      const uint64_t e = f.few[r.tid], m = f.few_q[r.tid];
+      uint64_t before = sh.cut_q;
+      for (uint32_t i = 0; i < few; ++i) before += f.few[i] < e ? f.few_q[i] : 0;
+      if (before < target) keep(e, m);
+      if (before < target && target <= before + m) sh.cut_c = e;
+    }
+    __syncthreads();
+    if (r.tid < ROW_SUMS) (&sh.part[0][0])[r.tid] += ((uint64_t)f.part[r.tid][1] << 20) + f.part[r.tid][0];
+    const uint64_t last = sh.cut_c, total = row_get(&rec.total);
+    __syncthreads();
     r.scan_parts(sh.part, row_draw(q.u, r.handed(sh.part)),
                  [&](float z, int j) -> uint64_t {
                    const float w = r.weight(z);
