@@ -36,6 +36,10 @@ constexpr uint32_t PART_MIN = 16u << 10;
 #define VSPART 16
 #endif
 constexpr uint64_t STREAM_ROWS = 1024;
+#ifndef VCTAS
+#define VCTAS 5
+#endif
+constexpr uint32_t STREAM_CTAS = VCTAS;  // CTAs an SM
 constexpr uint32_t STREAM_PART = VSPART << 10;
 
 uint32_t row_ctas(uint32_t vecs, uint64_t rows, int sm_count) {
@@ -76,7 +80,9 @@ size_t cluster_smem(uint32_t part_vecs) {
   const size_t part = (size_t)part_vecs * 16;
   return ROW_SHARED_BYTES + (part > sizeof(RowFinish) ? part : sizeof(RowFinish));
 }
-constexpr size_t FINISH_SMEM = ROW_SHARED_BYTES + sizeof(RowFinish);
+// The passes' shared memory: the copies in flight, which the last CTA's working memory lies over.
+constexpr size_t RING_SMEM = ROW_SHARED_BYTES + sizeof(RowRing);
+static_assert(sizeof(RowFinish) <= sizeof(RowRing) && sizeof(RowWide) <= sizeof(RowRing) && RING_SMEM <= 48 << 10, "fits");
 
 // Small batches: one cluster a row.
 template <typename T, bool BEST> int launch_clusters(fs_sorter* s, const SorterView& v, RowArgs& a, int* launches) {
@@ -103,8 +109,8 @@ template <typename T, bool BEST> int launch_clusters(fs_sorter* s, const SorterV
 template <typename T, bool BEST> int launch_passes(fs_sorter* s, const SorterView& v, RowArgs& a, int* launches) {
   const uint32_t vecs = row_vecs(a, RowElem<T>::N);
   RowStream st{};
-  // as many parts as fill the GPU once (four CTAs an SM), of at least STREAM_PART bytes
-  st.parts = (uint32_t)v.sm_count * 4 / a.rows;
+  // as many parts as fill the GPU once, of at least STREAM_PART bytes
+  st.parts = (uint32_t)v.sm_count * STREAM_CTAS / a.rows;
   if (st.parts > vecs * 16 / STREAM_PART) st.parts = vecs * 16 / STREAM_PART;
   if (st.parts > ROW_MAX_CLUSTER) st.parts = ROW_MAX_CLUSTER;
   if (st.parts < 1) st.parts = 1;
@@ -138,15 +144,15 @@ template <typename T, bool BEST> int launch_passes(fs_sorter* s, const SorterVie
   const unsigned grid = a.rows * st.parts;
   cudaError_t e = cudaMemsetAsync(mem, 0, zeroed, v.stream);
   if (e == cudaSuccess) {
-    k_stream_max<T, BEST><<<grid, ROW_THREADS, 0, v.stream>>>(args, st);
+    k_stream_max<T, BEST><<<grid, ROW_THREADS, RING_SMEM, v.stream>>>(args, st);
     e = cudaGetLastError();
   }
-  if (e == cudaSuccess) e = chained(v, k_stream_weigh<T, BEST>, grid, FINISH_SMEM, 0, args, st);
+  if (e == cudaSuccess) e = chained(v, k_stream_weigh<T, BEST>, grid, RING_SMEM, 0, args, st);
   if constexpr (!BEST) {
     if (narrows) {
       const unsigned most = (unsigned)v.sm_count * 3, few = grid < most ? grid : most;
-      if (e == cudaSuccess) e = chained(v, k_stream_bins<T>, few, 0, 0, args, st);
-      if (e == cudaSuccess) e = chained(v, k_stream_cut<T>, few, ROW_SHARED_BYTES + sizeof(RowWide), 0, args, st);
+      if (e == cudaSuccess) e = chained(v, k_stream_bins<T>, few, RING_SMEM, 0, args, st);
+      if (e == cudaSuccess) e = chained(v, k_stream_cut<T>, few, RING_SMEM, 0, args, st);
       *launches += 2;
     }
   }

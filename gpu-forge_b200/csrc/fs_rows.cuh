@@ -356,7 +356,8 @@ template <typename T> struct Row {
   uint4* data;
   const int tid, lane, wid;
   const uint32_t rank, ctas;
-  const bool again;  // the cluster works on one row after another
+  const bool again;      // the cluster works on one row after another
+  const uint32_t lists;  // of published maxima
   // the row in memory, cut into 16-byte vectors at memory's boundaries
   const T* x;
   const uint4* vecs;
@@ -369,7 +370,7 @@ template <typename T> struct Row {
   float m, c;
 
   // CTA `part` of the `parts` of a row; d: where it keeps its part (null: nowhere).
-  __device__ __forceinline__ Row(RowShared& s, uint4* d, const RowArgs& a, uint32_t row, uint32_t part, uint32_t parts)
+  __device__ __forceinline__ Row(RowShared& s, uint4* d, const RowArgs& a, uint32_t row, uint32_t part, uint32_t parts, uint32_t lists_a_warp = 1)
       : cluster(cg::this_cluster()),
         sh(s),
         data(d),
@@ -378,7 +379,8 @@ template <typename T> struct Row {
         wid(threadIdx.x >> 5),
         rank(part),
         ctas(parts),
-        again(a.only != nullptr) {
+        again(a.only != nullptr),
+        lists(parts * ROW_WARPS * lists_a_warp) {
     sh.edge_n[tid] = 0;
     if (tid == 0) sh.count = 0, sh.first = ~0u;
     x = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
@@ -477,7 +479,7 @@ template <typename T> struct Row {
   // The row's maximum from the published ones.
   __device__ __forceinline__ void find_max() {
     uint32_t best = ~0u;
-    for (uint32_t i = lane; i < ctas * ROW_WARPS; i += 32) best = min(best, sh.tops[i * top_count()]);
+    for (uint32_t i = lane; i < lists; i += 32) best = min(best, sh.tops[i * top_count()]);
     m = row_unkey(__reduce_min_sync(~0u, best));
   }
   // The edge of the candidates of a cut; infinity where they are too many to list.
@@ -493,9 +495,9 @@ template <typename T> struct Row {
     const float edge = edge_of(n, ROW_EDGE_SCALE * ROW_LOG2E, -ROW_F32_MAX);
     return edge == -ROW_F32_MAX ? edge_of(n, far_scale(), -ROW_F32_MAX) : edge;
   }
-  __device__ __forceinline__ uint32_t most_tops() const { return top_count() * ctas * ROW_WARPS * 3 / 4; }
+  __device__ __forceinline__ uint32_t most_tops() const { return top_count() * lists * 3 / 4; }
   // How many of its 32 sorted thread maxima a warp publishes.
-  __device__ __forceinline__ uint32_t top_count() const { return min(32u, (uint32_t)ROW_TOPS / (ctas * ROW_WARPS)); }
+  __device__ __forceinline__ uint32_t top_count() const { return min(32u, (uint32_t)ROW_TOPS / lists); }
 
   // f(x, index) for every entry of this thread
   template <typename F> __device__ __forceinline__ void each(F f) const {
@@ -631,7 +633,7 @@ template <typename T> struct Row {
   // more than k.  Every warp scans the histogram for itself, which spares a
   // barrier.
   __device__ __forceinline__ float edge_of(uint32_t k, float scale, float last) {
-    const uint32_t tops = top_count() * ctas * ROW_WARPS;
+    const uint32_t tops = top_count() * lists;
     scale = fminf(scale, ROW_F32_MAX);
     for (uint32_t i = tid; i < tops; i += ROW_THREADS) {
       const float z = row_unkey(sh.tops[i]);
@@ -660,7 +662,7 @@ template <typename T> struct Row {
   // Its scale where 42 octaves of weight are too short: up to the smallest
   // maximum, or 512.  Empties the bins again.
   __device__ __forceinline__ float far_scale() {
-    const uint32_t tops = top_count() * ctas * ROW_WARPS;
+    const uint32_t tops = top_count() * lists;
     float low = m;
     for (uint32_t i = lane; i < tops; i += 32) {
       const float z = row_unkey(sh.tops[i]);
@@ -796,18 +798,16 @@ template <typename T> struct Row {
                   by_mass ? __float_as_uint(w) & 0x7fffffu : 1u);
     }
   }
-  // From the bins' sums over the row, by one CTA: warp 0 gets the first entry
-  // of the interval that the prefix ends in, warp 1 its last.  sh.b1 = sh.b2 =
-  // ~0 and sh.last = 0 before; sh.above: entries before the interval (counts).
-  // The prefix ends in b1 or later, and in b2 or before: where a sum of
+  // From the bins' sums over the row, by one CTA: the bins sh.b1 to sh.b2 that
+  // the prefix ends in (both ~0 before, and at most sh.last, 0 before), and for
+  // counts the entries before them, sh.above.  The prefix ends in b1 or later, and in b2 or before: where a sum of
   // estimates, 2^-12 of it and in the first round 2^-20 of the largest weight
   // added, and taken off, reaches the goal.  (An estimate is off by half a unit
   // of 4060 and less than 2^-14; the weights' rounding to q by at most 2^-22
   // together; from the second round on estimates follow q.  Counts are exact.)
   // Else it ends in the last bin with anything; a count that is not reached,
   // beyond all of them.
-  __device__ __forceinline__ uint64_t end_of(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n,
-                                             float top_w, float c42, int shift, uint64_t lo, uint64_t hi) {
+  __device__ __forceinline__ void end_bins(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n, float top_w) {
     constexpr int PER = ROW_BINS / ROW_THREADS;
     float s[PER], own = 0, all;
     uint32_t filled = 0;
@@ -832,6 +832,9 @@ template <typename T> struct Row {
       if (run * (1.0f - slack) - more >= goal) atomicMin(&sh.b2, (uint32_t)(tid * PER + i));
     }
     __syncthreads();
+  }
+  // Of the interval of those bins: warp 0 gets the first entry, warp 1 the last.
+  __device__ __forceinline__ uint64_t end_of(bool by_mass, bool by_weight, float c42, int shift, uint64_t lo, uint64_t hi) {
     if (wid >= 2) return 0;
     const uint32_t end = by_mass ? sh.last : (uint32_t)ROW_BINS - 1;
     const uint32_t b = wid ? min(sh.b2, end) + 1 : min(sh.b1, end);
@@ -910,7 +913,8 @@ template <typename T> struct Row {
       cluster.sync();
       if (rank == 0) {
         const float goal = by_mass ? (float)(target - above_q) * 0x1p-28f : (float)(target - above_n);
-        const uint64_t at = end_of(by_mass, by_weight, round == 0, goal, above_n, top_w, c42, shift, lo, hi);
+        end_bins(by_mass, by_weight, round == 0, goal, above_n, top_w);
+        const uint64_t at = end_of(by_mass, by_weight, c42, shift, lo, hi);
         if (wid < 2) {
           if (lane < (int)ctas) {
             *cluster.map_shared_rank(wid ? &sh.hi : &sh.lo, lane) = at;

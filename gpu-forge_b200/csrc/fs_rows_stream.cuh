@@ -69,23 +69,42 @@ __device__ __forceinline__ bool row_last(uint32_t* done, uint32_t parts, uint32_
   return true;
 }
 
-// f(vector, number) for the vectors of warp r.wid's stretch of part r.rank,
-// U of them in flight.
-template <int U, typename T, typename F> __device__ __forceinline__ void row_stream(const Row<T>& r, bool dirty, F f) {
+// Each thread keeps ROW_AHEAD vectors in flight, in slots of its own in shared
+// memory: no registers, and nothing to wait for but its own copies.
+constexpr int ROW_AHEAD = 8;
+using RowRing = uint4[ROW_AHEAD][ROW_THREADS];
+
+// f(vector, number) for the vectors of warp r.wid's stretch of part r.rank.
+template <typename T, typename F> __device__ __forceinline__ void row_stream(const Row<T>& r, RowRing& ring, bool dirty, F f) {
   uint32_t v0, v1;
   r.stretch(r.rank, r.wid, v0, v1);
-  uint32_t i = v0 + r.lane;
-  for (; i + 32 * (U - 1) < v1; i += 32 * U) {
-    uint4 v[U];
+  const bool head = v0 < v1 && !r.inside(v0), tail = v0 + head < v1 && !r.inside(v1 - 1);
+  const uint32_t end = v1 - tail;
+  uint32_t i = v0 + head + r.lane, next = i;
+  const uint32_t slot = smem_of(&ring[0][r.tid]);
+  auto fetch = [&](int s) {
+    if (next < end)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + s * (uint32_t)sizeof(ring[0])), "l"(r.vecs + next) : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    next += 32;
+  };
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = r.inside(i + 32 * u) ? row_load(r.vecs + i + 32 * u) : r.ragged(i + 32 * u);
+  for (int s = 0; s < ROW_AHEAD; ++s) fetch(s);
+  while (i < end) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) f(dirty ? r.cleaned(v[u]) : v[u], i + 32 * u);
+    for (int s = 0; s < ROW_AHEAD; ++s) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(ROW_AHEAD - 1) : "memory");
+      if (i < end) {
+        const uint4 v = ring[s][r.tid];
+        f(dirty ? r.cleaned(v) : v, i);
+        i += 32;
+      }
+      fetch(s);
+    }
   }
-  for (; i < v1; i += 32) {
-    const uint4 v = r.inside(i) ? row_load(r.vecs + i) : r.ragged(i);
-    f(dirty ? r.cleaned(v) : v, i);
-  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (head && r.lane == 0) f(r.cleaned(r.ragged(v0)), v0);
+  if (tail && r.lane == 1) f(r.cleaned(r.ragged(v1 - 1)), v1 - 1);
 }
 // f(x, index) for the entries of a vector that mask names
 template <typename T, typename F> __device__ __forceinline__ void row_each(const Row<T>& r, uint32_t mask, const uint4& v, uint32_t i, F f) {
@@ -98,34 +117,45 @@ template <typename T, typename F> __device__ __forceinline__ void row_each(const
 template <typename V> __device__ __forceinline__ V row_get(const V* p) { return __ldcg(p); }  // written by other CTAs
 
 template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream_max(const RowArgs a, const RowStream s) {
-  __shared__ RowShared sh;
+  extern __shared__ __align__(16) unsigned char row_smem[];
+  RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
+  RowRing& ring = *reinterpret_cast<RowRing*>(row_smem + ROW_SHARED_BYTES);
   asm volatile("griddepcontrol.launch_dependents;");
   using E = RowElem<T>;
   const uint32_t row = blockIdx.x / s.parts;
-  Row<T> r(sh, nullptr, a, row, blockIdx.x % s.parts, s.parts);
+  Row<T> r(sh, nullptr, a, row, blockIdx.x % s.parts, s.parts, 2);
   RowRecord& rec = s.rec[row];
   bool tops = true;
   if constexpr (!BEST) {
     const RowParams q(a, row);
     tops = q.by_k || q.by_p;
   }
-  typename E::Top top = E::top0();
-  row_stream<8>(r, false, [&](const uint4& v, uint32_t) { top = E::top(top, v); });
-  r.mine = E::value(top);
-  if (!(r.mine <= ROW_F32_MAX)) {
-    rec.dirty = 1;
-    top = E::top0();
-    row_stream<1>(r, true, [&](const uint4& v, uint32_t) { top = E::top(top, v); });
-    r.mine = E::value(top);
+  // two maxima a thread, of its vectors of even and odd numbers
+  typename E::Top top[2] = {E::top0(), E::top0()};
+  row_stream(r, ring, false, [&](const uint4& v, uint32_t i) {
+    if (i & 32)
+      top[1] = E::top(top[1], v);
+    else
+      top[0] = E::top(top[0], v);
+  });
+  if (__any_sync(~0u, !(E::value(top[0]) <= ROW_F32_MAX && E::value(top[1]) <= ROW_F32_MAX))) {
+    rec.dirty = 1;  // the warp looks through its stretch again
+    uint32_t v0, v1;
+    r.stretch(r.rank, r.wid, v0, v1);
+    top[0] = top[1] = E::top0();
+    for (uint32_t i = v0 + r.lane; i < v1; i += 32) top[0] = E::top(top[0], r.from_memory(i));
   }
-  __syncwarp();
-  const uint32_t key = tops ? r.sorted_tops() : __reduce_min_sync(~0u, row_key(r.mine));
   const uint32_t per = r.top_count();
   uint32_t* const all = s.tops + (size_t)row * ROW_TOPS;
-  if (r.lane < (int)(tops ? per : 1)) all[(r.rank * ROW_WARPS + r.wid) * per + r.lane] = key;
+#pragma unroll
+  for (int l = 0; l < 2; ++l) {
+    r.mine = E::value(top[l]);
+    const uint32_t key = tops ? r.sorted_tops() : __reduce_min_sync(~0u, row_key(r.mine));
+    if (r.lane < (int)(tops ? per : 1)) all[((r.rank * ROW_WARPS + r.wid) * 2 + l) * per + r.lane] = key;
+  }
   if (!row_last(&rec.done[0], s.parts, sh.found)) return;
 
-  for (uint32_t i = r.tid; i < per * s.parts * ROW_WARPS; i += ROW_THREADS) sh.tops[i] = row_get(all + i);
+  for (uint32_t i = r.tid; i < per * r.lists; i += ROW_THREADS) sh.tops[i] = row_get(all + i);
   __syncthreads();
   r.find_max();
   float edge = INFINITY;
@@ -154,8 +184,9 @@ template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, 
   extern __shared__ __align__(16) unsigned char row_smem[];
   RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
   RowFinish& f = *reinterpret_cast<RowFinish*>(row_smem + ROW_SHARED_BYTES);
+  RowRing& ring = *reinterpret_cast<RowRing*>(row_smem + ROW_SHARED_BYTES);  // until the row's last CTA finishes
   const uint32_t row = a.rows - 1 - blockIdx.x / s.parts;
-  Row<T> r(sh, nullptr, a, row, blockIdx.x % s.parts, s.parts);
+  Row<T> r(sh, nullptr, a, row, blockIdx.x % s.parts, s.parts, 2);
   RowRecord& rec = s.rec[row];
   __syncthreads();
   row_chain_wait();
@@ -165,7 +196,7 @@ template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, 
   bool greedy = false;
   if constexpr (!BEST) greedy = a.temperature && !(a.temperature[row] > 0.0f);
   typename Row<T>::Sum sum(r.m, r.c);
-  row_stream<8>(r, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t i) {
+  row_stream(r, ring, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t i) {
     sum.template add<false>(v, 0.0f);
     if (RowElem<T>::value(RowElem<T>::top(RowElem<T>::top0(), v)) >= edge)
       row_each(r, r.hits(v, edge, INFINITY), v, i, [&](float z, int j) {
@@ -256,21 +287,23 @@ __device__ __forceinline__ uint32_t row_wide_parts(RowArgs& a, uint32_t n, uint3
 }
 
 template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream_bins(const RowArgs args, const RowStream s) {
-  __shared__ RowShared sh;
+  extern __shared__ __align__(16) unsigned char row_smem[];
+  RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
+  RowRing& ring = *reinterpret_cast<RowRing*>(row_smem + ROW_SHARED_BYTES);
   row_chain_wait();
   RowArgs a = args;
   const uint32_t wide = row_get(&s.counts[0]), parts = row_wide_parts(a, wide, s.parts * args.part_vecs);
   for (uint32_t item = blockIdx.x; item < wide * parts; item += gridDim.x) {
     const uint32_t slot = item / parts, row = row_get(&s.wide[slot]);
     __syncthreads();
-    Row<T> r(sh, nullptr, a, row, item % parts, parts);
+    Row<T> r(sh, nullptr, a, row, item % parts, parts, 2);
     RowRecord& rec = s.rec[row];
     r.m = row_get(&rec.m), r.c = row_get(&rec.c);
     const float c42 = fminf(r.c * ROW_BIN_SCALE, ROW_F32_MAX);
     for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS) sh.bins[b] = 0;
     if (r.tid == 0) sh.b1 = sh.b2 = ~0u, sh.last = 0;
     __syncthreads();
-    row_stream<4>(r, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t) { r.count_bins(v, true, c42); });
+    row_stream(r, ring, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t) { r.count_bins(v, true, c42); });
     __syncthreads();
     uint32_t* const bins = s.bins + (size_t)slot * ROW_BINS;
     for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS)
@@ -278,10 +311,16 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 4) k_stream
     if (!row_last(&rec.done[2], parts, sh.found)) continue;
     for (int b = r.tid; b < ROW_BINS; b += ROW_THREADS) sh.bins[b] = row_get(bins + b);
     __syncthreads();
-    const uint64_t lo = (uint64_t)row_key(r.m) << ROW_IDX_BITS,
-                   hi = (uint64_t)row_key(-ROW_F32_MAX) << ROW_IDX_BITS | (ROW_MAX_COLS - 1);
-    const uint64_t at = r.end_of(true, true, true, (float)row_get(&rec.target) * 0x1p-28f, 0, 1.0f, c42, 0, lo, hi);
-    if (r.wid < 2 && r.lane == 0) *(r.wid ? &rec.hi : &rec.lo) = at;
+    r.end_bins(true, true, true, (float)row_get(&rec.target) * 0x1p-28f, 0, 1.0f);
+    if (r.tid == 0) {
+      // the bins' bounds in x, by more than their rounding; what that adds is only more entries to look at
+      const float b1 = (float)min(sh.b1, sh.last), b2 = (float)min(sh.b2, sh.last);
+      const float slack = fabsf(r.m) * 0x1p-21f;
+      const float up = fminf(r.m - (b1 - 0.5f) / c42 * (1.0f - 0x1p-18f) + slack, r.m);
+      const float down = fmaxf(r.m - (b2 + 0.5f) / c42 * (1.0f + 0x1p-18f) - slack, -ROW_F32_MAX);
+      rec.lo = (uint64_t)row_key(up) << ROW_IDX_BITS;
+      rec.hi = (uint64_t)row_key(down) << ROW_IDX_BITS | (ROW_MAX_COLS - 1);
+    }
   }
 }
 
@@ -289,13 +328,14 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_stream
   extern __shared__ __align__(16) unsigned char row_smem[];
   RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
   RowWide& f = *reinterpret_cast<RowWide*>(row_smem + ROW_SHARED_BYTES);
+  RowRing& ring = *reinterpret_cast<RowRing*>(row_smem + ROW_SHARED_BYTES);  // until the row's last CTA finishes
   row_chain_wait();
   RowArgs a = args;
   const uint32_t wide = row_get(&s.counts[0]), parts = row_wide_parts(a, wide, s.parts * args.part_vecs);
   for (uint32_t item = blockIdx.x; item < wide * parts; item += gridDim.x) {
     const uint32_t slot = item / parts, row = row_get(&s.wide[slot]);
     __syncthreads();
-    Row<T> r(sh, nullptr, a, row, item % parts, parts);
+    Row<T> r(sh, nullptr, a, row, item % parts, parts, 2);
     RowRecord& rec = s.rec[row];
     const RowParams q(a, row);
     r.m = row_get(&rec.m), r.c = row_get(&rec.c);
@@ -304,7 +344,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_stream
     __syncthreads();
     typename Row<T>::Sum sum(r.m, r.c);
     uint64_t kept = 0;
-    row_stream<4>(r, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t i) {
+    row_stream(r, ring, row_get(&rec.dirty) != 0, [&](const uint4& v, uint32_t i) {
       sum.template add<true>(v, over);
       row_each(r, r.hits(v, least, over), v, i, [&](float z, int j) {
         const uint32_t at = atomicAdd(&sh.count, 1u);
@@ -335,7 +375,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 3) k_stream
     __syncthreads();
     if (!row_last(&rec.done[3], parts, sh.found)) continue;
 
-    // the entry of the interval at which the mass reaches the target: by bins of the interval, then among a bin's entries
+    // the entry of the interval at which the mass reaches the target: by bins of the interval, then among a bin's
     n = row_get(&rec.pool_n);
     auto leave = [&] {
       if (r.tid == 0) s.left[atomicAdd(&s.counts[1], 1u)] = row;
