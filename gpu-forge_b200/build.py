@@ -30,7 +30,7 @@ TARGETS = {
                            "fs_hoststage.h"],
             "fs_multi.cu": ["fs_device.cuh"],
             "fs_datagen.cu": ["fs_device.cuh"],
-            "fs_rows.cu": ["fs_internal.h", "fs_device.cuh", "fs_rows.cuh", "fs_rows_stream.cuh"],
+            "fs_rows.cu": ["fs_internal.h", "fs_device.cuh", "fs_rows.cuh"],
             "fs_slots.cu": ["fs_internal.h", "fs_device.cuh"],
         },
         "hdrs": ["forgesort.h", "forgesort_bench.h"],

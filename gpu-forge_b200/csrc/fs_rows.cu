@@ -3,7 +3,6 @@
 #include "forgesort.h"
 #include "fs_internal.h"
 #include "fs_rows.cuh"
-#include "fs_rows_stream.cuh"
 
 #include <atomic>
 
@@ -25,48 +24,13 @@ size_t elem_bytes(int dtype) { return dtype == FS_LOGITS_F32 ? 4 : 2; }
 // CTAs per row: as many as cut it into parts of PART bytes, of which three fit
 // an SM, and more while the batch has fewer CTAs than the GPU has SMs and a
 // part keeps PART_MIN bytes.
-#ifndef VPART
-#define VPART 64
-#endif
-constexpr uint32_t PART = VPART << 10;
+constexpr uint32_t PART = 64u << 10;
 constexpr uint32_t PART_MIN = 16u << 10;
-// Large batches go in passes over all rows, in groups of STREAM_ROWS rows
-// (of 25 KB of scratch each), cut into parts of STREAM_PART bytes.
-#ifndef VSPART
-#define VSPART 16
-#endif
-constexpr uint64_t STREAM_ROWS = 1024;
-#ifndef VCTAS
-#define VCTAS 5
-#endif
-constexpr uint32_t STREAM_CTAS = VCTAS;  // CTAs an SM
-constexpr uint32_t STREAM_PART = VSPART << 10;
 
-uint32_t row_ctas(uint32_t vecs, uint64_t rows, int sm_count) {
-  const uint32_t bytes = vecs * 16;
+uint32_t row_ctas(uint32_t bytes, uint64_t rows, int sm_count) {
   uint32_t c = (bytes + PART - 1) / PART;
   while (c < 8 && rows * c * 2 <= (uint64_t)sm_count && bytes / (2 * c) >= PART_MIN) c *= 2;
   return c < ROW_MAX_CLUSTER ? c : ROW_MAX_CLUSTER;
-}
-
-// A launch behind the call's previous one (fs_rows_stream.cuh), scheduled
-// while that one drains; every such kernel waits for it first.
-template <typename Kern, typename... Args>
-cudaError_t chained(const SorterView& v, Kern kern, unsigned grid, size_t smem, uint32_t cluster, const Args&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(ROW_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = v.stream;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = cluster;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = cluster ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
 // 16-byte vectors of a row: with the worst lead, unless every row begins at a
@@ -76,22 +40,28 @@ uint32_t row_vecs(const RowArgs& a, int lanes) {
   const bool aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && step % lanes == 0;
   return (a.cols + (aligned ? lanes - 1 : 2 * lanes - 2)) / lanes;
 }
-size_t cluster_smem(uint32_t part_vecs) {
-  const size_t part = (size_t)part_vecs * 16;
-  return ROW_SHARED_BYTES + (part > sizeof(RowFinish) ? part : sizeof(RowFinish));
-}
-// The passes' shared memory: the copies in flight, which the last CTA's working memory lies over.
-constexpr size_t RING_SMEM = ROW_SHARED_BYTES + sizeof(RowRing);
-static_assert(sizeof(RowFinish) <= sizeof(RowRing) && sizeof(RowWide) <= sizeof(RowRing) && RING_SMEM <= 48 << 10, "fits");
 
-// Small batches: one cluster a row.
-template <typename T, bool BEST> int launch_clusters(fs_sorter* s, const SorterView& v, RowArgs& a, int* launches) {
-  const uint32_t vecs = row_vecs(a, RowElem<T>::N), ctas = row_ctas(vecs, a.rows, v.sm_count);
+// Sets, once per device, what a kernel needs beyond the defaults.
+template <typename Kern> cudaError_t configure(std::atomic<bool>& done, Kern kern, size_t smem, bool clusters) {
+  if (done.load()) return cudaSuccess;  // idempotent: two threads may both get here
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess && clusters) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done.store(true);
+  return e;
+}
+
+// One cluster a row.
+template <typename T, bool BEST> int launch_clusters(fs_sorter* s, const SorterView& v, RowArgs& a) {
+  using R = Row<T, ROW_CLUSTER_THREADS, false>;
+  static std::atomic<bool> configured[SORTER_MAX_DEVICES];
+  FS_ROWS_CUDA(s, configure(configured[v.device], k_row_cluster<T, BEST>, R::SHARED_BYTES + ROW_PART_MAX, true));
+  const uint32_t vecs = row_vecs(a, RowElem<T>::N), ctas = row_ctas(vecs * 16, a.rows, v.sm_count);
   a.part_vecs = (vecs + ctas - 1) / ctas;
+  const size_t part = (size_t)a.part_vecs * 16;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.rows * ctas);
-  cfg.blockDim = dim3(ROW_THREADS);
-  cfg.dynamicSmemBytes = cluster_smem(a.part_vecs);
+  cfg.blockDim = dim3(ROW_CLUSTER_THREADS);
+  cfg.dynamicSmemBytes = R::SHARED_BYTES + (part > sizeof(RowFinish) ? part : sizeof(RowFinish));
   cfg.stream = v.stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -99,119 +69,35 @@ template <typename T, bool BEST> int launch_clusters(fs_sorter* s, const SorterV
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  FS_ROWS_CUDA(s, cudaLaunchKernelEx(&cfg, k_rows<T, BEST>, static_cast<const RowArgs>(a)));
-  *launches += 1;
+  FS_ROWS_CUDA(s, cudaLaunchKernelEx(&cfg, k_row_cluster<T, BEST>, static_cast<const RowArgs>(a)));
   return FS_OK;
 }
 
-// Large batches: passes over all rows, with scratch from the stream-ordered
-// allocator, so that a call keeps nothing and may be captured.
-template <typename T, bool BEST> int launch_passes(fs_sorter* s, const SorterView& v, RowArgs& a, int* launches) {
-  const uint32_t vecs = row_vecs(a, RowElem<T>::N);
-  RowStream st{};
-  // as many parts as fill the GPU once, of at least STREAM_PART bytes
-  st.parts = (uint32_t)v.sm_count * STREAM_CTAS / a.rows;
-  if (st.parts > vecs * 16 / STREAM_PART) st.parts = vecs * 16 / STREAM_PART;
-  if (st.parts > ROW_MAX_CLUSTER) st.parts = ROW_MAX_CLUSTER;
-  if (st.parts < 1) st.parts = 1;
-  a.part_vecs = (vecs + st.parts - 1) / st.parts;
-  const bool narrows = !BEST && a.top_p;  // rows may have wide nuclei
-  size_t bytes = 0;
-  auto take = [&](size_t n) {
-    const size_t at = bytes;
-    bytes += (n + 255) / 256 * 256;
-    return at;
-  };
-  const size_t R = a.rows;
-  const size_t o_rec = take(R * sizeof(RowRecord)), o_counts = take(8), zeroed = bytes;
-  const size_t o_tops = take(R * ROW_TOPS * 4), o_mass = take(R * ROW_SUMS * 8), o_list = take(R * ROW_LIST * 8), o_left = take(R * 4);
-  const size_t o_wide = take(narrows ? R * 4 : 0), o_part = take(narrows ? R * ROW_SUMS * 8 : 0);
-  const size_t o_bins = take(narrows ? R * ROW_BINS * 4 : 0), o_pool = take(narrows ? R * ROW_WIDE_POOL * 8 : 0);
-  void* mem = nullptr;
-  FS_ROWS_CUDA(s, cudaMallocFromPoolAsync(&mem, bytes, v.pool, v.stream));
-  unsigned char* const b = static_cast<unsigned char*>(mem);
-  st.rec = reinterpret_cast<RowRecord*>(b + o_rec);
-  st.counts = reinterpret_cast<uint32_t*>(b + o_counts);
-  st.tops = reinterpret_cast<uint32_t*>(b + o_tops);
-  st.mass = reinterpret_cast<uint64_t*>(b + o_mass);
-  st.list = reinterpret_cast<uint64_t*>(b + o_list);
-  st.left = reinterpret_cast<uint32_t*>(b + o_left);
-  st.wide = reinterpret_cast<uint32_t*>(b + o_wide);
-  st.part = reinterpret_cast<uint64_t*>(b + o_part);
-  st.bins = reinterpret_cast<uint32_t*>(b + o_bins);
-  st.pool = reinterpret_cast<uint64_t*>(b + o_pool);
-  const RowArgs args = a;
-  const unsigned grid = a.rows * st.parts;
-  cudaError_t e = cudaMemsetAsync(mem, 0, zeroed, v.stream);
-  if (e == cudaSuccess) {
-    k_stream_max<T, BEST><<<grid, ROW_THREADS, RING_SMEM, v.stream>>>(args, st);
-    e = cudaGetLastError();
-  }
-  if (e == cudaSuccess) e = chained(v, k_stream_weigh<T, BEST>, grid, RING_SMEM, 0, args, st);
-  if constexpr (!BEST) {
-    if (narrows) {
-      const unsigned most = (unsigned)v.sm_count * 3, few = grid < most ? grid : most;
-      if (e == cudaSuccess) e = chained(v, k_stream_bins<T>, few, RING_SMEM, 0, args, st);
-      if (e == cudaSuccess) e = chained(v, k_stream_cut<T>, few, RING_SMEM, 0, args, st);
-      *launches += 2;
-    }
-  }
-  if (e == cudaSuccess && (BEST || a.top_k || a.top_p || a.min_p)) {
-    RowArgs left = a;
-    left.only = st.left;
-    left.only_n = st.counts + 1;
-    const uint32_t ctas = row_ctas(vecs, 1, v.sm_count), most = (uint32_t)v.sm_count / ctas;
-    left.part_vecs = (vecs + ctas - 1) / ctas;
-    e = chained(v, k_rows<T, BEST>, (a.rows < most ? a.rows : most) * ctas, cluster_smem(left.part_vecs), ctas,
-                static_cast<const RowArgs>(left));
-    *launches += 1;
-  }
-  *launches += 2;
-  const cudaError_t freed = cudaFreeAsync(mem, v.stream);
-  FS_ROWS_CUDA(s, e);
-  FS_ROWS_CUDA(s, freed);
-  return FS_OK;
-}
-
-template <typename T, bool BEST> int launch(fs_sorter* s, const SorterView& v, RowArgs a, int* launches) {
+// One CTA of NT threads a row.
+template <typename T, int NT, bool BEST> int launch_solo(fs_sorter* s, const SorterView& v, RowArgs& a) {
+  using R = Row<T, NT, true>;
+  static_assert(sizeof(RowFinish) <= R::RING_BYTES, "fits");
+  constexpr size_t smem = R::SHARED_BYTES + R::RING_BYTES;
   static std::atomic<bool> configured[SORTER_MAX_DEVICES];
-  if (!configured[v.device].load()) {  // idempotent: two threads may both get here
-    FS_ROWS_CUDA(s, cudaFuncSetAttribute(k_rows<T, BEST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(ROW_SHARED_BYTES + ROW_PART_MAX)));
-    FS_ROWS_CUDA(s, cudaFuncSetAttribute(k_rows<T, BEST>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    configured[v.device].store(true);
-  }
-  const uint64_t total = a.rows;
-  if (total * a.cols * sizeof(T) < v.row_pass_min) return launch_clusters<T, BEST>(s, v, a, launches);
-  for (uint64_t r = 0; r < total; r += STREAM_ROWS) {
-    RowArgs g = a;
-    g.rows = (uint32_t)(total - r < STREAM_ROWS ? total - r : STREAM_ROWS);
-    g.x = static_cast<const T*>(a.x) + (int64_t)r * a.stride;
-    if constexpr (BEST) {
-      g.best_idx = a.best_idx + r * a.n;
-      g.best_logprob = a.best_logprob + r * a.n;
-      g.lse = a.lse ? a.lse + r : nullptr;
-    } else {
-      g.temperature = a.temperature ? a.temperature + r : nullptr;
-      g.top_k = a.top_k ? a.top_k + r : nullptr;
-      g.top_p = a.top_p ? a.top_p + r : nullptr;
-      g.min_p = a.min_p ? a.min_p + r : nullptr;
-      g.uniform = a.uniform + r;
-      g.tokens = a.tokens + r;
-      g.logprobs = a.logprobs ? a.logprobs + r : nullptr;
-    }
-    const int rc = launch_passes<T, BEST>(s, v, g, launches);
-    if (rc) return rc;
-  }
+  FS_ROWS_CUDA(s, configure(configured[v.device], k_row_solo<T, NT, BEST>, smem, false));
+  a.part_vecs = row_vecs(a, RowElem<T>::N);
+  k_row_solo<T, NT, BEST><<<a.rows, NT, smem, v.stream>>>(a);
+  FS_ROWS_CUDA(s, cudaGetLastError());
   return FS_OK;
 }
 
-template <bool BEST> int launch_rows(fs_sorter* s, const SorterView& v, int dtype, const RowArgs& a, int sync) {
-  int launches = 0;
-  const int rc = dtype == FS_LOGITS_F32   ? launch<float, BEST>(s, v, a, &launches)
-                 : dtype == FS_LOGITS_F16 ? launch<__half, BEST>(s, v, a, &launches)
-                                          : launch<__nv_bfloat16, BEST>(s, v, a, &launches);
-  return rc ? rc : sorter_finish(s, v, launches, sync);
+template <typename T, bool BEST> int launch(fs_sorter* s, const SorterView& v, RowArgs& a) {
+  const int form = v.row_form ? v.row_form : a.rows * 2 < (uint64_t)v.sm_count ? 1 : a.rows > (uint64_t)v.sm_count ? 2 : 3;
+  if (form == 1) return launch_clusters<T, BEST>(s, v, a);
+  if (form == 2) return launch_solo<T, 512, BEST>(s, v, a);
+  return launch_solo<T, 1024, BEST>(s, v, a);
+}
+
+template <bool BEST> int launch_rows(fs_sorter* s, const SorterView& v, int dtype, RowArgs& a, int sync) {
+  const int rc = dtype == FS_LOGITS_F32   ? launch<float, BEST>(s, v, a)
+                 : dtype == FS_LOGITS_F16 ? launch<__half, BEST>(s, v, a)
+                                          : launch<__nv_bfloat16, BEST>(s, v, a);
+  return rc ? rc : sorter_finish(s, v, 1, sync);
 }
 
 int check_rows(fs_sorter* s, int dtype, const void* logits, uint64_t rows, uint64_t cols, int64_t stride) {

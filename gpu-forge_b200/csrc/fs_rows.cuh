@@ -27,24 +27,19 @@ namespace fs {
 
 namespace cg = cooperative_groups;
 
-constexpr int ROW_THREADS = 256;
-#ifndef ROW_MINB
-#define ROW_MINB 3
-#endif
-constexpr int ROW_WARPS = ROW_THREADS / 32;
 constexpr int ROW_MAX_CLUSTER = 16;
 constexpr int ROW_IDX_BITS = 19;
 constexpr uint32_t ROW_MAX_COLS = 1u << ROW_IDX_BITS;
 constexpr int ROW_LIST = 640;   // candidates of a row above its edge
 constexpr int ROW_POOL = 1024;  // undecided entries of a row that narrowing leaves
-constexpr int ROW_FEW = 256;    // ... where they are ranked in place
+constexpr int ROW_FEW = 256;    // entries that are ranked in place, by comparing all of them
 constexpr int ROW_BEST_MAX = 1024;
 constexpr int ROW_TOPS = 512;   // thread maxima that a cluster's warps publish
 // A nucleus is first looked for among about this many entries.
 constexpr uint32_t ROW_NUCLEUS_GUESS = 128;
 // Bins linear in y: of the published maxima (1/6 octave of weight each, 42 in
 // all; entries with q > 0 have y < 41), and of all entries (1/42 octave).
-constexpr int ROW_EDGE_BINS = 256;  // one a thread
+constexpr int ROW_EDGE_BINS = 256;
 constexpr float ROW_EDGE_SCALE = 6.0f;
 constexpr int ROW_BINS = 1792;
 constexpr float ROW_BIN_SCALE = 42.0f;
@@ -60,8 +55,6 @@ struct RowArgs {
   int64_t stride;       // elements between rows
   uint32_t rows, cols;
   uint32_t part_vecs;   // 16-byte vectors of a row per CTA of its cluster
-  const uint32_t* only; // null, or the rows to work on, of number *only_n
-  const uint32_t* only_n;
   // sampling (null: off)
   const float* temperature;
   const int* top_k;
@@ -88,6 +81,16 @@ __device__ __forceinline__ float fmax_nan(float a, float b) {
   return r;
 }
 
+// Word k of a vector, by selections (an index would put it in local memory).
+__device__ __forceinline__ uint32_t row_word(const uint4& v, int k) {
+  uint32_t w = v.x;
+  asm("{\n .reg .pred p, q, r;\n setp.eq.s32 p, %4, 1;\n setp.eq.s32 q, %4, 2;\n setp.eq.s32 r, %4, 3;\n"
+      " @p mov.b32 %0, %1;\n @q mov.b32 %0, %2;\n @r mov.b32 %0, %3;\n}"
+      : "+r"(w)
+      : "r"(v.y), "r"(v.z), "r"(v.w), "r"(k));
+  return w;
+}
+
 template <typename T> struct RowElem;
 template <> struct RowElem<float> {
   static constexpr int N = 4;
@@ -102,10 +105,7 @@ template <> struct RowElem<float> {
   static __device__ __forceinline__ uint32_t clean(uint32_t v) {
     return __float_as_uint(fminf(fmaxf(__uint_as_float(v), -INFINITY), ROW_F32_MAX));
   }
-  static __device__ __forceinline__ float one(const uint4* v, uint32_t i) { return reinterpret_cast<const float*>(v)[i]; }
-  static __device__ __forceinline__ float at(const uint4& v, int e) {
-    return __uint_as_float(e < 2 ? (e ? v.y : v.x) : (e & 1 ? v.w : v.z));
-  }
+  static __device__ __forceinline__ float at(const uint4& v, int e) { return __uint_as_float(row_word(v, e)); }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
@@ -131,11 +131,8 @@ template <> struct RowElem<__nv_bfloat16> {
     asm("min.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7f7f7f7fu));
     return v;
   }
-  static __device__ __forceinline__ float one(const uint4* v, uint32_t i) {
-    return __uint_as_float((uint32_t) reinterpret_cast<const unsigned short*>(v)[i] << 16);
-  }
   static __device__ __forceinline__ float at(const uint4& v, int e) {
-    const uint32_t w = e < 4 ? (e < 2 ? v.x : v.y) : (e < 6 ? v.z : v.w);
+    const uint32_t w = row_word(v, e >> 1);
     return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
   }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
@@ -169,11 +166,8 @@ template <> struct RowElem<__half> {
     asm("min.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0x7bff7bffu));
     return v;
   }
-  static __device__ __forceinline__ float one(const uint4* v, uint32_t i) {
-    return __half2float(__ushort_as_half(reinterpret_cast<const unsigned short*>(v)[i]));
-  }
   static __device__ __forceinline__ float at(const uint4& v, int e) {
-    const uint32_t w = e < 4 ? (e < 2 ? v.x : v.y) : (e < 6 ? v.z : v.w);
+    const uint32_t w = row_word(v, e >> 1);
     return __half2float(__ushort_as_half((unsigned short)(e & 1 ? w >> 16 : w)));
   }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
@@ -272,11 +266,6 @@ __device__ __forceinline__ void smem_add_if(bool yes, uint32_t* p, uint32_t v) {
                "r"(v), "r"((uint32_t)yes)
                : "memory");
 }
-// Where kernels of one call are launched one behind the other before the
-// first has ended: waits until it has, with all that it wrote.
-__device__ __forceinline__ void row_chain_wait() {
-  asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
-}
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ uint64_t row_target(float p, uint64_t mass) {  // ceil(p mass), at least 1
@@ -315,7 +304,7 @@ struct RowParams {
 };
 
 // ---- shared state ---------------------------------------------------------------
-struct RowShared {
+template <int CTAS, int WARPS> struct RowShared {
   union {
     struct {
       uint64_t list[ROW_LIST];         // candidates: key << 19 | index
@@ -325,16 +314,15 @@ struct RowShared {
     uint32_t bins[ROW_BINS];  // while a cut is narrowed down: weights or counts,
     uint64_t pool[ROW_POOL];  // then the undecided entries
   };
-  uint64_t mass[ROW_MAX_CLUSTER][ROW_WARPS];  // of each warp of the cluster
-  uint64_t part[ROW_MAX_CLUSTER][ROW_WARPS];  // of its candidates; of its kept entries
-  uint64_t scan_q[ROW_WARPS];
-  uint32_t scan_n[ROW_WARPS];
-  uint32_t n[ROW_MAX_CLUSTER];
+  uint64_t mass[CTAS][WARPS];  // of each warp of the cluster
+  uint64_t part[CTAS][WARPS];  // of its candidates; of its kept entries
+  uint64_t scan_q[WARPS];
+  uint32_t scan_n[WARPS];
+  uint32_t n[CTAS];
   uint64_t lo, hi, cut_q, cut_c;
-  uint32_t cut_n, count, above, first, b1, b2, last, found;
+  uint32_t cut_n, count, above, first, b1, b2, last, found, dirty;
 };
-constexpr size_t ROW_SHARED_BYTES = (sizeof(RowShared) + 15) / 16 * 16;
-static_assert(3 * (ROW_SHARED_BYTES + (64 << 10) + 1024) <= 228 << 10, "three CTAs on an SM");
+constexpr int ROW_SUMS = 128;  // warps of the CTAs that share a row
 
 // What the first CTA lays over its part of the row when only the listed
 // entries (or the copy in memory) matter any more.
@@ -343,20 +331,31 @@ struct RowFinish {
   uint64_t loose[ROW_POOL];
   uint64_t sorted[ROW_POOL];
   uint64_t input[ROW_LIST];
-  uint32_t part[ROW_MAX_CLUSTER * ROW_WARPS][2];  // masses of a stretch's entries in the interval: their low 20 bits, the rest
+  uint32_t part[ROW_SUMS][2];  // masses of a stretch's entries in the interval: their low 20 bits, the rest
 };
 
 // ---- one row --------------------------------------------------------------------
-template <typename T> struct Row {
+// NT threads a CTA.  MEM: one CTA has the row to itself and streams it from
+// memory (L2) as often as it looks at it; else a cluster shares it and each CTA
+// keeps its part in shared memory.
+template <typename T, int NT, bool MEM> struct Row {
   using E = RowElem<T>;
+  static constexpr int WARPS = NT / 32;
+  static constexpr int CTAS = MEM ? 1 : ROW_MAX_CLUSTER;
+  static_assert(CTAS * WARPS <= ROW_SUMS, "sums");
+  using Shared = RowShared<CTAS, WARPS>;
+  static constexpr size_t SHARED_BYTES = (sizeof(Shared) + 15) / 16 * 16;
+  using Sums = uint64_t[CTAS][WARPS];
+  // vectors that each thread keeps in flight, in slots of its own in shared memory
+  static constexpr int AHEAD = 8;
+  static constexpr size_t RING_BYTES = MEM ? (size_t)AHEAD * NT * 16 : 0;
   static constexpr int N = E::N;
 
   cg::cluster_group cluster;
-  RowShared& sh;
+  Shared& sh;
   uint4* data;
   const int tid, lane, wid;
   const uint32_t rank, ctas;
-  const bool again;      // the cluster works on one row after another
   const uint32_t lists;  // of published maxima
   // the row in memory, cut into 16-byte vectors at memory's boundaries
   const T* x;
@@ -367,10 +366,11 @@ template <typename T> struct Row {
   uint32_t seg0, seg1;  // this warp's vectors of the CTA's part
   int first;            // index of the part's element 0 (negative inside the row's leading fill)
   float mine;           // this thread's maximum
+  bool dirty = false;   // the row has NaN or +inf (MEM)
   float m, c;
 
   // CTA `part` of the `parts` of a row; d: where it keeps its part (null: nowhere).
-  __device__ __forceinline__ Row(RowShared& s, uint4* d, const RowArgs& a, uint32_t row, uint32_t part, uint32_t parts, uint32_t lists_a_warp = 1)
+  __device__ __forceinline__ Row(Shared& s, uint4* d, const RowArgs& a, uint32_t row, uint32_t part, uint32_t parts, uint32_t lists_a_warp = 1)
       : cluster(cg::this_cluster()),
         sh(s),
         data(d),
@@ -379,10 +379,10 @@ template <typename T> struct Row {
         wid(threadIdx.x >> 5),
         rank(part),
         ctas(parts),
-        again(a.only != nullptr),
-        lists(parts * ROW_WARPS * lists_a_warp) {
-    sh.edge_n[tid] = 0;
-    if (tid == 0) sh.count = 0, sh.first = ~0u;
+        lists(parts * WARPS * lists_a_warp) {
+    for (int b = tid; b < ROW_EDGE_BINS; b += NT) sh.edge_n[b] = 0;
+    if (tid == 0) sh.count = 0, sh.first = ~0u, sh.dirty = 0;
+    if constexpr (MEM) __syncthreads();
     x = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
     cols = a.cols;
     part_vecs = a.part_vecs;
@@ -417,9 +417,37 @@ template <typename T> struct Row {
   // vectors [v0, v1) of warp w's stretch of CTA r's part
   __device__ __forceinline__ void stretch(uint32_t r, uint32_t w, uint32_t& v0, uint32_t& v1) const {
     const uint32_t p0 = min(r * part_vecs, total_vecs), p1 = min(p0 + part_vecs, total_vecs);
-    const uint32_t sv = (p1 - p0 + ROW_WARPS - 1) / ROW_WARPS;
+    const uint32_t sv = (p1 - p0 + WARPS - 1) / WARPS;
     v0 = min(p0 + w * sv, p1);
     v1 = min(v0 + sv, p1);
+  }
+
+  // Finds the row's maximum from memory; two maxima a thread, of every other
+  // vector each.
+  __device__ __forceinline__ void load_memory(bool tops) {
+    first = -lead;
+    typename E::Top top[2] = {E::top0(), E::top0()};
+    stream<false, false>([&](const uint4& v, uint32_t) {  // the two take turns
+      const typename E::Top t = E::top(top[0], v);
+      top[0] = top[1];
+      top[1] = t;
+    }, [] {});
+    const bool bad = !(E::value(top[0]) <= ROW_F32_MAX && E::value(top[1]) <= ROW_F32_MAX);
+    if (__any_sync(~0u, bad)) {  // NaN or +inf: the warp looks through its stretch again
+      sh.dirty = 1;
+      top[0] = top[1] = E::top0();
+      stream<true, false>([&](const uint4& v, uint32_t) { top[0] = E::top(top[0], v); }, [] {});
+    }
+    const uint32_t per = top_count();
+#pragma unroll
+    for (int l = 0; l < 2; ++l) {
+      mine = E::value(top[l]);
+      const uint32_t k = tops ? sorted_tops() : __reduce_min_sync(~0u, row_key(mine));
+      if (lane < (int)(tops ? per : 1)) sh.tops[(wid * 2 + l) * per + lane] = k;
+    }
+    __syncthreads();
+    dirty = sh.dirty != 0;
+    find_max();
   }
 
   // Reads this CTA's part into shared memory and finds the row's maximum.
@@ -428,6 +456,10 @@ template <typename T> struct Row {
   // nothing but its own copies has to be waited for.
   // With `tops`, the warps also publish their threads' largest maxima.
   __device__ __forceinline__ void load(bool tops) {
+    if constexpr (MEM) {
+      load_memory(tops);
+      return;
+    }
     cluster.barrier_arrive();  // waited for below: no CTA writes into one that has not started
     const uint32_t p0 = min(rank * part_vecs, total_vecs);
     stretch(rank, wid, seg0, seg1);
@@ -458,7 +490,7 @@ template <typename T> struct Row {
     const uint32_t per = top_count();
     for (uint32_t i0 = 0; i0 < per * ctas; i0 += 32) {
       const uint32_t to = (i0 + lane) / per, e = i0 + lane - to * per, v = __shfl_sync(~0u, k, e);
-      if (to < ctas && (tops || e == 0)) *cluster.map_shared_rank(&sh.tops[(rank * ROW_WARPS + wid) * per + e], to) = v;
+      if (to < ctas && (tops || e == 0)) *cluster.map_shared_rank(&sh.tops[(rank * WARPS + wid) * per + e], to) = v;
     }
     cluster.sync();
     find_max();
@@ -499,15 +531,67 @@ template <typename T> struct Row {
   // How many of its 32 sorted thread maxima a warp publishes.
   __device__ __forceinline__ uint32_t top_count() const { return min(32u, (uint32_t)ROW_TOPS / lists); }
 
+  // f(vector, number in the part) for this thread's vectors, two side by side;
+  // from memory, with +inf and NaN as they are unless CLEAN; now_and_then() is
+  // called every AHEAD vectors.  BACK: from the
+  // stretch's end, which was read last and is in L2 for the longest.
+  template <bool CLEAN, bool BACK, typename F, typename G> __device__ __forceinline__ void stream(F f, G now_and_then) const {
+    uint32_t v0, v1;
+    stretch(0, wid, v0, v1);
+    const bool head = v0 < v1 && !inside(v0), tail = v0 + head < v1 && !inside(v1 - 1);
+    const uint32_t lo = v0 + head, end = v1 - tail;
+    uint32_t i = lo + lane, next = i;
+    auto number = [&](uint32_t n) { return BACK ? lo + end - 1 - n : n; };
+    const uint32_t slot = smem_of(data + tid);
+    auto fetch = [&](int k) {
+      if (next < end)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + k * (NT * 16)), "l"(vecs + number(next)) : "memory");
+      next += 32;
+    };
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    auto get = [&](int k) {
+      const uint4 v = data[k * NT + tid];
+      return CLEAN ? cleaned(v) : v;
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; k += 2) fetch(k), fetch(k + 1), commit();
+    for (; i + 32 * (AHEAD - 1) < end; i += 32 * AHEAD) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; k += 2) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD / 2 - 1) : "memory");
+        const uint4 a = get(k), b = get(k + 1);
+        f(a, number(i + 32 * k));
+        f(b, number(i + 32 * k + 32));
+        fetch(k), fetch(k + 1), commit();
+      }
+      now_and_then();
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+    for (int k = 0; i < end; ++k, i += 32) f(get(k), number(i));
+    if (head && lane == 0) f(cleaned(ragged(v0)), v0);
+    if (tail && lane == 1) f(cleaned(ragged(v1 - 1)), v1 - 1);
+  }
+  template <typename F> __device__ __forceinline__ void vectors(F f) const {
+    vectors(f, [] {});
+  }
+  template <typename F, typename G> __device__ __forceinline__ void vectors(F f, G now_and_then) const {
+    if constexpr (MEM) {
+      stream<true, true>(f, now_and_then);
+    } else {
+#pragma unroll 2
+      for (uint32_t i = seg0 + lane; i < seg1; i += 32) f(data[i], i);
+    }
+  }
   // f(x, index) for every entry of this thread
   template <typename F> __device__ __forceinline__ void each(F f) const {
-    for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
-      float v[N];
-      E::get(data[i], v);
+    vectors([&](const uint4& v, uint32_t i) {
+      float z[N];
+      E::get(v, z);
       const int j0 = first + (int)(i * N);
 #pragma unroll
-      for (int e = 0; e < N; ++e) f(v[e], j0 + e);
-    }
+      for (int e = 0; e < N; ++e) f(z[e], j0 + e);
+    });
   }
 
   __device__ __forceinline__ float weight(float v) const { return row_exp2(row_neg_y(v, m, c)); }
@@ -524,7 +608,7 @@ template <typename T> struct Row {
     V before = 0;
     all = 0;
 #pragma unroll
-    for (int w = 0; w < ROW_WARPS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const V s = scratch[w];
       if (w < wid) before += s;
       all += s;
@@ -536,9 +620,9 @@ template <typename T> struct Row {
   // The mass of this thread's entries (ABOVE: of those over `over`, and
   // f(x, index) for those from `low` to `over`).  Per entry: a half of four
   // packed additions, a half of one packed multiplication, the exponential and
-  // one integer addition.  At most 256 entries
-  // come between folds, so that neither 32-bit sum of hi < 2^23 or |lo| <= 2^17
-  // wraps.
+  // one integer addition.  Fewer than 512 entries
+  // come between folds (a part in shared memory has fewer a thread), so that
+  // neither 32-bit sum of hi < 2^23 or |lo| <= 2^17 wraps.
   struct Sum {
     uint64_t m2, c2;
     uint64_t folded = 0;
@@ -563,10 +647,10 @@ template <typename T> struct Row {
         lo += __float_as_uint(b0) + __float_as_uint(b1);
       }
       n += N;
-      if (n == 256) {
-        folded = mass();
-        hi = lo = n = 0;
-      }
+    }
+    __device__ __forceinline__ void fold() {
+      folded = mass();
+      hi = lo = n = 0;
     }
     __device__ __forceinline__ uint64_t mass() const {
       return folded + row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
@@ -574,16 +658,37 @@ template <typename T> struct Row {
   };
   template <bool ABOVE, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, F f) const {
     Sum sum(m, c);
-#pragma unroll 2
-    for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
-      const uint4 v = data[i];
+    vectors([&](const uint4& v, uint32_t i) {
       sum.template add<ABOVE>(v, over);
-      if (ABOVE) each_of(hits(v, low, over), i, f);
-    }
+      if (ABOVE) each_of(hits(v, low, over), v, i, f);
+    }, [&] { sum.fold(); });
     return sum.mass();
   }
   __device__ __forceinline__ uint64_t weigh() const {
     return weigh<false>(0.0f, 0.0f, [](float, int) {});
+  }
+
+  // The same pass (from memory) also lists the entries of at least `edge`, or
+  // only finds the first of them.
+  template <bool CLEAN> __device__ __forceinline__ uint64_t weigh_and_list_of(float edge, bool only_first) {
+    Sum sum(m, c);
+    const bool lists_any = edge < INFINITY;
+    stream<CLEAN, true>([&](const uint4& v, uint32_t i) {
+      sum.template add<false>(v, 0.0f);
+      if (lists_any && E::value(E::top(E::top0(), v)) >= edge)
+        each_of(hits(v, edge, INFINITY), v, i, [&](float z, int j) {
+          if (only_first) {
+            atomicMin(&sh.first, (uint32_t)j);
+          } else {
+            const uint32_t at = atomicAdd(&sh.count, 1u);
+            if (at < ROW_LIST) sh.list[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+          }
+        });
+    }, [&] { sum.fold(); });
+    return sum.mass();
+  }
+  __device__ __forceinline__ uint64_t weigh_and_list(float edge, bool only_first) {
+    return dirty ? weigh_and_list_of<true>(edge, only_first) : weigh_and_list_of<false>(edge, only_first);
   }
 
   // Bits of the entries of a vector in [low, high].
@@ -596,23 +701,16 @@ template <typename T> struct Row {
     return mask;
   }
   // f(x, index) for the entries of vector i of this CTA's part that mask names
-  template <typename F> __device__ __forceinline__ void each_of(uint32_t mask, uint32_t i, F f) const {
+  template <typename F> __device__ __forceinline__ void each_of(uint32_t mask, const uint4& v, uint32_t i, F f) const {
     while (mask) {
       const int e = __ffs((int)mask) - 1;
       mask &= mask - 1;
-      f(E::one(data, i * N + e), first + (int)(i * N) + e);
+      f(E::at(v, e), first + (int)(i * N) + e);
     }
   }
   // Calls f(x, index) for the warp's entries in [low, high], many of them.
   template <typename F> __device__ __forceinline__ void between(float low, float high, F f) const {
-    constexpr int U = 4;
-    for (uint32_t i = seg0 + lane; i < seg1; i += 32 * U) {
-      uint32_t mask[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) mask[u] = i + 32 * u < seg1 ? hits(data[i + 32 * u], low, high) : 0;
-#pragma unroll
-      for (int u = 0; u < U; ++u) each_of(mask[u], i + 32 * u, f);
-    }
+    vectors([&](const uint4& v, uint32_t i) { each_of(hits(v, low, high), v, i, f); });
   }
   // The same, where few of the warp's threads have any above low: the warp
   // looks through the vectors of one such thread at a time.
@@ -621,7 +719,10 @@ template <typename T> struct Row {
     while (threads) {
       const uint32_t owner = __ffs((int)threads) - 1;
       threads &= threads - 1;
-      for (uint32_t i = seg0 + owner + 32 * lane; i < seg1; i += 32 * 32) each_of(hits(data[i], low, INFINITY), i, f);
+      for (uint32_t i = seg0 + owner + 32 * lane; i < seg1; i += 32 * 32) {
+        const uint4 v = data[i];
+        each_of(hits(v, low, INFINITY), v, i, f);
+      }
     }
   }
 
@@ -635,7 +736,7 @@ template <typename T> struct Row {
   __device__ __forceinline__ float edge_of(uint32_t k, float scale, float last) {
     const uint32_t tops = top_count() * lists;
     scale = fminf(scale, ROW_F32_MAX);
-    for (uint32_t i = tid; i < tops; i += ROW_THREADS) {
+    for (uint32_t i = tid; i < tops; i += NT) {
       const float z = row_unkey(sh.tops[i]);
       if (z > -INFINITY)
         atomicAdd(&sh.edge_n[(uint32_t)fminf(__fmul_rn(__fsub_rn(m, z), scale), (float)(ROW_EDGE_BINS - 1))], 1u);
@@ -670,7 +771,7 @@ template <typename T> struct Row {
     }
     low = row_unkey(__reduce_max_sync(~0u, row_key(low)));
     __syncthreads();
-    sh.edge_n[tid] = 0;
+    for (int b = tid; b < ROW_EDGE_BINS; b += NT) sh.edge_n[b] = 0;
     __syncthreads();
     return (ROW_EDGE_BINS - 2) / fmaxf(m - low, 0x1p-20f);
   }
@@ -680,31 +781,34 @@ template <typename T> struct Row {
   }
 
   // Hands this warp's masses to the first CTA (ALL: to every CTA).
-  template <bool ALL> __device__ __forceinline__ void hand(uint64_t (&to)[ROW_MAX_CLUSTER][ROW_WARPS], uint64_t own) {
+  template <bool ALL> __device__ __forceinline__ void hand(Sums& to, uint64_t own) {
     own = warp_sum_u64(own);
     if (lane < (ALL ? (int)ctas : 1)) *cluster.map_shared_rank(&to[rank][wid], lane) = own;
   }
   // Sums of what was handed over.
-  __device__ __forceinline__ uint64_t handed(const uint64_t (&of)[ROW_MAX_CLUSTER][ROW_WARPS]) const {
+  __device__ __forceinline__ uint64_t handed(const Sums& of) const {
     uint64_t t = 0;
-    for (uint32_t i = lane; i < ctas * ROW_WARPS; i += 32) t += (&of[0][0])[i];
+    for (uint32_t i = lane; i < ctas * WARPS; i += 32) t += (&of[0][0])[i];
     return warp_sum_u64(t);
   }
   // The first CTA's list of candidates is divided among the CTAs.
   __device__ __forceinline__ uint32_t share() const { return ROW_LIST / ctas; }
   // Collects this CTA's entries of at least `edge` in its share of the first
-  // CTA's list, and tells every CTA their number (sh.count = 0 before).
+  // CTA's list (sh.count = 0 before); then tells every CTA their number.
   __device__ __forceinline__ void collect_above(float edge) {
     const uint32_t room = share();
     above(edge, [&](float z, int j) {
       const uint32_t at = atomicAdd(&sh.count, 1u);
       if (at < room) sh.list[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
     });
+  }
+  __device__ __forceinline__ void tell_list() {
+    const uint32_t room = share();
     __syncthreads();
     if (tid < (int)ctas) *cluster.map_shared_rank(&sh.n[rank], tid) = sh.count;
     if (rank) {
       uint64_t* const to = cluster.map_shared_rank(sh.list, 0) + rank * room;
-      for (uint32_t i = tid; i < min(sh.count, room); i += ROW_THREADS) to[i] = sh.list[i];
+      for (uint32_t i = tid; i < min(sh.count, room); i += NT) to[i] = sh.list[i];
     }
   }
   // Whether the candidates of all CTAs fit their shares; their total.
@@ -717,7 +821,7 @@ template <typename T> struct Row {
   // f(number, entry) for this thread's candidates, on the first CTA.
   template <typename F> __device__ __forceinline__ void each_listed(F f) const {
     const uint32_t room = share();
-    for (uint32_t s = tid; s < room * ctas; s += ROW_THREADS) {
+    for (uint32_t s = tid; s < room * ctas; s += NT) {
       uint32_t before = 0, mine_n = 0, at = s;
       for (uint32_t i = 0; i < ctas; ++i) {
         const bool in = s >= i * room;
@@ -743,17 +847,13 @@ template <typename T> struct Row {
     }
     if (n <= room && rank) {
       uint64_t* const to = cluster.map_shared_rank(sh.pool, 0) + base;
-      for (uint32_t i = tid; i < sh.n[rank]; i += ROW_THREADS) to[i] = sh.pool[i];
+      for (uint32_t i = tid; i < sh.n[rank]; i += NT) to[i] = sh.pool[i];
     }
     return n;
   }
   // The end of the cluster's common work: true on the first CTA, once the
   // others' writes into it are there; the others are done.
   __device__ __forceinline__ bool last_part() {
-    if (again) {  // another row follows
-      cluster.sync();
-      return rank == 0;
-    }
     cluster.barrier_arrive();
     if (rank) return false;
     cluster.barrier_wait();
@@ -808,13 +908,13 @@ template <typename T> struct Row {
   // Else it ends in the last bin with anything; a count that is not reached,
   // beyond all of them.
   __device__ __forceinline__ void end_bins(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n, float top_w) {
-    constexpr int PER = ROW_BINS / ROW_THREADS;
+    constexpr int PER = (ROW_BINS + NT - 1) / NT;
     float s[PER], own = 0, all;
     uint32_t filled = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int b = tid * PER + i;
-      s[i] = (float)sh.bins[b];
+      s[i] = b < ROW_BINS ? (float)sh.bins[b] : 0.0f;
       if (s[i] > 0.0f) filled = b;
       if (by_mass) s[i] *= by_weight ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w;
       own += s[i];
@@ -826,6 +926,7 @@ template <typename T> struct Row {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const bool last = tid * PER + i == ROW_BINS - 1;
+      if (tid * PER + i >= ROW_BINS) break;
       if (run < goal && (run + s[i] >= goal || last)) sh.above = above_n + (uint32_t)run;  // read for counts alone
       run += s[i];
       if (run * (1.0f + slack) + more >= goal) atomicMin(&sh.b1, (uint32_t)(tid * PER + i));
@@ -867,23 +968,35 @@ template <typename T> struct Row {
   static __device__ __forceinline__ float held(float w) {
     return w < 0x1p-17f ? __fsub_rn(__fadd_rn(w, ROW_MAGIC), ROW_MAGIC) : w;
   }
-  __device__ __noinline__ void narrow(bool by_mass, uint64_t target, float least_w, uint32_t most, uint32_t& n,
-                                      uint32_t& above_n) {
+  struct Left {
+    uint32_t n, above_n;
+  };
+  __device__ __forceinline__ Left narrow(bool by_mass, uint64_t target, float least_w, uint32_t most) const {
+    return narrow_copy(*this, by_mass, target, least_w, most);
+  }
+  // Not inlined, for its size; on a copy, so that the row's own members may
+  // stay in registers everywhere else.
+  static __device__ __noinline__ Left narrow_copy(Row r, bool by_mass, uint64_t target, float least_w, uint32_t most) {
+    Left left;
+    r.narrow_into(by_mass, target, least_w, most, left.n, left.above_n);
+    return left;
+  }
+  __device__ __forceinline__ void narrow_into(bool by_mass, uint64_t target, float least_w, uint32_t most, uint32_t& n,
+                                              uint32_t& above_n) {
     uint64_t lo = (uint64_t)row_key(m) << ROW_IDX_BITS, hi = (uint64_t)row_key(-ROW_F32_MAX) << ROW_IDX_BITS | (ROW_MAX_COLS - 1);
     uint64_t above_q = 0;
     above_n = 0;
     constexpr int ROUNDS = 16;
     for (int round = 0; round < ROUNDS; ++round) {
       cluster.sync();  // what was there has been read
-      for (int b = tid; b < ROW_BINS; b += ROW_THREADS) sh.bins[b] = 0;
+      for (int b = tid; b < ROW_BINS; b += NT) sh.bins[b] = 0;
       if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ~0u, sh.last = 0;
       __syncthreads();
       const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
       const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w, c42 = fminf(c * ROW_BIN_SCALE, ROW_F32_MAX);
       const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), c42)) >= bin_at(place_of(value_of(lo), c42)) + 3);
       if (round == 0) {
-#pragma unroll 2
-        for (uint32_t i = seg0 + lane; i < seg1; i += 32) count_bins(data[i], by_mass, c42);
+        vectors([&](const uint4& v, uint32_t) { count_bins(v, by_mass, c42); });
       } else {
         between(value_of(hi), value_of(lo), [&](float z, int j) {
           const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
@@ -901,7 +1014,7 @@ template <typename T> struct Row {
       cluster.sync();
       // each CTA sums a slice of the bins over the cluster, into the first CTA's
       const uint32_t slice = (ROW_BINS + ctas - 1) / ctas;
-      for (uint32_t i = tid; i < slice; i += ROW_THREADS) {
+      for (uint32_t i = tid; i < slice; i += NT) {
         const uint32_t b = rank * slice + i;
         if (b < ROW_BINS) {
           uint32_t v = 0;
@@ -964,11 +1077,13 @@ template <typename T> struct Row {
   // its bin, which grows with c.  A counting sort by bin; what shares a bin is
   // then ranked by comparing.  Returns their number.
   template <typename F> __device__ __forceinline__ uint32_t order(RowFinish& f, F in) {
-    constexpr int PER = ROW_POOL / ROW_THREADS;
+    constexpr int PER = ROW_POOL / NT;
     uint64_t c[PER];
     uint32_t bin[PER], at[PER];
-    static_assert(ROW_SORT_BINS == 4 * ROW_THREADS, "four bins a thread");
-    *reinterpret_cast<uint4*>(&f.start[4 * tid]) = make_uint4(0, 0, 0, 0);
+    constexpr int BINS = ROW_SORT_BINS / NT;
+    static_assert(BINS * NT == ROW_SORT_BINS && PER * NT == ROW_POOL, "bins and entries a thread");
+#pragma unroll
+    for (int i = 0; i < BINS; ++i) f.start[tid * BINS + i] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -976,10 +1091,12 @@ template <typename T> struct Row {
       if (in(i, c[i], bin[i])) at[i] = atomicAdd(&f.start[bin[i]], 1u);
     }
     __syncthreads();
-    const uint4 n = *reinterpret_cast<uint4*>(&f.start[4 * tid]);
-    uint32_t all;
-    const uint32_t s = block_scan(n.x + n.y + n.z + n.w, sh.scan_n, all);
-    *reinterpret_cast<uint4*>(&f.start[4 * tid]) = make_uint4(s, s + n.x, s + n.x + n.y, s + n.x + n.y + n.z);
+    uint32_t n[BINS], own = 0, all;
+#pragma unroll
+    for (int i = 0; i < BINS; ++i) n[i] = f.start[tid * BINS + i], own += n[i];
+    uint32_t before = block_scan(own, sh.scan_n, all);
+#pragma unroll
+    for (int i = 0; i < BINS; ++i) f.start[tid * BINS + i] = before, before += n[i];
     if (tid == 0) f.start[ROW_SORT_BINS] = all;
     __syncthreads();
 #pragma unroll
@@ -1007,8 +1124,8 @@ template <typename T> struct Row {
     float scale = fmaxf((ROW_SORT_BINS - 1) / (m - low), (ROW_SORT_BINS - 1) / ROW_MASS_END * c);
     if (!(scale <= ROW_F32_MAX)) scale = 0.0f;  // all equal
     order(f, [&](int i, uint64_t& e, uint32_t& bin) {
-      if (tid + i * ROW_THREADS >= n) return false;
-      e = from[tid + i * ROW_THREADS];
+      if (tid + i * NT >= n) return false;
+      e = from[tid + i * NT];
       bin = (uint32_t)fminf(__fmul_rn(__fsub_rn(m, value_of(e)), scale), (float)(ROW_SORT_BINS - 1));
       return true;
     });
@@ -1017,8 +1134,8 @@ template <typename T> struct Row {
   __device__ __forceinline__ void order_by_place(RowFinish& f, const uint64_t* from, uint32_t n, uint64_t lo, uint64_t hi) {
     const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
     order(f, [&](int i, uint64_t& e, uint32_t& bin) {
-      if (tid + i * ROW_THREADS >= n) return false;
-      e = from[tid + i * ROW_THREADS];
+      if (tid + i * NT >= n) return false;
+      e = from[tid + i * NT];
       bin = (uint32_t)((e - lo) >> shift);
       return true;
     });
@@ -1038,7 +1155,7 @@ template <typename T> struct Row {
     __syncthreads();
   }
 
-  // Cuts the n <= ROW_THREADS entries of f.loose to the first k (0: all),
+  // Cuts the n <= ROW_FEW entries of f.loose to the first k (0: all),
   // then to the shortest prefix of at least p of their mass (without k: of the
   // row's, `total`), then to w >= least_w, and draws: each thread
   // compares its entry with all others, once in descending order and once in
@@ -1050,7 +1167,7 @@ template <typename T> struct Row {
     const uint64_t e = in ? f.loose[tid] : ~0ull;
     const float z = value_of(e), w = in ? weight(z) : 0.0f;
     const uint64_t q = row_q(w);
-    f.sorted[tid] = q;
+    if (tid < ROW_FEW) f.sorted[tid] = q;
     if (tid == 0) sh.cut_q = total, sh.cut_c = ~0ull;
     __syncthreads();
     uint32_t rank_of = 0;
@@ -1086,7 +1203,7 @@ template <typename T> struct Row {
       if (own) hit(z, (int)(e & (ROW_MAX_COLS - 1)));
       return;
     }
-    f.sorted[tid] = own;  // kept masses
+    if (tid < ROW_FEW) f.sorted[tid] = own;  // kept masses
     __syncthreads();
     if (wid * 32 >= (int)n) return;
     const uint32_t j = (uint32_t)e & (ROW_MAX_COLS - 1);
@@ -1103,18 +1220,18 @@ template <typename T> struct Row {
   // `mass`: the entry at which the running mass in index order exceeds t.
   template <typename H> __device__ __forceinline__ void draw(RowFinish& f, uint32_t n, float least_w, uint64_t t, H hit) {
     const int shift = max(0, 32 - __clz((int)cols) - 10);
-    constexpr int PER = ROW_POOL / ROW_THREADS;
+    constexpr int PER = ROW_POOL / NT;
     uint64_t e[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) e[i] = tid + i * ROW_THREADS < n ? f.sorted[tid + i * ROW_THREADS] : 0;
+    for (int i = 0; i < PER; ++i) e[i] = tid + i * NT < n ? f.sorted[tid + i * NT] : 0;
     order(f, [&](int i, uint64_t& c, uint32_t& bin) {
-      if (tid + i * ROW_THREADS >= n) return false;
+      if (tid + i * NT >= n) return false;
       const uint32_t j = (uint32_t)e[i] & (ROW_MAX_COLS - 1);
       c = (uint64_t)j << 32 | (uint32_t)(e[i] >> ROW_IDX_BITS);
       bin = j >> shift;
       return true;
     });
-    const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    const uint32_t per = (n + NT - 1) / NT, i0 = min(tid * per, n), i1 = min(i0 + per, n);
     auto mass_at = [&](uint32_t i) {
       const float w = weight(row_unkey((uint32_t)f.sorted[i]));
       return w >= least_w ? row_q(w) : 0;
@@ -1134,13 +1251,13 @@ template <typename T> struct Row {
   // the threads, else at f.input, above `edge`: by sorting.
   template <typename H>
   __device__ __forceinline__ void finish_listed(RowFinish& f, uint32_t n, float edge, const RowParams& q, uint64_t total, H hit) {
-    if (n <= (uint32_t)ROW_THREADS) {
+    if (n <= (uint32_t)ROW_FEW) {
       finish_few(f, n, q.by_k ? q.k : 0, q.p, q.least_w, q.u, total, hit);
       return;
     }
     order_by_value(f, f.input, n, edge);
     // running masses in descending order, `per` entries a thread
-    const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    const uint32_t per = (n + NT - 1) / NT, i0 = min(tid * per, n), i1 = min(i0 + per, n);
     uint64_t sum = 0, all;
     for (uint32_t i = i0; i < i1; ++i) sum += mass(value_of(f.sorted[i]));
     const uint64_t before = block_scan(sum, sh.scan_q, all);
@@ -1170,7 +1287,7 @@ template <typename T> struct Row {
     uint64_t left = sh.cut_q;
     if (q.by_w) {
       sum = 0;
-      for (uint32_t i = tid; i < cut; i += ROW_THREADS) {
+      for (uint32_t i = tid; i < cut; i += NT) {
         const float w = weight(value_of(f.sorted[i]));
         if (w >= q.least_w) sum += row_q(w);
       }
@@ -1189,7 +1306,7 @@ template <typename T> struct Row {
     order_by_place(f, sh.pool, n, lo, hi);
     uint32_t cut = n;
     if (p.by_p) {
-      const uint32_t per = (n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+      const uint32_t per = (n + NT - 1) / NT, i0 = min(tid * per, n), i1 = min(i0 + per, n);
       uint64_t sum = 0, all;
       for (uint32_t i = i0; i < i1; ++i) sum += mass(value_of(f.sorted[i]));
       uint64_t run = above + block_scan(sum, sh.scan_q, all);
@@ -1207,29 +1324,29 @@ template <typename T> struct Row {
     }
     const uint64_t last = cut ? f.sorted[cut - 1] : hi;
     // the warps' kept masses: before the interval, and those of its entries
-    if (tid < ROW_MAX_CLUSTER * ROW_WARPS) f.part[tid][0] = f.part[tid][1] = 0;
+    if (tid < ROW_SUMS) f.part[tid][0] = f.part[tid][1] = 0;
     __syncthreads();
-    for (uint32_t i = tid; i < cut; i += ROW_THREADS) {
+    for (uint32_t i = tid; i < cut; i += NT) {
       const uint64_t e = f.sorted[i];
       const float w = weight(value_of(e));
       const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + lead) / N;
       const uint32_t cta = v / part_vecs, p0 = cta * part_vecs, p1 = min(p0 + part_vecs, total_vecs);
-      const uint32_t warp = (v - p0) / ((p1 - p0 + ROW_WARPS - 1) / ROW_WARPS);
+      const uint32_t warp = (v - p0) / ((p1 - p0 + WARPS - 1) / WARPS);
       if (w >= p.least_w) {
         const uint64_t q = row_q(w);
-        atomicAdd(&f.part[cta * ROW_WARPS + warp][0], (uint32_t)q & 0xfffffu);
-        atomicAdd(&f.part[cta * ROW_WARPS + warp][1], (uint32_t)(q >> 20));
+        atomicAdd(&f.part[cta * WARPS + warp][0], (uint32_t)q & 0xfffffu);
+        atomicAdd(&f.part[cta * WARPS + warp][1], (uint32_t)(q >> 20));
       }
     }
     __syncthreads();
-    if (tid < ROW_MAX_CLUSTER * ROW_WARPS) (&sh.part[0][0])[tid] += ((uint64_t)f.part[tid][1] << 20) + f.part[tid][0];
+    if (tid < CTAS * WARPS) (&sh.part[0][0])[tid] += ((uint64_t)f.part[tid][1] << 20) + f.part[tid][0];
     __syncthreads();
     return last;
   }
 
   // Writes the first `have` of f.sorted as the row's best.
   __device__ __forceinline__ void put_best(const RowArgs& a, uint32_t row, const RowFinish& f, uint32_t have, float ln) const {
-    for (int i = tid; i < a.n; i += ROW_THREADS) {
+    for (int i = tid; i < a.n; i += NT) {
       const bool in = i < (int)have;
       const uint64_t e = in ? f.sorted[i] : 0;
       a.best_idx[(int64_t)row * a.n + i] = in ? (int)(e & (ROW_MAX_COLS - 1)) : -1;
@@ -1237,7 +1354,7 @@ template <typename T> struct Row {
     }
   }
   __device__ __forceinline__ void put_nothing(const RowArgs& a, uint32_t row) const {
-    for (int i = tid; i < a.n; i += ROW_THREADS)
+    for (int i = tid; i < a.n; i += NT)
       a.best_idx[(int64_t)row * a.n + i] = -1, a.best_logprob[(int64_t)row * a.n + i] = -INFINITY;
     if (a.lse && tid == 0) a.lse[row] = -INFINITY;
   }
@@ -1247,7 +1364,7 @@ template <typename T> struct Row {
   // exceeds t calls hit(x, index), on one thread.
   template <typename V, typename H>
   __device__ __forceinline__ void scan_memory(uint32_t v0, uint32_t v1, uint64_t t, V value, H hit) {
-    for (uint32_t i0 = v0; i0 < v1; i0 += ROW_THREADS) {
+    for (uint32_t i0 = v0; i0 < v1; i0 += NT) {
       const uint32_t i = i0 + tid;
       const uint4 v = i < v1 ? from_memory(i) : nothing();
       const int j0 = (int)(i * N) - lead;
@@ -1274,10 +1391,10 @@ template <typename T> struct Row {
   }
   // The same over the cluster's parts, given the sum of each warp's stretch.
   template <typename V, typename H>
-  __device__ __forceinline__ void scan_parts(const uint64_t (&of)[ROW_MAX_CLUSTER][ROW_WARPS], uint64_t t, V value, H hit) {
+  __device__ __forceinline__ void scan_parts(const Sums& of, uint64_t t, V value, H hit) {
     // each warp finds the stretch for itself: lanes hold up to four sums each, in order
-    constexpr int PER = ROW_MAX_CLUSTER * ROW_WARPS / 32;
-    const uint32_t count = ctas * ROW_WARPS;
+    constexpr int PER = (CTAS * WARPS + 31) / 32;
+    const uint32_t count = ctas * WARPS;
     uint64_t s[PER], own = 0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
@@ -1299,7 +1416,7 @@ template <typename T> struct Row {
     which = __shfl_sync(~0u, which, owner) - 1;
     left = __shfl_sync(~0u, left, owner);
     uint32_t v0, v1;
-    stretch(which / ROW_WARPS, which % ROW_WARPS, v0, v1);
+    stretch(which / WARPS, which % WARPS, v0, v1);
     scan_memory(v0, v1, left, value, hit);
   }
 };
@@ -1314,9 +1431,10 @@ template <typename T> struct Row {
 //
 // A cut that does not end among the candidates (a nucleus beyond the guess,
 // a large top_k, many equal values) keeps the cluster to narrow it down.
-template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, RowShared& sh, uint4* data) {
+template <typename T, int NT, bool MEM>
+__device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typename Row<T, NT, MEM>::Shared& sh, uint4* data) {
   RowFinish& f = *reinterpret_cast<RowFinish*>(data);
-  Row<T> r(sh, data, a, row, cg::this_cluster().block_rank(), cg::this_cluster().num_blocks());
+  Row<T, NT, MEM> r(sh, data, a, row, MEM ? 0 : cg::this_cluster().block_rank(), MEM ? 1 : cg::this_cluster().num_blocks(), MEM ? 2 : 1);
   const RowParams q(a, row);
   r.load(q.by_k || q.by_p);
   if (r.m == -INFINITY) {
@@ -1334,9 +1452,14 @@ template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& 
     a.tokens[row] = j;
     if (a.logprobs) a.logprobs[row] = row_neg_y(z, r.m, r.c) * ROW_LN2 - logf((float)total * 0x1p-40f);
   };
-  if (q.greedy)
-    r.above(r.m, [&](float, int j) { atomicMin(r.cluster.map_shared_rank(&sh.first, 0), (uint32_t)j); });
-  const uint64_t own = r.weigh();
+  const float edge = q.cuts() ? r.edge_for(q) : q.greedy ? r.m : INFINITY;
+  uint64_t own;
+  if constexpr (MEM) {
+    own = r.weigh_and_list(edge, q.greedy);
+  } else {
+    if (q.greedy) r.above(r.m, [&](float, int j) { atomicMin(r.cluster.map_shared_rank(&sh.first, 0), (uint32_t)j); });
+    own = r.weigh();
+  }
   if (!q.cuts()) {
     r.template hand<false>(sh.mass, own);
     if (!r.last_part()) return;
@@ -1349,13 +1472,13 @@ template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& 
   }
 
   // ---- candidates ----
-  const float edge = r.edge_for(q);
   r.template hand<true>(sh.mass, own);
   if (edge < INFINITY) {
-    r.collect_above(edge);
+    if constexpr (!MEM) r.collect_above(edge);
+    r.tell_list();
     if (q.by_p && !q.by_k) {
       uint64_t part = 0;
-      for (uint32_t i = r.tid; i < min(sh.count, r.share()); i += ROW_THREADS) part += r.mass(r.value_of(sh.list[i]));
+      for (uint32_t i = r.tid; i < min(sh.count, r.share()); i += NT) part += r.mass(r.value_of(sh.list[i]));
       r.template hand<true>(sh.part, part);
     }
   }
@@ -1370,7 +1493,7 @@ template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& 
   if (enough && !q.by_k && q.by_p) enough = r.handed(sh.part) >= row_target(q.p, total);
   if (enough) {
     if (r.rank) return;
-    uint64_t* const to = n <= (uint32_t)ROW_THREADS ? f.loose : f.input;
+    uint64_t* const to = n <= (uint32_t)ROW_FEW ? f.loose : f.input;
     r.each_listed([&](uint32_t i, uint64_t e) { to[i] = e; });
     __syncthreads();
     r.finish_listed(f, n, edge, q, total, store);
@@ -1380,9 +1503,10 @@ template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& 
   // ---- a cut beyond the candidates ----
   uint64_t last = ~0ull;  // the last entry of the cut
   if (q.by_k || q.by_p) {
-    uint32_t above_n;
+    typename Row<T, NT, MEM>::Left left{0, 0};
     uint64_t target = k;
-    if (q.by_k) r.narrow(false, k, least_w, q.by_p ? ROW_FEW : ROW_POOL, n, above_n);
+    if (q.by_k) left = r.narrow(false, k, least_w, q.by_p ? ROW_FEW : ROW_POOL);
+    const uint32_t above_n = left.above_n;
     if (q.by_p) {
       uint64_t mass = total;
       if (q.by_k) {
@@ -1392,7 +1516,7 @@ template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& 
           r.cluster.barrier_wait();
           if (r.tid == 0) sh.cut_q = total - above;
           __syncthreads();
-          r.nth_of_few(n, k - above_n);
+          r.nth_of_few(left.n, k - above_n);
           if (r.tid < (int)r.ctas) *r.cluster.map_shared_rank(&sh.cut_q, r.tid) = above + sh.cut_q;
         } else {
           r.cluster.sync();
@@ -1401,10 +1525,10 @@ template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& 
         mass = sh.cut_q;
       }
       target = row_target(q.p, mass);
-      r.narrow(true, target, least_w, ROW_POOL, n, above_n);
+      left = r.narrow(true, target, least_w, ROW_POOL);
     }
     if (!r.last_part()) return;
-    last = r.finish_pool(f, n, q, q.by_p ? target : k - above_n);
+    last = r.finish_pool(f, left.n, q, q.by_p ? target : k - above_n);
   } else {  // min_p alone
     uint64_t kept = 0;
     r.each([&](float z, int) {
@@ -1426,9 +1550,10 @@ template <typename T> __device__ __forceinline__ void row_sample(const RowArgs& 
 
 // ---- the n best ---------------------------------------------------------------------
 // As a sampling row with top_k = n, whose ordered candidates are the answer.
-template <typename T> __device__ __forceinline__ void row_best(const RowArgs& a, uint32_t row, RowShared& sh, uint4* data) {
+template <typename T, int NT, bool MEM>
+__device__ __forceinline__ void row_best(const RowArgs& a, uint32_t row, typename Row<T, NT, MEM>::Shared& sh, uint4* data) {
   RowFinish& f = *reinterpret_cast<RowFinish*>(data);
-  Row<T> r(sh, data, a, row, cg::this_cluster().block_rank(), cg::this_cluster().num_blocks());
+  Row<T, NT, MEM> r(sh, data, a, row, MEM ? 0 : cg::this_cluster().block_rank(), MEM ? 1 : cg::this_cluster().num_blocks(), MEM ? 2 : 1);
   r.load(true);
   if (r.m == -INFINITY) {
     if (r.rank == 0) r.put_nothing(a, row);
@@ -1436,10 +1561,14 @@ template <typename T> __device__ __forceinline__ void row_best(const RowArgs& a,
   }
   r.c = ROW_LOG2E;
   const uint32_t k = (uint32_t)a.n;
-  float edge = INFINITY;
-  r.template hand<true>(sh.mass, r.weigh());
-  edge = r.edge_for_best(k);
-  if (edge < INFINITY) r.collect_above(edge);
+  float edge = r.edge_for_best(k);
+  if constexpr (MEM) {
+    r.template hand<true>(sh.mass, r.weigh_and_list(edge, false));
+  } else {
+    r.template hand<true>(sh.mass, r.weigh());
+    if (edge < INFINITY) r.collect_above(edge);
+  }
+  r.tell_list();
   r.cluster.sync();
   uint32_t n = 0;
   const bool listed = edge < INFINITY && r.all_listed(n);
@@ -1451,11 +1580,10 @@ template <typename T> __device__ __forceinline__ void row_best(const RowArgs& a,
     __syncthreads();
   } else {
     // the n-th entry, then the entries up to it
-    uint32_t above_n;
-    r.narrow(false, k, 0.0f, ROW_FEW, n, above_n);
+    const auto left = r.narrow(false, k, 0.0f, ROW_FEW);
     r.cluster.sync();
     if (r.rank == 0) {
-      r.nth_of_few(n, k - above_n);
+      r.nth_of_few(left.n, k - left.above_n);
       if (r.tid > 0 && r.tid < (int)r.ctas) *r.cluster.map_shared_rank(&sh.hi, r.tid) = sh.hi;
     }
     if (r.tid == 0) sh.count = 0;
@@ -1478,19 +1606,25 @@ template <typename T> __device__ __forceinline__ void row_best(const RowArgs& a,
   r.put_best(a, row, f, min(n, k), ln);
 }
 
-// One cluster a row, or the listed rows in turn.
-template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_THREADS, ROW_MINB) k_rows(const RowArgs a) {
+// One cluster a row.
+constexpr int ROW_CLUSTER_THREADS = 256;
+template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_CLUSTER_THREADS, 3) k_row_cluster(const RowArgs a) {
   extern __shared__ __align__(16) unsigned char row_smem[];
-  RowShared& sh = *reinterpret_cast<RowShared*>(row_smem);
-  uint4* const data = reinterpret_cast<uint4*>(row_smem + ROW_SHARED_BYTES);
-  const uint32_t ctas = cg::this_cluster().num_blocks(), id = blockIdx.x / ctas;
-  if (a.only) row_chain_wait();
-  const uint32_t n = a.only ? *a.only_n : a.rows, step = a.only ? gridDim.x / ctas : a.rows;
-  for (uint32_t i = id; i < n; i += step) {
-    const uint32_t row = a.only ? a.only[i] : i;
-    BEST ? row_best<T>(a, row, sh, data) : row_sample<T>(a, row, sh, data);
-    if (a.only) cg::this_cluster().sync();  // nobody's shared memory is written any more
-  }
+  using R = Row<T, ROW_CLUSTER_THREADS, false>;
+  static_assert(3 * (R::SHARED_BYTES + (64 << 10) + 1024) <= 228 << 10, "three CTAs on an SM");
+  typename R::Shared& sh = *reinterpret_cast<typename R::Shared*>(row_smem);
+  uint4* const data = reinterpret_cast<uint4*>(row_smem + R::SHARED_BYTES);
+  const uint32_t row = blockIdx.x / cg::this_cluster().num_blocks();
+  BEST ? row_best<T, ROW_CLUSTER_THREADS, false>(a, row, sh, data) : row_sample<T, ROW_CLUSTER_THREADS, false>(a, row, sh, data);
+}
+
+// One CTA a row.
+template <typename T, int NT, bool BEST> __global__ void __launch_bounds__(NT, 1024 / NT) k_row_solo(const RowArgs a) {
+  extern __shared__ __align__(16) unsigned char row_smem[];
+  using R = Row<T, NT, true>;
+  typename R::Shared& sh = *reinterpret_cast<typename R::Shared*>(row_smem);
+  uint4* const data = reinterpret_cast<uint4*>(row_smem + R::SHARED_BYTES);
+  BEST ? row_best<T, NT, true>(a, blockIdx.x, sh, data) : row_sample<T, NT, true>(a, blockIdx.x, sh, data);
 }
 
 }  // namespace fs

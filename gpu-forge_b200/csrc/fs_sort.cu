@@ -91,8 +91,7 @@ struct fs_sorter {
   static constexpr int MAX_TIMED = 24;
   cudaEvent_t ev[2 * MAX_TIMED] = {};
   int ev_used = 0;
-  cudaMemPool_t pool = nullptr;  // stream-ordered scratch of the serving operators
-  uint64_t row_pass_min = 8ull << 20;  // FORGESORT_ROW_PASS_MIN_BYTES
+  int row_form = 0;  // FORGESORT_ROW_FORM
   HostStage stage;  // page-locked chunk ring for pageable host-slice copies
   int test_withhold = 0;    // fs_test_inject(FS_TEST_WITHHOLD_COPY): next radix sort
   int test_fail_alloc = 0;  // fs_test_inject(FS_TEST_FAIL_ALLOC): countdown to a failed growth
@@ -1176,22 +1175,7 @@ namespace fs {
 int sorter_view(fs_sorter* s, void* stream, SorterView* v) {
   const int rc = set_device(s);
   if (rc) return rc;
-  if (!s->pool) {
-    cudaMemPoolProps props{};
-    props.allocType = cudaMemAllocationTypePinned;
-    props.location.type = cudaMemLocationTypeDevice;
-    props.location.id = s->device;
-    cudaMemPool_t pool = nullptr;
-    FS_CUDA(s, cudaMemPoolCreate(&pool, &props));
-    uint64_t keep = ~0ull;  // freed scratch stays with the pool
-    const cudaError_t e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
-    if (e != cudaSuccess) {
-      cudaMemPoolDestroy(pool);
-      return cuda_fail(s, e, "cudaMemPoolSetAttribute");
-    }
-    s->pool = pool;
-  }
-  *v = SorterView{s->device, s->sm_count, stream ? static_cast<cudaStream_t>(stream) : s->stream, s->host_err_dev, s->pool, s->row_pass_min};
+  *v = SorterView{s->device, s->sm_count, stream ? static_cast<cudaStream_t>(stream) : s->stream, s->host_err_dev, s->row_form};
   return FS_OK;
 }
 
@@ -1270,9 +1254,9 @@ int fs_create(int device, void* stream, fs_sorter** out) {
     const long long v = atoll(t);
     s->coop_max_bytes = v <= 0 ? 0ull : (uint64_t)v;
   }
-  if (const char* t = getenv("FORGESORT_ROW_PASS_MIN_BYTES")) {
-    const long long v = atoll(t);
-    s->row_pass_min = v < 0 ? 0ull : (uint64_t)v;
+  if (const char* t = getenv("FORGESORT_ROW_FORM")) {
+    const int v = atoi(t);
+    s->row_form = v >= 1 && v <= 3 ? v : 0;
   }
   if (const char* t = getenv("FORGESORT_H16_MIN_KEYS")) {  // keys; 0: never the histogram fill
     const long long v = atoll(t);
@@ -1308,7 +1292,6 @@ int fs_destroy(fs_sorter* s) {
   for (void* b : bufs)
     if (b) cudaFree(b);
   if (s->host_err) cudaFreeHost(s->host_err);
-  if (s->pool) cudaMemPoolDestroy(s->pool);
   for (cudaEvent_t e : s->ev)
     if (e) cudaEventDestroy(e);
   if (s->own_stream) cudaStreamDestroy(s->own_stream);

@@ -14,12 +14,12 @@ pytestmark = pytest.mark.gpu
 DT = ["f32", "f16", "bf16"]
 
 
-@pytest.fixture(scope="module", params=["clusters", "passes"])
+@pytest.fixture(scope="module", params=[1, 2, 3], ids=["cluster", "solo512", "solo1024"])
 def gs(request):
-    """Both forms for every case: one cluster a row, and passes over the batch."""
+    """Every form for every case: a cluster a row, and a CTA of 512 or 1024 threads a row."""
     import forge_sort
     with pytest.MonkeyPatch.context() as mp:
-        mp.setenv("FORGESORT_ROW_PASS_MIN_BYTES", "0" if request.param == "passes" else str(1 << 40))
+        mp.setenv("FORGESORT_ROW_FORM", str(request.param))
         s = forge_sort.GpuSampler.new()
     yield s
     s.close()
