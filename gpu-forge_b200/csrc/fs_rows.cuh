@@ -81,6 +81,11 @@ __device__ __forceinline__ float fmax_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ uint4 smem_load(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
 // Word k of a vector, by selections (an index would put it in local memory).
 __device__ __forceinline__ uint32_t row_word(const uint4& v, int k) {
   uint32_t w = v.x;
@@ -209,7 +214,7 @@ __device__ __forceinline__ float row_neg_y(float x, float m, float c) { return _
 // push the unwanted bits out of the mantissa: hi = w to a multiple of 2^-23
 // (the mantissa bits of w + 1), lo = the rest to a multiple of 2^-40 (the
 // mantissa bits of rest + 1.5 2^-17).  Each addition rounds half to even and
-// w - hi is exact.  (A conversion to an integer runs at the rate of the
+// w - hi, and 1 + 1.5 2^-17 - (w + 1), are exact.  (A conversion to an integer runs at the rate of the
 // exponential, an eighth of that of these additions.)
 constexpr float ROW_MAGIC = 1.5f / 131072.0f;
 constexpr uint32_t ROW_ONE_BITS = 0x3f800000u;    // 1.0f
@@ -533,7 +538,7 @@ template <typename T, int NT, bool MEM> struct Row {
 
   // f(vector, number in the part) for this thread's vectors, two side by side;
   // from memory, with +inf and NaN as they are unless CLEAN; now_and_then() is
-  // called every AHEAD vectors.  BACK: from the
+  // called every 32 vectors.  BACK: from the
   // stretch's end, which was read last and is in L2 for the longest.
   template <bool CLEAN, bool BACK, typename F, typename G> __device__ __forceinline__ void stream(F f, G now_and_then) const {
     uint32_t v0, v1;
@@ -542,33 +547,34 @@ template <typename T, int NT, bool MEM> struct Row {
     const uint32_t lo = v0 + head, end = v1 - tail;
     uint32_t i = lo + lane, next = i;
     auto number = [&](uint32_t n) { return BACK ? lo + end - 1 - n : n; };
-    const uint32_t slot = smem_of(data + tid);
-    auto fetch = [&](int k) {
+    constexpr uint32_t STEP = NT * 16;
+    const uint32_t slots = smem_of(data + tid);
+    auto fetch = [&](uint32_t slot) {
       if (next < end)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + k * (NT * 16)), "l"(vecs + number(next)) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot), "l"(vecs + number(next)) : "memory");
       next += 32;
     };
     auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-    auto get = [&](int k) {
-      const uint4 v = data[k * NT + tid];
+    auto get = [&](uint32_t slot) {
+      const uint4 v = smem_load(slot);
       return CLEAN ? cleaned(v) : v;
     };
 #pragma unroll
-    for (int k = 0; k < AHEAD; k += 2) fetch(k), fetch(k + 1), commit();
-    for (; i + 32 * (AHEAD - 1) < end; i += 32 * AHEAD) {
-#pragma unroll
-      for (int k = 0; k < AHEAD; k += 2) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD / 2 - 1) : "memory");
-        const uint4 a = get(k), b = get(k + 1);
-        f(a, number(i + 32 * k));
-        f(b, number(i + 32 * k + 32));
-        fetch(k), fetch(k + 1), commit();
-      }
-      now_and_then();
+    for (int k = 0; k < AHEAD; k += 2) fetch(slots + k * STEP), fetch(slots + (k + 1) * STEP), commit();
+    uint32_t slot = slots, turns = 0;
+#pragma unroll 1
+    for (; i + 32 < end; i += 64) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD / 2 - 1) : "memory");
+      const uint4 a = get(slot), b = get(slot + STEP);
+      f(a, number(i));
+      f(b, number(i + 32));
+      fetch(slot), fetch(slot + STEP), commit();
+      slot += 2 * STEP;
+      if (slot == slots + AHEAD * STEP) slot = slots;
+      if (++turns % 16 == 0) now_and_then();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 1
-    for (int k = 0; i < end; ++k, i += 32) f(get(k), number(i));
+    if (i < end) f(get(slot), number(i));
     if (head && lane == 0) f(cleaned(ragged(v0)), v0);
     if (tail && lane == 1) f(cleaned(ragged(v1 - 1)), v1 - 1);
   }
@@ -629,7 +635,7 @@ template <typename T, int NT, bool MEM> struct Row {
     uint32_t hi = 0, lo = 0, n = 0;
     __device__ __forceinline__ Sum(float m, float c) : m2(f2_pack(-m, -m)), c2(f2_pack(c, c)) {}
     template <bool ABOVE> __device__ __forceinline__ void add(const uint4& v, float over) {
-      const uint64_t one = f2_pack(1.0f, 1.0f), none = f2_pack(-1.0f, -1.0f), magic = f2_pack(ROW_MAGIC, ROW_MAGIC);
+      const uint64_t one = f2_pack(1.0f, 1.0f), none = f2_pack(-1.0f, -1.0f), both = f2_pack(1.0f + ROW_MAGIC, 1.0f + ROW_MAGIC);
       float z[N];
       E::get(v, z);
 #pragma unroll
@@ -640,7 +646,7 @@ template <typename T, int NT, bool MEM> struct Row {
         if (ABOVE) w0 = z[e] > over ? w0 : 0.0f, w1 = z[e + 1] > over ? w1 : 0.0f;
         const uint64_t w = f2_pack(w0, w1);
         const uint64_t a = f2_add(w, one);
-        const uint64_t b = f2_add(f2_fma(f2_add(a, none), none, w), magic);
+        const uint64_t b = f2_add(w, f2_fma(a, none, both));  // 1 + MAGIC - a is exact
         f2_unpack(a, a0, a1);
         f2_unpack(b, b0, b1);
         hi += __float_as_uint(a0) + __float_as_uint(a1);
