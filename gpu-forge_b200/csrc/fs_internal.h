@@ -16,7 +16,7 @@ struct SorterView {
   int sm_count;
   cudaStream_t stream;
   int* host_err;  // device alias of the mapped error word (DEV_ERR_*)
-  int row_form;   // FORGESORT_ROW_FORM: 0 by size, 1 a cluster a row, 2 / 3 a CTA of 512 / 1024 threads a row
+  int row_form;   // FORGESORT_ROW_FORM: 0 by size, 1 a cluster a row, 2 a CTA a row
 };
 
 // Makes the sorter's device current and fills *v; stream NULL: the sorter's.

@@ -73,24 +73,23 @@ template <typename T, bool BEST> int launch_clusters(fs_sorter* s, const SorterV
   return FS_OK;
 }
 
-// One CTA of NT threads a row.
-template <typename T, int NT, bool BEST> int launch_solo(fs_sorter* s, const SorterView& v, RowArgs& a) {
-  using R = Row<T, NT, true>;
+// One CTA a row.
+template <typename T, bool BEST> int launch_solo(fs_sorter* s, const SorterView& v, RowArgs& a) {
+  using R = Row<T, ROW_SOLO_THREADS, true>;
   static_assert(sizeof(RowFinish) <= R::RING_BYTES, "fits");
   constexpr size_t smem = R::SHARED_BYTES + R::RING_BYTES;
   static std::atomic<bool> configured[SORTER_MAX_DEVICES];
-  FS_ROWS_CUDA(s, configure(configured[v.device], k_row_solo<T, NT, BEST>, smem, false));
+  FS_ROWS_CUDA(s, configure(configured[v.device], k_row_solo<T, BEST>, smem, false));
   a.part_vecs = row_vecs(a, RowElem<T>::N);
-  k_row_solo<T, NT, BEST><<<a.rows, NT, smem, v.stream>>>(a);
+  k_row_solo<T, BEST><<<a.rows, ROW_SOLO_THREADS, smem, v.stream>>>(a);
   FS_ROWS_CUDA(s, cudaGetLastError());
   return FS_OK;
 }
 
 template <typename T, bool BEST> int launch(fs_sorter* s, const SorterView& v, RowArgs& a) {
-  const int form = v.row_form ? v.row_form : a.rows * 2 < (uint64_t)v.sm_count ? 1 : a.rows > (uint64_t)v.sm_count ? 2 : 3;
-  if (form == 1) return launch_clusters<T, BEST>(s, v, a);
-  if (form == 2) return launch_solo<T, 512, BEST>(s, v, a);
-  return launch_solo<T, 1024, BEST>(s, v, a);
+  const uint32_t ctas = row_ctas(row_vecs(a, RowElem<T>::N) * 16, a.rows, v.sm_count);
+  const bool solo = v.row_form ? v.row_form == 2 : ctas > 1 && (uint64_t)ctas * a.rows > 3ull * v.sm_count;
+  return solo ? launch_solo<T, BEST>(s, v, a) : launch_clusters<T, BEST>(s, v, a);
 }
 
 template <bool BEST> int launch_rows(fs_sorter* s, const SorterView& v, int dtype, RowArgs& a, int sync) {

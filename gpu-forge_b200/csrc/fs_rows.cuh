@@ -664,10 +664,18 @@ template <typename T, int NT, bool MEM> struct Row {
   };
   template <bool ABOVE, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, F f) const {
     Sum sum(m, c);
+    uint64_t has = 0;  // which of the thread's vectors f wants: they are looked at again afterwards, few and together
     vectors([&](const uint4& v, uint32_t i) {
       sum.template add<ABOVE>(v, over);
-      if (ABOVE) each_of(hits(v, low, over), v, i, f);
+      if (ABOVE && MEM) each_of(hits(v, low, over), v, i, f);
+      if (ABOVE && !MEM) has |= (uint64_t)any_hit(v, low, over) << ((i - seg0) / 32);
     }, [&] { sum.fold(); });
+    while (ABOVE && !MEM && has) {
+      const uint32_t i = seg0 + lane + 32 * (__ffsll((long long)has) - 1);
+      has &= has - 1;
+      const uint4 v = data[i];
+      each_of(hits(v, low, over), v, i, f);
+    }
     return sum.mass();
   }
   __device__ __forceinline__ uint64_t weigh() const {
@@ -705,6 +713,14 @@ template <typename T, int NT, bool MEM> struct Row {
 #pragma unroll
     for (int e = 0; e < N; ++e) mask |= (uint32_t)(z[e] >= low && z[e] <= high) << e;
     return mask;
+  }
+  static __device__ __forceinline__ bool any_hit(const uint4& v, float low, float high) {
+    float z[N];
+    E::get(v, z);
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) any |= z[e] >= low && z[e] <= high;
+    return any;
   }
   // f(x, index) for the entries of vector i of this CTA's part that mask names
   template <typename F> __device__ __forceinline__ void each_of(uint32_t mask, const uint4& v, uint32_t i, F f) const {
@@ -892,7 +908,7 @@ template <typename T, int NT, bool MEM> struct Row {
   // A vector's entries by bin of 1/42 octave: their number, or their weights as
   // 4096 2^-(y - b) / 42 by the power's tangent, made a whole number by another
   // addition of 2^23.
-  __device__ __forceinline__ void count_bins(const uint4& v, bool by_mass, float c42) const {
+  __device__ __forceinline__ void count_bins(const uint4& v, bool by_mass, float c42, float y_end) const {
     float z[N];
     E::get(v, z);
 #pragma unroll
@@ -900,7 +916,7 @@ template <typename T, int NT, bool MEM> struct Row {
       const float y = place_of(z[e], c42);
       const float b = __fadd_rn(fminf(y, (float)(ROW_BINS - 1)), 0x1p23f);
       const float w = __fmaf_rn(__fsub_rn(y, __fsub_rn(b, 0x1p23f)), -4096.0f * ROW_LN2 / ROW_BIN_SCALE, 0x1p23f + 4096.0f);
-      smem_add_if(by_mass ? y < ROW_MASS_END * ROW_BIN_SCALE : z[e] > -INFINITY, &sh.bins[__float_as_uint(b) & 0x7fffffu],
+      smem_add_if(by_mass ? y < y_end : z[e] > -INFINITY, &sh.bins[__float_as_uint(b) & 0x7fffffu],
                   by_mass ? __float_as_uint(w) & 0x7fffffu : 1u);
     }
   }
@@ -929,23 +945,41 @@ template <typename T, int NT, bool MEM> struct Row {
     if (lane == 0) atomicMax(&sh.last, filled);
     float run = block_scan(own, reinterpret_cast<float*>(sh.scan_n), all);
     const float slack = by_mass ? 0x1p-12f : 0.0f, more = by_mass && first_round ? 0x1p-8f : 0.0f;
+    uint32_t b1 = ~0u, b2 = ~0u;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const bool last = tid * PER + i == ROW_BINS - 1;
       if (tid * PER + i >= ROW_BINS) break;
       if (run < goal && (run + s[i] >= goal || last)) sh.above = above_n + (uint32_t)run;  // read for counts alone
       run += s[i];
-      if (run * (1.0f + slack) + more >= goal) atomicMin(&sh.b1, (uint32_t)(tid * PER + i));
-      if (run * (1.0f - slack) - more >= goal) atomicMin(&sh.b2, (uint32_t)(tid * PER + i));
+      if (run * (1.0f + slack) + more >= goal) b1 = min(b1, (uint32_t)(tid * PER + i));
+      if (run * (1.0f - slack) - more >= goal) b2 = min(b2, (uint32_t)(tid * PER + i));
+    }
+    b1 = __reduce_min_sync(~0u, b1), b2 = __reduce_min_sync(~0u, b2);
+    if (lane == 0) {
+      if (b1 != ~0u) atomicMin(&sh.b1, b1);
+      if (b2 != ~0u) atomicMin(&sh.b2, b2);
     }
     __syncthreads();
   }
   // Of the interval of those bins: warp 0 gets the first entry, warp 1 the last.
-  __device__ __forceinline__ uint64_t end_of(bool by_mass, bool by_weight, float c42, int shift, uint64_t lo, uint64_t hi) {
+  // In the first round by mass a little before and behind them, by more than
+  // the rounding of a bin's bound, which spares the search; counts, and the
+  // rounds that have to shorten the interval, need the bounds themselves.
+  __device__ __forceinline__ uint64_t end_of(bool by_mass, bool by_weight, bool first_round, float c42, int shift, uint64_t lo,
+                                             uint64_t hi) {
     if (wid >= 2) return 0;
     const uint32_t end = by_mass ? sh.last : (uint32_t)ROW_BINS - 1;
     const uint32_t b = wid ? min(sh.b2, end) + 1 : min(sh.b1, end);
     uint64_t at;
+    if (by_mass && first_round) {
+      const float d = __fdiv_rn((float)b - 0.5f, c42), by = fabsf(m) * 0x1p-21f;
+      if (wid) {
+        const float z = m - d * (1.0f + 0x1p-18f) - by;
+        return b < (uint32_t)ROW_BINS && z > -ROW_F32_MAX ? (uint64_t)row_key(z) << ROW_IDX_BITS | (ROW_MAX_COLS - 1) : hi;
+      }
+      return b ? max(lo, (uint64_t)row_key(fminf(fmaxf(m - d * (1.0f - 0x1p-18f) + by, -ROW_F32_MAX), m)) << ROW_IDX_BITS) : lo;
+    }
     if (by_weight)
       at = b < (uint32_t)ROW_BINS ? max(lo, (uint64_t)first_key(b, c42) << ROW_IDX_BITS) : hi + 1;
     else
@@ -977,18 +1011,18 @@ template <typename T, int NT, bool MEM> struct Row {
   struct Left {
     uint32_t n, above_n;
   };
-  __device__ __forceinline__ Left narrow(bool by_mass, uint64_t target, float least_w, uint32_t most) const {
-    return narrow_copy(*this, by_mass, target, least_w, most);
+  __device__ __forceinline__ Left narrow(bool by_mass, uint64_t target, uint64_t rest, float least_w, uint32_t most) const {
+    return narrow_copy(*this, by_mass, target, rest, least_w, most);
   }
   // Not inlined, for its size; on a copy, so that the row's own members may
   // stay in registers everywhere else.
-  static __device__ __noinline__ Left narrow_copy(Row r, bool by_mass, uint64_t target, float least_w, uint32_t most) {
+  static __device__ __noinline__ Left narrow_copy(Row r, bool by_mass, uint64_t target, uint64_t rest, float least_w, uint32_t most) {
     Left left;
-    r.narrow_into(by_mass, target, least_w, most, left.n, left.above_n);
+    r.narrow_into(by_mass, target, rest, least_w, most, left.n, left.above_n);
     return left;
   }
-  __device__ __forceinline__ void narrow_into(bool by_mass, uint64_t target, float least_w, uint32_t most, uint32_t& n,
-                                              uint32_t& above_n) {
+  __device__ __forceinline__ void narrow_into(bool by_mass, uint64_t target, uint64_t rest, float least_w, uint32_t most,
+                                              uint32_t& n, uint32_t& above_n) {
     uint64_t lo = (uint64_t)row_key(m) << ROW_IDX_BITS, hi = (uint64_t)row_key(-ROW_F32_MAX) << ROW_IDX_BITS | (ROW_MAX_COLS - 1);
     uint64_t above_q = 0;
     above_n = 0;
@@ -1002,7 +1036,9 @@ template <typename T, int NT, bool MEM> struct Row {
       const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w, c42 = fminf(c * ROW_BIN_SCALE, ROW_F32_MAX);
       const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), c42)) >= bin_at(place_of(value_of(lo), c42)) + 3);
       if (round == 0) {
-        vectors([&](const uint4& v, uint32_t) { count_bins(v, by_mass, c42); });
+        // what the prefix leaves is at least `rest`: its first entry has at least rest / cols
+        const float y_end = ROW_BIN_SCALE * fminf(ROW_MASS_END, 41.125f - log2f(fmaxf((float)rest / (float)cols, 0x1p-8f)));
+        vectors([&](const uint4& v, uint32_t) { count_bins(v, by_mass, c42, y_end); });
       } else {
         between(value_of(hi), value_of(lo), [&](float z, int j) {
           const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
@@ -1033,7 +1069,7 @@ template <typename T, int NT, bool MEM> struct Row {
       if (rank == 0) {
         const float goal = by_mass ? (float)(target - above_q) * 0x1p-28f : (float)(target - above_n);
         end_bins(by_mass, by_weight, round == 0, goal, above_n, top_w);
-        const uint64_t at = end_of(by_mass, by_weight, c42, shift, lo, hi);
+        const uint64_t at = end_of(by_mass, by_weight, round == 0, c42, shift, lo, hi);
         if (wid < 2) {
           if (lane < (int)ctas) {
             *cluster.map_shared_rank(wid ? &sh.hi : &sh.lo, lane) = at;
@@ -1133,16 +1169,6 @@ template <typename T, int NT, bool MEM> struct Row {
       if (tid + i * NT >= n) return false;
       e = from[tid + i * NT];
       bin = (uint32_t)fminf(__fmul_rn(__fsub_rn(m, value_of(e)), scale), (float)(ROW_SORT_BINS - 1));
-      return true;
-    });
-  }
-  // The same by bins linear in (key, index) over [lo, hi].
-  __device__ __forceinline__ void order_by_place(RowFinish& f, const uint64_t* from, uint32_t n, uint64_t lo, uint64_t hi) {
-    const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
-    order(f, [&](int i, uint64_t& e, uint32_t& bin) {
-      if (tid + i * NT >= n) return false;
-      e = from[tid + i * NT];
-      bin = (uint32_t)((e - lo) >> shift);
       return true;
     });
   }
@@ -1306,43 +1332,94 @@ template <typename T, int NT, bool MEM> struct Row {
   // Cuts the n entries in sh.pool, those of [sh.lo, sh.hi], where the prefix of
   // `target` of them (by_p: of mass `target` with what sh.mass holds) ends, and
   // adds the kept ones' masses to their stretches' in sh.part.  Returns the
-  // last entry of the cut.
+  // last entry of the cut.  Their exact sums by bins linear in (key, index)
+  // leave those of one bin, and so on until few enough to be compared with
+  // each other are left: equal values, which 16-bit logits have many of, cost
+  // no more than others.
   __device__ __forceinline__ uint64_t finish_pool(RowFinish& f, uint32_t n, const RowParams& p, uint64_t target) {
-    const uint64_t lo = sh.lo, hi = sh.hi, above = handed(sh.mass);
-    order_by_place(f, sh.pool, n, lo, hi);
-    uint32_t cut = n;
-    if (p.by_p) {
-      const uint32_t per = (n + NT - 1) / NT, i0 = min(tid * per, n), i1 = min(i0 + per, n);
-      uint64_t sum = 0, all;
-      for (uint32_t i = i0; i < i1; ++i) sum += mass(value_of(f.sorted[i]));
-      uint64_t run = above + block_scan(sum, sh.scan_q, all);
-      if (tid == 0) sh.cut_n = n;
+    constexpr int PER = ROW_POOL / NT, BINS = ROW_SORT_BINS / NT;
+    constexpr uint32_t FEW = 64;
+    static_assert(BINS * NT == ROW_SORT_BINS && PER * NT == ROW_POOL, "bins and entries a thread");
+    uint32_t* const low = reinterpret_cast<uint32_t*>(f.loose);  // a bin's mass: the low 20 bits of each
+    uint32_t* const high = low + ROW_SORT_BINS;                  // and the rest
+    uint64_t lo = sh.lo, hi = sh.hi, left = p.by_p ? target - handed(sh.mass) : target;
+    const uint64_t end = hi;
+    uint64_t e[PER], q[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      e[i] = tid + i * NT < n ? sh.pool[tid + i * NT] : ~0ull;
+      q[i] = p.by_p ? mass(value_of(e[i])) : 1;
+    }
+    uint32_t undecided = n;
+    while (undecided > FEW) {
+      const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
+#pragma unroll
+      for (int i = 0; i < BINS; ++i) f.start[tid + i * NT] = low[tid + i * NT] = high[tid + i * NT] = 0;
       __syncthreads();
-      for (uint32_t i = i0; i < i1; ++i) {
-        const uint64_t q = mass(value_of(f.sorted[i]));
-        if (run < target && target <= run + q) sh.cut_n = i + 1;
-        run += q;
+      if (tid == 0) sh.cut_n = ~0u;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (e[i] >= lo && e[i] <= hi) {
+          const uint32_t b = (uint32_t)((e[i] - lo) >> shift);
+          atomicAdd(&f.start[b], 1u);
+          atomicAdd(&low[b], (uint32_t)q[i] & 0xfffffu);
+          atomicAdd(&high[b], (uint32_t)(q[i] >> 20));
+        }
+      __syncthreads();
+      uint64_t s[BINS], own = 0, all;
+#pragma unroll
+      for (int i = 0; i < BINS; ++i) {
+        const uint32_t b = tid * BINS + i;
+        s[i] = ((uint64_t)high[b] << 20) + low[b];
+        own += s[i];
+      }
+      uint64_t run = block_scan(own, sh.scan_q, all);
+#pragma unroll
+      for (int i = 0; i < BINS; ++i) {
+        if (run < left && left <= run + s[i]) sh.cut_n = tid * BINS + i, sh.cut_q = run, sh.above = f.start[tid * BINS + i];
+        run += s[i];
       }
       __syncthreads();
-      cut = sh.cut_n;
-    } else {
-      cut = (uint32_t)min((uint64_t)n, target);
+      if (sh.cut_n == ~0u) break;  // not reached: the cut takes them all
+      left -= sh.cut_q;
+      undecided = sh.above;
+      lo += (uint64_t)sh.cut_n << shift;
+      hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
     }
-    const uint64_t last = cut ? f.sorted[cut - 1] : hi;
+    __syncthreads();
+    if (tid == 0) sh.count = 0, sh.cut_c = end;
+    __syncthreads();
+    if (undecided <= FEW) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (e[i] >= lo && e[i] <= hi) {
+          const uint32_t at = atomicAdd(&sh.count, 1u);
+          f.sorted[at] = e[i], f.input[at] = q[i];
+        }
+      __syncthreads();
+      if (tid < (int)undecided) {
+        const uint64_t mine_e = f.sorted[tid];
+        uint64_t before = 0;
+        for (uint32_t i = 0; i < undecided; ++i) before += f.sorted[i] < mine_e ? f.input[i] : 0;
+        if (before < left && left <= before + f.input[tid]) sh.cut_c = mine_e;
+      }
+      __syncthreads();
+    }
+    const uint64_t last = sh.cut_c;
     // the warps' kept masses: before the interval, and those of its entries
     if (tid < ROW_SUMS) f.part[tid][0] = f.part[tid][1] = 0;
     __syncthreads();
-    for (uint32_t i = tid; i < cut; i += NT) {
-      const uint64_t e = f.sorted[i];
-      const float w = weight(value_of(e));
-      const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + lead) / N;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (e[i] > last) continue;  // none, too
+      const float w = weight(value_of(e[i]));
+      if (w < p.least_w) continue;
+      const uint32_t v = (((uint32_t)e[i] & (ROW_MAX_COLS - 1)) + lead) / N;
       const uint32_t cta = v / part_vecs, p0 = cta * part_vecs, p1 = min(p0 + part_vecs, total_vecs);
-      const uint32_t warp = (v - p0) / ((p1 - p0 + WARPS - 1) / WARPS);
-      if (w >= p.least_w) {
-        const uint64_t q = row_q(w);
-        atomicAdd(&f.part[cta * WARPS + warp][0], (uint32_t)q & 0xfffffu);
-        atomicAdd(&f.part[cta * WARPS + warp][1], (uint32_t)(q >> 20));
-      }
+      const uint32_t at = cta * WARPS + (v - p0) / ((p1 - p0 + WARPS - 1) / WARPS);
+      const uint64_t kept = row_q(w);
+      atomicAdd(&f.part[at][0], (uint32_t)kept & 0xfffffu);
+      atomicAdd(&f.part[at][1], (uint32_t)(kept >> 20));
     }
     __syncthreads();
     if (tid < CTAS * WARPS) (&sh.part[0][0])[tid] += ((uint64_t)f.part[tid][1] << 20) + f.part[tid][0];
@@ -1370,22 +1447,28 @@ template <typename T, int NT, bool MEM> struct Row {
   // exceeds t calls hit(x, index), on one thread.
   template <typename V, typename H>
   __device__ __forceinline__ void scan_memory(uint32_t v0, uint32_t v1, uint64_t t, V value, H hit) {
-    for (uint32_t i0 = v0; i0 < v1; i0 += NT) {
-      const uint32_t i = i0 + tid;
-      const uint4 v = i < v1 ? from_memory(i) : nothing();
-      const int j0 = (int)(i * N) - lead;
-      float f[N];
-      E::get(v, f);
+    constexpr int PER = 2;  // vectors a thread, side by side
+    for (uint32_t i0 = v0; i0 < v1; i0 += NT * PER) {
+      float z[PER * N];
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const uint32_t i = i0 + tid * PER + k;
+        float of[N];
+        E::get(i < v1 ? from_memory(i) : nothing(), of);
+#pragma unroll
+        for (int e = 0; e < N; ++e) z[k * N + e] = of[e];
+      }
+      const int j0 = (int)((i0 + tid * PER) * N) - lead;
       uint64_t own = 0, all;
 #pragma unroll
-      for (int e = 0; e < N; ++e) own += value(f[e], j0 + e);
+      for (int e = 0; e < PER * N; ++e) own += value(z[e], j0 + e);
       uint64_t run = block_scan(own, sh.scan_q, all);
       if (t < all) {
         if (t >= run && t < run + own) {
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const uint64_t q = value(f[e], j0 + e);
-            if (t >= run && t < run + q) hit(f[e], j0 + e);
+          for (int e = 0; e < PER * N; ++e) {
+            const uint64_t q = value(z[e], j0 + e);
+            if (t >= run && t < run + q) hit(z[e], j0 + e);
             run += q;
           }
         }
@@ -1511,7 +1594,7 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
   if (q.by_k || q.by_p) {
     typename Row<T, NT, MEM>::Left left{0, 0};
     uint64_t target = k;
-    if (q.by_k) left = r.narrow(false, k, least_w, q.by_p ? ROW_FEW : ROW_POOL);
+    if (q.by_k) left = r.narrow(false, k, 0, least_w, q.by_p ? ROW_FEW : ROW_POOL);
     const uint32_t above_n = left.above_n;
     if (q.by_p) {
       uint64_t mass = total;
@@ -1531,7 +1614,7 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
         mass = sh.cut_q;
       }
       target = row_target(q.p, mass);
-      left = r.narrow(true, target, least_w, ROW_POOL);
+      left = r.narrow(true, target, mass - target, least_w, ROW_POOL);
     }
     if (!r.last_part()) return;
     last = r.finish_pool(f, left.n, q, q.by_p ? target : k - above_n);
@@ -1586,7 +1669,7 @@ __device__ __forceinline__ void row_best(const RowArgs& a, uint32_t row, typenam
     __syncthreads();
   } else {
     // the n-th entry, then the entries up to it
-    const auto left = r.narrow(false, k, 0.0f, ROW_FEW);
+    const auto left = r.narrow(false, k, 0, 0.0f, ROW_FEW);
     r.cluster.sync();
     if (r.rank == 0) {
       r.nth_of_few(left.n, k - left.above_n);
@@ -1625,12 +1708,13 @@ template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_CLUSTER_T
 }
 
 // One CTA a row.
-template <typename T, int NT, bool BEST> __global__ void __launch_bounds__(NT, 1024 / NT) k_row_solo(const RowArgs a) {
+constexpr int ROW_SOLO_THREADS = 512;
+template <typename T, bool BEST> __global__ void __launch_bounds__(ROW_SOLO_THREADS, 2) k_row_solo(const RowArgs a) {
   extern __shared__ __align__(16) unsigned char row_smem[];
-  using R = Row<T, NT, true>;
+  using R = Row<T, ROW_SOLO_THREADS, true>;
   typename R::Shared& sh = *reinterpret_cast<typename R::Shared*>(row_smem);
   uint4* const data = reinterpret_cast<uint4*>(row_smem + R::SHARED_BYTES);
-  BEST ? row_best<T, NT, true>(a, blockIdx.x, sh, data) : row_sample<T, NT, true>(a, blockIdx.x, sh, data);
+  BEST ? row_best<T, ROW_SOLO_THREADS, true>(a, blockIdx.x, sh, data) : row_sample<T, ROW_SOLO_THREADS, true>(a, blockIdx.x, sh, data);
 }
 
 }  // namespace fs

@@ -1256,7 +1256,7 @@ int fs_create(int device, void* stream, fs_sorter** out) {
   }
   if (const char* t = getenv("FORGESORT_ROW_FORM")) {
     const int v = atoi(t);
-    s->row_form = v >= 1 && v <= 3 ? v : 0;
+    s->row_form = v == 1 || v == 2 ? v : 0;
   }
   if (const char* t = getenv("FORGESORT_H16_MIN_KEYS")) {  // keys; 0: never the histogram fill
     const long long v = atoll(t);

@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 DT = ["f32", "f16", "bf16"]
 
 
-@pytest.fixture(scope="module", params=[1, 2, 3], ids=["cluster", "solo512", "solo1024"])
+@pytest.fixture(scope="module", params=[1, 2], ids=["cluster", "solo"])
 def gs(request):
     """Every form for every case: a cluster a row, and a CTA of 512 or 1024 threads a row."""
     import forge_sort
