@@ -96,6 +96,15 @@ __device__ __forceinline__ uint32_t row_word(const uint4& v, int k) {
   return w;
 }
 
+// The same word replaced.
+__device__ __forceinline__ void row_put_word(uint4& v, int k, uint32_t w) {
+  v.x = k == 0 ? w : v.x, v.y = k == 1 ? w : v.y, v.z = k == 2 ? w : v.z, v.w = k == 3 ? w : v.w;
+}
+__device__ __forceinline__ void row_put_half(uint4& v, int e, uint32_t h) {
+  const uint32_t w = row_word(v, e >> 1);
+  row_put_word(v, e >> 1, e & 1 ? (w & 0xffffu) | h << 16 : (w & 0xffff0000u) | h);
+}
+
 template <typename T> struct RowElem;
 template <> struct RowElem<float> {
   static constexpr int N = 4;
@@ -111,6 +120,7 @@ template <> struct RowElem<float> {
     return __float_as_uint(fminf(fmaxf(__uint_as_float(v), -INFINITY), ROW_F32_MAX));
   }
   static __device__ __forceinline__ float at(const uint4& v, int e) { return __uint_as_float(row_word(v, e)); }
+  static __device__ __forceinline__ void put(uint4& v, int e, const float* x) { row_put_word(v, e, __float_as_uint(*x)); }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
@@ -139,6 +149,9 @@ template <> struct RowElem<__nv_bfloat16> {
   static __device__ __forceinline__ float at(const uint4& v, int e) {
     const uint32_t w = row_word(v, e >> 1);
     return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+  }
+  static __device__ __forceinline__ void put(uint4& v, int e, const __nv_bfloat16* x) {
+    row_put_half(v, e, *reinterpret_cast<const unsigned short*>(x));
   }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -174,6 +187,9 @@ template <> struct RowElem<__half> {
   static __device__ __forceinline__ float at(const uint4& v, int e) {
     const uint32_t w = row_word(v, e >> 1);
     return __half2float(__ushort_as_half((unsigned short)(e & 1 ? w >> 16 : w)));
+  }
+  static __device__ __forceinline__ void put(uint4& v, int e, const __half* x) {
+    row_put_half(v, e, *reinterpret_cast<const unsigned short*>(x));
   }
   static __device__ __forceinline__ void get(const uint4& v, float (&x)[N]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -385,6 +401,7 @@ template <typename T, int NT, bool MEM> struct Row {
         rank(part),
         ctas(parts),
         lists(parts * WARPS * lists_a_warp) {
+#pragma unroll 1
     for (int b = tid; b < ROW_EDGE_BINS; b += NT) sh.edge_n[b] = 0;
     if (tid == 0) sh.count = 0, sh.first = ~0u, sh.dirty = 0;
     if constexpr (MEM) __syncthreads();
@@ -407,14 +424,13 @@ template <typename T, int NT, bool MEM> struct Row {
     const int j0 = (int)(v * N) - lead;
     return j0 >= 0 && j0 + N <= (int)cols;
   }
-  __device__ __forceinline__ uint4 ragged(uint32_t v) const {  // the row's first or last vector
-    const int j0 = (int)(v * N) - lead;
-    union { uint4 v; T e[N]; } u;
-    u.v = nothing();
-#pragma unroll
+  __device__ __forceinline__ uint4 ragged(uint32_t i) const {  // the row's first or last vector
+    const int j0 = (int)(i * N) - lead;
+    uint4 v = nothing();
+#pragma unroll 1
     for (int e = 0; e < N; ++e)
-      if (j0 + e >= 0 && j0 + e < (int)cols) u.e[e] = x[j0 + e];
-    return u.v;
+      if (j0 + e >= 0 && j0 + e < (int)cols) E::put(v, e, x + j0 + e);
+    return v;
   }
   __device__ __forceinline__ uint4 from_memory(uint32_t v) const {
     return cleaned(inside(v) ? __ldg(vecs + v) : ragged(v));
@@ -432,7 +448,7 @@ template <typename T, int NT, bool MEM> struct Row {
   __device__ __forceinline__ void load_memory(bool tops) {
     first = -lead;
     typename E::Top top[2] = {E::top0(), E::top0()};
-    stream<false, false>([&](const uint4& v, uint32_t) {  // the two take turns
+    stream<false, false, true>([&](const uint4& v, uint32_t) {  // the two take turns
       const typename E::Top t = E::top(top[0], v);
       top[0] = top[1];
       top[1] = t;
@@ -441,7 +457,7 @@ template <typename T, int NT, bool MEM> struct Row {
     if (__any_sync(~0u, bad)) {  // NaN or +inf: the warp looks through its stretch again
       sh.dirty = 1;
       top[0] = top[1] = E::top0();
-      stream<true, false>([&](const uint4& v, uint32_t) { top[0] = E::top(top[0], v); }, [] {});
+      stream<true, false, false>([&](const uint4& v, uint32_t) { top[0] = E::top(top[0], v); }, [] {});
     }
     const uint32_t per = top_count();
 #pragma unroll
@@ -470,6 +486,7 @@ template <typename T, int NT, bool MEM> struct Row {
     stretch(rank, wid, seg0, seg1);
     seg0 -= p0, seg1 -= p0;
     first = (int)(p0 * N) - lead;
+#pragma unroll 1
     for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
       if (inside(p0 + i))
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_of(data + i)), "l"(vecs + p0 + i) : "memory");
@@ -483,6 +500,7 @@ template <typename T, int NT, bool MEM> struct Row {
     mine = E::value(top);
     if (!(mine <= ROW_F32_MAX)) {  // NaN or +inf among this thread's entries
       top = E::top0();
+#pragma unroll 1
       for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
         const uint4 v = cleaned(data[i]);
         data[i] = v;
@@ -493,6 +511,7 @@ template <typename T, int NT, bool MEM> struct Row {
     const uint32_t k = tops ? sorted_tops() : __reduce_min_sync(~0u, row_key(mine));
     cluster.barrier_wait();
     const uint32_t per = top_count();
+#pragma unroll 1
     for (uint32_t i0 = 0; i0 < per * ctas; i0 += 32) {
       const uint32_t to = (i0 + lane) / per, e = i0 + lane - to * per, v = __shfl_sync(~0u, k, e);
       if (to < ctas && (tops || e == 0)) *cluster.map_shared_rank(&sh.tops[(rank * WARPS + wid) * per + e], to) = v;
@@ -516,6 +535,7 @@ template <typename T, int NT, bool MEM> struct Row {
   // The row's maximum from the published ones.
   __device__ __forceinline__ void find_max() {
     uint32_t best = ~0u;
+#pragma unroll 1
     for (uint32_t i = lane; i < lists; i += 32) best = min(best, sh.tops[i * top_count()]);
     m = row_unkey(__reduce_min_sync(~0u, best));
   }
@@ -539,8 +559,10 @@ template <typename T, int NT, bool MEM> struct Row {
   // f(vector, number in the part) for this thread's vectors, two side by side;
   // from memory, with +inf and NaN as they are unless CLEAN; now_and_then() is
   // called every 32 vectors.  BACK: from the
-  // stretch's end, which was read last and is in L2 for the longest.
-  template <bool CLEAN, bool BACK, typename F, typename G> __device__ __forceinline__ void stream(F f, G now_and_then) const {
+  // stretch's end, which was read last and is in L2 for the longest.  f appears
+  // in the code once or twice (WIDE) in the loop and once behind it: the code of
+  // a row is run once or twice by a CTA, so its size is time.
+  template <bool CLEAN, bool BACK, bool WIDE, typename F, typename G> __device__ __forceinline__ void stream(F f, G now_and_then) const {
     uint32_t v0, v1;
     stretch(0, wid, v0, v1);
     const bool head = v0 < v1 && !inside(v0), tail = v0 + head < v1 && !inside(v1 - 1);
@@ -565,39 +587,37 @@ template <typename T, int NT, bool MEM> struct Row {
 #pragma unroll 1
     for (; i + 32 < end; i += 64) {
       asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD / 2 - 1) : "memory");
-      const uint4 a = get(slot), b = get(slot + STEP);
-      f(a, number(i));
-      f(b, number(i + 32));
+      if constexpr (WIDE) {
+        const uint4 a = get(slot), b = get(slot + STEP);
+        f(a, number(i));
+        f(b, number(i + 32));
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) f(get(slot + k * STEP), number(i + 32 * k));
+      }
       fetch(slot), fetch(slot + STEP), commit();
       slot += 2 * STEP;
       if (slot == slots + AHEAD * STEP) slot = slots;
       if (++turns % 16 == 0) now_and_then();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (i < end) f(get(slot), number(i));
-    if (head && lane == 0) f(cleaned(ragged(v0)), v0);
-    if (tail && lane == 1) f(cleaned(ragged(v1 - 1)), v1 - 1);
+    // what is left: a vector of the loop's, then on one thread each the row's ends
+    const bool at_head = head && lane == 0, at_tail = tail && lane == 1;
+    const uint32_t ragged_at = at_head ? v0 : v1 - 1;
+#pragma unroll 1
+    for (int k = i < end ? 0 : 1; k < (at_head || at_tail ? 2 : 1); ++k)
+      f(k ? cleaned(ragged(ragged_at)) : get(slot), k ? ragged_at : number(i));
   }
-  template <typename F> __device__ __forceinline__ void vectors(F f) const {
-    vectors(f, [] {});
-  }
-  template <typename F, typename G> __device__ __forceinline__ void vectors(F f, G now_and_then) const {
+  template <bool WIDE, typename F, typename G> __device__ __forceinline__ void vectors(F f, G now_and_then) const {
     if constexpr (MEM) {
-      stream<true, true>(f, now_and_then);
-    } else {
+      stream<true, true, WIDE>(f, now_and_then);
+    } else if constexpr (WIDE) {
 #pragma unroll 2
       for (uint32_t i = seg0 + lane; i < seg1; i += 32) f(data[i], i);
+    } else {
+#pragma unroll 1
+      for (uint32_t i = seg0 + lane; i < seg1; i += 32) f(data[i], i);
     }
-  }
-  // f(x, index) for every entry of this thread
-  template <typename F> __device__ __forceinline__ void each(F f) const {
-    vectors([&](const uint4& v, uint32_t i) {
-      float z[N];
-      E::get(v, z);
-      const int j0 = first + (int)(i * N);
-#pragma unroll
-      for (int e = 0; e < N; ++e) f(z[e], j0 + e);
-    });
   }
 
   __device__ __forceinline__ float weight(float v) const { return row_exp2(row_neg_y(v, m, c)); }
@@ -624,17 +644,19 @@ template <typename T, int NT, bool MEM> struct Row {
 
   // ---- the one pass over all weights ----
   // The mass of this thread's entries (ABOVE: of those over `over`, and
-  // f(x, index) for those from `low` to `over`).  Per entry: a half of four
+  // f(x, index) for those from `low` to `over`; HEAVY: of those over
+  // `over` with w >= least_w).  Per entry: a half of four
   // packed additions, a half of one packed multiplication, the exponential and
   // one integer addition.  Fewer than 512 entries
   // come between folds (a part in shared memory has fewer a thread), so that
   // neither 32-bit sum of hi < 2^23 or |lo| <= 2^17 wraps.
+  enum { ALL, ABOVE, HEAVY };
   struct Sum {
     uint64_t m2, c2;
     uint64_t folded = 0;
     uint32_t hi = 0, lo = 0, n = 0;
     __device__ __forceinline__ Sum(float m, float c) : m2(f2_pack(-m, -m)), c2(f2_pack(c, c)) {}
-    template <bool ABOVE> __device__ __forceinline__ void add(const uint4& v, float over) {
+    template <int KIND> __device__ __forceinline__ void add(const uint4& v, float over, float least_w) {
       const uint64_t one = f2_pack(1.0f, 1.0f), none = f2_pack(-1.0f, -1.0f), both = f2_pack(1.0f + ROW_MAGIC, 1.0f + ROW_MAGIC);
       float z[N];
       E::get(v, z);
@@ -643,7 +665,8 @@ template <typename T, int NT, bool MEM> struct Row {
         float w0, w1, a0, a1, b0, b1;
         f2_unpack(f2_mul(f2_add(f2_pack(z[e], z[e + 1]), m2), c2), w0, w1);
         w0 = row_exp2(w0), w1 = row_exp2(w1);
-        if (ABOVE) w0 = z[e] > over ? w0 : 0.0f, w1 = z[e + 1] > over ? w1 : 0.0f;
+        if (KIND == HEAVY) w0 = w0 >= least_w ? w0 : 0.0f, w1 = w1 >= least_w ? w1 : 0.0f;
+        if (KIND != ALL) w0 = z[e] > over ? w0 : 0.0f, w1 = z[e + 1] > over ? w1 : 0.0f;
         const uint64_t w = f2_pack(w0, w1);
         const uint64_t a = f2_add(w, one);
         const uint64_t b = f2_add(w, f2_fma(a, none, both));  // 1 + MAGIC - a is exact
@@ -662,15 +685,16 @@ template <typename T, int NT, bool MEM> struct Row {
       return folded + row_mass(hi - n * ROW_ONE_BITS, (int)(lo - n * ROW_MAGIC_BITS));
     }
   };
-  template <bool ABOVE, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, F f) const {
+  template <int KIND, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, float least_w, F f) const {
     Sum sum(m, c);
     uint64_t has = 0;  // which of the thread's vectors f wants: they are looked at again afterwards, few and together
-    vectors([&](const uint4& v, uint32_t i) {
-      sum.template add<ABOVE>(v, over);
-      if (ABOVE && MEM) each_of(hits(v, low, over), v, i, f);
-      if (ABOVE && !MEM) has |= (uint64_t)any_hit(v, low, over) << ((i - seg0) / 32);
+    vectors<KIND == ALL>([&](const uint4& v, uint32_t i) {
+      sum.template add<KIND>(v, over, least_w);
+      if (KIND == ABOVE && MEM) each_of(hits(v, low, over), v, i, f);
+      if (KIND == ABOVE && !MEM) has |= (uint64_t)any_hit(v, low, over) << ((i - seg0) / 32);
     }, [&] { sum.fold(); });
-    while (ABOVE && !MEM && has) {
+#pragma unroll 1
+    while (KIND == ABOVE && !MEM && has) {
       const uint32_t i = seg0 + lane + 32 * (__ffsll((long long)has) - 1);
       has &= has - 1;
       const uint4 v = data[i];
@@ -679,7 +703,10 @@ template <typename T, int NT, bool MEM> struct Row {
     return sum.mass();
   }
   __device__ __forceinline__ uint64_t weigh() const {
-    return weigh<false>(0.0f, 0.0f, [](float, int) {});
+    return weigh<ALL>(0.0f, 0.0f, 0.0f, [](float, int) {});
+  }
+  __device__ __forceinline__ uint64_t heavy(float over, float least_w) const {
+    return weigh<HEAVY>(over, 0.0f, least_w, [](float, int) {});
   }
 
   // The same pass (from memory) also lists the entries of at least `edge`, or
@@ -687,8 +714,8 @@ template <typename T, int NT, bool MEM> struct Row {
   template <bool CLEAN> __device__ __forceinline__ uint64_t weigh_and_list_of(float edge, bool only_first) {
     Sum sum(m, c);
     const bool lists_any = edge < INFINITY;
-    stream<CLEAN, true>([&](const uint4& v, uint32_t i) {
-      sum.template add<false>(v, 0.0f);
+    stream<CLEAN, true, !CLEAN>([&](const uint4& v, uint32_t i) {
+      sum.template add<ALL>(v, 0.0f, 0.0f);
       if (lists_any && E::value(E::top(E::top0(), v)) >= edge)
         each_of(hits(v, edge, INFINITY), v, i, [&](float z, int j) {
           if (only_first) {
@@ -724,6 +751,7 @@ template <typename T, int NT, bool MEM> struct Row {
   }
   // f(x, index) for the entries of vector i of this CTA's part that mask names
   template <typename F> __device__ __forceinline__ void each_of(uint32_t mask, const uint4& v, uint32_t i, F f) const {
+#pragma unroll 1
     while (mask) {
       const int e = __ffs((int)mask) - 1;
       mask &= mask - 1;
@@ -732,15 +760,17 @@ template <typename T, int NT, bool MEM> struct Row {
   }
   // Calls f(x, index) for the warp's entries in [low, high], many of them.
   template <typename F> __device__ __forceinline__ void between(float low, float high, F f) const {
-    vectors([&](const uint4& v, uint32_t i) { each_of(hits(v, low, high), v, i, f); });
+    vectors<false>([&](const uint4& v, uint32_t i) { each_of(hits(v, low, high), v, i, f); }, [] {});
   }
   // The same, where few of the warp's threads have any above low: the warp
   // looks through the vectors of one such thread at a time.
   template <typename F> __device__ __forceinline__ void above(float low, F f) const {
     uint32_t threads = __ballot_sync(~0u, mine >= low);
+#pragma unroll 1
     while (threads) {
       const uint32_t owner = __ffs((int)threads) - 1;
       threads &= threads - 1;
+#pragma unroll 1
       for (uint32_t i = seg0 + owner + 32 * lane; i < seg1; i += 32 * 32) {
         const uint4 v = data[i];
         each_of(hits(v, low, INFINITY), v, i, f);
@@ -758,6 +788,7 @@ template <typename T, int NT, bool MEM> struct Row {
   __device__ __forceinline__ float edge_of(uint32_t k, float scale, float last) {
     const uint32_t tops = top_count() * lists;
     scale = fminf(scale, ROW_F32_MAX);
+#pragma unroll 1
     for (uint32_t i = tid; i < tops; i += NT) {
       const float z = row_unkey(sh.tops[i]);
       if (z > -INFINITY)
@@ -787,12 +818,14 @@ template <typename T, int NT, bool MEM> struct Row {
   __device__ __forceinline__ float far_scale() {
     const uint32_t tops = top_count() * lists;
     float low = m;
+#pragma unroll 1
     for (uint32_t i = lane; i < tops; i += 32) {
       const float z = row_unkey(sh.tops[i]);
       if (z > m - 512.0f) low = fminf(low, z);
     }
     low = row_unkey(__reduce_max_sync(~0u, row_key(low)));
     __syncthreads();
+#pragma unroll 1
     for (int b = tid; b < ROW_EDGE_BINS; b += NT) sh.edge_n[b] = 0;
     __syncthreads();
     return (ROW_EDGE_BINS - 2) / fmaxf(m - low, 0x1p-20f);
@@ -810,26 +843,33 @@ template <typename T, int NT, bool MEM> struct Row {
   // Sums of what was handed over.
   __device__ __forceinline__ uint64_t handed(const Sums& of) const {
     uint64_t t = 0;
+#pragma unroll 1
     for (uint32_t i = lane; i < ctas * WARPS; i += 32) t += (&of[0][0])[i];
     return warp_sum_u64(t);
   }
   // The first CTA's list of candidates is divided among the CTAs.
   __device__ __forceinline__ uint32_t share() const { return ROW_LIST / ctas; }
   // Collects this CTA's entries of at least `edge` in its share of the first
-  // CTA's list (sh.count = 0 before); then tells every CTA their number.
-  __device__ __forceinline__ void collect_above(float edge) {
+  // CTA's list (sh.count = 0 before), or only finds the first of them.
+  __device__ __forceinline__ void collect_above(float edge, bool only_first) {
     const uint32_t room = share();
     above(edge, [&](float z, int j) {
+      if (only_first) {
+        atomicMin(cluster.map_shared_rank(&sh.first, 0), (uint32_t)j);
+        return;
+      }
       const uint32_t at = atomicAdd(&sh.count, 1u);
       if (at < room) sh.list[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
     });
   }
+  // Hands them to the first CTA and tells every CTA their number.
   __device__ __forceinline__ void tell_list() {
     const uint32_t room = share();
     __syncthreads();
     if (tid < (int)ctas) *cluster.map_shared_rank(&sh.n[rank], tid) = sh.count;
     if (rank) {
       uint64_t* const to = cluster.map_shared_rank(sh.list, 0) + rank * room;
+#pragma unroll 1
       for (uint32_t i = tid; i < min(sh.count, room); i += NT) to[i] = sh.list[i];
     }
   }
@@ -837,14 +877,17 @@ template <typename T, int NT, bool MEM> struct Row {
   __device__ __forceinline__ bool all_listed(uint32_t& n) const {
     bool fit = true;
     n = 0;
+#pragma unroll 1
     for (uint32_t i = 0; i < ctas; ++i) n += sh.n[i], fit &= sh.n[i] <= share();
     return fit;
   }
   // f(number, entry) for this thread's candidates, on the first CTA.
   template <typename F> __device__ __forceinline__ void each_listed(F f) const {
     const uint32_t room = share();
+#pragma unroll 1
     for (uint32_t s = tid; s < room * ctas; s += NT) {
       uint32_t before = 0, mine_n = 0, at = s;
+#pragma unroll 1
       for (uint32_t i = 0; i < ctas; ++i) {
         const bool in = s >= i * room;
         if (in) at = s - i * room, mine_n = sh.n[i];
@@ -863,12 +906,14 @@ template <typename T, int NT, bool MEM> struct Row {
   // where they are at most `room`, the others' go behind the first CTA's.
   __device__ __forceinline__ uint32_t pooled(uint32_t room) {
     uint32_t n = 0, base = 0;
+#pragma unroll 1
     for (uint32_t i = 0; i < ctas; ++i) {
       if (i == rank) base = n;
       n += sh.n[i];
     }
     if (n <= room && rank) {
       uint64_t* const to = cluster.map_shared_rank(sh.pool, 0) + base;
+#pragma unroll 1
       for (uint32_t i = tid; i < sh.n[rank]; i += NT) to[i] = sh.pool[i];
     }
     return n;
@@ -893,6 +938,7 @@ template <typename T, int NT, bool MEM> struct Row {
   // 32 probes at a time.
   __device__ __forceinline__ uint32_t first_key(uint32_t b, float c42) const {
     uint32_t lo = row_key(m), hi = row_key(-ROW_F32_MAX) + 1;
+#pragma unroll 1
     while (lo < hi) {
       const uint32_t step = max(1u, (hi - lo) / 32), at = lo + lane * step;
       const bool past = at - lo >= hi - lo || bin_at(place_of(row_unkey(at), c42)) >= b;
@@ -931,29 +977,31 @@ template <typename T, int NT, bool MEM> struct Row {
   // beyond all of them.
   __device__ __forceinline__ void end_bins(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n, float top_w) {
     constexpr int PER = (ROW_BINS + NT - 1) / NT;
-    float s[PER], own = 0, all;
+    const int at = tid * PER, end = min(at + PER, ROW_BINS);
+    auto sum_of = [&](int b) {
+      const float v = (float)sh.bins[b];
+      return by_mass ? v * (by_weight ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w) : v;
+    };
+    float own = 0, all;
     uint32_t filled = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int b = tid * PER + i;
-      s[i] = b < ROW_BINS ? (float)sh.bins[b] : 0.0f;
-      if (s[i] > 0.0f) filled = b;
-      if (by_mass) s[i] *= by_weight ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w;
-      own += s[i];
+#pragma unroll 1
+    for (int b = at; b < end; ++b) {
+      const float v = sum_of(b);
+      if (v > 0.0f) filled = b;
+      own += v;
     }
     filled = __reduce_max_sync(~0u, filled);
     if (lane == 0) atomicMax(&sh.last, filled);
     float run = block_scan(own, reinterpret_cast<float*>(sh.scan_n), all);
     const float slack = by_mass ? 0x1p-12f : 0.0f, more = by_mass && first_round ? 0x1p-8f : 0.0f;
     uint32_t b1 = ~0u, b2 = ~0u;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const bool last = tid * PER + i == ROW_BINS - 1;
-      if (tid * PER + i >= ROW_BINS) break;
-      if (run < goal && (run + s[i] >= goal || last)) sh.above = above_n + (uint32_t)run;  // read for counts alone
-      run += s[i];
-      if (run * (1.0f + slack) + more >= goal) b1 = min(b1, (uint32_t)(tid * PER + i));
-      if (run * (1.0f - slack) - more >= goal) b2 = min(b2, (uint32_t)(tid * PER + i));
+#pragma unroll 1
+    for (int b = at; b < end; ++b) {
+      const float v = sum_of(b);
+      if (run < goal && (run + v >= goal || b == ROW_BINS - 1)) sh.above = above_n + (uint32_t)run;  // read for counts alone
+      run += v;
+      if (run * (1.0f + slack) + more >= goal) b1 = min(b1, (uint32_t)b);
+      if (run * (1.0f - slack) - more >= goal) b2 = min(b2, (uint32_t)b);
     }
     b1 = __reduce_min_sync(~0u, b1), b2 = __reduce_min_sync(~0u, b2);
     if (lane == 0) {
@@ -1027,8 +1075,10 @@ template <typename T, int NT, bool MEM> struct Row {
     uint64_t above_q = 0;
     above_n = 0;
     constexpr int ROUNDS = 16;
+#pragma unroll 1
     for (int round = 0; round < ROUNDS; ++round) {
       cluster.sync();  // what was there has been read
+#pragma unroll 1
       for (int b = tid; b < ROW_BINS; b += NT) sh.bins[b] = 0;
       if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ~0u, sh.last = 0;
       __syncthreads();
@@ -1038,7 +1088,7 @@ template <typename T, int NT, bool MEM> struct Row {
       if (round == 0) {
         // what the prefix leaves is at least `rest`: its first entry has at least rest / cols
         const float y_end = ROW_BIN_SCALE * fminf(ROW_MASS_END, 41.125f - log2f(fmaxf((float)rest / (float)cols, 0x1p-8f)));
-        vectors([&](const uint4& v, uint32_t) { count_bins(v, by_mass, c42, y_end); });
+        vectors<false>([&](const uint4& v, uint32_t) { count_bins(v, by_mass, c42, y_end); }, [] {});
       } else {
         between(value_of(hi), value_of(lo), [&](float z, int j) {
           const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
@@ -1056,6 +1106,7 @@ template <typename T, int NT, bool MEM> struct Row {
       cluster.sync();
       // each CTA sums a slice of the bins over the cluster, into the first CTA's
       const uint32_t slice = (ROW_BINS + ctas - 1) / ctas;
+#pragma unroll 1
       for (uint32_t i = tid; i < slice; i += NT) {
         const uint32_t b = rank * slice + i;
         if (b < ROW_BINS) {
@@ -1084,22 +1135,18 @@ template <typename T, int NT, bool MEM> struct Row {
       uint64_t before = 0, kept;
       const float over = value_of(lo);
       const bool cuts_equals = (lo & (ROW_MAX_COLS - 1)) != 0;  // equal values lie on both sides of lo
-      before = weigh<true>(over, value_of(hi), [&](float z, int j) {
+      before = weigh<ABOVE>(over, value_of(hi), 0.0f, [&](float z, int j) {
         const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
         if (e < lo || e > hi) return;
         const uint32_t at = atomicAdd(&sh.count, 1u);
         if (at < ROW_POOL) sh.pool[at] = e;
       });
-      if (cuts_equals)
-        between(over, over, [&](float z, int j) {
-          if (((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) < lo) before += mass(z);
-        });
-      kept = before;
-      if (least_w > 0.0f) {
-        kept = 0;
-        each([&](float z, int j) {
-          const float w = weight(z);
-          if (w >= least_w && ((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) < lo) kept += row_q(w);
+      // where the weight there is clearly more, all that comes before has at least least_w
+      kept = weight(over) * (1.0f - 0x1p-12f) >= least_w ? before : heavy(over, least_w);
+      if (cuts_equals) {
+        const float w = weight(over);
+        between(over, over, [&](float, int j) {
+          if ((uint32_t)j < ((uint32_t)lo & (ROW_MAX_COLS - 1))) before += row_q(w), kept += w >= least_w ? row_q(w) : 0;
         });
       }
       hand<true>(sh.mass, before);
@@ -1151,6 +1198,7 @@ template <typename T, int NT, bool MEM> struct Row {
         const uint32_t b0 = f.start[bin[i]], b1 = f.start[bin[i] + 1];
         uint32_t r = b0;
         if (b1 - b0 > 1)
+#pragma unroll 1
           for (uint32_t k = b0; k < b1; ++k) r += f.loose[k] < c[i];
         f.sorted[r] = c[i];
       }
@@ -1181,6 +1229,7 @@ template <typename T, int NT, bool MEM> struct Row {
     __syncthreads();
     uint32_t rank_in = 0;
     uint64_t upto = 0;
+#pragma unroll 1
     for (uint32_t i = 0; i < n; ++i)
       if (sh.pool[i] <= e) ++rank_in, upto += q[i];
     if (tid < n && rank_in == nth) sh.hi = e, sh.cut_q = upto;
@@ -1269,9 +1318,11 @@ template <typename T, int NT, bool MEM> struct Row {
       return w >= least_w ? row_q(w) : 0;
     };
     uint64_t own = 0, all;
+#pragma unroll 1
     for (uint32_t i = i0; i < i1; ++i) own += mass_at(i);
     uint64_t run = block_scan(own, sh.scan_q, all);
     if (t < run || t >= run + own) return;
+#pragma unroll 1
     for (uint32_t i = i0; i < i1; ++i) {
       const uint64_t q = mass_at(i);
       if (t >= run && t < run + q) hit(row_unkey((uint32_t)f.sorted[i]), (int)(f.sorted[i] >> 32));
@@ -1291,12 +1342,14 @@ template <typename T, int NT, bool MEM> struct Row {
     // running masses in descending order, `per` entries a thread
     const uint32_t per = (n + NT - 1) / NT, i0 = min(tid * per, n), i1 = min(i0 + per, n);
     uint64_t sum = 0, all;
+#pragma unroll 1
     for (uint32_t i = i0; i < i1; ++i) sum += mass(value_of(f.sorted[i]));
     const uint64_t before = block_scan(sum, sh.scan_q, all);
     if (tid == 0) sh.cut_n = n, sh.cut_q = q.by_k ? all : total;
     __syncthreads();
     uint64_t run = before;
     if (q.by_k && n > q.k) {
+#pragma unroll 1
       for (uint32_t i = i0; i < i1; ++i) {
         run += mass(value_of(f.sorted[i]));
         if (i == q.k - 1) sh.cut_n = q.k, sh.cut_q = run;
@@ -1308,6 +1361,7 @@ template <typename T, int NT, bool MEM> struct Row {
       const uint64_t target = row_target(q.p, sh.cut_q);
       __syncthreads();
       run = before;
+#pragma unroll 1
       for (uint32_t i = i0; i < i1 && i < cut; ++i) {
         const uint64_t qi = mass(value_of(f.sorted[i]));
         if (run < target && target <= run + qi) sh.cut_n = i + 1, sh.cut_q = run + qi;
@@ -1319,6 +1373,7 @@ template <typename T, int NT, bool MEM> struct Row {
     uint64_t left = sh.cut_q;
     if (q.by_w) {
       sum = 0;
+#pragma unroll 1
       for (uint32_t i = tid; i < cut; i += NT) {
         const float w = weight(value_of(f.sorted[i]));
         if (w >= q.least_w) sum += row_q(w);
@@ -1330,27 +1385,28 @@ template <typename T, int NT, bool MEM> struct Row {
   }
 
   // Cuts the n entries in sh.pool, those of [sh.lo, sh.hi], where the prefix of
-  // `target` of them (by_p: of mass `target` with what sh.mass holds) ends, and
+  // `target` of them (by_mass: of mass `target` with what sh.mass holds) ends, and
   // adds the kept ones' masses to their stretches' in sh.part.  Returns the
   // last entry of the cut.  Their exact sums by bins linear in (key, index)
   // leave those of one bin, and so on until few enough to be compared with
   // each other are left: equal values, which 16-bit logits have many of, cost
   // no more than others.
-  __device__ __forceinline__ uint64_t finish_pool(RowFinish& f, uint32_t n, const RowParams& p, uint64_t target) {
+  __device__ __forceinline__ uint64_t finish_pool(RowFinish& f, uint32_t n, bool by_mass, float least_w, uint64_t target) {
     constexpr int PER = ROW_POOL / NT, BINS = ROW_SORT_BINS / NT;
     constexpr uint32_t FEW = 64;
     static_assert(BINS * NT == ROW_SORT_BINS && PER * NT == ROW_POOL, "bins and entries a thread");
     uint32_t* const low = reinterpret_cast<uint32_t*>(f.loose);  // a bin's mass: the low 20 bits of each
     uint32_t* const high = low + ROW_SORT_BINS;                  // and the rest
-    uint64_t lo = sh.lo, hi = sh.hi, left = p.by_p ? target - handed(sh.mass) : target;
+    uint64_t lo = sh.lo, hi = sh.hi, left = by_mass ? target - handed(sh.mass) : target;
     const uint64_t end = hi;
     uint64_t e[PER], q[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       e[i] = tid + i * NT < n ? sh.pool[tid + i * NT] : ~0ull;
-      q[i] = p.by_p ? mass(value_of(e[i])) : 1;
+      q[i] = by_mass ? mass(value_of(e[i])) : 1;
     }
     uint32_t undecided = n;
+#pragma unroll 1
     while (undecided > FEW) {
       const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
 #pragma unroll
@@ -1400,6 +1456,7 @@ template <typename T, int NT, bool MEM> struct Row {
       if (tid < (int)undecided) {
         const uint64_t mine_e = f.sorted[tid];
         uint64_t before = 0;
+#pragma unroll 1
         for (uint32_t i = 0; i < undecided; ++i) before += f.sorted[i] < mine_e ? f.input[i] : 0;
         if (before < left && left <= before + f.input[tid]) sh.cut_c = mine_e;
       }
@@ -1413,7 +1470,7 @@ template <typename T, int NT, bool MEM> struct Row {
     for (int i = 0; i < PER; ++i) {
       if (e[i] > last) continue;  // none, too
       const float w = weight(value_of(e[i]));
-      if (w < p.least_w) continue;
+      if (w < least_w) continue;
       const uint32_t v = (((uint32_t)e[i] & (ROW_MAX_COLS - 1)) + lead) / N;
       const uint32_t cta = v / part_vecs, p0 = cta * part_vecs, p1 = min(p0 + part_vecs, total_vecs);
       const uint32_t at = cta * WARPS + (v - p0) / ((p1 - p0 + WARPS - 1) / WARPS);
@@ -1429,6 +1486,7 @@ template <typename T, int NT, bool MEM> struct Row {
 
   // Writes the first `have` of f.sorted as the row's best.
   __device__ __forceinline__ void put_best(const RowArgs& a, uint32_t row, const RowFinish& f, uint32_t have, float ln) const {
+#pragma unroll 1
     for (int i = tid; i < a.n; i += NT) {
       const bool in = i < (int)have;
       const uint64_t e = in ? f.sorted[i] : 0;
@@ -1437,38 +1495,47 @@ template <typename T, int NT, bool MEM> struct Row {
     }
   }
   __device__ __forceinline__ void put_nothing(const RowArgs& a, uint32_t row) const {
+#pragma unroll 1
     for (int i = tid; i < a.n; i += NT)
       a.best_idx[(int64_t)row * a.n + i] = -1, a.best_logprob[(int64_t)row * a.n + i] = -INFINITY;
     if (a.lse && tid == 0) a.lse[row] = -INFINITY;
   }
 
   // ---- over the row in memory, by one CTA ----
-  // The entry of vectors [v0, v1) at which the running sum of value(x, index)
-  // exceeds t calls hit(x, index), on one thread.
-  template <typename V, typename H>
-  __device__ __forceinline__ void scan_memory(uint32_t v0, uint32_t v1, uint64_t t, V value, H hit) {
+  // Draws among the entries of vectors [v0, v1) up to `last` in (key, index)
+  // order, with w >= least_w: the one at which the running mass exceeds t.
+  template <typename H>
+  __device__ __forceinline__ void scan_memory(uint32_t v0, uint32_t v1, uint64_t t, float least_w, uint64_t last, H hit) {
+    const float low = last == ~0ull ? -INFINITY : value_of(last);
+    const int low_j = (int)(last & (ROW_MAX_COLS - 1));
+    auto value = [&](float z, int j) -> uint64_t {
+      const float w = weight(z);
+      return w >= least_w && (z > low || (z == low && j <= low_j)) ? row_q(w) : 0;
+    };
     constexpr int PER = 2;  // vectors a thread, side by side
+#pragma unroll 1
     for (uint32_t i0 = v0; i0 < v1; i0 += NT * PER) {
-      float z[PER * N];
+      const uint32_t i = i0 + tid * PER;
+      uint4 v[PER];
 #pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        const uint32_t i = i0 + tid * PER + k;
-        float of[N];
-        E::get(i < v1 ? from_memory(i) : nothing(), of);
-#pragma unroll
-        for (int e = 0; e < N; ++e) z[k * N + e] = of[e];
-      }
-      const int j0 = (int)((i0 + tid * PER) * N) - lead;
+      for (int k = 0; k < PER; ++k) v[k] = i + k < v1 ? from_memory(i + k) : nothing();
+      const int j0 = (int)(i * N) - lead;
       uint64_t own = 0, all;
 #pragma unroll
-      for (int e = 0; e < PER * N; ++e) own += value(z[e], j0 + e);
+      for (int k = 0; k < PER; ++k) {
+        float z[N];
+        E::get(v[k], z);
+#pragma unroll
+        for (int e = 0; e < N; ++e) own += value(z[e], j0 + k * N + e);
+      }
       uint64_t run = block_scan(own, sh.scan_q, all);
       if (t < all) {
         if (t >= run && t < run + own) {
-#pragma unroll
+#pragma unroll 1
           for (int e = 0; e < PER * N; ++e) {
-            const uint64_t q = value(z[e], j0 + e);
-            if (t >= run && t < run + q) hit(z[e], j0 + e);
+            const float z = E::at(e < N ? v[0] : v[1], e % N);
+            const uint64_t q = value(z, j0 + e);
+            if (t >= run && t < run + q) hit(z, j0 + e);
             run += q;
           }
         }
@@ -1479,8 +1546,8 @@ template <typename T, int NT, bool MEM> struct Row {
     }
   }
   // The same over the cluster's parts, given the sum of each warp's stretch.
-  template <typename V, typename H>
-  __device__ __forceinline__ void scan_parts(const Sums& of, uint64_t t, V value, H hit) {
+  template <typename H>
+  __device__ __forceinline__ void scan_parts(const Sums& of, uint64_t t, float least_w, uint64_t last, H hit) {
     // each warp finds the stretch for itself: lanes hold up to four sums each, in order
     constexpr int PER = (CTAS * WARPS + 31) / 32;
     const uint32_t count = ctas * WARPS;
@@ -1506,7 +1573,7 @@ template <typename T, int NT, bool MEM> struct Row {
     left = __shfl_sync(~0u, left, owner);
     uint32_t v0, v1;
     stretch(which / WARPS, which % WARPS, v0, v1);
-    scan_memory(v0, v1, left, value, hit);
+    scan_memory(v0, v1, left, least_w, last, hit);
   }
 };
 
@@ -1546,66 +1613,66 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
   if constexpr (MEM) {
     own = r.weigh_and_list(edge, q.greedy);
   } else {
-    if (q.greedy) r.above(r.m, [&](float, int j) { atomicMin(r.cluster.map_shared_rank(&sh.first, 0), (uint32_t)j); });
+    if (edge < INFINITY) r.collect_above(edge, q.greedy);
     own = r.weigh();
   }
-  if (!q.cuts()) {
-    r.template hand<false>(sh.mass, own);
-    if (!r.last_part()) return;
-    total = r.handed(sh.mass);
-    if (!q.greedy)
-      r.scan_parts(sh.mass, row_draw(q.u, total), [&](float z, int) { return r.mass(z); }, store);
-    else if (r.tid == 0)
-      store(r.m, (int)sh.first);
-    return;
-  }
-
-  // ---- candidates ----
-  r.template hand<true>(sh.mass, own);
-  if (edge < INFINITY) {
-    if constexpr (!MEM) r.collect_above(edge);
-    r.tell_list();
-    if (q.by_p && !q.by_k) {
-      uint64_t part = 0;
-      for (uint32_t i = r.tid; i < min(sh.count, r.share()); i += NT) part += r.mass(r.value_of(sh.list[i]));
-      r.template hand<true>(sh.part, part);
-    }
-  }
-  r.cluster.sync();
-  uint32_t n = 0;
-  bool enough = false;
-  if (edge < INFINITY) {
-    enough = r.all_listed(n);
-    if (q.by_k && enough && r.rank) return;
-  }
-  total = r.handed(sh.mass);
-  if (enough && !q.by_k && q.by_p) enough = r.handed(sh.part) >= row_target(q.p, total);
-  if (enough) {
-    if (r.rank) return;
-    uint64_t* const to = n <= (uint32_t)ROW_FEW ? f.loose : f.input;
-    r.each_listed([&](uint32_t i, uint64_t e) { to[i] = e; });
-    __syncthreads();
-    r.finish_listed(f, n, edge, q, total, store);
-    return;
-  }
-
-  // ---- a cut beyond the candidates ----
   uint64_t last = ~0ull;  // the last entry of the cut
-  if (q.by_k || q.by_p) {
-    typename Row<T, NT, MEM>::Left left{0, 0};
-    uint64_t target = k;
-    if (q.by_k) left = r.narrow(false, k, 0, least_w, q.by_p ? ROW_FEW : ROW_POOL);
-    const uint32_t above_n = left.above_n;
-    if (q.by_p) {
-      uint64_t mass = total;
-      if (q.by_k) {
+  if (!q.cuts()) {
+    r.template hand<false>(sh.part, own);
+    if (!r.last_part()) return;
+    total = r.handed(sh.part);
+    if (q.greedy) {
+      if (r.tid == 0) store(r.m, (int)sh.first);
+      return;
+    }
+  } else {
+    // ---- candidates ----
+    r.template hand<true>(sh.mass, own);
+    if (edge < INFINITY) {
+      r.tell_list();
+      if (q.by_p && !q.by_k) {
+        uint64_t part = 0;
+#pragma unroll 1
+        for (uint32_t i = r.tid; i < min(sh.count, r.share()); i += NT) part += r.mass(r.value_of(sh.list[i]));
+        r.template hand<true>(sh.part, part);
+      }
+    }
+    r.cluster.sync();
+    uint32_t n = 0;
+    bool enough = false;
+    if (edge < INFINITY) {
+      enough = r.all_listed(n);
+      if (q.by_k && enough && r.rank) return;
+    }
+    total = r.handed(sh.mass);
+    if (enough && !q.by_k && q.by_p) enough = r.handed(sh.part) >= row_target(q.p, total);
+    if (enough) {
+      if (r.rank) return;
+      uint64_t* const to = n <= (uint32_t)ROW_FEW ? f.loose : f.input;
+      r.each_listed([&](uint32_t i, uint64_t e) { to[i] = e; });
+      __syncthreads();
+      r.finish_listed(f, n, edge, q, total, store);
+      return;
+    }
+
+    // ---- a cut beyond the candidates ----
+    if (q.by_k || q.by_p) {
+      typename Row<T, NT, MEM>::Left left{0, 0};
+      uint32_t above_n = 0;
+      uint64_t mass = total, target = k;
+      // the top k, then the nucleus in their mass
+#pragma unroll 1
+      for (int by_mass = q.by_k ? 0 : 1; by_mass <= (q.by_p ? 1 : 0); ++by_mass) {
+        if (by_mass) target = row_target(q.p, mass);
+        left = r.narrow(by_mass, target, by_mass ? mass - target : 0, least_w, !by_mass && q.by_p ? ROW_FEW : ROW_POOL);
+        if (by_mass || !q.by_p) continue;
         if (!r.rank) {  // the mass of the top k
           const uint64_t above = r.handed(sh.mass);
           r.cluster.barrier_arrive();  // the others' entries
           r.cluster.barrier_wait();
           if (r.tid == 0) sh.cut_q = total - above;
           __syncthreads();
-          r.nth_of_few(left.n, k - above_n);
+          r.nth_of_few(left.n, k - left.above_n);
           if (r.tid < (int)r.ctas) *r.cluster.map_shared_rank(&sh.cut_q, r.tid) = above + sh.cut_q;
         } else {
           r.cluster.sync();
@@ -1613,28 +1680,18 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
         r.cluster.sync();
         mass = sh.cut_q;
       }
-      target = row_target(q.p, mass);
-      left = r.narrow(true, target, mass - target, least_w, ROW_POOL);
+      if (!q.by_p) above_n = left.above_n;
+      if (!r.last_part()) return;
+      last = r.finish_pool(f, left.n, q.by_p, least_w, target - above_n);
+    } else {  // min_p alone
+      const uint64_t kept = r.heavy(-INFINITY, least_w);
+      r.cluster.sync();  // every CTA has read the sums before the next ones
+      r.template hand<false>(sh.part, kept);
+      if (!r.last_part()) return;
     }
-    if (!r.last_part()) return;
-    last = r.finish_pool(f, left.n, q, q.by_p ? target : k - above_n);
-  } else {  // min_p alone
-    uint64_t kept = 0;
-    r.each([&](float z, int) {
-      const float w = r.weight(z);
-      if (w >= least_w) kept += row_q(w);
-    });
-    r.cluster.sync();  // every CTA has read the sums before the next ones
-    r.template hand<false>(sh.part, kept);
-    if (!r.last_part()) return;
+    __syncthreads();
   }
-  __syncthreads();
-  r.scan_parts(sh.part, row_draw(q.u, r.handed(sh.part)),
-               [&](float z, int j) -> uint64_t {
-                 const float w = r.weight(z);
-                 return w >= least_w && ((uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j) <= last ? row_q(w) : 0;
-               },
-               store);
+  r.scan_parts(sh.part, row_draw(q.u, r.handed(sh.part)), least_w, last, store);
 }
 
 // ---- the n best ---------------------------------------------------------------------
@@ -1655,7 +1712,7 @@ __device__ __forceinline__ void row_best(const RowArgs& a, uint32_t row, typenam
     r.template hand<true>(sh.mass, r.weigh_and_list(edge, false));
   } else {
     r.template hand<true>(sh.mass, r.weigh());
-    if (edge < INFINITY) r.collect_above(edge);
+    if (edge < INFINITY) r.collect_above(edge, false);
   }
   r.tell_list();
   r.cluster.sync();
