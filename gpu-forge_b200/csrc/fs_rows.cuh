@@ -351,7 +351,7 @@ struct RowFinish {
   uint32_t start[ROW_SORT_BINS + 4];
   uint64_t loose[ROW_POOL];
   uint64_t sorted[ROW_POOL];
-  uint64_t input[ROW_LIST];
+  uint64_t input[ROW_POOL];
   uint32_t part[ROW_SUMS][2];  // masses of a stretch's entries in the interval: their low 20 bits, the rest
 };
 
@@ -378,6 +378,8 @@ template <typename T, int NT, bool MEM> struct Row {
   const int tid, lane, wid;
   const uint32_t rank, ctas;
   const uint32_t lists;  // of published maxima
+  const uint32_t per;    // how many of its 32 sorted thread maxima a warp publishes
+  const uint32_t room;   // a CTA's share of the first CTA's list of candidates
   // the row in memory, cut into 16-byte vectors at memory's boundaries
   const T* x;
   const uint4* vecs;
@@ -400,7 +402,9 @@ template <typename T, int NT, bool MEM> struct Row {
         wid(threadIdx.x >> 5),
         rank(part),
         ctas(parts),
-        lists(parts * WARPS * lists_a_warp) {
+        lists(parts * WARPS * lists_a_warp),
+        per(min(32u, (uint32_t)ROW_TOPS / lists)),
+        room(ROW_LIST / parts) {
 #pragma unroll 1
     for (int b = tid; b < ROW_EDGE_BINS; b += NT) sh.edge_n[b] = 0;
     if (tid == 0) sh.count = 0, sh.first = ~0u, sh.dirty = 0;
@@ -459,7 +463,6 @@ template <typename T, int NT, bool MEM> struct Row {
       top[0] = top[1] = E::top0();
       stream<true, false, false>([&](const uint4& v, uint32_t) { top[0] = E::top(top[0], v); }, [] {});
     }
-    const uint32_t per = top_count();
 #pragma unroll
     for (int l = 0; l < 2; ++l) {
       mine = E::value(top[l]);
@@ -510,7 +513,6 @@ template <typename T, int NT, bool MEM> struct Row {
     }
     const uint32_t k = tops ? sorted_tops() : __reduce_min_sync(~0u, row_key(mine));
     cluster.barrier_wait();
-    const uint32_t per = top_count();
 #pragma unroll 1
     for (uint32_t i0 = 0; i0 < per * ctas; i0 += 32) {
       const uint32_t to = (i0 + lane) / per, e = i0 + lane - to * per, v = __shfl_sync(~0u, k, e);
@@ -536,7 +538,7 @@ template <typename T, int NT, bool MEM> struct Row {
   __device__ __forceinline__ void find_max() {
     uint32_t best = ~0u;
 #pragma unroll 1
-    for (uint32_t i = lane; i < lists; i += 32) best = min(best, sh.tops[i * top_count()]);
+    for (uint32_t i = lane; i < lists; i += 32) best = min(best, sh.tops[i * per]);
     m = row_unkey(__reduce_min_sync(~0u, best));
   }
   // The edge of the candidates of a cut; infinity where they are too many to list.
@@ -552,9 +554,7 @@ template <typename T, int NT, bool MEM> struct Row {
     const float edge = edge_of(n, ROW_EDGE_SCALE * ROW_LOG2E, -ROW_F32_MAX);
     return edge == -ROW_F32_MAX ? edge_of(n, far_scale(), -ROW_F32_MAX) : edge;
   }
-  __device__ __forceinline__ uint32_t most_tops() const { return top_count() * lists * 3 / 4; }
-  // How many of its 32 sorted thread maxima a warp publishes.
-  __device__ __forceinline__ uint32_t top_count() const { return min(32u, (uint32_t)ROW_TOPS / lists); }
+  __device__ __forceinline__ uint32_t most_tops() const { return per * lists * 3 / 4; }
 
   // f(vector, number in the part) for this thread's vectors, two side by side;
   // from memory, with +inf and NaN as they are unless CLEAN; now_and_then() is
@@ -627,7 +627,8 @@ template <typename T, int NT, bool MEM> struct Row {
   }
 
   // Exclusive sum over the block, and the block's sum.
-  template <typename V> __device__ __forceinline__ V block_scan(V v, V* scratch, V& all) const {
+  template <typename V> static __device__ __forceinline__ V block_scan(V v, V* scratch, V& all) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     const V in = warp_scan(v, lane);
     if (lane == 31) scratch[wid] = in;
     __syncthreads();
@@ -786,7 +787,7 @@ template <typename T, int NT, bool MEM> struct Row {
   // more than k.  Every warp scans the histogram for itself, which spares a
   // barrier.
   __device__ __forceinline__ float edge_of(uint32_t k, float scale, float last) {
-    const uint32_t tops = top_count() * lists;
+    const uint32_t tops = per * lists;
     scale = fminf(scale, ROW_F32_MAX);
 #pragma unroll 1
     for (uint32_t i = tid; i < tops; i += NT) {
@@ -816,7 +817,7 @@ template <typename T, int NT, bool MEM> struct Row {
   // Its scale where 42 octaves of weight are too short: up to the smallest
   // maximum, or 512.  Empties the bins again.
   __device__ __forceinline__ float far_scale() {
-    const uint32_t tops = top_count() * lists;
+    const uint32_t tops = per * lists;
     float low = m;
 #pragma unroll 1
     for (uint32_t i = lane; i < tops; i += 32) {
@@ -847,12 +848,9 @@ template <typename T, int NT, bool MEM> struct Row {
     for (uint32_t i = lane; i < ctas * WARPS; i += 32) t += (&of[0][0])[i];
     return warp_sum_u64(t);
   }
-  // The first CTA's list of candidates is divided among the CTAs.
-  __device__ __forceinline__ uint32_t share() const { return ROW_LIST / ctas; }
   // Collects this CTA's entries of at least `edge` in its share of the first
   // CTA's list (sh.count = 0 before), or only finds the first of them.
   __device__ __forceinline__ void collect_above(float edge, bool only_first) {
-    const uint32_t room = share();
     above(edge, [&](float z, int j) {
       if (only_first) {
         atomicMin(cluster.map_shared_rank(&sh.first, 0), (uint32_t)j);
@@ -864,7 +862,6 @@ template <typename T, int NT, bool MEM> struct Row {
   }
   // Hands them to the first CTA and tells every CTA their number.
   __device__ __forceinline__ void tell_list() {
-    const uint32_t room = share();
     __syncthreads();
     if (tid < (int)ctas) *cluster.map_shared_rank(&sh.n[rank], tid) = sh.count;
     if (rank) {
@@ -875,25 +872,18 @@ template <typename T, int NT, bool MEM> struct Row {
   }
   // Whether the candidates of all CTAs fit their shares; their total.
   __device__ __forceinline__ bool all_listed(uint32_t& n) const {
-    bool fit = true;
-    n = 0;
-#pragma unroll 1
-    for (uint32_t i = 0; i < ctas; ++i) n += sh.n[i], fit &= sh.n[i] <= share();
-    return fit;
+    const uint32_t of = lane < (int)ctas ? sh.n[lane] : 0;
+    n = __reduce_add_sync(~0u, of);
+    return __all_sync(~0u, of <= room);
   }
   // f(number, entry) for this thread's candidates, on the first CTA.
   template <typename F> __device__ __forceinline__ void each_listed(F f) const {
-    const uint32_t room = share();
+    const uint32_t of = lane < (int)ctas ? sh.n[lane] : 0, upto = warp_scan(of, lane);
 #pragma unroll 1
-    for (uint32_t s = tid; s < room * ctas; s += NT) {
-      uint32_t before = 0, mine_n = 0, at = s;
+    for (uint32_t r = MEM ? 0 : wid; r < ctas; r += WARPS) {
+      const uint32_t have = __shfl_sync(~0u, of, r), before = __shfl_sync(~0u, upto, r) - have;
 #pragma unroll 1
-      for (uint32_t i = 0; i < ctas; ++i) {
-        const bool in = s >= i * room;
-        if (in) at = s - i * room, mine_n = sh.n[i];
-        if (s >= (i + 1) * room) before += sh.n[i];
-      }
-      if (at < mine_n) f(before + at, sh.list[s]);
+      for (uint32_t i = MEM ? tid : lane; i < have; i += MEM ? NT : 32) f(before + i, sh.list[r * room + i]);
     }
   }
   // Tells every CTA the number of entries that this one has put at the start
@@ -1236,191 +1226,46 @@ template <typename T, int NT, bool MEM> struct Row {
     __syncthreads();
   }
 
-  // Cuts the n <= ROW_FEW entries of f.loose to the first k (0: all),
-  // then to the shortest prefix of at least p of their mass (without k: of the
-  // row's, `total`), then to w >= least_w, and draws: each thread
-  // compares its entry with all others, once in descending order and once in
-  // index order.
-  template <typename H>
-  __device__ __forceinline__ void finish_few(RowFinish& f, uint32_t n, uint32_t k, float p, float least_w, float u, uint64_t total,
-                                             H hit) {
-    const bool in = tid < n;
-    const uint64_t e = in ? f.loose[tid] : ~0ull;
-    const float z = value_of(e), w = in ? weight(z) : 0.0f;
-    const uint64_t q = row_q(w);
-    if (tid < ROW_FEW) f.sorted[tid] = q;
-    if (tid == 0) sh.cut_q = total, sh.cut_c = ~0ull;
-    __syncthreads();
-    uint32_t rank_of = 0;
-    uint64_t before = 0;
-    if (wid * 32 < (int)n) {
-#pragma unroll 4
-      for (uint32_t i = 0; i < n; ++i) {
-        const bool less = f.loose[i] < e;
-        const uint64_t qi = f.sorted[i];
-        rank_of += less;
-        before += less ? qi : 0;
-      }
-    }
-    if (k) {
-      if (in && rank_of == min(k, n) - 1) sh.cut_c = e, sh.cut_q = before + q;
-      __syncthreads();
-    }
-    uint64_t last = sh.cut_c, mass = sh.cut_q;
-    if (p < 1.0f) {
-      const uint64_t target = row_target(p, mass);
-      __syncthreads();
-      if (in && before < target && target <= before + q) sh.cut_c = e, sh.cut_q = before + q;
-      __syncthreads();
-      last = sh.cut_c, mass = sh.cut_q;
-    }
-    if (least_w > 0.0f) {
-      __syncthreads();
-      block_scan(in && e <= last && w >= least_w ? q : 0, sh.scan_q, mass);
-    }
-    const uint64_t t = row_draw(u, mass);
-    const uint64_t own = in && e <= last && w >= least_w ? q : 0;
-    if (__syncthreads_or(own && own == mass)) {  // one entry is left
-      if (own) hit(z, (int)(e & (ROW_MAX_COLS - 1)));
-      return;
-    }
-    if (tid < ROW_FEW) f.sorted[tid] = own;  // kept masses
-    __syncthreads();
-    if (wid * 32 >= (int)n) return;
-    const uint32_t j = (uint32_t)e & (ROW_MAX_COLS - 1);
-    before = 0;
-#pragma unroll 4
-    for (uint32_t i = 0; i < n; ++i) {
-      const uint64_t qi = f.sorted[i];
-      before += ((uint32_t)f.loose[i] & (ROW_MAX_COLS - 1)) < j ? qi : 0;
-    }
-    if (own && before <= t && t < before + own) hit(z, (int)j);
-  }
-
-  // Draws among the first n of f.sorted, kept where w >= least_w, of together
-  // `mass`: the entry at which the running mass in index order exceeds t.
-  template <typename H> __device__ __forceinline__ void draw(RowFinish& f, uint32_t n, float least_w, uint64_t t, H hit) {
-    const int shift = max(0, 32 - __clz((int)cols) - 10);
-    constexpr int PER = ROW_POOL / NT;
-    uint64_t e[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) e[i] = tid + i * NT < n ? f.sorted[tid + i * NT] : 0;
-    order(f, [&](int i, uint64_t& c, uint32_t& bin) {
-      if (tid + i * NT >= n) return false;
-      const uint32_t j = (uint32_t)e[i] & (ROW_MAX_COLS - 1);
-      c = (uint64_t)j << 32 | (uint32_t)(e[i] >> ROW_IDX_BITS);
-      bin = j >> shift;
-      return true;
-    });
-    const uint32_t per = (n + NT - 1) / NT, i0 = min(tid * per, n), i1 = min(i0 + per, n);
-    auto mass_at = [&](uint32_t i) {
-      const float w = weight(row_unkey((uint32_t)f.sorted[i]));
-      return w >= least_w ? row_q(w) : 0;
-    };
-    uint64_t own = 0, all;
-#pragma unroll 1
-    for (uint32_t i = i0; i < i1; ++i) own += mass_at(i);
-    uint64_t run = block_scan(own, sh.scan_q, all);
-    if (t < run || t >= run + own) return;
-#pragma unroll 1
-    for (uint32_t i = i0; i < i1; ++i) {
-      const uint64_t q = mass_at(i);
-      if (t >= run && t < run + q) hit(row_unkey((uint32_t)f.sorted[i]), (int)(f.sorted[i] >> 32));
-      run += q;
-    }
-  }
-
-  // The same for n <= ROW_LIST entries, at f.loose where they are no more than
-  // the threads, else at f.input, above `edge`: by sorting.
-  template <typename H>
-  __device__ __forceinline__ void finish_listed(RowFinish& f, uint32_t n, float edge, const RowParams& q, uint64_t total, H hit) {
-    if (n <= (uint32_t)ROW_FEW) {
-      finish_few(f, n, q.by_k ? q.k : 0, q.p, q.least_w, q.u, total, hit);
-      return;
-    }
-    order_by_value(f, f.input, n, edge);
-    // running masses in descending order, `per` entries a thread
-    const uint32_t per = (n + NT - 1) / NT, i0 = min(tid * per, n), i1 = min(i0 + per, n);
-    uint64_t sum = 0, all;
-#pragma unroll 1
-    for (uint32_t i = i0; i < i1; ++i) sum += mass(value_of(f.sorted[i]));
-    const uint64_t before = block_scan(sum, sh.scan_q, all);
-    if (tid == 0) sh.cut_n = n, sh.cut_q = q.by_k ? all : total;
-    __syncthreads();
-    uint64_t run = before;
-    if (q.by_k && n > q.k) {
-#pragma unroll 1
-      for (uint32_t i = i0; i < i1; ++i) {
-        run += mass(value_of(f.sorted[i]));
-        if (i == q.k - 1) sh.cut_n = q.k, sh.cut_q = run;
-      }
-      __syncthreads();
-    }
-    uint32_t cut = sh.cut_n;
-    if (q.by_p) {
-      const uint64_t target = row_target(q.p, sh.cut_q);
-      __syncthreads();
-      run = before;
-#pragma unroll 1
-      for (uint32_t i = i0; i < i1 && i < cut; ++i) {
-        const uint64_t qi = mass(value_of(f.sorted[i]));
-        if (run < target && target <= run + qi) sh.cut_n = i + 1, sh.cut_q = run + qi;
-        run += qi;
-      }
-      __syncthreads();
-      cut = sh.cut_n;
-    }
-    uint64_t left = sh.cut_q;
-    if (q.by_w) {
-      sum = 0;
-#pragma unroll 1
-      for (uint32_t i = tid; i < cut; i += NT) {
-        const float w = weight(value_of(f.sorted[i]));
-        if (w >= q.least_w) sum += row_q(w);
-      }
-      __syncthreads();
-      block_scan(sum, sh.scan_q, left);
-    }
-    draw(f, cut, q.least_w, row_draw(q.u, left), hit);
-  }
-
-  // Cuts the n entries in sh.pool, those of [sh.lo, sh.hi], where the prefix of
-  // `target` of them (by_mass: of mass `target` with what sh.mass holds) ends, and
-  // adds the kept ones' masses to their stretches' in sh.part.  Returns the
-  // last entry of the cut.  Their exact sums by bins linear in (key, index)
-  // leave those of one bin, and so on until few enough to be compared with
-  // each other are left: equal values, which 16-bit logits have many of, cost
-  // no more than others.
-  __device__ __forceinline__ uint64_t finish_pool(RowFinish& f, uint32_t n, bool by_mass, float least_w, uint64_t target) {
-    constexpr int PER = ROW_POOL / NT, BINS = ROW_SORT_BINS / NT;
+  // Of the n <= ROW_POOL entries with places f.sorted, all different, and sums
+  // f.input: the one at which the running sum in order of place reaches `goal`
+  // (~0: none does), and the sum up to it.  Exact sums by bins leave the
+  // entries of one bin, and so on until few enough to be compared with each
+  // other are left.  Bins are linear in the place over [lo, hi]; scale >= 0: the first
+  // are linear in x, 1 / scale from m down.  Empties f.input of what drops out.
+  // One copy of this serves all cuts and draws of a row.
+  struct Reached {
+    uint64_t at, upto;
+  };
+  static __device__ __noinline__ Reached reach(RowFinish& f, Shared& sh, uint32_t n, uint64_t goal, uint64_t lo, uint64_t hi, float m,
+                                               float scale) {
+    constexpr int BINS = ROW_SORT_BINS / NT;
     constexpr uint32_t FEW = 64;
-    static_assert(BINS * NT == ROW_SORT_BINS && PER * NT == ROW_POOL, "bins and entries a thread");
-    uint32_t* const low = reinterpret_cast<uint32_t*>(f.loose);  // a bin's mass: the low 20 bits of each
+    static_assert(BINS * NT == ROW_SORT_BINS, "bins a thread");
+    const uint32_t tid = threadIdx.x;
+    uint32_t* const low = reinterpret_cast<uint32_t*>(f.loose);  // a bin's sum: the low 20 bits of each
     uint32_t* const high = low + ROW_SORT_BINS;                  // and the rest
-    uint64_t lo = sh.lo, hi = sh.hi, left = by_mass ? target - handed(sh.mass) : target;
-    const uint64_t end = hi;
-    uint64_t e[PER], q[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      e[i] = tid + i * NT < n ? sh.pool[tid + i * NT] : ~0ull;
-      q[i] = by_mass ? mass(value_of(e[i])) : 1;
-    }
+    uint64_t left = goal;
     uint32_t undecided = n;
 #pragma unroll 1
     while (undecided > FEW) {
       const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
+      auto bin_of = [&](uint64_t e) {
+        return scale >= 0.0f ? (uint32_t)fminf(__fmul_rn(__fsub_rn(m, value_of(e)), scale), (float)(ROW_SORT_BINS - 1))
+                             : (uint32_t)((e - lo) >> shift);
+      };
 #pragma unroll
       for (int i = 0; i < BINS; ++i) f.start[tid + i * NT] = low[tid + i * NT] = high[tid + i * NT] = 0;
       __syncthreads();
       if (tid == 0) sh.cut_n = ~0u;
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (e[i] >= lo && e[i] <= hi) {
-          const uint32_t b = (uint32_t)((e[i] - lo) >> shift);
-          atomicAdd(&f.start[b], 1u);
-          atomicAdd(&low[b], (uint32_t)q[i] & 0xfffffu);
-          atomicAdd(&high[b], (uint32_t)(q[i] >> 20));
-        }
+#pragma unroll 1
+      for (uint32_t i = tid; i < n; i += NT) {
+        const uint64_t q = f.input[i];
+        if (!q) continue;
+        const uint32_t b = bin_of(f.sorted[i]);
+        atomicAdd(&f.start[b], 1u);
+        atomicAdd(&low[b], (uint32_t)q & 0xfffffu);
+        atomicAdd(&high[b], (uint32_t)(q >> 20));
+      }
       __syncthreads();
       uint64_t s[BINS], own = 0, all;
 #pragma unroll
@@ -1430,48 +1275,172 @@ template <typename T, int NT, bool MEM> struct Row {
         own += s[i];
       }
       uint64_t run = block_scan(own, sh.scan_q, all);
+      if (run < left && left <= run + own) {
 #pragma unroll
-      for (int i = 0; i < BINS; ++i) {
-        if (run < left && left <= run + s[i]) sh.cut_n = tid * BINS + i, sh.cut_q = run, sh.above = f.start[tid * BINS + i];
-        run += s[i];
+        for (int i = 0; i < BINS; ++i) {
+          if (run < left && left <= run + s[i]) sh.cut_n = tid * BINS + i, sh.cut_q = run, sh.above = f.start[tid * BINS + i];
+          run += s[i];
+        }
       }
       __syncthreads();
-      if (sh.cut_n == ~0u) break;  // not reached: the cut takes them all
+      const uint32_t cut = sh.cut_n;
+      if (cut == ~0u) break;
       left -= sh.cut_q;
       undecided = sh.above;
-      lo += (uint64_t)sh.cut_n << shift;
-      hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+#pragma unroll 1
+      for (uint32_t i = tid; i < n; i += NT)
+        if (f.input[i] && bin_of(f.sorted[i]) != cut) f.input[i] = 0;
+      if (scale < 0.0f) lo += (uint64_t)cut << shift, hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+      scale = -1.0f;
     }
     __syncthreads();
-    if (tid == 0) sh.count = 0, sh.cut_c = end;
+    if (tid == 0) sh.count = 0, sh.cut_c = ~0ull;
     __syncthreads();
     if (undecided <= FEW) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (e[i] >= lo && e[i] <= hi) {
+      uint64_t* const c = f.loose;
+      uint64_t* const q = f.loose + FEW;
+#pragma unroll 1
+      for (uint32_t i = tid; i < n; i += NT)
+        if (f.input[i]) {
           const uint32_t at = atomicAdd(&sh.count, 1u);
-          f.sorted[at] = e[i], f.input[at] = q[i];
+          c[at] = f.sorted[i], q[at] = f.input[i];
         }
       __syncthreads();
-      if (tid < (int)undecided) {
-        const uint64_t mine_e = f.sorted[tid];
-        uint64_t before = 0;
-#pragma unroll 1
-        for (uint32_t i = 0; i < undecided; ++i) before += f.sorted[i] < mine_e ? f.input[i] : 0;
-        if (before < left && left <= before + f.input[tid]) sh.cut_c = mine_e;
+      const uint32_t few = sh.count;
+      if (tid < few) {
+        const uint64_t own = c[tid];
+        uint64_t upto = 0;
+#pragma unroll 2
+        for (uint32_t i = 0; i < few; ++i) upto += c[i] <= own ? q[i] : 0;
+        if (upto >= left && upto - q[tid] < left) sh.cut_c = own, sh.cut_q = upto;
       }
       __syncthreads();
     }
-    const uint64_t last = sh.cut_c;
+    return {sh.cut_c, goal - left + sh.cut_q};
+  }
+
+  // The same sums for n <= NT entries and for each of them, by comparing it
+  // with all: entry tid / each of `each` neighbouring threads, which share its
+  // comparisons.  less(i) says whether entry i comes before it, q its f.input;
+  // returns the sum before it, and their number.
+  template <typename L> static __device__ __forceinline__ uint64_t before_of(const RowFinish& f, uint32_t n, uint32_t each, uint32_t& number, L less) {
+    uint64_t sum = 0;
+    number = 0;
+#pragma unroll 2
+    for (uint32_t i = threadIdx.x & (each - 1); i < n; i += each) {
+      const uint64_t q = f.input[i];
+      const bool yes = less(f.sorted[i]);
+      number += yes;
+      sum += yes ? q : 0;
+    }
+#pragma unroll 1
+    for (uint32_t d = 1; d < each; d <<= 1) {
+      sum += __shfl_xor_sync(~0u, sum, d);
+      number += __shfl_xor_sync(~0u, number, d);
+    }
+    return sum;
+  }
+  // finish_listed() for n <= NT / 2 entries.
+  template <typename H>
+  __device__ __forceinline__ void finish_few(RowFinish& f, uint32_t n, const RowParams& p, uint64_t total, H hit) {
+    const uint32_t each = n <= NT / 8 ? 8 : n <= NT / 4 ? 4 : 2, slot = tid / each;
+    const bool in = slot < n, works = wid * (32 / each) < n;
+    const uint64_t e = in ? f.sorted[slot] : ~0ull;
+    const float z = value_of(e), w = in ? weight(z) : 0.0f;
+    const uint64_t q = row_q(w);
+    if (in) f.input[slot] = q;
+    if (tid == 0) sh.cut_q = total, sh.cut_c = ~0ull;
+    __syncthreads();
+    uint32_t rank_of = 0, number;
+    uint64_t before = 0;
+    if (works) before = before_of(f, n, each, rank_of, [&](uint64_t other) { return other < e; });
+    if (p.by_k) {
+      if (in && rank_of == min(p.k, n) - 1) sh.cut_c = e, sh.cut_q = before + q;
+      __syncthreads();
+    }
+    uint64_t last = sh.cut_c, mass = sh.cut_q;
+    if (p.by_p) {
+      const uint64_t target = row_target(p.p, mass);
+      __syncthreads();
+      if (in && before < target && target <= before + q) sh.cut_c = e, sh.cut_q = before + q;
+      __syncthreads();
+      last = sh.cut_c, mass = sh.cut_q;
+    }
+    const uint64_t own = in && e <= last && w >= p.least_w ? q : 0;
+    if (p.by_w) {
+      __syncthreads();
+      block_scan(tid % each ? 0 : own, sh.scan_q, mass);
+    }
+    if (__syncthreads_or(own && own == mass)) {  // one entry is left
+      if (own && tid % each == 0) hit(z, (int)(e & (ROW_MAX_COLS - 1)));
+      return;
+    }
+    const uint64_t t = row_draw(p.u, mass);
+    if (in) f.input[slot] = own;  // kept masses
+    __syncthreads();
+    if (!works) return;
+    const uint32_t j = (uint32_t)e & (ROW_MAX_COLS - 1);
+    before = before_of(f, n, each, number, [&](uint64_t other) { return ((uint32_t)other & (ROW_MAX_COLS - 1)) < j; });
+    if (tid % each == 0 && own && before <= t && t < before + own) hit(z, (int)j);
+  }
+
+  // Cuts the n entries of f.sorted, those above `edge`, to the first k, then to
+  // the shortest prefix of at least p of their mass (without k: of the row's,
+  // `total`), then to w >= least_w, and draws, in index order.
+  template <typename H>
+  __device__ __forceinline__ void finish_listed(RowFinish& f, uint32_t n, float edge, const RowParams& q, uint64_t total, H hit) {
+    if (n <= (uint32_t)NT / 2) {
+      finish_few(f, n, q, total, hit);
+      return;
+    }
+    float scale = fmaxf((ROW_SORT_BINS - 1) / (m - edge), (ROW_SORT_BINS - 1) / ROW_MASS_END * c);
+    if (!(scale <= ROW_F32_MAX)) scale = 0.0f;  // all equal
+    uint64_t last = ~0ull;
+#pragma unroll 1
+    for (int step = q.by_k ? 0 : q.by_p ? 1 : 2; step < 3; step += step == 0 && !q.by_p ? 2 : 1) {
+      uint64_t own = 0, all;
+#pragma unroll 1
+      for (uint32_t i = tid; i < n; i += NT) {
+        const uint64_t e = f.sorted[i];
+        const float w = weight(value_of(e));
+        const uint64_t v = e <= last && (step < 2 || w >= q.least_w) ? row_q(w) : 0;
+        own += v;
+        f.input[i] = step ? v : 1;
+        if (step == 2) f.sorted[i] = (e & (ROW_MAX_COLS - 1)) << 32 | e >> ROW_IDX_BITS;
+      }
+      block_scan(own, sh.scan_q, all);
+      const uint64_t goal = step == 0 ? q.k : step == 1 ? row_target(q.p, q.by_k ? all : total) : row_draw(q.u, all) + 1;
+      const uint64_t lo = step < 2 ? (uint64_t)row_key(m) << ROW_IDX_BITS : 0;
+      const uint64_t hi = step < 2 ? (uint64_t)row_key(edge) << ROW_IDX_BITS | (ROW_MAX_COLS - 1) : (uint64_t)cols << 32;
+      const Reached r = reach(f, sh, n, goal, lo, hi, m, step < 2 ? scale : -1.0f);
+      if (step < 2)
+        last = min(last, r.at);
+      else if (tid == 0)
+        hit(row_unkey((uint32_t)r.at), (int)(r.at >> 32));
+    }
+  }
+
+  // Cuts the n entries in sh.pool, those of [sh.lo, sh.hi], where the prefix of
+  // `target` of them (by_mass: of mass `target` with what sh.mass holds) ends, and
+  // adds the kept ones' masses to their stretches' in sh.part.  Returns the
+  // last entry of the cut.
+  __device__ __forceinline__ uint64_t finish_pool(RowFinish& f, uint32_t n, bool by_mass, float least_w, uint64_t target) {
+#pragma unroll 1
+    for (uint32_t i = tid; i < n; i += NT) {
+      f.sorted[i] = sh.pool[i];
+      f.input[i] = by_mass ? mass(value_of(sh.pool[i])) : 1;
+    }
+    const uint64_t end = sh.hi, left = by_mass ? target - handed(sh.mass) : target;
+    const uint64_t last = min(end, reach(f, sh, n, left, sh.lo, end, m, -1.0f).at);
     // the warps' kept masses: before the interval, and those of its entries
     if (tid < ROW_SUMS) f.part[tid][0] = f.part[tid][1] = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (e[i] > last) continue;  // none, too
-      const float w = weight(value_of(e[i]));
-      if (w < least_w) continue;
-      const uint32_t v = (((uint32_t)e[i] & (ROW_MAX_COLS - 1)) + lead) / N;
+#pragma unroll 1
+    for (uint32_t i = tid; i < n; i += NT) {
+      const uint64_t e = f.sorted[i];
+      const float w = weight(value_of(e));
+      if (e > last || w < least_w) continue;
+      const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + lead) / N;
       const uint32_t cta = v / part_vecs, p0 = cta * part_vecs, p1 = min(p0 + part_vecs, total_vecs);
       const uint32_t at = cta * WARPS + (v - p0) / ((p1 - p0 + WARPS - 1) / WARPS);
       const uint64_t kept = row_q(w);
@@ -1512,6 +1481,7 @@ template <typename T, int NT, bool MEM> struct Row {
       const float w = weight(z);
       return w >= least_w && (z > low || (z == low && j <= low_j)) ? row_q(w) : 0;
     };
+    const bool takes_equals = last != ~0ull && weight(low) >= least_w;
     constexpr int PER = 2;  // vectors a thread, side by side
 #pragma unroll 1
     for (uint32_t i0 = v0; i0 < v1; i0 += NT * PER) {
@@ -1520,18 +1490,21 @@ template <typename T, int NT, bool MEM> struct Row {
 #pragma unroll
       for (int k = 0; k < PER; ++k) v[k] = i + k < v1 ? from_memory(i + k) : nothing();
       const int j0 = (int)(i * N) - lead;
-      uint64_t own = 0, all;
+      Sum sum(m, c);
 #pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        float z[N];
-        E::get(v[k], z);
-#pragma unroll
-        for (int e = 0; e < N; ++e) own += value(z[e], j0 + k * N + e);
+      for (int k = 0; k < PER; ++k) sum.template add<HEAVY>(v[k], low, least_w);
+      uint64_t own = sum.mass(), all;
+      if (takes_equals) {
+#pragma unroll 1
+        for (int k = 0; k < PER; ++k) {
+          const uint4 of = k ? v[1] : v[0];
+          each_of(hits(of, low, low), of, 0, [&](float z, int e) { own += j0 + k * N + e - first <= low_j ? mass(z) : 0; });
+        }
       }
       uint64_t run = block_scan(own, sh.scan_q, all);
       if (t < all) {
         if (t >= run && t < run + own) {
-#pragma unroll 1
+#pragma unroll 4
           for (int e = 0; e < PER * N; ++e) {
             const float z = E::at(e < N ? v[0] : v[1], e % N);
             const uint64_t q = value(z, j0 + e);
@@ -1633,7 +1606,7 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
       if (q.by_p && !q.by_k) {
         uint64_t part = 0;
 #pragma unroll 1
-        for (uint32_t i = r.tid; i < min(sh.count, r.share()); i += NT) part += r.mass(r.value_of(sh.list[i]));
+        for (uint32_t i = r.tid; i < min(sh.count, r.room); i += NT) part += r.mass(r.value_of(sh.list[i]));
         r.template hand<true>(sh.part, part);
       }
     }
@@ -1648,8 +1621,7 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
     if (enough && !q.by_k && q.by_p) enough = r.handed(sh.part) >= row_target(q.p, total);
     if (enough) {
       if (r.rank) return;
-      uint64_t* const to = n <= (uint32_t)ROW_FEW ? f.loose : f.input;
-      r.each_listed([&](uint32_t i, uint64_t e) { to[i] = e; });
+      r.each_listed([&](uint32_t i, uint64_t e) { f.sorted[i] = e; });
       __syncthreads();
       r.finish_listed(f, n, edge, q, total, store);
       return;
