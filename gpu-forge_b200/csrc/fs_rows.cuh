@@ -280,11 +280,9 @@ template <typename V> __device__ __forceinline__ V warp_scan(V v, int lane) {  /
   }
   return v;
 }
-// *p += v in shared memory where yes, without a branch.
-__device__ __forceinline__ void smem_add_if(bool yes, uint32_t* p, uint32_t v) {
-  asm volatile("{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n @q red.shared.add.u32 [%0], %1;\n}" ::"r"(
-                   (uint32_t)__cvta_generic_to_shared(p)),
-               "r"(v), "r"((uint32_t)yes)
+// Adds v to a word in shared memory where yes, without a branch.
+__device__ __forceinline__ void smem_add_if(bool yes, uint32_t at, uint32_t v) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n @q red.shared.add.u32 [%0], %1;\n}" ::"r"(at), "r"(v), "r"((uint32_t)yes)
                : "memory");
 }
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -941,19 +939,36 @@ template <typename T, int NT, bool MEM> struct Row {
     return lo;
   }
 
-  // A vector's entries by bin of 1/42 octave: their number, or their weights as
+  // A vector's entries by bin of 1/42 octave.  Their weights, up to y_end, as
   // 4096 2^-(y - b) / 42 by the power's tangent, made a whole number by another
-  // addition of 2^23.
-  __device__ __forceinline__ void count_bins(const uint4& v, bool by_mass, float c42, float y_end) const {
-    float z[N];
+  // addition of 2^23.  Two entries an instruction, and all of a vector's places
+  // before the first addition: few warps share an SM here, so what counts is
+  // the length of the chain.
+  __device__ __forceinline__ void weigh_bins(const uint4& v, uint32_t bins, float c42, float y_end) const {
+    constexpr uint32_t MAGIC = 0x4b000000u;  // 2^23
+    const uint64_t magic = f2_pack(0x1p23f, 0x1p23f), minus = f2_pack(-0x1p23f, -0x1p23f), none = f2_pack(-1.0f, -1.0f);
+    const uint64_t tangent = f2_pack(-4096.0f * ROW_LN2 / ROW_BIN_SCALE, -4096.0f * ROW_LN2 / ROW_BIN_SCALE);
+    const uint64_t unit = f2_pack(0x1p23f + 4096.0f, 0x1p23f + 4096.0f), m2 = f2_pack(m, m), c2 = f2_pack(c42, c42);
+    float z[N], y[N], b[N], w[N];
     E::get(v, z);
 #pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const uint64_t place = f2_mul(f2_fma(f2_pack(z[e], z[e + 1]), none, m2), c2);
+      const uint64_t bin = f2_add(place, magic);
+      f2_unpack(place, y[e], y[e + 1]);
+      f2_unpack(bin, b[e], b[e + 1]);
+      f2_unpack(f2_fma(f2_fma(f2_add(bin, minus), none, place), tangent, unit), w[e], w[e + 1]);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      smem_add_if(y[e] < y_end, bins + (__float_as_uint(b[e]) - MAGIC) * 4, __float_as_uint(w[e]) - MAGIC);
+  }
+  // Their numbers.
+  __device__ __forceinline__ void count_bins(const uint4& v, uint32_t bins, float c42) const {
+#pragma unroll 1
     for (int e = 0; e < N; ++e) {
-      const float y = place_of(z[e], c42);
-      const float b = __fadd_rn(fminf(y, (float)(ROW_BINS - 1)), 0x1p23f);
-      const float w = __fmaf_rn(__fsub_rn(y, __fsub_rn(b, 0x1p23f)), -4096.0f * ROW_LN2 / ROW_BIN_SCALE, 0x1p23f + 4096.0f);
-      smem_add_if(by_mass ? y < y_end : z[e] > -INFINITY, &sh.bins[__float_as_uint(b) & 0x7fffffu],
-                  by_mass ? __float_as_uint(w) & 0x7fffffu : 1u);
+      const float z = E::at(v, e);
+      smem_add_if(z > -INFINITY, bins + bin_at(place_of(z, c42)) * 4, 1u);
     }
   }
   // From the bins' sums over the row, by one CTA: the bins sh.b1 to sh.b2 that
@@ -1078,7 +1093,13 @@ template <typename T, int NT, bool MEM> struct Row {
       if (round == 0) {
         // what the prefix leaves is at least `rest`: its first entry has at least rest / cols
         const float y_end = ROW_BIN_SCALE * fminf(ROW_MASS_END, 41.125f - log2f(fmaxf((float)rest / (float)cols, 0x1p-8f)));
-        vectors<false>([&](const uint4& v, uint32_t) { count_bins(v, by_mass, c42, y_end); }, [] {});
+        const uint32_t bins = smem_of(sh.bins);
+        vectors<false>([&](const uint4& v, uint32_t) {
+          if (by_mass)
+            weigh_bins(v, bins, c42, y_end);
+          else
+            count_bins(v, bins, c42);
+        }, [] {});
       } else {
         between(value_of(hi), value_of(lo), [&](float z, int j) {
           const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
