@@ -42,7 +42,8 @@ constexpr uint32_t ROW_NUCLEUS_GUESS = 128;
 constexpr int ROW_EDGE_BINS = 256;
 constexpr float ROW_EDGE_SCALE = 6.0f;
 constexpr int ROW_BINS = 1792;
-constexpr float ROW_BIN_SCALE = 42.0f;
+constexpr int ROW_BINS_END = ROW_BINS - 28;  // of weights
+constexpr float ROW_BIN_SCALE = 42.0f;        // of counts, an octave
 constexpr float ROW_MASS_END = 42.0f;  // octaves: no mass beyond
 constexpr int ROW_SORT_BINS = 1024;
 
@@ -918,18 +919,18 @@ template <typename T, int NT, bool MEM> struct Row {
   // ---- narrowing a cut down, by the whole cluster ----
   // Bins of 1/42 octave: y c 42 to the nearest whole number, by an addition
   // that pushes the fraction out of the mantissa.
-  __device__ __forceinline__ float place_of(float v, float c42) const { return __fmul_rn(__fsub_rn(m, v), c42); }
+  __device__ __forceinline__ float place_of(float v, float cs) const { return __fmul_rn(__fsub_rn(m, v), cs); }
   static __device__ __forceinline__ uint32_t bin_at(float place) {
     return __float_as_uint(__fadd_rn(fminf(place, (float)(ROW_BINS - 1)), 0x1p23f)) & 0x7fffffu;
   }
   // The smallest key from the maximum's on whose bin is b or later; one warp,
   // 32 probes at a time.
-  __device__ __forceinline__ uint32_t first_key(uint32_t b, float c42) const {
+  __device__ __forceinline__ uint32_t first_key(uint32_t b, float cs) const {
     uint32_t lo = row_key(m), hi = row_key(-ROW_F32_MAX) + 1;
 #pragma unroll 1
     while (lo < hi) {
       const uint32_t step = max(1u, (hi - lo) / 32), at = lo + lane * step;
-      const bool past = at - lo >= hi - lo || bin_at(place_of(row_unkey(at), c42)) >= b;
+      const bool past = at - lo >= hi - lo || bin_at(place_of(row_unkey(at), cs)) >= b;
       const uint32_t has = __ballot_sync(~0u, past);
       if (has & 1) break;
       const int f = has ? __ffs((int)has) - 1 : 32;
@@ -944,11 +945,12 @@ template <typename T, int NT, bool MEM> struct Row {
   // addition of 2^23.  Two entries an instruction, and all of a vector's places
   // before the first addition: few warps share an SM here, so what counts is
   // the length of the chain.
-  __device__ __forceinline__ void weigh_bins(const uint4& v, uint32_t bins, float c42, float y_end) const {
+  __device__ __forceinline__ void weigh_bins(const uint4& v, uint32_t bins, float cs, float per_octave) const {
     constexpr uint32_t MAGIC = 0x4b000000u;  // 2^23
     const uint64_t magic = f2_pack(0x1p23f, 0x1p23f), minus = f2_pack(-0x1p23f, -0x1p23f), none = f2_pack(-1.0f, -1.0f);
-    const uint64_t tangent = f2_pack(-4096.0f * ROW_LN2 / ROW_BIN_SCALE, -4096.0f * ROW_LN2 / ROW_BIN_SCALE);
-    const uint64_t unit = f2_pack(0x1p23f + 4096.0f, 0x1p23f + 4096.0f), m2 = f2_pack(m, m), c2 = f2_pack(c42, c42);
+    const float slope = -4096.0f * ROW_LN2 / per_octave;
+    const uint64_t tangent = f2_pack(slope, slope);
+    const uint64_t unit = f2_pack(0x1p23f + 4096.0f, 0x1p23f + 4096.0f), m2 = f2_pack(m, m), c2 = f2_pack(cs, cs);
     float z[N], y[N], b[N], w[N];
     E::get(v, z);
 #pragma unroll
@@ -961,14 +963,14 @@ template <typename T, int NT, bool MEM> struct Row {
     }
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      smem_add_if(y[e] < y_end, bins + (__float_as_uint(b[e]) - MAGIC) * 4, __float_as_uint(w[e]) - MAGIC);
+      smem_add_if(y[e] < (float)ROW_BINS_END, bins + (__float_as_uint(b[e]) - MAGIC) * 4, __float_as_uint(w[e]) - MAGIC);
   }
   // Their numbers.
-  __device__ __forceinline__ void count_bins(const uint4& v, uint32_t bins, float c42) const {
+  __device__ __forceinline__ void count_bins(const uint4& v, uint32_t bins, float cs) const {
 #pragma unroll 1
     for (int e = 0; e < N; ++e) {
       const float z = E::at(v, e);
-      smem_add_if(z > -INFINITY, bins + bin_at(place_of(z, c42)) * 4, 1u);
+      smem_add_if(z > -INFINITY, bins + bin_at(place_of(z, cs)) * 4, 1u);
     }
   }
   // From the bins' sums over the row, by one CTA: the bins sh.b1 to sh.b2 that
@@ -980,12 +982,13 @@ template <typename T, int NT, bool MEM> struct Row {
   // together; from the second round on estimates follow q.  Counts are exact.)
   // Else it ends in the last bin with anything; a count that is not reached,
   // beyond all of them.
-  __device__ __forceinline__ void end_bins(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n, float top_w) {
+  __device__ __forceinline__ void end_bins(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n, float top_w,
+                                           float octaves) {
     constexpr int PER = (ROW_BINS + NT - 1) / NT;
     const int at = tid * PER, end = min(at + PER, ROW_BINS);
     auto sum_of = [&](int b) {
       const float v = (float)sh.bins[b];
-      return by_mass ? v * (by_weight ? row_exp2((float)b * (-1.0f / ROW_BIN_SCALE)) : top_w) : v;
+      return by_mass ? v * (by_weight ? row_exp2((float)b * -octaves) : top_w) : v;
     };
     float own = 0, all;
     uint32_t filled = 0;
@@ -1019,14 +1022,14 @@ template <typename T, int NT, bool MEM> struct Row {
   // In the first round by mass a little before and behind them, by more than
   // the rounding of a bin's bound, which spares the search; counts, and the
   // rounds that have to shorten the interval, need the bounds themselves.
-  __device__ __forceinline__ uint64_t end_of(bool by_mass, bool by_weight, bool first_round, float c42, int shift, uint64_t lo,
+  __device__ __forceinline__ uint64_t end_of(bool by_mass, bool by_weight, bool first_round, float cs, int shift, uint64_t lo,
                                              uint64_t hi) {
     if (wid >= 2) return 0;
     const uint32_t end = by_mass ? sh.last : (uint32_t)ROW_BINS - 1;
     const uint32_t b = wid ? min(sh.b2, end) + 1 : min(sh.b1, end);
     uint64_t at;
     if (by_mass && first_round) {
-      const float d = __fdiv_rn((float)b - 0.5f, c42), by = fabsf(m) * 0x1p-21f;
+      const float d = __fdiv_rn((float)b - 0.5f, cs), by = fabsf(m) * 0x1p-21f;
       if (wid) {
         const float z = m - d * (1.0f + 0x1p-18f) - by;
         return b < (uint32_t)ROW_BINS && z > -ROW_F32_MAX ? (uint64_t)row_key(z) << ROW_IDX_BITS | (ROW_MAX_COLS - 1) : hi;
@@ -1034,7 +1037,7 @@ template <typename T, int NT, bool MEM> struct Row {
       return b ? max(lo, (uint64_t)row_key(fminf(fmaxf(m - d * (1.0f - 0x1p-18f) + by, -ROW_F32_MAX), m)) << ROW_IDX_BITS) : lo;
     }
     if (by_weight)
-      at = b < (uint32_t)ROW_BINS ? max(lo, (uint64_t)first_key(b, c42) << ROW_IDX_BITS) : hi + 1;
+      at = b < (uint32_t)ROW_BINS ? max(lo, (uint64_t)first_key(b, cs) << ROW_IDX_BITS) : hi + 1;
     else
       at = lo + ((uint64_t)b << shift);
     at = min(at, hi + 1);
@@ -1079,6 +1082,11 @@ template <typename T, int NT, bool MEM> struct Row {
     uint64_t lo = (uint64_t)row_key(m) << ROW_IDX_BITS, hi = (uint64_t)row_key(-ROW_F32_MAX) << ROW_IDX_BITS | (ROW_MAX_COLS - 1);
     uint64_t above_q = 0;
     above_n = 0;
+    // Bins an octave of weight.  What a nucleus leaves is at least `rest`, and so its last entry has at least rest / cols:
+    // the bins of weights end an octave further on (or at the last weight that q holds).
+    const float per_octave =
+        by_mass ? ROW_BINS_END / fminf(ROW_MASS_END, 41.125f - log2f(fmaxf((float)rest / (float)cols, 0x1p-8f))) : ROW_BIN_SCALE;
+    const float octaves = 1.0f / per_octave, cs = fminf(c * per_octave, ROW_F32_MAX);
     constexpr int ROUNDS = 16;
 #pragma unroll 1
     for (int round = 0; round < ROUNDS; ++round) {
@@ -1088,17 +1096,15 @@ template <typename T, int NT, bool MEM> struct Row {
       if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ~0u, sh.last = 0;
       __syncthreads();
       const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
-      const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w, c42 = fminf(c * ROW_BIN_SCALE, ROW_F32_MAX);
-      const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), c42)) >= bin_at(place_of(value_of(lo), c42)) + 3);
+      const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w;
+      const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), cs)) >= bin_at(place_of(value_of(lo), cs)) + 3);
       if (round == 0) {
-        // what the prefix leaves is at least `rest`: its first entry has at least rest / cols
-        const float y_end = ROW_BIN_SCALE * fminf(ROW_MASS_END, 41.125f - log2f(fmaxf((float)rest / (float)cols, 0x1p-8f)));
         const uint32_t bins = smem_of(sh.bins);
         vectors<false>([&](const uint4& v, uint32_t) {
           if (by_mass)
-            weigh_bins(v, bins, c42, y_end);
+            weigh_bins(v, bins, cs, per_octave);
           else
-            count_bins(v, bins, c42);
+            count_bins(v, bins, cs);
         }, [] {});
       } else {
         between(value_of(hi), value_of(lo), [&](float z, int j) {
@@ -1107,8 +1113,8 @@ template <typename T, int NT, bool MEM> struct Row {
           if (!by_mass) {
             atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], 1u);
           } else if (by_weight) {
-            const uint32_t b = bin_at(place_of(z, c42));
-            atomicAdd(&sh.bins[b], (uint32_t)(held(weight(z)) * row_exp2((float)b * (1.0f / ROW_BIN_SCALE) + 12.0f) + 0.5f));
+            const uint32_t b = bin_at(place_of(z, cs));
+            atomicAdd(&sh.bins[b], (uint32_t)(held(weight(z)) * row_exp2((float)b * octaves + 12.0f) + 0.5f));
           } else {
             atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], (uint32_t)(held(weight(z)) * scale + 0.5f));
           }
@@ -1130,8 +1136,8 @@ template <typename T, int NT, bool MEM> struct Row {
       cluster.sync();
       if (rank == 0) {
         const float goal = by_mass ? (float)(target - above_q) * 0x1p-28f : (float)(target - above_n);
-        end_bins(by_mass, by_weight, round == 0, goal, above_n, top_w);
-        const uint64_t at = end_of(by_mass, by_weight, round == 0, c42, shift, lo, hi);
+        end_bins(by_mass, by_weight, round == 0, goal, above_n, top_w, octaves);
+        const uint64_t at = end_of(by_mass, by_weight, round == 0, cs, shift, lo, hi);
         if (wid < 2) {
           if (lane < (int)ctas) {
             *cluster.map_shared_rank(wid ? &sh.hi : &sh.lo, lane) = at;
