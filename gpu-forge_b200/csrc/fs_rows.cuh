@@ -917,8 +917,8 @@ template <typename T, int NT, bool MEM> struct Row {
   }
 
   // ---- narrowing a cut down, by the whole cluster ----
-  // Bins of 1/42 octave: y c 42 to the nearest whole number, by an addition
-  // that pushes the fraction out of the mantissa.
+  // Bins of weight: (m - x) cs, that is y by the bins an octave, to the nearest
+  // whole number, by an addition that pushes the fraction out of the mantissa.
   __device__ __forceinline__ float place_of(float v, float cs) const { return __fmul_rn(__fsub_rn(m, v), cs); }
   static __device__ __forceinline__ uint32_t bin_at(float place) {
     return __float_as_uint(__fadd_rn(fminf(place, (float)(ROW_BINS - 1)), 0x1p23f)) & 0x7fffffu;
@@ -940,17 +940,21 @@ template <typename T, int NT, bool MEM> struct Row {
     return lo;
   }
 
-  // A vector's entries by bin of 1/42 octave.  Their weights, up to y_end, as
-  // 4096 2^-(y - b) / 42 by the power's tangent, made a whole number by another
-  // addition of 2^23.  Two entries an instruction, and all of a vector's places
+  // The unit of a weight in its bin: with it 32 bits hold the sum of every
+  // entry that a CTA has.
+  static constexpr float UNIT = MEM ? 0x1p12f : 0x1p16f;
+  static constexpr int UNIT_BITS = MEM ? 12 : 16;
+  // A vector's entries by bin.  Their weights, up to the last bin, as
+  // UNIT 2^-(y - b) / per_octave by the power's tangent, made a whole number by
+  // another addition of 2^23.  Two entries an instruction, and all of a vector's places
   // before the first addition: few warps share an SM here, so what counts is
   // the length of the chain.
   __device__ __forceinline__ void weigh_bins(const uint4& v, uint32_t bins, float cs, float per_octave) const {
     constexpr uint32_t MAGIC = 0x4b000000u;  // 2^23
     const uint64_t magic = f2_pack(0x1p23f, 0x1p23f), minus = f2_pack(-0x1p23f, -0x1p23f), none = f2_pack(-1.0f, -1.0f);
-    const float slope = -4096.0f * ROW_LN2 / per_octave;
+    const float slope = -UNIT * ROW_LN2 / per_octave;
     const uint64_t tangent = f2_pack(slope, slope);
-    const uint64_t unit = f2_pack(0x1p23f + 4096.0f, 0x1p23f + 4096.0f), m2 = f2_pack(m, m), c2 = f2_pack(cs, cs);
+    const uint64_t unit = f2_pack(0x1p23f + UNIT, 0x1p23f + UNIT), m2 = f2_pack(m, m), c2 = f2_pack(cs, cs);
     float z[N], y[N], b[N], w[N];
     E::get(v, z);
 #pragma unroll
@@ -976,10 +980,11 @@ template <typename T, int NT, bool MEM> struct Row {
   // From the bins' sums over the row, by one CTA: the bins sh.b1 to sh.b2 that
   // the prefix ends in (both ~0 before, and at most sh.last, 0 before), and for
   // counts the entries before them, sh.above.  The prefix ends in b1 or later, and in b2 or before: where a sum of
-  // estimates, 2^-12 of it and in the first round 2^-20 of the largest weight
+  // estimates, its slack and in the first round 2^-20 of the largest weight
   // added, and taken off, reaches the goal.  (An estimate is off by half a unit
-  // of 4060 and less than 2^-14; the weights' rounding to q by at most 2^-22
-  // together; from the second round on estimates follow q.  Counts are exact.)
+  // and, a tangent at most half a bin from where it touches, by a 16th of the
+  // bin's width squared; the weights' rounding to q by at most 2^-22 together;
+  // from the second round on estimates follow q.  Counts are exact.)
   // Else it ends in the last bin with anything; a count that is not reached,
   // beyond all of them.
   __device__ __forceinline__ void end_bins(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n, float top_w,
@@ -987,7 +992,7 @@ template <typename T, int NT, bool MEM> struct Row {
     constexpr int PER = (ROW_BINS + NT - 1) / NT;
     const int at = tid * PER, end = min(at + PER, ROW_BINS);
     auto sum_of = [&](int b) {
-      const float v = (float)sh.bins[b];
+      const float v = __uint_as_float(sh.bins[b]);
       return by_mass ? v * (by_weight ? row_exp2((float)b * -octaves) : top_w) : v;
     };
     float own = 0, all;
@@ -1001,7 +1006,7 @@ template <typename T, int NT, bool MEM> struct Row {
     filled = __reduce_max_sync(~0u, filled);
     if (lane == 0) atomicMax(&sh.last, filled);
     float run = block_scan(own, reinterpret_cast<float*>(sh.scan_n), all);
-    const float slack = by_mass ? 0x1p-12f : 0.0f, more = by_mass && first_round ? 0x1p-8f : 0.0f;
+    const float slack = by_mass ? 1.25f / UNIT + 0.0625f * octaves * octaves : 0.0f, more = by_mass && first_round ? UNIT * 0x1p-20f : 0.0f;
     uint32_t b1 = ~0u, b2 = ~0u;
 #pragma unroll 1
     for (int b = at; b < end; ++b) {
@@ -1052,12 +1057,12 @@ template <typename T, int NT, bool MEM> struct Row {
   //   of entries with w >= least_w in sh.part, on all CTAs,
   //   the number of entries before it in above_n (counts alone).
   // Each round counts the undecided entries by bin, or sums their weights, each
-  // to 13 bits of its bin's, which tells the bin, or next to its bounds the two
+  // to 13 or 17 bits of its bin's, which tells the bin, or next to its bounds the two
   // or three, that the prefix ends in; a second pass takes what comes before by
   // its exact mass, so that the estimates of the next round err by a part of
-  // the rest alone.  Bins are of 1/42 octave of weight, and of a 2^-10th of the
-  // interval once it is shorter than three of those (for counts: after the
-  // first round).  (key, index) has no ties: an interval can always be cut.
+  // the rest alone.  Bins are of a 42nd octave of weight or less, by how far
+  // the nucleus may reach, and of a 2^-10th of the interval once it is shorter
+  // than three of those (for counts: after the first round).  (key, index) has no ties: an interval can always be cut.
   // `rounds` bounds them all the same; it takes two or three, and far in the
   // tail, where the rest shrinks by 2^-12 a round, up to eight.
   // A weight as q holds it.
@@ -1096,7 +1101,7 @@ template <typename T, int NT, bool MEM> struct Row {
       if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ~0u, sh.last = 0;
       __syncthreads();
       const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
-      const float top_w = weight(value_of(lo)), scale = 4096.0f / top_w;
+      const float top_w = weight(value_of(lo)), scale = UNIT / top_w;
       const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), cs)) >= bin_at(place_of(value_of(lo), cs)) + 3);
       if (round == 0) {
         const uint32_t bins = smem_of(sh.bins);
@@ -1114,7 +1119,7 @@ template <typename T, int NT, bool MEM> struct Row {
             atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], 1u);
           } else if (by_weight) {
             const uint32_t b = bin_at(place_of(z, cs));
-            atomicAdd(&sh.bins[b], (uint32_t)(held(weight(z)) * row_exp2((float)b * octaves + 12.0f) + 0.5f));
+            atomicAdd(&sh.bins[b], (uint32_t)(held(weight(z)) * row_exp2((float)b * octaves + (float)UNIT_BITS) + 0.5f));
           } else {
             atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], (uint32_t)(held(weight(z)) * scale + 0.5f));
           }
@@ -1127,15 +1132,15 @@ template <typename T, int NT, bool MEM> struct Row {
       for (uint32_t i = tid; i < slice; i += NT) {
         const uint32_t b = rank * slice + i;
         if (b < ROW_BINS) {
-          uint32_t v = 0;
+          float v = 0;
 #pragma unroll 8
-          for (uint32_t k = 0; k < ctas; ++k) v += cluster.map_shared_rank(sh.bins, k)[b];
-          cluster.map_shared_rank(sh.bins, 0)[b] = v;
+          for (uint32_t k = 0; k < ctas; ++k) v += (float)cluster.map_shared_rank(sh.bins, k)[b];
+          cluster.map_shared_rank(sh.bins, 0)[b] = __float_as_uint(v);
         }
       }
       cluster.sync();
       if (rank == 0) {
-        const float goal = by_mass ? (float)(target - above_q) * 0x1p-28f : (float)(target - above_n);
+        const float goal = by_mass ? (float)(target - above_q) * (UNIT * 0x1p-40f) : (float)(target - above_n);
         end_bins(by_mass, by_weight, round == 0, goal, above_n, top_w, octaves);
         const uint64_t at = end_of(by_mass, by_weight, round == 0, cs, shift, lo, hi);
         if (wid < 2) {
