@@ -86,10 +86,20 @@ template <typename T, bool BEST> int launch_solo(fs_sorter* s, const SorterView&
   return FS_OK;
 }
 
+// A cluster a row, or one CTA that streams it.  While one wave of clusters
+// takes the batch, clusters: they read a row once and several CTAs share its
+// work (16 rows of 128256 bf16, n = 20: 11.7 us against 20.8; 96 rows: 19.2
+// against 21.4).  Beyond, a streaming CTA has no partners to wait for (148 rows:
+// 23.9 us against 28.4; 1024 rows: 102 against 118; 1024 x 128256 f32: 166
+// against 195), but not for rows of a single part (512 x 32000 bf16: 30.5 us against
+// 26.4).  Nor for nuclei: a row whose cut lies far down takes several times as
+// long as the rest of the batch, and less so on several CTAs (256 x 131072 bf16
+// peaked rows, a sixth of them such: 80 us by clusters, 109 streaming; where
+// all rows are such, 256 x 128256 bf16, 126 and 115).
 template <typename T, bool BEST> int launch(fs_sorter* s, const SorterView& v, RowArgs& a) {
   const uint32_t ctas = row_ctas(row_vecs(a, RowElem<T>::N) * 16, a.rows, v.sm_count);
-  const bool solo = v.row_form ? v.row_form == 2 : ctas > 1 && (uint64_t)ctas * a.rows > 3ull * v.sm_count;
-  return solo ? launch_solo<T, BEST>(s, v, a) : launch_clusters<T, BEST>(s, v, a);
+  const bool streams = !a.top_p && ctas > 1 && (uint64_t)ctas * a.rows > 3ull * v.sm_count;
+  return (v.row_form ? v.row_form == 2 : streams) ? launch_solo<T, BEST>(s, v, a) : launch_clusters<T, BEST>(s, v, a);
 }
 
 template <bool BEST> int launch_rows(fs_sorter* s, const SorterView& v, int dtype, RowArgs& a, int sync) {
