@@ -43,15 +43,20 @@ struct SlotArgs {
   uint64_t capacity;
   int32_t* cursor_out;
   int* host_err;
+  bool wide;  // positions, request_of and slots begin at 16-byte boundaries
 };
 
 template <typename I> __device__ __forceinline__ int64_t length_of(const void* p, uint32_t r) {
   const int64_t v = static_cast<const I*>(p)[r];
   return v > 0 ? v : 0;
 }
+// A division of 64-bit numbers takes several times as long as one of 32.
+__device__ __forceinline__ int64_t div_page(int64_t tokens, uint32_t page) {
+  return (uint64_t)tokens >> 32 ? tokens / page : (int64_t)((uint32_t)tokens / page);
+}
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, uint32_t page, uint32_t width) {
-  const int64_t n = tokens / page + (tokens % page != 0);
-  return n < width ? n : width;
+  const int64_t n = div_page(tokens, page), all = n + (n * page != tokens);
+  return all < width ? all : width;
 }
 
 constexpr int SLOT_THREADS = 512;
@@ -72,6 +77,7 @@ __device__ __forceinline__ void block_scan(int64_t& x, int64_t& y, int64_t (*war
   __syncthreads();
   all_x = all_y = 0;
   int64_t bx = 0, by = 0;
+#pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     if (w == wid) bx = all_x, by = all_y;
     all_x += warp[w][0], all_y += warp[w][1];
@@ -80,11 +86,22 @@ __device__ __forceinline__ void block_scan(int64_t& x, int64_t& y, int64_t (*war
 }
 
 // Every CTA takes both sums over all requests, SLOT_CHUNK of them at a time,
-// and plans the tokens of its own tiles of SLOT_THREADS tokens that belong to
+// and plans the tokens of its own tiles of SLOT_THREADS x TOK tokens that belong to
 // the chunk; the first CTA writes what is one per request.  The sums are taken
 // again by each CTA (two numbers per request from L2) instead of handed on:
-// one launch, no scratch, nobody waits.
-template <typename I> __global__ void __launch_bounds__(SLOT_THREADS) k_plan_slots(const SlotArgs a) {
+// one launch, no scratch, nobody waits.  A thread plans TOK neighbouring
+// tokens: it looks its request up once and writes 16 bytes at a time.
+template <typename I, int TOK> __device__ __forceinline__ void put(I* to, const I (&v)[TOK]) {
+  constexpr int PER = 16 / sizeof(I) < TOK ? 16 / sizeof(I) : TOK;
+#pragma unroll
+  for (int k = 0; k < TOK; k += PER) {
+    union { I e[PER]; uint4 v; } u;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) u.e[e] = v[k + e];
+    *reinterpret_cast<uint4*>(to + k) = u.v;
+  }
+}
+template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k_plan_slots(const SlotArgs a) {
   __shared__ int64_t warp[SLOT_THREADS / 32][2];
   __shared__ int32_t start[SLOT_CHUNK + 1];  // of the chunk's requests
   __shared__ int64_t took[SLOT_CHUNK];
@@ -125,40 +142,72 @@ template <typename I> __global__ void __launch_bounds__(SLOT_THREADS) k_plan_slo
     tokens += all_t, pages += all_p;
     __syncthreads();
     // the first of this CTA's tiles that reaches into [from, to)
-    int64_t tile = from / SLOT_THREADS;
+    constexpr int TILE = SLOT_THREADS * TOK;
+    int64_t tile = from / TILE;
     tile += ((int64_t)blockIdx.x - tile % gridDim.x + gridDim.x) % gridDim.x;
-    for (int64_t i = tile * SLOT_THREADS + tid; i - tid < to; i += (int64_t)gridDim.x * SLOT_THREADS) {
-      if (i < from || i >= to) continue;
-      int lo = 0, hi = n;  // the chunk's last request that starts at or before i
+    for (int64_t i0 = tile * TILE + tid * TOK; i0 - tid * TOK < to; i0 += (int64_t)gridDim.x * TILE) {
+      const int64_t i1 = max(i0, from), i2 = min(i0 + TOK, to);
+      if (i1 >= i2) continue;
+      int lo = 0, hi = n;  // the chunk's last request that starts at or before i1
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (start[mid] <= i)
+        if (start[mid] <= i1)
           lo = mid;
         else
           hi = mid;
       }
-      const int64_t ctx = length_of<I>(a.ctx, r0 + lo);
-      const int64_t pos = ctx + i - start[lo];
-      const int64_t nth = pos / a.page, off = pos - nth * a.page;
+      int32_t request[TOK];
+      I position[TOK];
+      int64_t slot[TOK];
+      int64_t pos = 0, nth = 0, off = 0, have = 0;
+      int32_t* row = nullptr;
       int32_t id = -1;
-      if (nth < (int64_t)a.width) {
-        int32_t* entry = a.table + (int64_t)(r0 + lo) * a.table_stride + nth;
-        const int64_t have = pages_of(ctx, a.page, a.width);
-        if (nth < have) {
-          id = *entry;
+      bool look = true;  // the request is a new one
+#pragma unroll
+      for (int k = 0; k < TOK; ++k) {
+        const int64_t i = i0 + k;
+        if (i < i1 || i >= i2) continue;
+        while (lo + 1 < n && start[lo + 1] <= i) ++lo, look = true;
+        bool turn = look;  // the page is another one
+        if (look) {
+          const int64_t ctx = length_of<I>(a.ctx, r0 + lo);
+          pos = ctx + i - start[lo];
+          nth = div_page(pos, a.page), off = pos - nth * a.page;
+          have = pages_of(ctx, a.page, a.width);
+          row = a.table + (int64_t)(r0 + lo) * a.table_stride;
+          look = false;
         } else {
-          const uint64_t f = (uint64_t)(cursor + took[lo] + nth - have);
-          if (f < a.n_free) id = a.free_pages[f];
-          if (off == 0) *entry = id;
+          ++pos;
+          if (++off == a.page) ++nth, off = 0, turn = true;
         }
+        if (turn) {
+          id = -1;
+          if (nth < have) {
+            id = row[nth];
+          } else if (nth < (int64_t)a.width) {
+            const uint64_t f = (uint64_t)(cursor + took[lo] + nth - have);
+            if (f < a.n_free) id = a.free_pages[f];
+            if (off == 0) row[nth] = id;
+          }
+        }
+        missed |= id < 0 || i >= (int64_t)a.capacity;
+        request[k] = (int32_t)(r0 + lo);
+        position[k] = (I)pos;
+        slot[k] = id < 0 ? -1 : (int64_t)id * a.page + off;
       }
-      if (id < 0) missed = true;
-      if (i < (int64_t)a.capacity) {
-        a.request_of[i] = (int32_t)(r0 + lo);
-        static_cast<I*>(a.positions)[i] = (I)pos;
-        a.slots[i] = id < 0 ? -1 : (int64_t)id * a.page + off;
+      if (TOK > 1 && a.wide && i2 - i1 == TOK && i2 <= (int64_t)a.capacity) {
+        put(a.request_of + i0, request);
+        put(static_cast<I*>(a.positions) + i0, position);
+        put(a.slots + i0, slot);
       } else {
-        missed = true;
+#pragma unroll
+        for (int k = 0; k < TOK; ++k) {
+          const int64_t i = i0 + k;
+          if (i < i1 || i >= i2 || i >= (int64_t)a.capacity) continue;
+          a.request_of[i] = request[k];
+          static_cast<I*>(a.positions)[i] = position[k];
+          a.slots[i] = slot[k];
+        }
       }
     }
     __syncthreads();
@@ -178,11 +227,15 @@ template <typename I> __global__ void __launch_bounds__(SLOT_THREADS) k_plan_slo
   if (missed) *a.host_err = DEV_ERR_PAGES;
 }
 
-template <typename I> int launch_slots(fs_sorter* s, const SorterView& v, const SlotArgs& a) {
-  const uint64_t tiles = (a.capacity + SLOT_THREADS - 1) / SLOT_THREADS, cap = (uint64_t)v.sm_count * 2;
-  k_plan_slots<I><<<(unsigned)(tiles < 1 ? 1 : tiles < cap ? tiles : cap), SLOT_THREADS, 0, v.stream>>>(a);
+template <typename I, int TOK> int launch_tokens(fs_sorter* s, const SorterView& v, const SlotArgs& a) {
+  constexpr uint64_t TILE = SLOT_THREADS * TOK;
+  const uint64_t tiles = (a.capacity + TILE - 1) / TILE, cap = (uint64_t)v.sm_count * 4;
+  k_plan_slots<I, TOK><<<(unsigned)(tiles < 1 ? 1 : tiles < cap ? tiles : cap), SLOT_THREADS, 0, v.stream>>>(a);
   FS_SLOTS_CUDA(s, cudaGetLastError());
   return FS_OK;
+}
+template <typename I> int launch_slots(fs_sorter* s, const SorterView& v, const SlotArgs& a) {
+  return a.capacity > (uint64_t)v.sm_count * SLOT_THREADS ? launch_tokens<I, 4>(s, v, a) : launch_tokens<I, 1>(s, v, a);
 }
 
 }  // namespace
@@ -208,6 +261,8 @@ extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_
   if (!context_lens || !new_lens || !block_table || !cursor || !query_start || !seq_lens || !cursor_out ||
       (n_free && !free_pages) || (capacity && (!positions || !request_of || !slots)))
     return sorter_fail(s, FS_E_INVALID, "a required pointer is NULL");
+  if (seq_lens == context_lens || seq_lens == new_lens)
+    return sorter_fail(s, FS_E_INVALID, "seq_lens is the same memory as context_lens or new_lens");
   if (cursor == cursor_out) return sorter_fail(s, FS_E_INVALID, "cursor and cursor_out are the same memory");
   SorterView v;
   int rc = sorter_view(s, stream, &v);
@@ -241,6 +296,7 @@ extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_
   a.capacity = capacity;
   a.cursor_out = cursor_out;
   a.host_err = v.host_err;
+  a.wide = (reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(request_of) | reinterpret_cast<uintptr_t>(slots)) % 16 == 0;
   rc = index_bytes == 4 ? launch_slots<int32_t>(s, v, a) : launch_slots<int64_t>(s, v, a);
   return rc ? rc : sorter_finish(s, v, 1, sync);
 }

@@ -79,6 +79,11 @@ class GpuSampler:
 
     def _vec(self, t, name: str, n: int, dtype):
         """Device address of a contiguous tensor of n elements of dtype."""
+        try:  # the checks below in their cheapest form
+            if t.dtype is dtype and t.numel() == n and t.is_contiguous() and t.get_device() == self.device:
+                return t.data_ptr()
+        except AttributeError:
+            pass
         if not isinstance(t, self._torch.Tensor):
             raise TypeError(f"{name} must be a tensor")
         if t.dtype is not dtype:
@@ -104,11 +109,9 @@ class GpuSampler:
         if t is None:
             t = self._torch.empty(shape, dtype=dtype, device=self._dev)
             return t, t.data_ptr()
-        if tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        n = 1
-        for d in shape:
-            n *= d
+        if t.shape != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+        n = shape[0] if len(shape) == 1 else shape[0] * shape[1]
         return t, self._vec(t, name, n, dtype)
 
     def _rows(self, x):
@@ -123,7 +126,7 @@ class GpuSampler:
         stride, step = x.stride()
         if step != 1 and cols > 1:
             raise ValueError(f"logits must have stride 1 along the vocabulary, got {step}")
-        if x.device != self._dev:
+        if x.get_device() != self.device:
             raise ValueError(f"logits is on {x.device}, the sampler on {self._dev}")
         return code, rows, cols, stride
 
@@ -198,7 +201,7 @@ class GpuSampler:
         tstride, tstep = block_table.stride()
         if tstep != 1 and width > 1:
             raise ValueError("block_table must have stride 1 along a row")
-        if block_table.device != self._dev:
+        if block_table.get_device() != self.device:
             raise ValueError(f"block_table is on {block_table.device}, the sampler on {self._dev}")
         nf = free_pages.numel() if isinstance(free_pages, t.Tensor) else 0
         f = self._vec(free_pages, "free_pages", nf, t.int32)

@@ -85,6 +85,10 @@ int fs_create(int device, void* stream, fs_sorter** out);
  *                              radix passes of the top two digits and then
  *                              sort each top-16-bit group by counting its
  *                              low 16 bits; 0: always the four passes
+ *   FORGESORT_ROW_FORM         fs_sample_rows and fs_top_logprobs: 1: always a
+ *                              cluster of CTAs per row, 2: always one CTA that
+ *                              streams the row (default: by the batch's size;
+ *                              the results are the same)
  * and once per process:
  *   FORGESORT_CHAIN_LAUNCH     0: launch a sort's kernels without programmatic
  *                              stream serialization (default: chained) */
@@ -307,7 +311,8 @@ int fs_top_logprobs(fs_sorter* s, int dtype, const void* logits, uint64_t rows,
  * entries of pages held are read, the new ones written, no other touched).
  * Writes:
  *   query_start  requests + 1 entries: where each request's tokens start
- *   seq_lens     context + new of each request (index_bytes each)
+ *   seq_lens     context + new of each request (index_bytes each; not the
+ *                memory of either)
  *   positions    of each token in its request (index_bytes each), 0 beyond
  *                the last token
  *   request_of   the token's request, -1 beyond the last token
