@@ -29,6 +29,7 @@ struct SlotArgs {
   const void* neu;
   uint32_t requests;
   uint32_t page;
+  uint64_t page_part;  // (2^64 - 1) / page
   int32_t* table;
   uint32_t width;
   int64_t table_stride;
@@ -50,39 +51,47 @@ template <typename I> __device__ __forceinline__ int64_t length_of(const void* p
   const int64_t v = static_cast<const I*>(p)[r];
   return v > 0 ? v : 0;
 }
-// A division of 64-bit numbers takes several times as long as one of 32.
-__device__ __forceinline__ int64_t div_page(int64_t tokens, uint32_t page) {
-  return (uint64_t)tokens >> 32 ? tokens / page : (int64_t)((uint32_t)tokens / page);
+// tokens / page and what is left, for 0 <= tokens < 2^63: the product with
+// the page's reciprocal, which is at most one too small.  (The code of a step
+// runs once, from cold: a 64-bit division is an order of magnitude longer.)
+__device__ __forceinline__ int64_t div_page(int64_t tokens, const SlotArgs& a, int64_t& left) {
+  int64_t n = (int64_t)__umul64hi((uint64_t)tokens, a.page_part);
+  left = tokens - n * a.page;
+  if (left >= a.page) ++n, left -= a.page;
+  return n;
 }
-__device__ __forceinline__ int64_t pages_of(int64_t tokens, uint32_t page, uint32_t width) {
-  const int64_t n = div_page(tokens, page), all = n + (n * page != tokens);
-  return all < width ? all : width;
+__device__ __forceinline__ int64_t pages_of(int64_t tokens, const SlotArgs& a) {
+  int64_t left;
+  const int64_t n = div_page(tokens, a, left);
+  return min(n + (left != 0), (int64_t)a.width);
 }
 
 constexpr int SLOT_THREADS = 512;
 constexpr int SLOT_CHUNK = 4 * SLOT_THREADS;  // requests scanned at a time
 constexpr int64_t MOST_TOKENS = 0x7fffffff;   // query_start is of 32 bits
 
+// Sums of two numbers over the lanes up to each.
+__device__ __forceinline__ void warp_scan(int64_t& x, int64_t& y, int lane) {
+#pragma unroll 1
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t ox = __shfl_up_sync(~0u, x, d), oy = __shfl_up_sync(~0u, y, d);
+    if (lane >= d) x += ox, y += oy;
+  }
+}
 // Exclusive sums of two numbers over the block.
 __device__ __forceinline__ void block_scan(int64_t& x, int64_t& y, int64_t (*warp)[2], int64_t& all_x, int64_t& all_y) {
   constexpr int WARPS = SLOT_THREADS / 32;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t x0 = x, y0 = y;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t ox = __shfl_up_sync(~0u, x, d), oy = __shfl_up_sync(~0u, y, d);
-    if (lane >= d) x += ox, y += oy;
-  }
+  warp_scan(x, y, lane);
   if (lane == 31) warp[wid][0] = x, warp[wid][1] = y;
   __syncthreads();
-  all_x = all_y = 0;
-  int64_t bx = 0, by = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w == wid) bx = all_x, by = all_y;
-    all_x += warp[w][0], all_y += warp[w][1];
-  }
-  x += bx - x0, y += by - y0;
+  int64_t wx = lane < WARPS ? warp[lane][0] : 0, wy = lane < WARPS ? warp[lane][1] : 0;
+  const int64_t ox = wx, oy = wy;
+  warp_scan(wx, wy, lane);
+  all_x = __shfl_sync(~0u, wx, 31), all_y = __shfl_sync(~0u, wy, 31);
+  x += __shfl_sync(~0u, wx - ox, wid) - x0;
+  y += __shfl_sync(~0u, wy - oy, wid) - y0;
 }
 
 // Every CTA takes both sums over all requests, SLOT_CHUNK of them at a time,
@@ -104,7 +113,7 @@ template <typename I, int TOK> __device__ __forceinline__ void put(I* to, const 
 template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k_plan_slots(const SlotArgs a) {
   __shared__ int64_t warp[SLOT_THREADS / 32][2];
   __shared__ int32_t start[SLOT_CHUNK + 1];  // of the chunk's requests
-  __shared__ int64_t took[SLOT_CHUNK];
+  __shared__ int32_t took[SLOT_CHUNK];       // pages of those before, at most 2^31 - 1: there are no more free ones
   const int tid = threadIdx.x;
   const int64_t cursor = a.cursor[0] > 0 ? a.cursor[0] : 0;
   int64_t tokens = 0, pages = 0;  // of the chunks before
@@ -120,7 +129,7 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
       if (l < n) {
         const int64_t ctx = length_of<I>(a.ctx, r0 + l);
         neu[k] = length_of<I>(a.neu, r0 + l);
-        more[k] = pages_of(ctx + neu[k], a.page, a.width) - pages_of(ctx, a.page, a.width);
+        more[k] = pages_of(ctx + neu[k], a) - pages_of(ctx, a);
         if (blockIdx.x == 0) static_cast<I*>(a.seq_lens)[r0 + l] = (I)(ctx + neu[k]);
       }
       t += neu[k], p += more[k];
@@ -133,25 +142,28 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
       const int l = tid * PER + k;
       if (l < n) {
         start[l] = (int32_t)min(t, MOST_TOKENS);
-        took[l] = p;
+        took[l] = (int32_t)min(p, MOST_TOKENS);
         if (blockIdx.x == 0) a.query_start[r0 + l] = start[l];
       }
       t += neu[k], p += more[k];
     }
-    const int64_t from = min(tokens, MOST_TOKENS), to = min(tokens + all_t, MOST_TOKENS);
+    const uint32_t from = (uint32_t)min(tokens, MOST_TOKENS), to = (uint32_t)min(tokens + all_t, MOST_TOKENS);
     tokens += all_t, pages += all_p;
     __syncthreads();
     // the first of this CTA's tiles that reaches into [from, to)
     constexpr int TILE = SLOT_THREADS * TOK;
-    int64_t tile = from / TILE;
-    tile += ((int64_t)blockIdx.x - tile % gridDim.x + gridDim.x) % gridDim.x;
-    for (int64_t i0 = tile * TILE + tid * TOK; i0 - tid * TOK < to; i0 += (int64_t)gridDim.x * TILE) {
-      const int64_t i1 = max(i0, from), i2 = min(i0 + TOK, to);
+    uint32_t tile = from / TILE;
+    const uint32_t at = tile % gridDim.x;
+    tile += blockIdx.x >= at ? blockIdx.x - at : gridDim.x - at + blockIdx.x;
+#pragma unroll 1
+    for (uint32_t i0 = tile * TILE + tid * TOK; i0 - tid * TOK < to; i0 += gridDim.x * TILE) {
+      const uint32_t i1 = max(i0, from), i2 = min(i0 + TOK, to);
       if (i1 >= i2) continue;
       int lo = 0, hi = n;  // the chunk's last request that starts at or before i1
+#pragma unroll 1
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (start[mid] <= i1)
+        if ((uint32_t)start[mid] <= i1)
           lo = mid;
         else
           hi = mid;
@@ -165,15 +177,16 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
       bool look = true;  // the request is a new one
 #pragma unroll
       for (int k = 0; k < TOK; ++k) {
-        const int64_t i = i0 + k;
+        const uint32_t i = i0 + k;
         if (i < i1 || i >= i2) continue;
-        while (lo + 1 < n && start[lo + 1] <= i) ++lo, look = true;
+#pragma unroll 1
+        while (lo + 1 < n && (uint32_t)start[lo + 1] <= i) ++lo, look = true;
         bool turn = look;  // the page is another one
         if (look) {
           const int64_t ctx = length_of<I>(a.ctx, r0 + lo);
           pos = ctx + i - start[lo];
-          nth = div_page(pos, a.page), off = pos - nth * a.page;
-          have = pages_of(ctx, a.page, a.width);
+          nth = div_page(pos, a, off);
+          have = pages_of(ctx, a);
           row = a.table + (int64_t)(r0 + lo) * a.table_stride;
           look = false;
         } else {
@@ -190,20 +203,20 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
             if (off == 0) row[nth] = id;
           }
         }
-        missed |= id < 0 || i >= (int64_t)a.capacity;
+        missed |= id < 0 || i >= a.capacity;
         request[k] = (int32_t)(r0 + lo);
         position[k] = (I)pos;
         slot[k] = id < 0 ? -1 : (int64_t)id * a.page + off;
       }
-      if (TOK > 1 && a.wide && i2 - i1 == TOK && i2 <= (int64_t)a.capacity) {
+      if (TOK > 1 && a.wide && i2 - i1 == TOK && i2 <= a.capacity) {
         put(a.request_of + i0, request);
         put(static_cast<I*>(a.positions) + i0, position);
         put(a.slots + i0, slot);
       } else {
 #pragma unroll
         for (int k = 0; k < TOK; ++k) {
-          const int64_t i = i0 + k;
-          if (i < i1 || i >= i2 || i >= (int64_t)a.capacity) continue;
+          const uint32_t i = i0 + k;
+          if (i < i1 || i >= i2 || i >= a.capacity) continue;
           a.request_of[i] = request[k];
           static_cast<I*>(a.positions)[i] = position[k];
           a.slots[i] = slot[k];
@@ -229,7 +242,7 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
 
 template <typename I, int TOK> int launch_tokens(fs_sorter* s, const SorterView& v, const SlotArgs& a) {
   constexpr uint64_t TILE = SLOT_THREADS * TOK;
-  const uint64_t tiles = (a.capacity + TILE - 1) / TILE, cap = (uint64_t)v.sm_count * 4;
+  const uint64_t tiles = (a.capacity + TILE - 1) / TILE, cap = (uint64_t)v.sm_count * 2;  // as many as run at a time
   k_plan_slots<I, TOK><<<(unsigned)(tiles < 1 ? 1 : tiles < cap ? tiles : cap), SLOT_THREADS, 0, v.stream>>>(a);
   FS_SLOTS_CUDA(s, cudaGetLastError());
   return FS_OK;
@@ -282,6 +295,7 @@ extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_
   a.neu = new_lens;
   a.requests = (uint32_t)requests;
   a.page = page_size;
+  a.page_part = ~0ull / page_size;
   a.table = block_table;
   a.width = (uint32_t)table_width;
   a.table_stride = table_stride;

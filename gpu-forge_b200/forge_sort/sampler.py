@@ -49,6 +49,8 @@ class GpuSampler:
         self._last = self._fixed
         self._logits = {torch.float32: _lib.LOGITS_F32, torch.float16: _lib.LOGITS_F16,
                         torch.bfloat16: _lib.LOGITS_BF16}
+        # torch.cuda.current_stream() makes an object; this gives its handle alone
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._index = {torch.int32: 4, torch.int64: 8}
 
     @classmethod
@@ -74,7 +76,9 @@ class GpuSampler:
     # -- plumbing -----------------------------------------------------------------
     def _stream(self):
         if self._fixed is None:
-            self._last = self._torch.cuda.current_stream(self._dev).cuda_stream or 1  # 1: cudaStreamLegacy
+            raw = self._raw_stream
+            h = raw(self.device) if raw else self._torch.cuda.current_stream(self._dev).cuda_stream
+            self._last = h or 1  # 1: cudaStreamLegacy
         return self._last
 
     def _vec(self, t, name: str, n: int, dtype):
@@ -109,6 +113,11 @@ class GpuSampler:
         if t is None:
             t = self._torch.empty(shape, dtype=dtype, device=self._dev)
             return t, t.data_ptr()
+        try:
+            if t.shape == shape and t.dtype is dtype and t.is_contiguous() and t.get_device() == self.device:
+                return t, t.data_ptr()
+        except AttributeError:
+            raise TypeError(f"{name} must be a tensor") from None
         if t.shape != shape:
             raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
         n = shape[0] if len(shape) == 1 else shape[0] * shape[1]
