@@ -272,6 +272,46 @@ class GpuSorter {
     detail::check(fs_gather(h_, (int)sizeof(T), src, src_n, idx, dst, n, 1), h_);
   }
 
+  // -- serving: a decode step's calls on device memory (no reference counterpart;
+  // arguments as in forgesort.h).  They enqueue on `stream` (this sorter's where
+  // null) and do not wait unless sync --
+  struct Sampling {  // one value a row each; null: off
+    const float* temperature = nullptr;
+    const int32_t* top_k = nullptr;
+    const float* top_p = nullptr;
+    const float* min_p = nullptr;
+  };
+  void sample_rows(fs_logits_dtype dtype, const void* logits, uint64_t rows, uint64_t cols, int64_t row_stride,
+                   const Sampling& by, const float* uniform, int32_t* tokens, float* logprobs = nullptr,
+                   void* stream = nullptr, bool sync = false) {
+    detail::check(fs_sample_rows(h_, dtype, logits, rows, cols, row_stride, by.temperature, by.top_k, by.top_p, by.min_p,
+                                 uniform, tokens, logprobs, sync, stream),
+                  h_);
+  }
+  void top_logprobs(fs_logits_dtype dtype, const void* logits, uint64_t rows, uint64_t cols, int64_t row_stride, int n,
+                    int32_t* indices, float* logprobs, float* lse = nullptr, void* stream = nullptr, bool sync = false) {
+    detail::check(fs_top_logprobs(h_, dtype, logits, rows, cols, row_stride, n, indices, logprobs, lse, sync, stream), h_);
+  }
+  template <typename I> struct SlotPlan {  // what plan_slots writes
+    int32_t* query_start;
+    I* seq_lens;
+    I* positions;
+    int32_t* request_of;
+    int64_t* slots;
+    uint64_t capacity;  // of the last three
+    int32_t* cursor_out;
+  };
+  template <typename I>
+  void plan_slots(const I* context_lens, const I* new_lens, uint64_t requests, uint32_t page_size, int32_t* block_table,
+                  uint64_t table_width, int64_t table_stride, const int32_t* free_pages, uint64_t n_free,
+                  const int32_t* cursor, const SlotPlan<I>& to, void* stream = nullptr, bool sync = false) {
+    static_assert(sizeof(I) == 4 || sizeof(I) == 8, "lengths of 4 or 8 bytes");
+    detail::check(fs_plan_slots(h_, (int)sizeof(I), context_lens, new_lens, requests, page_size, block_table, table_width,
+                                table_stride, free_pages, n_free, cursor, to.query_start, to.seq_lens, to.positions,
+                                to.request_of, to.slots, to.capacity, to.cursor_out, sync, stream),
+                  h_);
+  }
+
   // -- stable key/value sort, u32 values (lib.rs:1923-2236, 2826-3015) --------
   void sort_pairs_u32(std::span<uint32_t> k, std::span<uint32_t> v) { pairs_host(k, v); }
   void sort_pairs_i32(std::span<int32_t> k, std::span<uint32_t> v) { pairs_host(k, v); }

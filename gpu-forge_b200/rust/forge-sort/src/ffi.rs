@@ -92,6 +92,21 @@ extern "C" {
     pub fn fs_stream_synchronize(stream: *mut c_void) -> c_int;
     pub fn fs_stream_destroy(stream: *mut c_void) -> c_int;
 
+    // serving: token sampling, best log-probabilities, slots of a paged cache
+    // (no reference counterpart)
+    pub fn fs_sample_rows(s: *mut FsSorter, dtype: c_int, logits: *const c_void, rows: u64, cols: u64, row_stride: i64,
+                          temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32,
+                          uniform: *const f32, tokens: *mut i32, logprobs: *mut f32, sync: c_int,
+                          stream: *mut c_void) -> c_int;
+    pub fn fs_top_logprobs(s: *mut FsSorter, dtype: c_int, logits: *const c_void, rows: u64, cols: u64,
+                           row_stride: i64, n: c_int, indices: *mut i32, logprobs: *mut f32, lse: *mut f32,
+                           sync: c_int, stream: *mut c_void) -> c_int;
+    pub fn fs_plan_slots(s: *mut FsSorter, index_bytes: c_int, context_lens: *const c_void, new_lens: *const c_void,
+                         requests: u64, page_size: u32, block_table: *mut i32, table_width: u64, table_stride: i64,
+                         free_pages: *const i32, n_free: u64, cursor: *const i32, query_start: *mut i32,
+                         seq_lens: *mut c_void, positions: *mut c_void, request_of: *mut i32, slots: *mut i64,
+                         capacity: u64, cursor_out: *mut i32, sync: c_int, stream: *mut c_void) -> c_int;
+
     // several GPUs of one process (no reference counterpart)
     pub fn fs_mg_create(devices: *const c_int, g: c_int, out: *mut *mut FsMg) -> c_int;
     pub fn fs_mg_destroy(mg: *mut FsMg) -> c_int;
