@@ -702,34 +702,53 @@ template <typename T, int NT, bool MEM> struct Row {
     }
     return sum.mass();
   }
-  __device__ __forceinline__ uint64_t weigh() const {
-    return weigh<ALL>(0.0f, 0.0f, 0.0f, [](float, int) {});
-  }
   __device__ __forceinline__ uint64_t heavy(float over, float least_w) const {
     return weigh<HEAVY>(over, 0.0f, least_w, [](float, int) {});
   }
 
-  // The same pass (from memory) also lists the entries of at least `edge`, or
-  // only finds the first of them.
+  // The same pass also lists the entries of at least `edge` in this CTA's share
+  // of the first CTA's list (sh.count = 0 before), or only finds the first of
+  // them.  Infinity: none.
+  __device__ __forceinline__ void list_entry(float z, int j, bool only_first) const {
+    if (only_first) {
+      atomicMin(cluster.map_shared_rank(&sh.first, 0), (uint32_t)j);
+    } else {
+      const uint32_t at = atomicAdd(&sh.count, 1u);
+      if (at < room) sh.list[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
+    }
+  }
   template <bool CLEAN> __device__ __forceinline__ uint64_t weigh_and_list_of(float edge, bool only_first) {
     Sum sum(m, c);
     const bool lists_any = edge < INFINITY;
     stream<CLEAN, true, !CLEAN>([&](const uint4& v, uint32_t i) {
       sum.template add<ALL>(v, 0.0f, 0.0f);
       if (lists_any && E::value(E::top(E::top0(), v)) >= edge)
-        each_of(hits(v, edge, INFINITY), v, i, [&](float z, int j) {
-          if (only_first) {
-            atomicMin(&sh.first, (uint32_t)j);
-          } else {
-            const uint32_t at = atomicAdd(&sh.count, 1u);
-            if (at < ROW_LIST) sh.list[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
-          }
-        });
+        each_of(hits(v, edge, INFINITY), v, i, [&](float z, int j) { list_entry(z, j, only_first); });
     }, [&] { sum.fold(); });
     return sum.mass();
   }
   __device__ __forceinline__ uint64_t weigh_and_list(float edge, bool only_first) {
-    return dirty ? weigh_and_list_of<true>(edge, only_first) : weigh_and_list_of<false>(edge, only_first);
+    if constexpr (MEM) {
+      return dirty ? weigh_and_list_of<true>(edge, only_first) : weigh_and_list_of<false>(edge, only_first);
+    } else {
+      Sum sum(m, c);
+      const bool lists_any = mine >= edge;
+      uint64_t has = 0;  // which of the thread's vectors have any: they are looked at again afterwards
+#pragma unroll 2
+      for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
+        const uint4 v = data[i];
+        sum.template add<ALL>(v, 0.0f, 0.0f);
+        if (lists_any) has |= (uint64_t)(E::value(E::top(E::top0(), v)) >= edge) << ((i - seg0) / 32);
+      }
+#pragma unroll 1
+      while (has) {
+        const uint32_t i = seg0 + lane + 32 * (__ffsll((long long)has) - 1);
+        has &= has - 1;
+        const uint4 v = data[i];
+        each_of(hits(v, edge, INFINITY), v, i, [&](float z, int j) { list_entry(z, j, only_first); });
+      }
+      return sum.mass();
+    }
   }
 
   // Bits of the entries of a vector in [low, high].
@@ -762,22 +781,6 @@ template <typename T, int NT, bool MEM> struct Row {
   template <typename F> __device__ __forceinline__ void between(float low, float high, F f) const {
     vectors<false>([&](const uint4& v, uint32_t i) { each_of(hits(v, low, high), v, i, f); }, [] {});
   }
-  // The same, where few of the warp's threads have any above low: the warp
-  // looks through the vectors of one such thread at a time.
-  template <typename F> __device__ __forceinline__ void above(float low, F f) const {
-    uint32_t threads = __ballot_sync(~0u, mine >= low);
-#pragma unroll 1
-    while (threads) {
-      const uint32_t owner = __ffs((int)threads) - 1;
-      threads &= threads - 1;
-#pragma unroll 1
-      for (uint32_t i = seg0 + owner + 32 * lane; i < seg1; i += 32 * 32) {
-        const uint4 v = data[i];
-        each_of(hits(v, low, INFINITY), v, i, f);
-      }
-    }
-  }
-
   // A value with at least `k` of the row's entries at or above it: the k-th
   // largest of the published thread maxima, rounded down to the bound of a bin
   // of 1 / scale and by more than the bound's rounding.  Where fewer are within
@@ -846,18 +849,6 @@ template <typename T, int NT, bool MEM> struct Row {
 #pragma unroll 1
     for (uint32_t i = lane; i < ctas * WARPS; i += 32) t += (&of[0][0])[i];
     return warp_sum_u64(t);
-  }
-  // Collects this CTA's entries of at least `edge` in its share of the first
-  // CTA's list (sh.count = 0 before), or only finds the first of them.
-  __device__ __forceinline__ void collect_above(float edge, bool only_first) {
-    above(edge, [&](float z, int j) {
-      if (only_first) {
-        atomicMin(cluster.map_shared_rank(&sh.first, 0), (uint32_t)j);
-        return;
-      }
-      const uint32_t at = atomicAdd(&sh.count, 1u);
-      if (at < room) sh.list[at] = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
-    });
   }
   // Hands them to the first CTA and tells every CTA their number.
   __device__ __forceinline__ void tell_list() {
@@ -1614,13 +1605,7 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
     if (a.logprobs) a.logprobs[row] = row_neg_y(z, r.m, r.c) * ROW_LN2 - logf((float)total * 0x1p-40f);
   };
   const float edge = q.cuts() ? r.edge_for(q) : q.greedy ? r.m : INFINITY;
-  uint64_t own;
-  if constexpr (MEM) {
-    own = r.weigh_and_list(edge, q.greedy);
-  } else {
-    if (edge < INFINITY) r.collect_above(edge, q.greedy);
-    own = r.weigh();
-  }
+  const uint64_t own = r.weigh_and_list(edge, q.greedy);
   uint64_t last = ~0ull;  // the last entry of the cut
   if (!q.cuts()) {
     r.template hand<false>(sh.part, own);
@@ -1712,12 +1697,7 @@ __device__ __forceinline__ void row_best(const RowArgs& a, uint32_t row, typenam
   r.c = ROW_LOG2E;
   const uint32_t k = (uint32_t)a.n;
   float edge = r.edge_for_best(k);
-  if constexpr (MEM) {
-    r.template hand<true>(sh.mass, r.weigh_and_list(edge, false));
-  } else {
-    r.template hand<true>(sh.mass, r.weigh());
-    if (edge < INFINITY) r.collect_above(edge, false);
-  }
+  r.template hand<true>(sh.mass, r.weigh_and_list(edge, false));
   r.tell_list();
   r.cluster.sync();
   uint32_t n = 0;
