@@ -668,7 +668,7 @@ template <typename T, int NT, bool MEM> struct Row {
     uint64_t folded = 0;
     uint32_t hi = 0, lo = 0, n = 0;
     __device__ __forceinline__ Sum(float m, float c) : m2(f2_pack(-m, -m)), c2(f2_pack(c, c)) {}
-    template <int KIND> __device__ __forceinline__ void add(const uint4& v, float over, float least_w) {
+    template <int KIND> __device__ __forceinline__ void add(const uint4& v, float over, float least_w, float* below = nullptr) {
       const uint64_t one = f2_pack(1.0f, 1.0f), none = f2_pack(-1.0f, -1.0f), both = f2_pack(1.0f + ROW_MAGIC, 1.0f + ROW_MAGIC);
       float z[N];
       E::get(v, z);
@@ -678,7 +678,11 @@ template <typename T, int NT, bool MEM> struct Row {
         f2_unpack(f2_mul(f2_add(f2_pack(z[e], z[e + 1]), m2), c2), w0, w1);
         w0 = row_exp2(w0), w1 = row_exp2(w1);
         if (KIND == HEAVY) w0 = w0 >= least_w ? w0 : 0.0f, w1 = w1 >= least_w ? w1 : 0.0f;
-        if (KIND != ALL) w0 = z[e] > over ? w0 : 0.0f, w1 = z[e + 1] > over ? w1 : 0.0f;
+        if (KIND != ALL) {
+          const bool in0 = z[e] > over, in1 = z[e + 1] > over;
+          w0 = in0 ? w0 : 0.0f, w1 = in1 ? w1 : 0.0f;
+          if (KIND == ABOVE) *below = fmaxf(fmaxf(*below, in0 ? -INFINITY : z[e]), in1 ? -INFINITY : z[e + 1]);
+        }
         const uint64_t w = f2_pack(w0, w1);
         const uint64_t a = f2_add(w, one);
         const uint64_t b = f2_add(w, f2_fma(a, none, both));  // 1 + MAGIC - a is exact
@@ -701,9 +705,10 @@ template <typename T, int NT, bool MEM> struct Row {
     Sum sum(m, c);
     uint64_t has = 0;  // which of the thread's vectors f wants: they are looked at again afterwards, few and together
     vectors<KIND == ALL>([&](const uint4& v, uint32_t i) {
-      sum.template add<KIND>(v, over, least_w);
-      if (KIND == ABOVE && MEM) each_of(hits(v, low, over), v, i, f);
-      if (KIND == ABOVE && !MEM) has |= (uint64_t)any_hit(v, low, over) << ((i - seg0) / 32);
+      float below = -INFINITY;  // the largest that is not above
+      sum.template add<KIND>(v, over, least_w, &below);
+      if (KIND == ABOVE && MEM && below >= low) each_of(hits(v, low, over), v, i, f);
+      if (KIND == ABOVE && !MEM) has |= (uint64_t)(below >= low) << ((i - seg0) / 32);
     }, [&] { sum.fold(); });
 #pragma unroll 1
     while (KIND == ABOVE && !MEM && has) {
@@ -771,14 +776,6 @@ template <typename T, int NT, bool MEM> struct Row {
 #pragma unroll
     for (int e = 0; e < N; ++e) mask |= (uint32_t)(z[e] >= low && z[e] <= high) << e;
     return mask;
-  }
-  static __device__ __forceinline__ bool any_hit(const uint4& v, float low, float high) {
-    float z[N];
-    E::get(v, z);
-    bool any = false;
-#pragma unroll
-    for (int e = 0; e < N; ++e) any |= z[e] >= low && z[e] <= high;
-    return any;
   }
   // f(x, index) for the entries of vector i of this CTA's part that mask names
   template <typename F> __device__ __forceinline__ void each_of(uint32_t mask, const uint4& v, uint32_t i, F f) const {
@@ -990,32 +987,29 @@ template <typename T, int NT, bool MEM> struct Row {
   // from the second round on estimates follow q.  Counts are exact.)
   // Else it ends in the last bin with anything; a count that is not reached,
   // beyond all of them.
-  __device__ __forceinline__ void end_bins(bool by_mass, bool by_weight, bool first_round, float goal, uint32_t above_n, float top_w,
-                                           float octaves) {
+  __device__ __forceinline__ void end_bins(bool by_mass, bool first_round, float goal, uint32_t above_n, float octaves) {
     constexpr int PER = (ROW_BINS + NT - 1) / NT;
-    const int at = tid * PER, end = min(at + PER, ROW_BINS);
-    auto sum_of = [&](int b) {
-      const float v = __uint_as_float(sh.bins[b]);
-      return by_mass ? v * (by_weight ? row_exp2((float)b * -octaves) : top_w) : v;
-    };
-    float own = 0, all;
+    const int at = tid * PER;
+    float v[PER], own = 0, all;
     uint32_t filled = 0;
-#pragma unroll 1
-    for (int b = at; b < end; ++b) {
-      const float v = sum_of(b);
-      if (v > 0.0f) filled = b;
-      own += v;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = at + i < ROW_BINS ? __uint_as_float(sh.bins[at + i]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (v[i] > 0.0f) filled = at + i;
+      own += v[i];
     }
     filled = __reduce_max_sync(~0u, filled);
     if (lane == 0) atomicMax(&sh.last, filled);
     float run = block_scan(own, reinterpret_cast<float*>(sh.scan_n), all);
     const float slack = by_mass ? 1.25f / UNIT + 0.0625f * octaves * octaves : 0.0f, more = by_mass && first_round ? UNIT * 0x1p-20f : 0.0f;
     uint32_t b1 = ~0u, b2 = ~0u;
-#pragma unroll 1
-    for (int b = at; b < end; ++b) {
-      const float v = sum_of(b);
-      if (run < goal && (run + v >= goal || b == ROW_BINS - 1)) sh.above = above_n + (uint32_t)run;  // read for counts alone
-      run += v;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int b = at + i;
+      if (b >= ROW_BINS) break;
+      if (run < goal && (run + v[i] >= goal || b == ROW_BINS - 1)) sh.above = above_n + (uint32_t)run;  // read for counts alone
+      run += v[i];
       if (run * (1.0f + slack) + more >= goal) b1 = min(b1, (uint32_t)b);
       if (run * (1.0f - slack) - more >= goal) b2 = min(b2, (uint32_t)b);
     }
@@ -1098,7 +1092,11 @@ template <typename T, int NT, bool MEM> struct Row {
     constexpr int ROUNDS = 16;
 #pragma unroll 1
     for (int round = 0; round < ROUNDS; ++round) {
-      cluster.sync();  // what was there has been read
+      // what was there has been read (before the first round: by this CTA alone, since the last barrier)
+      if (round)
+        cluster.sync();
+      else
+        __syncthreads();
 #pragma unroll 1
       for (int b = tid; b < ROW_BINS; b += NT) sh.bins[b] = 0;
       if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ~0u, sh.last = 0;
@@ -1138,13 +1136,14 @@ template <typename T, int NT, bool MEM> struct Row {
           float v = 0;
 #pragma unroll 8
           for (uint32_t k = 0; k < ctas; ++k) v += (float)cluster.map_shared_rank(sh.bins, k)[b];
+          if (by_mass) v *= by_weight ? row_exp2((float)b * -octaves) : top_w;
           cluster.map_shared_rank(sh.bins, 0)[b] = __float_as_uint(v);
         }
       }
       cluster.sync();
       if (rank == 0) {
         const float goal = by_mass ? (float)(target - above_q) * (UNIT * 0x1p-40f) : (float)(target - above_n);
-        end_bins(by_mass, by_weight, round == 0, goal, above_n, top_w, octaves);
+        end_bins(by_mass, round == 0, goal, above_n, octaves);
         const uint64_t at = end_of(by_mass, by_weight, round == 0, cs, shift, lo, hi);
         if (wid < 2) {
           if (lane < (int)ctas) {
