@@ -122,6 +122,7 @@ template <typename T> struct RowElem;
 template <> struct RowElem<float> {
   static constexpr int N = 4;
   static constexpr uint32_t NEG_INF = 0xff800000u;  // fills a 32-bit word
+  static constexpr int ZEROS = 0;                   // low bits of its 32-bit form that are always 0
   using Top = float;                                // running maximum
   static __device__ __forceinline__ Top top0() { return -INFINITY; }
   static __device__ __forceinline__ Top top(Top t, const uint4& v) {
@@ -141,6 +142,7 @@ template <> struct RowElem<float> {
 template <> struct RowElem<__nv_bfloat16> {
   static constexpr int N = 8;
   static constexpr uint32_t NEG_INF = 0xff80ff80u;
+  static constexpr int ZEROS = 16;
   using Top = uint32_t;
   static __device__ __forceinline__ Top top0() { return NEG_INF; }
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
@@ -175,6 +177,7 @@ template <> struct RowElem<__nv_bfloat16> {
 template <> struct RowElem<__half> {
   static constexpr int N = 8;
   static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+  static constexpr int ZEROS = 13;
   using Top = uint32_t;
   static __device__ __forceinline__ Top top0() { return NEG_INF; }
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
@@ -1454,6 +1457,16 @@ template <typename T, int NT, bool MEM> struct Row {
     }
   }
 
+  // (key, index) without the bits that no key of 16-bit logits has: neighbouring
+  // values are then as near as their entries are, and one round of bins parts
+  // both.  A key's low bits are all 1 or, below 0, all 0.
+  static __device__ __forceinline__ uint64_t squeezed(uint64_t e) {
+    return e >> (ROW_IDX_BITS + E::ZEROS) << ROW_IDX_BITS | (e & (ROW_MAX_COLS - 1));
+  }
+  static __device__ __forceinline__ uint64_t unsqueezed(uint64_t s) {
+    const uint32_t key = (uint32_t)(s >> ROW_IDX_BITS) << E::ZEROS;
+    return (uint64_t)(key >> 31 ? key : key | ((1u << E::ZEROS) - 1)) << ROW_IDX_BITS | (s & (ROW_MAX_COLS - 1));
+  }
   // Cuts the n entries in sh.pool, those of [sh.lo, sh.hi], where the prefix of
   // `target` of them (by_mass: of mass `target` with what sh.mass holds) ends, and
   // adds the kept ones' masses to their stretches' in sh.part.  Returns the
@@ -1461,17 +1474,20 @@ template <typename T, int NT, bool MEM> struct Row {
   __device__ __forceinline__ uint64_t finish_pool(RowFinish& f, uint32_t n, bool by_mass, float least_w, uint64_t target) {
 #pragma unroll 1
     for (uint32_t i = tid; i < n; i += NT) {
-      f.sorted[i] = sh.pool[i];
+      f.sorted[i] = squeezed(sh.pool[i]);
       f.input[i] = by_mass ? mass(value_of(sh.pool[i])) : 1;
     }
     const uint64_t end = sh.hi, left = by_mass ? target - handed(sh.mass) : target;
-    const uint64_t last = min(end, reach(f, sh, n, left, sh.lo, end, m, -1.0f).at);
+    // the interval's ends lie between values, too: of their own index only 32-bit logits can make use
+    const uint64_t any = E::ZEROS ? ROW_MAX_COLS - 1 : 0;
+    const uint64_t at = reach(f, sh, n, left, squeezed(sh.lo) & ~any, squeezed(end) | any, m, -1.0f).at;
+    const uint64_t last = at == ~0ull ? end : unsqueezed(at);
     // the warps' kept masses: before the interval, and those of its entries
     if (tid < ROW_SUMS) f.part[tid][0] = f.part[tid][1] = 0;
     __syncthreads();
 #pragma unroll 1
     for (uint32_t i = tid; i < n; i += NT) {
-      const uint64_t e = f.sorted[i];
+      const uint64_t e = sh.pool[i];
       const float w = weight(value_of(e));
       if (e > last || w < least_w) continue;
       const uint32_t v = (((uint32_t)e & (ROW_MAX_COLS - 1)) + lead) / N;
@@ -1537,14 +1553,15 @@ template <typename T, int NT, bool MEM> struct Row {
       }
       uint64_t run = block_scan(own, sh.scan_q, all);
       if (t < all) {
-        if (t >= run && t < run + own) {
-#pragma unroll 4
-          for (int e = 0; e < PER * N; ++e) {
-            const float z = E::at(e < N ? v[0] : v[1], e % N);
-            const uint64_t q = value(z, j0 + e);
-            if (t >= run && t < run + q) hit(z, j0 + e);
-            run += q;
-          }
+        // the thread whose vectors hold the draw: its warp takes an entry a lane
+        const uint32_t has = __ballot_sync(~0u, t >= run && t < run + own);
+        if (has) {
+          const int owner = __ffs((int)has) - 1;
+          const uint32_t at = __shfl_sync(~0u, i, owner) + lane / N;
+          const float z = E::at(lane < PER * N && at < v1 ? from_memory(at) : nothing(), lane % N);
+          const int j = (int)(at * N) - lead + lane % N;
+          const uint64_t q = lane < PER * N ? value(z, j) : 0, upto = __shfl_sync(~0u, run, owner) + warp_scan(q, lane);
+          if (t < upto && t >= upto - q) hit(z, j);
         }
         return;
       }
