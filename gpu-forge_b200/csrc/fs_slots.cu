@@ -99,8 +99,9 @@ __device__ __forceinline__ void block_scan(int64_t& x, int64_t& y, int64_t (*war
 // the chunk; the first CTA writes what is one per request.  The sums are taken
 // again by each CTA (two numbers per request from L2) instead of handed on:
 // one launch, no scratch, nobody waits.  A thread plans TOK neighbouring
-// tokens: it looks its request up once and writes 16 bytes at a time (TOK = 4
-// where that still gives every SM a CTA; else 1).
+// tokens: it looks its request up once and writes 16 bytes at a time.  TOK is 4
+// in steps of more tokens than an SM has threads for (2^20 tokens: 14.7 us, one
+// token a thread 18.5), else 1 (4096 tokens: 10.3 us, four 12.4).
 //
 // Bound: the writes of a large step (21 MB for 2^20 prompt tokens with 64-bit
 // positions, 3.2 us), else the chain load - scan - search - page - store of one CTA.

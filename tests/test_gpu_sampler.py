@@ -153,6 +153,23 @@ def test_masks_and_ties(gs, dtype, params):
     _check(gs, x, _uniform(len(rows), 3), top_k=2500, top_p=0.5)
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("step", [0.25, 0.0625, 3.0])
+@pytest.mark.parametrize("params", [dict(top_p=0.5), dict(top_p=0.97, min_p=0.01), dict(top_k=9000), dict(top_k=30000, top_p=0.8)],
+                         ids=["top_p", "top_p min_p", "top_k", "top_k top_p"])
+def test_wide_cuts_end_among_equal_values(gs, dtype, step, params):
+    """Logits of few values: a cut that lies far down ends inside hundreds to
+    thousands of equal ones, of either sign, and is told by the index alone."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.round(torch.randn(3, 70001, generator=g, device="cuda") * 1.5 / step) * step
+    x[1] -= 7.0
+    x[2] += 7.0
+    x = x.to(getattr(torch, {"f32": "float32", "f16": "float16", "bf16": "bfloat16"}[dtype]) if isinstance(dtype, str) else dtype)
+    for seed in (1, 2):
+        _check(gs, x, _uniform(3, seed), temperature=1.3, **params)
+
+
 def test_draw_ends(gs):
     """u at 0, just below 1, and outside [0, 1)."""
     import torch

@@ -174,6 +174,36 @@ def test_a_million_tokens(gs):
     assert torch.equal(p.slots, t[r, pos // page].long() * page + pos % page)
 
 
+@pytest.mark.parametrize("page", [1, 3, 100, 65536])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+@pytest.mark.parametrize("ints", ["int32", "int64"])
+def test_many_tokens_into_given_memory(gs, page, offset, ints):
+    """Enough tokens for the wide stores, into tensors that begin at 16-byte
+    boundaries and between them, with places behind the last token."""
+    import torch
+    I = getattr(torch, ints)
+    g = torch.Generator(device="cuda").manual_seed(page + offset)
+    R, T = 997, 90000
+    new = torch.randint(0, 181, (R,), generator=g, device="cuda")
+    new = (new * T // int(new.sum())).to(I)
+    ctx = torch.randint(0, 300, (R,), generator=g, device="cuda").to(I)
+    have, need = (ctx + page - 1) // page, (ctx + new + page - 1) // page
+    t = torch.full((R, int(need.max())), -1, dtype=torch.int32, device="cuda")
+    col = torch.arange(t.shape[1], device="cuda")[None]
+    t[col < have[:, None]] = torch.arange(int(have.sum()), dtype=torch.int32, device="cuda")
+    free = torch.arange(int(have.sum()), int(need.sum()), dtype=torch.int32, device="cuda")
+    out = lambda dt: torch.full((T + 8,), -5, dtype=dt, device="cuda")[offset:offset + T]  # noqa: E731
+    p = gs.plan_slots(ctx, new, t, free, torch.zeros(1, dtype=torch.int32, device="cuda"), page_size=page,
+                      positions=out(I), requests=out(torch.int32), slots=out(torch.int64), sync=True)
+    n = int(new.sum())
+    r = torch.repeat_interleave(torch.arange(R, device="cuda"), new.long())
+    pos = ctx.long()[r] + torch.arange(n, device="cuda") - (torch.cumsum(new.long(), 0) - new.long())[r]
+    assert torch.equal(p.requests[:n].long(), r) and torch.equal(p.positions[:n].long(), pos)
+    assert torch.equal(p.slots[:n], t[r, pos // page].long() * page + pos % page)
+    assert n < T and (p.requests[n:] == -1).all() and (p.positions[n:] == 0).all() and (p.slots[n:] == -1).all()
+    assert torch.equal(t[(col >= have[:, None]) & (col < need[:, None])], free)
+
+
 def test_refusals(gs):
     import torch
     i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
@@ -204,3 +234,7 @@ def test_refusals(gs):
     with pytest.raises(ValueError):
         gs.plan_slots(i(1, 2), i(1, 1), t, i(5), i(0), slots=torch.zeros(3, dtype=torch.int64, device="cuda"),
                       positions=i(0), page_size=16)
+    c, n = i(1, 2), i(1, 1)
+    for same in (c, n):  # lengths that would change while they are read
+        with pytest.raises(ValueError):
+            gs.plan_slots(c, n, t, i(5), i(0), seq_lens=same, **ok)
