@@ -505,13 +505,17 @@ template <typename T, int NT, bool MEM> struct Row {
     stretch(rank, wid, seg0, seg1);
     seg0 -= p0, seg1 -= p0;
     first = (int)(p0 * N) - lead;
-#pragma unroll 1
-    for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
-      if (inside(p0 + i))
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_of(data + i)), "l"(vecs + p0 + i) : "memory");
-      else
-        data[i] = ragged(p0 + i);
-    }
+    // the row's first and last vector, where they are not its own alone; the others are copied
+    const bool head = seg0 < seg1 && !inside(p0 + seg0), tail = seg0 + head < seg1 && !inside(p0 + seg1 - 1);
+    const uint32_t i0 = seg0 + lane, from = i0 + (head && lane == 0 ? 32 : 0), end = seg1 - tail;
+    uint32_t to = smem_of(data + from);
+    const uint4* of = vecs + p0 + from;
+#pragma unroll 4
+    for (uint32_t i = from; i < end; i += 32, to += 32 * 16, of += 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(of) : "memory");
+    const uint32_t last = seg1 - 1 - seg0;  // the last vector's thread copies it, too
+    if (head && lane == 0) data[seg0] = ragged(p0 + seg0);
+    if (tail && lane == (int)(last % 32)) data[seg1 - 1] = ragged(p0 + seg1 - 1);
     asm volatile("cp.async.wait_all;" ::: "memory");
     typename E::Top top = E::top0();
 #pragma unroll 4
@@ -755,19 +759,26 @@ template <typename T, int NT, bool MEM> struct Row {
     } else {
       Sum sum(m, c);
       const bool lists_any = mine >= edge;
-      uint64_t has = 0;  // which of the thread's vectors have any: they are looked at again afterwards
+      // which of the thread's vectors have any (the last bit: any of the 32nd and later ones): they are looked at again
+      uint32_t has = 0, bit = 1;
 #pragma unroll 2
       for (uint32_t i = seg0 + lane; i < seg1; i += 32) {
         const uint4 v = data[i];
         sum.template add<ALL>(v, 0.0f, 0.0f);
-        if (lists_any) has |= (uint64_t)(E::value(E::top(E::top0(), v)) >= edge) << ((i - seg0) / 32);
+        if (lists_any) {
+          if (E::value(E::top(E::top0(), v)) >= edge) has |= bit;
+          bit = bit << 1 | (bit & 0x80000000u);
+        }
       }
 #pragma unroll 1
       while (has) {
-        const uint32_t i = seg0 + lane + 32 * (__ffsll((long long)has) - 1);
+        const uint32_t k = __ffs((int)has) - 1;
         has &= has - 1;
-        const uint4 v = data[i];
-        each_of(hits(v, edge, INFINITY), v, i, [&](float z, int j) { list_entry(z, j, only_first); });
+#pragma unroll 1
+        for (uint32_t i = seg0 + lane + 32 * k; i < seg1; i += k == 31 ? 32 : part_vecs) {
+          const uint4 v = data[i];
+          each_of(hits(v, edge, INFINITY), v, i, [&](float z, int j) { list_entry(z, j, only_first); });
+        }
       }
       return sum.mass();
     }
