@@ -285,10 +285,12 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+// In three parts of 27 bits, whose sums over a warp fit 32: three reductions of
+// one instruction each against five exchanges of both halves.
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
-  return v;
+  const uint32_t a = __reduce_add_sync(~0u, (uint32_t)v & 0x7ffffffu), b = __reduce_add_sync(~0u, (uint32_t)(v >> 27) & 0x7ffffffu);
+  const uint32_t c = __reduce_add_sync(~0u, (uint32_t)(v >> 54));
+  return a + ((uint64_t)b << 27) + ((uint64_t)c << 54);
 }
 template <typename V> __device__ __forceinline__ V warp_scan(V v, int lane) {  // inclusive
 #pragma unroll
@@ -712,19 +714,27 @@ template <typename T, int NT, bool MEM> struct Row {
   };
   template <int KIND, typename F> __device__ __forceinline__ uint64_t weigh(float over, float low, float least_w, F f) const {
     Sum sum(m, c);
-    uint64_t has = 0;  // which of the thread's vectors f wants: they are looked at again afterwards, few and together
+    // which of the thread's vectors f wants (the last bit: any of the 32nd and later ones): they are looked at again
+    // afterwards, few and together
+    uint32_t has = 0, bit = 1;
     vectors<KIND == ALL>([&](const uint4& v, uint32_t i) {
       float below = -INFINITY;  // the largest that is not above
       sum.template add<KIND>(v, over, least_w, &below);
       if (KIND == ABOVE && MEM && below >= low) each_of(hits(v, low, over), v, i, f);
-      if (KIND == ABOVE && !MEM) has |= (uint64_t)(below >= low) << ((i - seg0) / 32);
+      if (KIND == ABOVE && !MEM) {
+        if (below >= low) has |= bit;
+        bit = bit << 1 | (bit & 0x80000000u);
+      }
     }, [&] { sum.fold(); });
 #pragma unroll 1
     while (KIND == ABOVE && !MEM && has) {
-      const uint32_t i = seg0 + lane + 32 * (__ffsll((long long)has) - 1);
+      const uint32_t k = __ffs((int)has) - 1;
       has &= has - 1;
-      const uint4 v = data[i];
-      each_of(hits(v, low, over), v, i, f);
+#pragma unroll 1
+      for (uint32_t i = seg0 + lane + 32 * k; i < seg1; i += k == 31 ? 32 : part_vecs) {
+        const uint4 v = data[i];
+        each_of(hits(v, low, over), v, i, f);
+      }
     }
     return sum.mass();
   }
