@@ -22,7 +22,7 @@
 // with the launch) and 20 to 40,000 beside two other CTAs on the SM, and 35,000
 // more where a nucleus lies beyond the candidates.  Each phase runs once or
 // twice per CTA, from a cold instruction cache: cutting the code of the sampling kernel from
-// 287 KB to 129 KB (loops rolled, one copy of each search) made every case 10
+// 287 KB to 124 KB (loops rolled, one copy of each search) made every case 10
 // to 35% faster, so loops are unrolled where a pass over the row is hot and
 // nowhere else.
 #pragma once
@@ -1635,11 +1635,11 @@ template <typename T, int NT, bool MEM> struct Row {
 // A cut that does not end among the candidates (a nucleus beyond the guess,
 // a large top_k, many equal values) keeps the cluster to narrow it down.
 //
-// Measured (B200, device time): 1 x 32768 f32 9.7 us; 16 x 131072 bf16 of mixed
-// parameters 23 us; 256 x 131072 bf16, nuclei, 77 us (a sixth of the rows are
-// narrowed down, and one of those among the last to start makes the tail); 200 x
+// Measured (B200, device time): 1 x 32768 f32 9.6 us; 16 x 131072 bf16 of mixed
+// parameters 14 to 21 us; 256 x 131072 bf16, nuclei, 67 us (a sixth of the rows
+// are narrowed down, and one of those among the last to start makes the tail); 200 x
 // 100003 f16 without cuts 29 us (1.4 TB/s); 64 x 131072 f32 with nuclei of tens
-// of thousands 60 us; 512 x 131072 f32 of mixed parameters 132 us (2.0 TB/s).
+// of thousands 55 us; 512 x 131072 f32 of mixed parameters 124 us (2.2 TB/s).
 template <typename T, int NT, bool MEM>
 __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typename Row<T, NT, MEM>::Shared& sh, uint4* data) {
   RowFinish& f = *reinterpret_cast<RowFinish*>(data);
@@ -1743,7 +1743,7 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
 // ---- the n best ---------------------------------------------------------------------
 // As a sampling row with top_k = n, whose ordered candidates are the answer.
 // Measured (B200, device time): n = 5 of 1 x 32768 f32 8.3 us, n = 20 of 128 x
-// 131072 bf16 19.7 us (1.7 TB/s), n = 8 of 1024 x 50021 f32 70 us (2.9 TB/s,
+// 131072 bf16 19.9 us (1.7 TB/s), n = 8 of 1024 x 50021 f32 70 us (2.9 TB/s,
 // one streaming CTA a row; bound by issue: 16 instructions an entry in the two
 // passes together).
 template <typename T, int NT, bool MEM>
