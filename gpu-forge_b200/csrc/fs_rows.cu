@@ -96,8 +96,9 @@ template <typename T, bool BEST> int launch_solo(fs_sorter* s, const SorterView&
 // against 195), but not for rows of a single part (512 x 32000 bf16: 30.5 us against
 // 26.4).  Nor for nuclei: a row whose cut lies far down takes several times as
 // long as the rest of the batch, and less so on several CTAs (256 x 131072 bf16
-// peaked rows, a sixth of them such: 73 us by clusters, 105 streaming; where
-// all rows are such, 256 x 128256 bf16, 110 and about as much).
+// peaked rows, a sixth of them such: 73 us by clusters, 105 streaming; 512
+// x 131072 f32, a twentieth of them, 131 and 147.  Where all rows are such, streaming
+// gains: 256 x 128256 bf16 110 and 111 us, 512 x 128256 f32 299 and 238).
 template <typename T, bool BEST> int launch(fs_sorter* s, const SorterView& v, RowArgs& a) {
   const uint32_t ctas = row_ctas(row_vecs(a, RowElem<T>::N) * 16, a.rows, v.sm_count);
   const bool streams = !a.top_p && ctas > 1 && (uint64_t)ctas * a.rows > 3ull * v.sm_count;
