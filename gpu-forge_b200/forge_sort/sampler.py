@@ -36,7 +36,7 @@ class GpuSampler:
 
     new() / GpuSampler() follow torch's current stream of device 0;
     with_context(device, stream) enqueues on the caller's stream, which the
-    arguments must be ready on."""
+    arguments must be ready on and which the results belong to."""
 
     def __init__(self, device: int = 0, stream=None):
         import torch
@@ -47,6 +47,14 @@ class GpuSampler:
         self._dev = torch.device("cuda", self.device)
         self._fixed = _stream_handle(stream)
         self._last = self._fixed
+        # With a stream of its own, what a call makes (outputs, numbers spread over the rows) is made on that stream:
+        # on torch's current one it might still be filled, or its memory still be used, when the kernel runs.
+        if self._fixed is None:
+            self._own = None
+        elif self._fixed == 1:  # cudaStreamLegacy
+            self._own = torch.cuda.default_stream(self._dev)
+        else:
+            self._own = torch.cuda.ExternalStream(self._fixed, device=self._dev)
         self._logits = {torch.float32: _lib.LOGITS_F32, torch.float16: _lib.LOGITS_F16,
                         torch.bfloat16: _lib.LOGITS_BF16}
         # torch.cuda.current_stream() makes an object; this gives its handle alone
@@ -81,6 +89,12 @@ class GpuSampler:
             self._last = h or 1  # 1: cudaStreamLegacy
         return self._last
 
+    def _made(self, make, *args, **kw):
+        if self._own is None:
+            return make(*args, **kw)
+        with self._torch.cuda.stream(self._own):
+            return make(*args, **kw)
+
     def _vec(self, t, name: str, n: int, dtype):
         """Device address of a contiguous tensor of n elements of dtype."""
         try:  # the checks below in their cheapest form
@@ -105,13 +119,13 @@ class GpuSampler:
         if v is None:
             return None
         if isinstance(v, (int, float)):
-            v = self._torch.full((n,), v, dtype=dtype, device=self._dev)
+            v = self._made(self._torch.full, (n,), v, dtype=dtype, device=self._dev)
             keep.append(v)  # until the call has been enqueued; later reuse is ordered by the stream
         return self._vec(v, name, n, dtype)
 
     def _out(self, t, name: str, shape, dtype):
         if t is None:
-            t = self._torch.empty(shape, dtype=dtype, device=self._dev)
+            t = self._made(self._torch.empty, shape, dtype=dtype, device=self._dev)
             return t, t.data_ptr()
         try:
             if t.shape == shape and t.dtype is dtype and t.is_contiguous() and t.get_device() == self.device:

@@ -312,6 +312,23 @@ def test_streams(gs):
     own.close()
 
 
+def test_numbers_on_a_stream_of_its_own(gs):
+    """Numbers for all rows are spread on the sampler's stream, not on torch's
+    current one, which is busy here."""
+    import forge_sort
+    import torch
+    x, u = _peaked(64, 50021, "f32", 3), _uniform(64, 3)
+    want, _ = gs.sample(x, u, temperature=0.7, top_k=40, top_p=0.9, min_p=0.01, sync=True)
+    torch.cuda.synchronize()
+    for st in (torch.cuda.Stream(), torch.cuda.default_stream()):
+        own = forge_sort.GpuSampler.with_context(0, st)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            torch.cuda._sleep(20_000_000)
+            got, _ = own.sample(x, u, temperature=0.7, top_k=40, top_p=0.9, min_p=0.01, sync=True)
+            assert torch.equal(got.cpu(), want.cpu())
+        own.close()
+
+
 def test_graph(gs):
     import torch
     x, u = _peaked(8, 30011, "bf16", 3), _uniform(8, 3)
