@@ -358,7 +358,7 @@ template <int CTAS, int WARPS> struct RowShared {
   uint64_t scan_q[WARPS];
   uint32_t scan_n[WARPS];
   uint32_t n[CTAS];
-  uint64_t lo, hi, cut_q, cut_c;
+  uint64_t lo, hi, mid, cut_q, cut_c;
   uint32_t cut_n, count, above, first, b1, b2, last, found, dirty;
 };
 constexpr int ROW_SUMS = 128;  // warps of the CTAs that share a row
@@ -1046,15 +1046,16 @@ template <typename T, int NT, bool MEM> struct Row {
     }
     __syncthreads();
   }
-  // Of the interval of those bins: warp 0 gets the first entry, warp 1 the last.
+  // Of the interval of those bins: warp 0 gets the first entry, warp 1 the last,
+  // warp 2 the last of bin b1.
   // In the first round by mass a little before and behind them, by more than
   // the rounding of a bin's bound, which spares the search; counts, and the
   // rounds that have to shorten the interval, need the bounds themselves.
   __device__ __forceinline__ uint64_t end_of(bool by_mass, bool by_weight, bool first_round, float cs, int shift, uint64_t lo,
                                              uint64_t hi) {
-    if (wid >= 2) return 0;
+    if (wid >= 3) return 0;
     const uint32_t end = by_mass ? sh.last : (uint32_t)ROW_BINS - 1;
-    const uint32_t b = wid ? min(sh.b2, end) + 1 : min(sh.b1, end);
+    const uint32_t b = min(wid == 1 ? sh.b2 : sh.b1, end) + (wid ? 1 : 0);
     uint64_t at;
     if (by_mass && first_round) {
       const float d = __fdiv_rn((float)b - 0.5f, cs), by = fabsf(m) * 0x1p-21f;
@@ -1080,14 +1081,19 @@ template <typename T, int NT, bool MEM> struct Row {
   //   of entries with w >= least_w in sh.part, on all CTAs,
   //   the number of entries before it in above_n (counts alone).
   // Each round counts the undecided entries by bin, or sums their weights, each
-  // to 13 or 17 bits of its bin's, which tells the bin, or next to its bounds the two
-  // or three, that the prefix ends in; a second pass takes what comes before by
-  // its exact mass, so that the estimates of the next round err by a part of
-  // the rest alone.  Bins are of a 42nd octave of weight or less, by how far
+  // to 13 or 17 bits of its bin's, which tells the bin b1 that the prefix ends in or,
+  // where it ends closer to b1's end than the sums' error, a range of bins from b1 on.  A
+  // second pass takes the exact masses of what comes before b1 and of b1, which
+  // tell b1 from what lies behind it: the next round has b1 alone, or has b1
+  // among what comes before, and its estimates err by a part of the rest alone.
+  // Bins are of a 42nd octave of weight or less, by how far
   // the nucleus may reach, and of a 2^-10th of the interval once it is shorter
-  // than three of those (for counts: after the first round).  (key, index) has no ties: an interval can always be cut.
-  // `rounds` bounds them all the same; it takes two or three, and far in the
-  // tail, where the rest shrinks by 2^-12 a round, up to eight.
+  // than three of those (for counts: after the first round).
+  // Most rows take two or three rounds.  A round that leaves b1 alone shortens the
+  // interval of 51-bit (key, index) to a bin: once by weight, then by 2^9 at
+  // least, so at most seven do.  One that leaves what lies behind b1
+  // shrinks the goal, below 2^59, to twice the estimates' error of it, 2^-10
+  // or less, so at most six do.
   // A weight as q holds it.
   static __device__ __forceinline__ float held(float w) {
     return w < 0x1p-17f ? __fsub_rn(__fadd_rn(w, ROW_MAGIC), ROW_MAGIC) : w;
@@ -1116,13 +1122,9 @@ template <typename T, int NT, bool MEM> struct Row {
         by_mass ? ROW_BINS_END / fminf(ROW_MASS_END, 41.125f - log2f(fmaxf((float)rest / (float)cols, 0x1p-8f))) : ROW_BIN_SCALE;
     const float octaves = 1.0f / per_octave, cs = fminf(c * per_octave, ROW_F32_MAX);
     constexpr int ROUNDS = 16;
+    __syncthreads();  // what was there has been read, by this CTA alone since the last barrier
 #pragma unroll 1
     for (int round = 0; round < ROUNDS; ++round) {
-      // what was there has been read (before the first round: by this CTA alone, since the last barrier)
-      if (round)
-        cluster.sync();
-      else
-        __syncthreads();
 #pragma unroll 1
       for (int b = tid; b < ROW_BINS; b += NT) sh.bins[b] = 0;
       if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ~0u, sh.last = 0;
@@ -1171,23 +1173,23 @@ template <typename T, int NT, bool MEM> struct Row {
         const float goal = by_mass ? (float)(target - above_q) * (UNIT * 0x1p-40f) : (float)(target - above_n);
         end_bins(by_mass, round == 0, goal, above_n, octaves);
         const uint64_t at = end_of(by_mass, by_weight, round == 0, cs, shift, lo, hi);
-        if (wid < 2) {
-          if (lane < (int)ctas) {
-            *cluster.map_shared_rank(wid ? &sh.hi : &sh.lo, lane) = at;
-            if (wid && lane) *cluster.map_shared_rank(&sh.above, lane) = sh.above;
-          }
+        if (wid < 3 && lane < (int)ctas) {
+          *cluster.map_shared_rank(wid == 0 ? &sh.lo : wid == 1 ? &sh.hi : &sh.mid, lane) = at;
+          if (wid == 1 && lane) *cluster.map_shared_rank(&sh.above, lane) = sh.above;
         }
       }
       cluster.sync();
       lo = sh.lo, hi = sh.hi;
       // exact sums of what comes before, and the entries of the interval
       above_n = by_mass ? 0 : sh.above;
-      uint64_t before = 0, kept;
+      const uint64_t mid = sh.mid;
+      uint64_t before = 0, kept, in_b1 = 0;
       const float over = value_of(lo);
       const bool cuts_equals = (lo & (ROW_MAX_COLS - 1)) != 0;  // equal values lie on both sides of lo
       before = weigh<ABOVE>(over, value_of(hi), 0.0f, [&](float z, int j) {
         const uint64_t e = (uint64_t)row_key(z) << ROW_IDX_BITS | (uint32_t)j;
         if (e < lo || e > hi) return;
+        if (by_mass && e <= mid) in_b1 += mass(z);
         const uint32_t at = atomicAdd(&sh.count, 1u);
         if (at < ROW_POOL) sh.pool[at] = e;
       });
@@ -1206,8 +1208,17 @@ template <typename T, int NT, bool MEM> struct Row {
       above_q = handed(sh.mass);
       n = pooled(most);
       if (n <= most) return;
+      if (by_mass) hand<true>(sh.part, in_b1);  // nobody reads its masses before the last round's
+      cluster.sync();
+      if (by_mass) {
+        in_b1 = handed(sh.part);
+        if (above_q + in_b1 >= target)
+          hi = mid;
+        else
+          lo = mid + 1, above_q += in_b1;
+      }
     }
-    n = 0;  // never: what the last round left undecided is cut off
+    n = 0;  // by the count above, never; a row without a kept mass would say so
   }
 
   // ---- ordering the candidates, on the first CTA alone ----
@@ -1646,13 +1657,13 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
   Row<T, NT, MEM> r(sh, data, a, row, MEM ? 0 : cg::this_cluster().block_rank(), MEM ? 1 : cg::this_cluster().num_blocks(), MEM ? 2 : 1);
   const RowParams q(a, row);
   r.load(q.by_k || q.by_p);
-  if (r.m == -INFINITY) {
+  auto store_nothing = [&] {
     if (r.rank == 0 && r.tid == 0) {
       a.tokens[row] = -1;
       if (a.logprobs) a.logprobs[row] = -INFINITY;
     }
-    return;
-  }
+  };
+  if (r.m == -INFINITY) return store_nothing();
   r.c = q.c();
   const uint32_t k = q.k;
   const float least_w = q.least_w;
@@ -1737,7 +1748,11 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
     }
     __syncthreads();
   }
-  r.scan_parts(sh.part, row_draw(q.u, r.handed(sh.part)), least_w, last, store);
+  const uint64_t mass = r.handed(sh.part);
+  if (mass)
+    r.scan_parts(sh.part, row_draw(q.u, mass), least_w, last, store);
+  else
+    store_nothing();
 }
 
 // ---- the n best ---------------------------------------------------------------------

@@ -1,0 +1,116 @@
+"""GPU tests of GpuSampler where a cut or a batch is at its edge, against the
+plain restatements of _serving.py: equal tokens, into outputs that hold
+something else before.  Every test runs in the default form, which goes by the
+batch's size, and in each form by itself."""
+import functools
+
+import numpy as np
+import pytest
+
+import _serving as ref
+
+pytestmark = pytest.mark.gpu
+
+DT = ["f32", "f16", "bf16"]
+
+
+@pytest.fixture(scope="module", params=[0, 1, 2], ids=["by size", "cluster", "solo"])
+def gs(request):
+    import forge_sort
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setenv("FORGESORT_ROW_FORM", str(request.param))
+        s = forge_sort.GpuSampler.new()
+    yield s
+    s.close()
+
+
+def _dtype(name):
+    import torch
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def _sample(gs, x, u, **params):
+    """Tokens of gs.sample as a list; params: numbers, or a list of one for each row."""
+    import torch
+    R = x.shape[0]
+    dev = lambda v, dt: torch.as_tensor(v, dtype=dt, device="cuda").expand(R).contiguous()  # noqa: E731
+    kw = {k: dev(v, torch.int32 if k == "top_k" else torch.float32) for k, v in params.items()}
+    tok = torch.full((R,), -7, dtype=torch.int32, device="cuda")
+    lp = torch.full((R,), 7.0, device="cuda")
+    gs.sample(x, dev(u, torch.float32), tokens=tok, logprobs=lp, sync=True, **kw)
+    assert int((tok == -7).sum()) == 0 and float(lp.max()) < 1e-6  # the logarithm of a sum's rounding may pass 0
+    return tok.tolist()
+
+
+def _draws(kept, spots):
+    """Numbers u that put the draw at the given shares of the kept mass of all
+    entries but the last, and the tokens that they give."""
+    run = np.cumsum(kept)
+    total, tail = int(run[-1]), int(run[-2])
+    us = [np.float32(min(s * tail / total, 1 - 2.0**-24)) for s in spots] + [np.float32(0.5)]
+    at = [min(int(np.floor(float(u) * float(total))), total - 1) for u in us]
+    return us, [int(np.searchsorted(run, t, side="right")) for t in at]
+
+
+def _tail(kind, n, rng):
+    if kind == "flat":
+        return np.zeros(n)
+    if kind == "two values":
+        return rng.integers(0, 2, n) * -3.0
+    return rng.standard_normal(n) * {"narrow": 0.5, "wide": 3.0}[kind]
+
+
+@functools.lru_cache(maxsize=None)
+def _close_cuts(dtype, heavy, share, top_k, V=20011):
+    """Four rows, and for each draw its row, top_p, number and token."""
+    import torch
+    rng = np.random.default_rng(int(share * 1e6) + heavy)
+    rows, of, ps, us, want = [], [], [], [], []
+    for kind in ("flat", "two values", "narrow", "wide"):
+        z = _tail(kind, V - heavy, rng)
+        z += np.log((1 - share) / share) - np.log(np.exp(z).sum())
+        # the heavy ones last, so that small numbers u draw from the tail
+        row = torch.from_numpy(np.concatenate([z, np.full(heavy, -np.log(heavy))]).astype(np.float32)).to(_dtype(dtype)).cuda()
+        x = ref.clean(row)
+        _, w = ref.weights(x, 1.0, row.device)
+        q = ref.kept(x, w, top_k=top_k)
+        least = q[-heavy:].sum() / q.sum()
+        for by in (-1e-5, 0.0, 1e-7, 1e-6, 1e-5, 3e-5, 1e-4, 1e-3, 1e-2):
+            p = float(np.float32(least * (1 + by)))
+            if not 0 < p < 1:
+                continue
+            k = ref.kept(x, w, top_k=top_k, top_p=p)
+            k = np.concatenate([k[:-heavy], [k[-heavy:].sum()]])
+            for u, t in zip(*_draws(k, (0.3, 0.9999))):
+                of.append(len(rows)), ps.append(p), us.append(u), want.append(t)
+        rows.append(row)
+    return torch.stack(rows), of, ps, np.array(us), want
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("heavy", [1, 3])
+@pytest.mark.parametrize("share", [0.5, 0.99, 0.999, 0.99999])
+@pytest.mark.parametrize("top_k", [0, 12000])
+def test_a_nucleus_that_ends_close_behind_its_heaviest_entries(gs, dtype, heavy, share, top_k):
+    """`heavy` equal entries hold `share` of the mass, and p asks for that much
+    and a little more, or less: where the nucleus ends among thousands of light
+    entries, no estimate of the heavy ones tells where."""
+    rows, of, ps, us, want = _close_cuts(dtype, heavy, share, top_k)
+    got = _sample(gs, rows[of], us, top_p=ps, top_k=top_k)
+    assert [min(t, rows.shape[1] - heavy) for t in got] == want
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("cols,share,p,spread", [(32000, 0.99997, 0.99999, 0.5), (131072, 0.99997, 0.99999, 2.0),
+                                                 (131072, 0.99999, 0.999999, 1.0), (131072, 0.999001, 0.999011, 0.5),
+                                                 (4096, 0.9900991, 0.990109, 0.0), (131072, 0.9900991, 0.990109, 0.0)])
+def test_confident_rows_with_top_p_close_to_one(gs, dtype, cols, share, p, spread):
+    import torch
+    rng = np.random.default_rng(cols)
+    z = rng.standard_normal(cols - 1) * spread
+    z += np.log((1 - share) / share) - np.log(np.exp(z).sum())
+    row = torch.from_numpy(np.concatenate([z, [0.0]]).astype(np.float32)).to(_dtype(dtype)).cuda()
+    x = ref.clean(row)
+    _, w = ref.weights(x, 1.0, row.device)
+    us, want = _draws(ref.kept(x, w, top_p=p), (0.001, 0.5, 0.99999))
+    assert _sample(gs, row.expand(len(us), -1), np.array(us), top_p=p) == want
