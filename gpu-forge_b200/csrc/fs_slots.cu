@@ -269,30 +269,31 @@ extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_
   if (!s) return FS_E_INVALID;
   if (index_bytes != 4 && index_bytes != 8)
     return sorter_fail(s, FS_E_INVALID, "lengths must be of 4 or 8 bytes, got %d", index_bytes);
-  if (requests == 0) return FS_OK;
   if (requests > (1u << 24)) return sorter_fail(s, FS_E_INVALID, "requests = %llu exceeds 2^24", (unsigned long long)requests);
   if (page_size == 0 || page_size > (1u << 20)) return sorter_fail(s, FS_E_INVALID, "page size %u outside [1, 2^20]", page_size);
-  if (table_width == 0 || table_width > 0x7fffffffull)
+  if ((requests && table_width == 0) || table_width > 0x7fffffffull)
     return sorter_fail(s, FS_E_INVALID, "block table width %llu outside [1, 2^31)", (unsigned long long)table_width);
   if (requests > 1 && table_stride < (int64_t)table_width)
     return sorter_fail(s, FS_E_INVALID, "block table rows overlap: stride %lld, width %llu", (long long)table_stride,
                        (unsigned long long)table_width);
   if (n_free > 0x7fffffffull) return sorter_fail(s, FS_E_INVALID, "more than 2^31 - 1 free pages");
   if (capacity > 0x7fffffffull) return sorter_fail(s, FS_E_INVALID, "more than 2^31 - 1 tokens");
-  if (!context_lens || !new_lens || !block_table || !cursor || !query_start || !seq_lens || !cursor_out ||
+  // without requests: places to fill and a cursor to hand on, but no lengths and no table
+  if ((requests && (!context_lens || !new_lens || !block_table || !seq_lens)) || !cursor || !query_start || !cursor_out ||
       (n_free && !free_pages) || (capacity && (!positions || !request_of || !slots)))
     return sorter_fail(s, FS_E_INVALID, "a required pointer is NULL");
-  if (seq_lens == context_lens || seq_lens == new_lens)
+  if (requests && (seq_lens == context_lens || seq_lens == new_lens))
     return sorter_fail(s, FS_E_INVALID, "seq_lens is the same memory as context_lens or new_lens");
   if (cursor == cursor_out) return sorter_fail(s, FS_E_INVALID, "cursor and cursor_out are the same memory");
   SorterView v;
   int rc = sorter_view(s, stream, &v);
   if (rc) return rc;
   const struct { const void* p; size_t bytes; const char* what; } ptrs[] = {
-      {context_lens, requests * index_bytes, "context_lens"}, {new_lens, requests * index_bytes, "new_lens"},
-      {block_table, ((size_t)(requests - 1) * table_stride + table_width) * 4, "block_table"},
+      {requests ? context_lens : nullptr, requests * index_bytes, "context_lens"},
+      {requests ? new_lens : nullptr, requests * index_bytes, "new_lens"},
+      {requests ? block_table : nullptr, ((size_t)(requests - 1) * table_stride + table_width) * 4, "block_table"},
       {n_free ? free_pages : nullptr, n_free * 4, "free_pages"}, {cursor, 4, "cursor"},
-      {query_start, (requests + 1) * 4, "query_start"}, {seq_lens, requests * index_bytes, "seq_lens"},
+      {query_start, (requests + 1) * 4, "query_start"}, {requests ? seq_lens : nullptr, requests * index_bytes, "seq_lens"},
       {capacity ? positions : nullptr, capacity * index_bytes, "positions"},
       {capacity ? request_of : nullptr, capacity * 4, "request_of"}, {capacity ? slots : nullptr, capacity * 8, "slots"},
       {cursor_out, 4, "cursor_out"}};

@@ -320,7 +320,8 @@ int fs_top_logprobs(fs_sorter* s, int dtype, const void* logits, uint64_t rows,
  *                token and where a token has no page
  *   cursor_out   cursor[0] + pages needed, at most n_free (not the same
  *                memory as cursor: a call may be repeated)
- * positions, request_of and slots hold `capacity` entries.  A token without a
+ * positions, request_of and slots hold `capacity` entries.  requests may be 0:
+ * the lengths, seq_lens and block_table are then not read and may be NULL.  A token without a
  * page (free pages used up, a row of the block table full, a negative entry
  * where a held page should be) or tokens beyond `capacity` are reported as
  * FS_E_GPU_EXECUTION at the next synchronisation; what has a page is still
