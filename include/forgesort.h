@@ -279,7 +279,8 @@ typedef enum fs_logits_dtype {
  *   top_p        then the shortest prefix of descending order that holds at
  *                least p of the mass of those; p >= 1: all; p <= 0: the best
  *   min_p        then the entries of at least min_p times the largest weight
- * uniform holds one number u of [0, 1) for each row (clamped to it): the
+ * A top_p or min_p of NaN is off.  uniform holds one number u of [0, 1) for
+ * each row (clamped to it, NaN reads as 0): the
  * token is the first index at which the running mass of the kept entries, in
  * index order, exceeds u times their sum.  Weights are 32-bit 2^-y with
  * y = (max - x) * (log2(e) / t), each rounded to a whole multiple of 2^-40,

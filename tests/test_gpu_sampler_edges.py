@@ -114,3 +114,21 @@ def test_confident_rows_with_top_p_close_to_one(gs, dtype, cols, share, p, sprea
     _, w = ref.weights(x, 1.0, row.device)
     us, want = _draws(ref.kept(x, w, top_p=p), (0.001, 0.5, 0.99999))
     assert _sample(gs, row.expand(len(us), -1), np.array(us), top_p=p) == want
+
+
+@pytest.mark.parametrize("params", [dict(top_p=float("nan")), dict(min_p=float("nan")), dict(top_k=40, top_p=float("nan"), min_p=float("nan")),
+                                    dict(top_p=0.8, min_p=float("nan"), temperature=1.5)], ids=["top_p", "min_p", "top_k", "top_p min_p"])
+def test_a_parameter_of_nan_is_off(gs, params):
+    import math
+    import torch
+    x = torch.randn(64, 5003, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") * 2
+    u = torch.rand(64, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").tolist()
+    off = {k: v for k, v in params.items() if not math.isnan(v)}
+    assert _sample(gs, x, u, **params) == [ref.sample(x[r], u[r], **off)[0] for r in range(64)]
+
+
+def test_a_number_of_nan_draws_the_first_kept(gs):
+    import torch
+    x = torch.randn(4, 5003, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    for kw in ({}, dict(top_k=9), dict(top_p=0.9)):
+        assert _sample(gs, x, [float("nan")] * 4, **kw) == [ref.sample(x[r], 0.0, **kw)[0] for r in range(4)]
