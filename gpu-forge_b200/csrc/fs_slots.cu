@@ -51,19 +51,22 @@ template <typename I> __device__ __forceinline__ int64_t length_of(const void* p
   const int64_t v = static_cast<const I*>(p)[r];
   return v > 0 ? v : 0;
 }
-// tokens / page and what is left, for 0 <= tokens < 2^63: the product with
+template <typename I> __device__ __forceinline__ constexpr int64_t longest() {
+  return sizeof(I) == 4 ? 0x7fffffffll : 0x7fffffffffffffffll;
+}
+// tokens / page and what is left: the product with
 // the page's reciprocal, which is at most one too small.  (The code of a step
 // runs once, from cold: a 64-bit division is an order of magnitude longer.)
-__device__ __forceinline__ int64_t div_page(int64_t tokens, const SlotArgs& a, int64_t& left) {
-  int64_t n = (int64_t)__umul64hi((uint64_t)tokens, a.page_part);
+__device__ __forceinline__ uint64_t div_page(uint64_t tokens, const SlotArgs& a, uint64_t& left) {
+  uint64_t n = __umul64hi(tokens, a.page_part);
   left = tokens - n * a.page;
   if (left >= a.page) ++n, left -= a.page;
   return n;
 }
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, const SlotArgs& a) {
-  int64_t left;
-  const int64_t n = div_page(tokens, a, left);
-  return min(n + (left != 0), (int64_t)a.width);
+  uint64_t left;
+  const uint64_t n = div_page((uint64_t)tokens, a, left);
+  return (int64_t)min(n + (left != 0), (uint64_t)a.width);
 }
 
 constexpr int SLOT_THREADS = 512;
@@ -137,8 +140,13 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
       if (l < n) {
         const int64_t ctx = length_of<I>(a.ctx, r0 + l);
         neu[k] = length_of<I>(a.neu, r0 + l);
-        more[k] = pages_of(ctx + neu[k], a) - pages_of(ctx, a);
-        if (blockIdx.x == 0) static_cast<I*>(a.seq_lens)[r0 + l] = (I)(ctx + neu[k]);
+        // no length passes its type's largest number, and no sum of 2^24 of them 64 bits
+        const uint64_t sum = (uint64_t)ctx + (uint64_t)neu[k];
+        const int64_t len = (int64_t)min(sum, (uint64_t)longest<I>());
+        if (sum > (uint64_t)longest<I>()) neu[k] = longest<I>() - ctx, missed = true;
+        neu[k] = min(neu[k], MOST_TOKENS);
+        more[k] = pages_of(len, a) - pages_of(ctx, a);
+        if (blockIdx.x == 0) static_cast<I*>(a.seq_lens)[r0 + l] = (I)len;
       }
       t += neu[k], p += more[k];
     }
@@ -179,7 +187,7 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
       int32_t request[TOK];
       I position[TOK];
       int64_t slot[TOK];
-      int64_t pos = 0, nth = 0, off = 0, have = 0;
+      uint64_t pos = 0, nth = 0, off = 0, have = 0;
       int32_t* row = nullptr;
       int32_t id = -1;
       bool look = true;  // the request is a new one
@@ -192,9 +200,9 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
         bool turn = look;  // the page is another one
         if (look) {
           const int64_t ctx = length_of<I>(a.ctx, r0 + lo);
-          pos = ctx + i - start[lo];
+          pos = (uint64_t)ctx + (i - (uint32_t)start[lo]);
           nth = div_page(pos, a, off);
-          have = pages_of(ctx, a);
+          have = (uint64_t)pages_of(ctx, a);
           row = a.table + (int64_t)(r0 + lo) * a.table_stride;
           look = false;
         } else {
@@ -205,8 +213,8 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
           id = -1;
           if (nth < have) {
             id = row[nth];
-          } else if (nth < (int64_t)a.width) {
-            const uint64_t f = (uint64_t)(cursor + took[lo] + nth - have);
+          } else if (nth < a.width) {
+            const uint64_t f = (uint64_t)cursor + (uint32_t)took[lo] + nth - have;
             if (f < a.n_free) id = a.free_pages[f];
             if (off == 0) row[nth] = id;
           }
@@ -214,7 +222,7 @@ template <typename I, int TOK> __global__ void __launch_bounds__(SLOT_THREADS) k
         missed |= id < 0 || i >= a.capacity;
         request[k] = (int32_t)(r0 + lo);
         position[k] = (I)pos;
-        slot[k] = id < 0 ? -1 : (int64_t)id * a.page + off;
+        slot[k] = id < 0 ? -1 : (int64_t)id * a.page + (int64_t)off;
       }
       if (TOK > 1 && a.wide && i2 - i1 == TOK && i2 <= a.capacity) {
         put(a.request_of + i0, request);

@@ -322,11 +322,12 @@ int fs_top_logprobs(fs_sorter* s, int dtype, const void* logits, uint64_t rows,
  *   cursor_out   cursor[0] + pages needed, at most n_free (not the same
  *                memory as cursor: a call may be repeated)
  * positions, request_of and slots hold `capacity` entries.  requests may be 0:
- * the lengths, seq_lens and block_table are then not read and may be NULL.  A token without a
- * page (free pages used up, a row of the block table full, a negative entry
- * where a held page should be) or tokens beyond `capacity` are reported as
- * FS_E_GPU_EXECUTION at the next synchronisation; what has a page is still
- * planned. */
+ * the lengths, seq_lens and block_table are then not read and may be NULL.  A
+ * token without a page (free pages used up, a row of the block table full, a
+ * negative entry where a held page should be), tokens beyond `capacity` and
+ * new tokens that would take a length past the largest number of index_bytes
+ * (they are left out) are reported as FS_E_GPU_EXECUTION at the next
+ * synchronisation; what has a page is still planned. */
 int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_lens,
                   const void* new_lens, uint64_t requests, uint32_t page_size,
                   int32_t* block_table, uint64_t table_width,

@@ -36,3 +36,89 @@ def test_no_requests(gs, ints, capacity, width, cursor, free):
     assert p.query_start.tolist() == [0] and p.seq_lens.shape == (0,)
     assert p.cursor_out.tolist() == [min(max(cursor, 0), free)]
     assert (p.positions == 0).all() and (p.requests == -1).all() and (p.slots == -1).all()
+
+
+MOST = {"int32": 2**31 - 1, "int64": 2**63 - 1}
+
+
+def _plan(context, new, page, held, top):
+    """What a plan holds, in whole numbers without end; no length passes `top`."""
+    start, seq, pos, req, slots = [0], [], [], [], []
+    for r, c in enumerate(context):
+        n = min(new[r], top - c)
+        for p in range(c, c + n):
+            page_of = p // page
+            pos.append(p), req.append(r), slots.append(held[r][page_of] * page + p % page if page_of < len(held[r]) else -1)
+        start.append(start[-1] + n), seq.append(c + n)
+    return start, seq, pos, req, slots
+
+
+@pytest.mark.parametrize("ints", ["int32", "int64"])
+@pytest.mark.parametrize("short,extra", [(1, 5), (5, 2), (5, 5), (5, 6), (0, 3), (3, 0)])
+def test_lengths_that_pass_their_type(gs, ints, short, extra):
+    """A request whose context and new tokens exceed the largest number of its
+    type, beside others that do not: reported, and planned up to that number."""
+    import torch
+    from forge_sort import GpuExecution
+    I, top, page = getattr(torch, ints), MOST[ints], 1 << 20
+    context, new, capacity = [7, top - short, 3], [4, extra, 9], 32
+    width = 2048  # all pages that 32-bit positions have; of 64-bit ones, none of the long request's
+    table = torch.arange(3 * width, dtype=torch.int32, device="cuda").view(3, width)
+    held = table.tolist()
+    args = (torch.tensor(context, device="cuda").to(I), torch.tensor(new, device="cuda").to(I), table,
+            torch.empty(0, dtype=torch.int32, device="cuda"), _i32(0))
+    p = gs.plan_slots(*args, page_size=page, capacity=capacity)
+    torch.cuda.synchronize()
+    start, seq, pos, req, slots = _plan(context, new, page, held, top)
+    if -1 in slots or extra > short:
+        with pytest.raises(GpuExecution, match="slot"):
+            gs.synchronize()
+    else:
+        gs.synchronize()
+    n = len(pos)
+    assert p.query_start.tolist() == start and p.seq_lens.tolist() == seq
+    assert p.positions.tolist() == pos + [0] * (capacity - n) and p.requests.tolist() == req + [-1] * (capacity - n)
+    assert p.slots.tolist() == slots + [-1] * (capacity - n)
+    assert table.tolist() == held
+
+
+@pytest.mark.parametrize("page", [1, 3, 16, 1 << 20])
+@pytest.mark.parametrize("capacity", [70000, 90000])  # both widths of the stores, enough CTAs for 2^31 tokens
+def test_lengths_near_two_to_the_63(gs, page, capacity):
+    """Sums of lengths that 64 bits do not hold: every step stays inside its
+    memory and ends, and what fits is planned."""
+    import torch
+    from forge_sort import GpuExecution
+    top = 2**63 - 1
+    context = [4, top, top - 1, top - 5, 0, top // 2, 0]
+    new = [2, top, top, 3, top, top, top]
+    table = torch.full((7, 4), -1, dtype=torch.int32, device="cuda")
+    table[0] = torch.arange(4, dtype=torch.int32, device="cuda")
+    p = gs.plan_slots(torch.tensor(context, device="cuda"), torch.tensor(new, device="cuda"), table,
+                      torch.empty(0, dtype=torch.int32, device="cuda"), _i32(0), page_size=page, capacity=capacity)
+    torch.cuda.synchronize()
+    with pytest.raises(GpuExecution, match="slot"):
+        gs.synchronize()
+    assert p.query_start.tolist() == [0, 2, 2, 3, 6] + [2**31 - 1] * 3
+    assert p.seq_lens.tolist() == [6, top, top, top - 2, top, top, top]
+    have = [k * page + at if k < 4 else -1 for k, at in (divmod(x, page) for x in (4, 5))]
+    assert p.slots.tolist() == have + [-1] * (capacity - 2)
+    assert p.positions.tolist() == [4, 5, top - 1, top - 5, top - 4, top - 3] + list(range(capacity - 6))
+    assert p.requests.tolist() == [0, 0, 2, 3, 3, 3] + [4] * (capacity - 6)
+    assert table.tolist() == [[0, 1, 2, 3]] + [[-1] * 4] * 6
+
+
+def test_many_long_requests(gs):
+    """A sum of new tokens that 64 bits do not hold, of lengths that they do."""
+    import torch
+    from forge_sort import GpuExecution
+    R, T = 5000, 70000
+    new = torch.full((R,), 2**62, device="cuda")
+    p = gs.plan_slots(torch.zeros_like(new), new, torch.full((R, 1), -1, dtype=torch.int32, device="cuda"), _i32(9, 8, 7), _i32(1),
+                      page_size=2, capacity=T)
+    torch.cuda.synchronize()
+    with pytest.raises(GpuExecution, match="slot"):
+        gs.synchronize()
+    assert p.query_start.tolist() == [0] + [2**31 - 1] * R
+    assert p.slots.tolist() == [16, 17] + [-1] * (T - 2) and p.positions.tolist() == list(range(T))
+    assert p.cursor_out.tolist() == [3] and (p.seq_lens == 2**62).all()
