@@ -290,21 +290,27 @@ extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_
   if ((requests && (!context_lens || !new_lens || !block_table || !seq_lens)) || !cursor || !query_start || !cursor_out ||
       (n_free && !free_pages) || (capacity && (!positions || !request_of || !slots)))
     return sorter_fail(s, FS_E_INVALID, "a required pointer is NULL");
-  if (requests && (seq_lens == context_lens || seq_lens == new_lens))
-    return sorter_fail(s, FS_E_INVALID, "seq_lens is the same memory as context_lens or new_lens");
-  if (cursor == cursor_out) return sorter_fail(s, FS_E_INVALID, "cursor and cursor_out are the same memory");
   SorterView v;
   int rc = sorter_view(s, stream, &v);
   if (rc) return rc;
+  // the outputs first, then what is read, then the table, which is both
+  constexpr int OUTPUTS = 6, PLAIN = 10;
   const struct { const void* p; size_t bytes; const char* what; } ptrs[] = {
-      {requests ? context_lens : nullptr, requests * index_bytes, "context_lens"},
-      {requests ? new_lens : nullptr, requests * index_bytes, "new_lens"},
-      {requests ? block_table : nullptr, ((size_t)(requests - 1) * table_stride + table_width) * 4, "block_table"},
-      {n_free ? free_pages : nullptr, n_free * 4, "free_pages"}, {cursor, 4, "cursor"},
       {query_start, (requests + 1) * 4, "query_start"}, {requests ? seq_lens : nullptr, requests * index_bytes, "seq_lens"},
       {capacity ? positions : nullptr, capacity * index_bytes, "positions"},
       {capacity ? request_of : nullptr, capacity * 4, "request_of"}, {capacity ? slots : nullptr, capacity * 8, "slots"},
-      {cursor_out, 4, "cursor_out"}};
+      {cursor_out, 4, "cursor_out"},
+      {requests ? context_lens : nullptr, requests * index_bytes, "context_lens"},
+      {requests ? new_lens : nullptr, requests * index_bytes, "new_lens"},
+      {n_free ? free_pages : nullptr, n_free * 4, "free_pages"}, {cursor, 4, "cursor"},
+      {requests ? block_table : nullptr, ((size_t)(requests - 1) * table_stride + table_width) * 4, "block_table"}};
+  // CTAs read all of the inputs while others write
+  for (int i = 0; i < OUTPUTS; ++i)
+    for (int j = i + 1; j < PLAIN; ++j) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(ptrs[i].p), y = reinterpret_cast<uintptr_t>(ptrs[j].p);
+      if (x && y && x < y + ptrs[j].bytes && y < x + ptrs[i].bytes)
+        return sorter_fail(s, FS_E_INVALID, "%s and %s overlap", ptrs[i].what, ptrs[j].what);
+    }
   for (const auto& q : ptrs)
     if (q.p && (rc = sorter_check(s, q.p, q.bytes, q.what))) return rc;
   SlotArgs a{};

@@ -312,15 +312,14 @@ int fs_top_logprobs(fs_sorter* s, int dtype, const void* logits, uint64_t rows,
  * entries of pages held are read, the new ones written, no other touched).
  * Writes:
  *   query_start  requests + 1 entries: where each request's tokens start
- *   seq_lens     context + new of each request (index_bytes each; not the
- *                memory of either)
+ *   seq_lens     context + new of each request (index_bytes each)
  *   positions    of each token in its request (index_bytes each), 0 beyond
  *                the last token
  *   request_of   the token's request, -1 beyond the last token
  *   slots        page * page_size + position % page_size, -1 beyond the last
  *                token and where a token has no page
- *   cursor_out   cursor[0] + pages needed, at most n_free (not the same
- *                memory as cursor: a call may be repeated)
+ *   cursor_out   cursor[0] + pages needed, at most n_free
+ * These overlap neither each other nor what is read, so a call may be repeated.
  * positions, request_of and slots hold `capacity` entries.  requests may be 0:
  * the lengths, seq_lens and block_table are then not read and may be NULL.  A
  * token without a page (free pages used up, a row of the block table full, a

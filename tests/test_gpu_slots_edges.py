@@ -122,3 +122,41 @@ def test_many_long_requests(gs):
     assert p.query_start.tolist() == [0] + [2**31 - 1] * R
     assert p.slots.tolist() == [16, 17] + [-1] * (T - 2) and p.positions.tolist() == list(range(T))
     assert p.cursor_out.tolist() == [3] and (p.seq_lens == 2**62).all()
+
+
+def _overlaps():
+    """name -> arguments of a plan in which an output shares some of its memory with something else."""
+    import torch
+    b = torch.zeros(64, dtype=torch.int32, device="cuda")
+    w = torch.zeros(64, dtype=torch.int64, device="cuda")
+    return {
+        "lengths, one on": dict(context_lens=b[0:3], seq_lens=b[1:4]), "lengths, one back": dict(new_lens=b[5:8], seq_lens=b[3:6]),
+        "positions of lengths": dict(context_lens=b[0:3], positions=b[2:14]), "starts of lengths": dict(new_lens=b[0:3], query_start=b[0:4]),
+        "requests of free pages": dict(free_pages=b[0:6], requests=b[5:17]), "cursor": dict(cursor=b[0:1], cursor_out=b[0:1]),
+        "cursor in starts": dict(cursor=b[3:4], query_start=b[0:4]), "cursors in requests": dict(cursor_out=b[4:5], requests=b[0:12]),
+        "positions and requests": dict(positions=b[0:12], requests=b[11:23]),
+        "slots and positions": dict(slots=w[0:12], positions=w[11:23].view(torch.int32)[:12]),
+    }
+
+
+@pytest.mark.parametrize("name", ["lengths, one on", "lengths, one back", "positions of lengths", "starts of lengths",
+                                  "requests of free pages", "cursor", "cursor in starts", "cursors in requests",
+                                  "positions and requests", "slots and positions"])
+def test_outputs_that_share_memory_are_refused(gs, name):
+    import torch
+    args = dict(context_lens=_i32(1, 2, 3), new_lens=_i32(4, 4, 4), block_table=torch.zeros(3, 4, dtype=torch.int32, device="cuda"),
+                free_pages=_i32(1, 2, 3, 4, 5, 6), cursor=_i32(0), page_size=16, capacity=12)
+    with pytest.raises(ValueError, match="overlap"):
+        gs.plan_slots(**{**args, **_overlaps()[name]})
+
+
+def test_outputs_side_by_side_are_taken(gs):
+    """Everything in one allocation, nothing shared."""
+    import torch
+    b = torch.zeros(64, dtype=torch.int32, device="cuda")
+    w = torch.zeros(16, dtype=torch.int64, device="cuda")
+    b[0:3], b[3:6], b[6:8], b[8] = _i32(1, 2, 3), _i32(1, 1, 2), _i32(5, 6), 0
+    table = torch.zeros(3, 4, dtype=torch.int32, device="cuda")
+    p = gs.plan_slots(b[0:3], b[3:6], table, b[6:8], b[8:9], page_size=16, query_start=b[9:13], seq_lens=b[13:16],
+                      positions=b[16:20], requests=b[20:24], cursor_out=b[24:25], slots=w[0:4], sync=True)
+    assert p.positions.tolist() == [1, 2, 3, 4] and p.requests.tolist() == [0, 1, 2, 2] and p.seq_lens.tolist() == [2, 3, 5]
