@@ -25,8 +25,8 @@ int sorter_view(fs_sorter* s, void* stream, SorterView* v);
 int sorter_fail(fs_sorter* s, int code, const char* fmt, ...) __attribute__((format(printf, 3, 4)));
 int sorter_cuda_fail(fs_sorter* s, cudaError_t e, const char* what);
 // Checks that p is device or managed memory of the sorter's device, as the
-// device-resident sorts do.
-int sorter_check(fs_sorter* s, const void* p, size_t bytes, const char* what);
+// device-resident sorts do, and aligned to its elements of `align` bytes.
+int sorter_check(fs_sorter* s, const void* p, size_t bytes, size_t align, const char* what);
 // Ends a call that enqueued `launches` kernels on v.stream: waits and reports
 // device-side failures when sync != 0.
 int sorter_finish(fs_sorter* s, const SorterView& v, int launches, int sync);

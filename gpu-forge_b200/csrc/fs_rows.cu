@@ -120,8 +120,6 @@ int check_rows(fs_sorter* s, int dtype, const void* logits, uint64_t rows, uint6
   if (rows > 1 && stride < 0)
     return sorter_fail(s, FS_E_INVALID, "row stride %lld is negative", (long long)stride);
   if (!logits) return sorter_fail(s, FS_E_INVALID, "logits is NULL");
-  if (reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype))
-    return sorter_fail(s, FS_E_INVALID, "logits is not aligned to its elements");
   return FS_OK;
 }
 
@@ -140,12 +138,13 @@ int fs_sample_rows(fs_sorter* s, int dtype, const void* logits, uint64_t rows, u
   SorterView v;
   if ((rc = sorter_view(s, stream, &v))) return rc;
   const size_t span = ((size_t)(rows - 1) * row_stride + cols) * elem_bytes(dtype);
+  if ((rc = sorter_check(s, logits, span, elem_bytes(dtype), "logits"))) return rc;
   const struct { const void* p; size_t bytes; const char* what; } ptrs[] = {
-      {logits, span, "logits"},          {uniform, rows * 4, "uniform"}, {tokens, rows * 4, "tokens"},
+      {uniform, rows * 4, "uniform"}, {tokens, rows * 4, "tokens"},
       {temperature, rows * 4, "temperature"}, {top_k, rows * 4, "top_k"}, {top_p, rows * 4, "top_p"},
       {min_p, rows * 4, "min_p"},        {logprobs, rows * 4, "logprobs"}};
   for (const auto& q : ptrs)
-    if (q.p && (rc = sorter_check(s, q.p, q.bytes, q.what))) return rc;
+    if (q.p && (rc = sorter_check(s, q.p, q.bytes, 4, q.what))) return rc;
   RowArgs a{};
   a.x = logits;
   a.stride = row_stride;
@@ -172,8 +171,10 @@ int fs_top_logprobs(fs_sorter* s, int dtype, const void* logits, uint64_t rows, 
   SorterView v;
   if ((rc = sorter_view(s, stream, &v))) return rc;
   const size_t span = ((size_t)(rows - 1) * row_stride + cols) * elem_bytes(dtype);
-  if ((rc = sorter_check(s, logits, span, "logits")) || (rc = sorter_check(s, indices, rows * n * 4, "indices")) ||
-      (rc = sorter_check(s, logprobs, rows * n * 4, "logprobs")) || (lse && (rc = sorter_check(s, lse, rows * 4, "lse"))))
+  if ((rc = sorter_check(s, logits, span, elem_bytes(dtype), "logits")) ||
+      (rc = sorter_check(s, indices, rows * n * 4, 4, "indices")) ||
+      (rc = sorter_check(s, logprobs, rows * n * 4, 4, "logprobs")) ||
+      (lse && (rc = sorter_check(s, lse, rows * 4, 4, "lse"))))
     return rc;
   RowArgs a{};
   a.x = logits;

@@ -295,15 +295,16 @@ extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_
   if (rc) return rc;
   // the outputs first, then what is read, then the table, which is both
   constexpr int OUTPUTS = 6, PLAIN = 10;
-  const struct { const void* p; size_t bytes; const char* what; } ptrs[] = {
-      {query_start, (requests + 1) * 4, "query_start"}, {requests ? seq_lens : nullptr, requests * index_bytes, "seq_lens"},
-      {capacity ? positions : nullptr, capacity * index_bytes, "positions"},
-      {capacity ? request_of : nullptr, capacity * 4, "request_of"}, {capacity ? slots : nullptr, capacity * 8, "slots"},
-      {cursor_out, 4, "cursor_out"},
-      {requests ? context_lens : nullptr, requests * index_bytes, "context_lens"},
-      {requests ? new_lens : nullptr, requests * index_bytes, "new_lens"},
-      {n_free ? free_pages : nullptr, n_free * 4, "free_pages"}, {cursor, 4, "cursor"},
-      {requests ? block_table : nullptr, ((size_t)(requests - 1) * table_stride + table_width) * 4, "block_table"}};
+  const size_t I = index_bytes;
+  const struct { const void* p; size_t bytes, align; const char* what; } ptrs[] = {
+      {query_start, (requests + 1) * 4, 4, "query_start"}, {requests ? seq_lens : nullptr, requests * I, I, "seq_lens"},
+      {capacity ? positions : nullptr, capacity * I, I, "positions"},
+      {capacity ? request_of : nullptr, capacity * 4, 4, "request_of"}, {capacity ? slots : nullptr, capacity * 8, 8, "slots"},
+      {cursor_out, 4, 4, "cursor_out"},
+      {requests ? context_lens : nullptr, requests * I, I, "context_lens"},
+      {requests ? new_lens : nullptr, requests * I, I, "new_lens"},
+      {n_free ? free_pages : nullptr, n_free * 4, 4, "free_pages"}, {cursor, 4, 4, "cursor"},
+      {requests ? block_table : nullptr, ((size_t)(requests - 1) * table_stride + table_width) * 4, 4, "block_table"}};
   // CTAs read all of the inputs while others write
   for (int i = 0; i < OUTPUTS; ++i)
     for (int j = i + 1; j < PLAIN; ++j) {
@@ -312,7 +313,7 @@ extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_
         return sorter_fail(s, FS_E_INVALID, "%s and %s overlap", ptrs[i].what, ptrs[j].what);
     }
   for (const auto& q : ptrs)
-    if (q.p && (rc = sorter_check(s, q.p, q.bytes, q.what))) return rc;
+    if (q.p && (rc = sorter_check(s, q.p, q.bytes, q.align, q.what))) return rc;
   SlotArgs a{};
   a.ctx = context_lens;
   a.neu = new_lens;

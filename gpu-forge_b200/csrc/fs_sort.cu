@@ -1190,7 +1190,8 @@ int sorter_fail(fs_sorter* s, int code, const char* fmt, ...) {
 
 int sorter_cuda_fail(fs_sorter* s, cudaError_t e, const char* what) { return cuda_fail(s, e, what); }
 
-int sorter_check(fs_sorter* s, const void* p, size_t bytes, const char* what) {
+int sorter_check(fs_sorter* s, const void* p, size_t bytes, size_t align, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % align) return fail(s, FS_E_INVALID, "%s is not aligned to its elements", what);
   return prepare_ptr(s, p, bytes, what);
 }
 

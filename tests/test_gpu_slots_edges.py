@@ -160,3 +160,33 @@ def test_outputs_side_by_side_are_taken(gs):
     p = gs.plan_slots(b[0:3], b[3:6], table, b[6:8], b[8:9], page_size=16, query_start=b[9:13], seq_lens=b[13:16],
                       positions=b[16:20], requests=b[20:24], cursor_out=b[24:25], slots=w[0:4], sync=True)
     assert p.positions.tolist() == [1, 2, 3, 4] and p.requests.tolist() == [0, 1, 2, 2] and p.seq_lens.tolist() == [2, 3, 5]
+
+
+def test_addresses_between_elements_are_refused(gs):
+    """The C entries refuse them before a launch, with the argument's name."""
+    import torch
+    from forge_sort import _lib
+    L, h = _lib.load(), gs._s._h
+    b = torch.zeros(4096, dtype=torch.int64, device="cuda")
+    at = lambda k: b[64 * k:].data_ptr()  # noqa: E731
+    plan = dict(context_lens=at(0), new_lens=at(1), requests=2, page_size=16, block_table=at(2), width=4, stride=4, free_pages=at(3),
+                n_free=3, cursor=at(4), query_start=at(5), seq_lens=at(6), positions=at(7), request_of=at(8), slots=at(9),
+                capacity=4, cursor_out=at(10))
+    rows = dict(logits=at(11), rows=2, cols=8, stride=8, temperature=at(12), top_k=at(13), top_p=at(14), min_p=at(15),
+                uniform=at(16), tokens=at(17), logprobs=at(18))
+    best = dict(logits=at(11), rows=2, cols=8, stride=8, n=2, indices=at(19), logprobs=at(20), lse=at(21))
+    calls = [(lambda a: L.fs_plan_slots(h, 4, *a.values(), 1, None), plan, 4, {"slots": 8}),
+             (lambda a: L.fs_plan_slots(h, 8, *a.values(), 1, None), plan, 4,
+              dict.fromkeys(("context_lens", "new_lens", "seq_lens", "positions", "slots"), 8)),
+             (lambda a: L.fs_sample_rows(h, 0, *a.values(), 1, None), rows, 4, {}),
+             (lambda a: L.fs_sample_rows(h, 2, *a.values(), 1, None), rows, 4, {"logits": 2}),
+             (lambda a: L.fs_top_logprobs(h, 0, *a.values(), 1, None), best, 4, {})]
+    for call, args, size, own in calls:
+        assert call(args) == _lib.OK
+        for name, v in args.items():
+            if v < 4096:  # a number
+                continue
+            off = own.get(name, size) // 2
+            assert call({**args, name: v + off}) == _lib.E_INVALID, name
+            text = L.fs_last_error(h).decode()
+            assert name in text and "aligned" in text
