@@ -28,8 +28,9 @@ int sorter_cuda_fail(fs_sorter* s, cudaError_t e, const char* what);
 // device-resident sorts do, and aligned to its elements of `align` bytes.
 int sorter_check(fs_sorter* s, const void* p, size_t bytes, size_t align, const char* what);
 // Ends a call that enqueued `launches` kernels on v.stream: waits and reports
-// device-side failures when sync != 0.
-int sorter_finish(fs_sorter* s, const SorterView& v, int launches, int sync);
+// device-side failures when sync != 0.  may_fail: they use v.host_err, so
+// fs_synchronize and fs_destroy wait for them.
+int sorter_finish(fs_sorter* s, const SorterView& v, int launches, int sync, bool may_fail);
 
 // Device ordinals that per-device caches cover (fs_create refuses more).
 constexpr int SORTER_MAX_DEVICES = 64;

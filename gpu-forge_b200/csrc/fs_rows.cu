@@ -109,7 +109,7 @@ template <bool BEST> int launch_rows(fs_sorter* s, const SorterView& v, int dtyp
   const int rc = dtype == FS_LOGITS_F32   ? launch<float, BEST>(s, v, a)
                  : dtype == FS_LOGITS_F16 ? launch<__half, BEST>(s, v, a)
                                           : launch<__nv_bfloat16, BEST>(s, v, a);
-  return rc ? rc : sorter_finish(s, v, 1, sync);
+  return rc ? rc : sorter_finish(s, v, 1, sync, false);
 }
 
 int check_rows(fs_sorter* s, int dtype, const void* logits, uint64_t rows, uint64_t cols, int64_t stride) {

@@ -336,5 +336,5 @@ extern "C" int fs_plan_slots(fs_sorter* s, int index_bytes, const void* context_
   a.host_err = v.host_err;
   a.wide = (reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(request_of) | reinterpret_cast<uintptr_t>(slots)) % 16 == 0;
   rc = index_bytes == 4 ? launch_slots<int32_t>(s, v, a) : launch_slots<int64_t>(s, v, a);
-  return rc ? rc : sorter_finish(s, v, 1, sync);
+  return rc ? rc : sorter_finish(s, v, 1, sync, true);
 }

@@ -21,6 +21,7 @@
 #include <string>
 #include <type_traits>
 #include <unordered_map>
+#include <vector>
 
 using namespace fs;
 
@@ -92,6 +93,14 @@ struct fs_sorter {
   cudaEvent_t ev[2 * MAX_TIMED] = {};
   int ev_used = 0;
   int row_form = 0;  // FORGESORT_ROW_FORM
+  // the last call on each of the callers' streams that may use the error word,
+  // which fs_synchronize reads and fs_destroy frees
+  struct Elsewhere {
+    unsigned long long stream = 0;  // cudaStreamGetId: a handle may come again for another stream
+    cudaEvent_t done = nullptr;
+    bool pending = false;
+  };
+  std::vector<Elsewhere> elsewhere;
   HostStage stage;  // page-locked chunk ring for pageable host-slice copies
   int test_withhold = 0;    // fs_test_inject(FS_TEST_WITHHOLD_COPY): next radix sort
   int test_fail_alloc = 0;  // fs_test_inject(FS_TEST_FAIL_ALLOC): countdown to a failed growth
@@ -1117,6 +1126,42 @@ int finish_on(fs_sorter* s, cudaStream_t stream, int sync) {
 
 int finish(fs_sorter* s, int sync) { return finish_on(s, s->stream, sync); }
 
+// Marks the end of a call on a caller's stream.  One that is captured has no
+// end: its graph's launches are the caller's to wait for.
+int mark_elsewhere(fs_sorter* s, cudaStream_t stream) {
+  cudaStreamCaptureStatus capture;
+  FS_CUDA(s, cudaStreamIsCapturing(stream, &capture));
+  if (capture != cudaStreamCaptureStatusNone) return FS_OK;
+  unsigned long long id;
+  FS_CUDA(s, cudaStreamGetId(stream, &id));
+  fs_sorter::Elsewhere* at = nullptr;
+  for (auto& e : s->elsewhere)
+    if (e.stream == id) at = &e;
+  if (!at) {  // the event of a stream that is done, or a new one
+    for (auto& e : s->elsewhere)
+      if (!e.pending || cudaEventQuery(e.done) == cudaSuccess) at = &e;
+    cudaGetLastError();  // not ready
+  }
+  if (!at) {
+    cudaEvent_t ev;
+    FS_CUDA(s, cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
+    s->elsewhere.push_back({0, ev, false});
+    at = &s->elsewhere.back();
+  }
+  at->stream = id;
+  at->pending = true;
+  FS_CUDA(s, cudaEventRecord(at->done, stream));
+  return FS_OK;
+}
+
+int wait_elsewhere(fs_sorter* s) {
+  for (auto& e : s->elsewhere) {
+    if (e.pending) FS_CUDA(s, cudaEventSynchronize(e.done));
+    e.pending = false;
+  }
+  return FS_OK;
+}
+
 int check_common(fs_sorter* s, int dtype, uint64_t n) {
   if (!s) return FS_E_INVALID;
   if (dtype < FS_U32 || dtype > FS_F64) return fail(s, FS_E_INVALID, "unknown dtype %d", dtype);
@@ -1195,9 +1240,10 @@ int sorter_check(fs_sorter* s, const void* p, size_t bytes, size_t align, const 
   return prepare_ptr(s, p, bytes, what);
 }
 
-int sorter_finish(fs_sorter* s, const SorterView& v, int launches, int sync) {
+int sorter_finish(fs_sorter* s, const SorterView& v, int launches, int sync, bool may_fail) {
   s->last_launches = launches;
-  return finish_on(s, v.stream, sync);
+  const int rc = finish_on(s, v.stream, sync);
+  return rc || sync || !may_fail || v.stream == s->stream ? rc : mark_elsewhere(s, v.stream);
 }
 
 }  // namespace fs
@@ -1271,6 +1317,7 @@ int fs_destroy(fs_sorter* s) {
   if (!s) return FS_OK;
   cudaSetDevice(s->device);
   if (s->stream) cudaStreamSynchronize(s->stream);
+  for (auto& e : s->elsewhere) cudaEventSynchronize(e.done), cudaEventDestroy(e.done);
   for (auto& kv : s->allocs) {
     if (s->managed.count(kv.first))
       cudaFreeHost(kv.first);
@@ -1324,6 +1371,7 @@ int fs_synchronize(fs_sorter* s) {
   for (auto& sl : s->pipe)
     if (sl.used) FS_CUDA(s, cudaStreamWaitEvent(s->stream, sl.out_done, 0));
   s->pipe_open = false;
+  if ((rc = wait_elsewhere(s))) return rc;
   return finish(s, 1);
 }
 

@@ -7,8 +7,9 @@ No counterpart in the reference.  Arguments are torch tensors on the
 sampler's device; what a call returns are tensors too, new ones or those the
 caller passes to be written.  Calls enqueue on torch's current stream (or the
 stream the sampler was made with) and return without waiting unless
-sync=True; a device-side failure (a token without a slot) is raised by
-sync=True or by the next synchronize().  They keep no state between them.
+sync=True.  A device-side failure (a token without a slot) is raised, once, by
+whatever waits next on the sampler: synchronize(), or any call with sync=True,
+one that succeeded itself among them.  They keep no state between them.
 """
 from __future__ import annotations
 
@@ -73,7 +74,9 @@ class GpuSampler:
         self._s.close()
 
     def synchronize(self) -> None:
-        """Wait for the last call's stream and report device-side failures."""
+        """Wait for the last call's stream and for the slot plans on all others,
+        and report device-side failures.  Replays of a captured graph on another
+        stream are the caller's to wait for before."""
         if self._last is not None and self._L.fs_stream_synchronize(self._last):
             raise GpuExecution(self._L.fs_last_error(None).decode())
         self._s.synchronize()
@@ -96,9 +99,9 @@ class GpuSampler:
             return make(*args, **kw)
 
     def _vec(self, t, name: str, n: int, dtype):
-        """Device address of a contiguous tensor of n elements of dtype."""
+        """Device address of a contiguous tensor of n elements (None: any number) of dtype."""
         try:  # the checks below in their cheapest form
-            if t.dtype is dtype and t.numel() == n and t.is_contiguous() and t.get_device() == self.device:
+            if t.dtype is dtype and (n is None or t.numel() == n) and t.is_contiguous() and t.get_device() == self.device:
                 return t.data_ptr()
         except AttributeError:
             pass
@@ -106,7 +109,7 @@ class GpuSampler:
             raise TypeError(f"{name} must be a tensor")
         if t.dtype is not dtype:
             raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
-        if t.numel() != n:
+        if n is not None and t.numel() != n:
             raise ValueError(f"{name} has {t.numel()} elements, expected {n}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
@@ -218,16 +221,17 @@ class GpuSampler:
         w = self._vec(new_lens, "new_lens", R, I)
         if not isinstance(block_table, t.Tensor) or block_table.dtype is not t.int32:
             raise TypeError("block_table must be a tensor of int32")
-        if block_table.dim() != 2 or block_table.shape[0] != R:
-            raise ValueError(f"block_table must be [{R}, width], got {tuple(block_table.shape)}")
-        width = block_table.shape[1]
+        shape = block_table.shape
+        if len(shape) != 2 or shape[0] != R:
+            raise ValueError(f"block_table must be [{R}, width], got {tuple(shape)}")
+        width = shape[1]
         tstride, tstep = block_table.stride()
         if tstep != 1 and width > 1:
             raise ValueError("block_table must have stride 1 along a row")
         if block_table.get_device() != self.device:
             raise ValueError(f"block_table is on {block_table.device}, the sampler on {self._dev}")
-        nf = free_pages.numel() if isinstance(free_pages, t.Tensor) else 0
-        f = self._vec(free_pages, "free_pages", nf, t.int32)
+        f = self._vec(free_pages, "free_pages", None, t.int32)
+        nf = free_pages.numel()
         cur = self._vec(cursor, "cursor", 1, t.int32)
         if capacity is None:
             for o in (slots, positions, requests):

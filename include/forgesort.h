@@ -101,9 +101,10 @@ const char* fs_last_error(const fs_sorter* s);
 
 /* Replace the stream the sorter enqueues on (NULL = its private stream). */
 int fs_set_stream(fs_sorter* s, void* stream);
-/* Wait for all work enqueued by `s`, then report any device-side failure
- * (a bounded wait that ran out, an out-of-range scatter) that an
- * asynchronous call left behind. */
+/* Wait for all work enqueued by `s` (on its stream; of the calls that take a
+ * stream of their own, for what may report a failure), then report any
+ * device-side failure (a bounded wait that ran out, an out-of-range scatter, a
+ * token without a slot) that an asynchronous call left behind. */
 int fs_synchronize(fs_sorter* s);
 
 /* ---- memory (SortBuffer backing) --------------------------------------- */
@@ -259,8 +260,15 @@ int fs_gather(fs_sorter* s, int width, const void* src, uint64_t src_n,
  * sorter's device, ready on `stream` (a cudaStream_t, or NULL for the
  * sorter's own), on which the work is enqueued; they keep no scratch, so calls
  * on several streams may overlap and a call may be captured into a graph
- * (with sync == 0).  sync != 0 waits for `stream` and reports device failures,
- * as fs_synchronize does later for sync == 0. */
+ * (with sync == 0).  sync != 0 waits for `stream` and reports device failures.
+ * With sync == 0, fs_synchronize does so later for fs_plan_slots, on whatever
+ * stream it ran, and fs_destroy waits for it, too; the other two cannot fail on
+ * the device, and the caller waits for their stream.  Launches of a graph that
+ * holds calls are the caller's to wait for before fs_synchronize, and must all
+ * be done before fs_destroy.  Failures belong to the sorter, not to a call: one
+ * that an asynchronous call left behind is reported, once, by whatever
+ * synchronises next on the sorter, be it a call that succeeded itself.
+ * What a call writes overlaps none of its other arguments. */
 
 /* Types of logits. */
 typedef enum fs_logits_dtype {

@@ -190,3 +190,107 @@ def test_addresses_between_elements_are_refused(gs):
             assert call({**args, name: v + off}) == _lib.E_INVALID, name
             text = L.fs_last_error(h).decode()
             assert name in text and "aligned" in text
+
+
+def _short_plan():
+    """Arguments of a plan that finds no page for its only token."""
+    import torch
+    return dict(context_lens=_i32(0), new_lens=_i32(1), block_table=torch.full((1, 1), -1, dtype=torch.int32, device="cuda"),
+                free_pages=_i32(), cursor=_i32(0), page_size=16, capacity=1)
+
+
+def test_synchronize_waits_for_every_stream(gs):
+    """A failure on one stream is reported although the last call was on another."""
+    import torch
+    from forge_sort import GpuExecution
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    x, u, plan = torch.zeros(2, 64, device="cuda"), torch.zeros(2, device="cuda"), _short_plan()
+    torch.cuda.synchronize()
+    try:
+        for asleep in (1000, 200_000_000):  # the first time for the allocations, which wait for the device
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(asleep)
+                gs.plan_slots(**plan)
+            with torch.cuda.stream(b):
+                gs.sample(x, u)
+            if asleep == 1000:
+                torch.cuda.synchronize()
+            else:
+                assert not a.query()
+            with pytest.raises(GpuExecution, match="slot"):
+                gs.synchronize()
+            assert a.query() and b.query()
+            gs.synchronize()  # reported once
+    finally:
+        torch.cuda.synchronize()
+
+
+def test_fs_synchronize_waits_for_the_callers_streams():
+    import torch
+    import forge_sort
+    from forge_sort import _lib
+    L = _lib.load()
+    s = forge_sort.GpuSorter.new()
+    st = torch.cuda.Stream()
+    v = _i32(0, 1, 0, 0, 0, 0, 0, 0, 0)
+    table, slots = _i32(-1), torch.zeros(1, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    p = [v[k:].data_ptr() for k in range(9)]
+    try:
+        with torch.cuda.stream(st):
+            torch.cuda._sleep(200_000_000)
+        assert L.fs_plan_slots(s._h, 4, p[0], p[1], 1, 16, table.data_ptr(), 1, 1, None, 0, p[2], p[3], p[5], p[6], p[7],
+                               slots.data_ptr(), 1, p[8], 0, st.cuda_stream) == _lib.OK
+        assert L.fs_synchronize(s._h) == _lib.E_GPU_EXECUTION
+        assert st.query() and slots.tolist() == [-1]
+        assert L.fs_synchronize(s._h) == _lib.OK
+    finally:
+        torch.cuda.synchronize()
+        s.close()
+
+
+def test_close_waits_for_the_callers_streams():
+    """A failing plan writes the sorter's error word, which close() frees."""
+    import torch
+    import forge_sort
+    plan, st = _short_plan(), torch.cuda.Stream()
+    for asleep in (1000, 200_000_000):
+        gs = forge_sort.GpuSampler.new()
+        with torch.cuda.stream(st):
+            torch.cuda._sleep(asleep)
+            gs.plan_slots(**plan)
+        gs.close()
+        assert st.query()
+
+
+def test_many_streams(gs):
+    """More streams than are busy at a time, a captured call among them."""
+    import torch
+    from forge_sort import GpuExecution
+    plan, good = _short_plan(), {**_short_plan(), "free_pages": _i32(4)}
+    good["block_table"] = torch.full((1, 1), -1, dtype=torch.int32, device="cuda")
+    out = gs.plan_slots(**plan)
+    into = {k: getattr(out, k) for k in ("query_start", "seq_lens", "positions", "requests", "slots", "cursor_out")}
+    streams = [torch.cuda.Stream() for _ in range(12)]
+    torch.cuda.synchronize()
+    with pytest.raises(GpuExecution):
+        gs.synchronize()
+    for bad in (0, 7, 11, None):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                torch.cuda._sleep(2_000_000)
+                gs.plan_slots(**(plan if k == bad else good), **into)
+        if bad is not None:
+            with pytest.raises(GpuExecution, match="slot"):
+                gs.synchronize()
+        gs.synchronize()
+        assert all(st.query() for st in streams)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        gs.plan_slots(**plan, **into)
+    gs.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(GpuExecution, match="slot"):
+        gs.synchronize()
+    gs.synchronize()
