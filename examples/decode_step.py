@@ -34,7 +34,9 @@ class PagedModel:
         self.embed, self.place = w(vocab, dim) * 8, w(page_size * pages, dim) * 8
         self.qkv, self.out = w(3 * dim, dim), w(vocab, dim) * 4
         self.heads, self.page_size = heads, page_size
-        self.cache = torch.zeros(2, pages * page_size, dim, device="cuda")
+        # one row more than the pages have: slots of -1 (a token without a page, a place beyond the last token) index
+        # the last row, which belongs to nobody
+        self.cache = torch.zeros(2, pages * page_size + 1, dim, device="cuda")
 
     def forward(self, ids, plan, block_table):
         x = self.embed[ids] + self.place[plan.positions]

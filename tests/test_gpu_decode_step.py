@@ -64,3 +64,19 @@ def test_out_of_pages_is_reported(ex):
     model = ex.PagedModel(pages=256)
     with pytest.raises(Exception, match="free pages"):
         ex.generate(model, [[1] * 40, [2] * 40], 2, temperature=0.0, pages=3)
+
+
+def test_tokens_without_a_slot_touch_no_page(ex):
+    """A token without a page and a place beyond the last token (slots of -1)
+    leave every page as it was; the keys of the others are written."""
+    from forge_sort import SlotPlan
+    model = ex.PagedModel(pages=8, page_size=4)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    mark = torch.full((2, 8 * 4, model.embed.shape[1]), 3.0, device="cuda")
+    model.cache[:, :8 * 4] = mark
+    plan = SlotPlan(query_start=i32(0, 1, 2), seq_lens=i32(1, 1), positions=i32(0, 0, 0), requests=i32(0, 1, -1),
+                    slots=torch.tensor([-1, 9, -1], device="cuda"), cursor_out=i32(1))
+    logits = model.forward(torch.tensor([5, 6, 0], device="cuda"), plan, i32(-1, 2).view(2, 1))
+    changed = (model.cache[:, :8 * 4] != mark).any(-1)
+    assert changed.nonzero().tolist() == [[0, 9], [1, 9]]
+    assert logits.shape[0] == 2 and logits[1].isfinite().all()
