@@ -968,7 +968,9 @@ template <typename T, int NT, bool MEM> struct Row {
   }
 
   // The unit of a weight in its bin: with it 32 bits hold the sum of every
-  // entry that a CTA has.
+  // entry that a CTA has, of up to twice the unit less a little.  (The tangents
+  // are within 1% of the unit; what q holds is up to 4/3 of the weight, and
+  // below 2^-40, where it is up to twice the weight, the unit is that of 2^-40.)
   static constexpr float UNIT = MEM ? 0x1p12f : 0x1p16f;
   static constexpr int UNIT_BITS = MEM ? 12 : 16;
   // A vector's entries by bin.  Their weights, up to the last bin, as
@@ -1131,7 +1133,9 @@ template <typename T, int NT, bool MEM> struct Row {
       if (tid == 0) sh.count = 0, sh.b1 = sh.b2 = ~0u, sh.last = 0;
       __syncthreads();
       const int shift = max(0, 64 - __clzll((long long)((hi - lo) | 1)) - 10);
-      const float top_w = weight(value_of(lo)), scale = UNIT / top_w;
+      const float top_w = fmaxf(weight(value_of(lo)), 0x1p-40f), scale = UNIT / top_w;
+      // octaves down to the weight whose unit bin b has
+      auto down = [&](uint32_t b) { return round ? fminf((float)b * octaves, 40.0f) : (float)b * octaves; };
       const bool by_weight = round == 0 || (by_mass && bin_at(place_of(value_of(hi), cs)) >= bin_at(place_of(value_of(lo), cs)) + 3);
       if (round == 0) {
         const uint32_t bins = smem_of(sh.bins);
@@ -1149,7 +1153,7 @@ template <typename T, int NT, bool MEM> struct Row {
             atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], 1u);
           } else if (by_weight) {
             const uint32_t b = bin_at(place_of(z, cs));
-            atomicAdd(&sh.bins[b], (uint32_t)(held(weight(z)) * row_exp2((float)b * octaves + (float)UNIT_BITS) + 0.5f));
+            atomicAdd(&sh.bins[b], (uint32_t)(held(weight(z)) * row_exp2(down(b) + (float)UNIT_BITS) + 0.5f));
           } else {
             atomicAdd(&sh.bins[(uint32_t)((e - lo) >> shift)], (uint32_t)(held(weight(z)) * scale + 0.5f));
           }
@@ -1165,7 +1169,7 @@ template <typename T, int NT, bool MEM> struct Row {
           float v = 0;
 #pragma unroll 8
           for (uint32_t k = 0; k < ctas; ++k) v += (float)cluster.map_shared_rank(sh.bins, k)[b];
-          if (by_mass) v *= by_weight ? row_exp2((float)b * -octaves) : top_w;
+          if (by_mass) v *= by_weight ? row_exp2(-down(b)) : top_w;
           cluster.map_shared_rank(sh.bins, 0)[b] = __float_as_uint(v);
         }
       }

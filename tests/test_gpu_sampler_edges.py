@@ -132,3 +132,83 @@ def test_a_number_of_nan_draws_the_first_kept(gs):
     x = torch.randn(4, 5003, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
     for kw in ({}, dict(top_k=9), dict(top_p=0.9)):
         assert _sample(gs, x, [float("nan")] * 4, **kw) == [ref.sample(x[r], 0.0, **kw)[0] for r in range(4)]
+
+
+@pytest.fixture()
+def managed():
+    """f(numpy array) -> address of a copy in managed memory."""
+    import ctypes
+    import torch
+    rt = ctypes.CDLL("libcudart.so.12")  # torch has loaded it
+    held = []
+
+    def put(a):
+        p = ctypes.c_void_p()
+        assert rt.cudaMallocManaged(ctypes.byref(p), ctypes.c_size_t(a.nbytes), ctypes.c_uint(1)) == 0
+        held.append(p)
+        ctypes.memmove(p, a.ctypes.data, a.nbytes)
+        return p.value
+
+    torch.zeros(1, device="cuda")
+    yield put
+    torch.cuda.synchronize()
+    for p in held:
+        rt.cudaFree(p)
+
+
+@pytest.mark.parametrize("sorters", ["own", "legacy"])
+def test_managed_logits(managed, sorters):
+    """Logits in managed memory, on a stream other than the sorter's: at once and under a capture."""
+    import torch
+    import forge_sort
+    from forge_sort import _lib
+    L = _lib.load()
+    s = forge_sort.GpuSorter(0, None if sorters == "own" else torch.cuda.default_stream())
+    x = (np.random.default_rng(3).standard_normal((4, 70001)) * 2).astype(np.float32)
+    u = np.array([0.1, 0.5, 0.9, 0.99], np.float32)
+    want = [ref.sample(torch.from_numpy(x[r]).cuda(), float(u[r]))[0] for r in range(4)]
+    at, au = managed(x), managed(u)
+    tok = torch.full((4,), -7, dtype=torch.int32, device="cuda")
+    call = lambda: L.fs_sample_rows(s._h, 0, at, 4, 70001, 70001, None, None, None, None, au, tok.data_ptr(), None, 0,  # noqa: E731
+                                    torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        assert call() == _lib.OK
+    torch.cuda.synchronize()
+    assert tok.tolist() == want
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        rc = call()
+    assert rc == _lib.OK
+    tok.fill_(-7)
+    g.replay()
+    torch.cuda.synchronize()
+    assert tok.tolist() == want
+    s.close()
+
+
+@pytest.mark.parametrize("dtype,cols,rows", [("bf16", 131072, 40), ("f16", 131072, 40), ("f32", 1 << 19, 5)])
+def test_a_nucleus_of_the_lightest_weights(gs, dtype, cols, rows):
+    """Thousands of entries of hardly more than 2^-41 of the largest weight,
+    which the whole-number masses hold as 2^-40: as many as a CTA of a cluster
+    has in one bin, of the greatest sum that a bin can have."""
+    import torch
+    part = 32768  # entries of a CTA
+    x = torch.full((cols,), -32.0, dtype=_dtype(dtype), device="cuda")
+    x[cols - part:] = -float("inf")
+    x[cols - 1] = 0
+    T = float(np.float32(ref.LOG2E * 32 / 40.995))
+    h = ref.clean(x)
+    _, w = ref.weights(h, T, x.device)
+    p = 1 - 2.0**-24
+    kept = ref.kept(h, w, top_p=p)
+    tail = int((kept[:-1] > 0).sum())
+    assert 2.0**-41 < w[0] < 2.0**-40.99 and kept[0] == 1 and part // 2 <= tail < cols - part - 1
+    at = [0, 1, part // 2, tail - 1, tail]
+    u = [(t + 0.5) / int(kept.sum()) for t in at]
+    want = [ref.sample(x, v, temperature=T, top_p=p)[0] for v in u]
+    assert want[:-1] == at[:-1] and want[-1] == cols - 1
+    of = torch.arange(rows) % len(u)
+    got = _sample(gs, x.expand(rows, -1), np.array(u, np.float32)[of], top_p=p, temperature=T)
+    assert got == [want[k] for k in of]
