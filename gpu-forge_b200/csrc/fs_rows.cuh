@@ -326,8 +326,7 @@ struct RowParams {
     t = a.temperature ? a.temperature[row] : 1.0f;
     const int k_arg = a.top_k ? a.top_k[row] : 0;
     p = a.top_p ? a.top_p[row] : 1.0f;
-    const float w = a.min_p ? a.min_p[row] : 0.0f;
-    least_w = w > 0.0f ? fminf(w, 1.0f) : 0.0f;  // NaN: off
+    least_w = a.min_p ? __saturatef(a.min_p[row]) : 0.0f;  // NaN: 0, off
     u = a.uniform[row];
     k = (uint32_t)k_arg;
     greedy = !(t > 0.0f);
