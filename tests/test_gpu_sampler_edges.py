@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 import _serving as ref
+from test_gpu_sampler import _check, _check_best, _peaked, _uniform
 
 pytestmark = pytest.mark.gpu
 
@@ -212,3 +213,62 @@ def test_a_nucleus_of_the_lightest_weights(gs, dtype, cols, rows):
     of = torch.arange(rows) % len(u)
     got = _sample(gs, x.expand(rows, -1), np.array(u, np.float32)[of], top_p=p, temperature=T)
     assert got == [want[k] for k in of]
+
+
+def _across(dtype, n):
+    """Rows that several CTAs of a cluster share, whose entries above -inf, or whose entries that are to be cleaned, lie
+    in some of their parts only."""
+    import torch
+    dt, inf = _dtype(dtype), float("inf")
+    base = _peaked(1, n, dtype, 5)[0]
+    full = lambda v: torch.full((n,), v, dtype=dt, device="cuda")  # noqa: E731
+
+    def only(a, b, x=base, rest=-inf):
+        y = full(rest)
+        y[a:b] = x[a:b]
+        return y
+
+    def put(at, v, x=base):
+        y = x.clone()
+        y[at] = v
+        return y
+
+    low = torch.finfo(dt).min
+    return [full(-inf), full(float("nan")), only(0, 1), only(n - 1, n), only(n // 2, n // 2 + 1), only(0, 30), only(n - 30, n),
+            only(n // 2 - 300, n // 2 + 300), only(n // 3, n // 3 + 5, rest=low), only(n - 9000, n), only(0, 9000, full(0.5)),
+            put(n // 2, inf), put(n - 1, inf, put(0, inf)), put(n - 2, float("nan")), put(slice(n // 4, n // 2), float("nan")),
+            put(slice(0, n, 2), -inf), put(slice(0, n, 2), low), put(n - 3, inf, full(-inf)), full(low), full(2.0)]
+
+
+@pytest.mark.parametrize("dtype,cols", [("f32", 70001), ("f16", 70001), ("bf16", 70001), ("f32", 200003), ("bf16", 262139)])
+@pytest.mark.parametrize("params", [{}, dict(temperature=0.0), dict(top_k=50), dict(top_k=5000), dict(top_p=0.9), dict(min_p=0.05),
+                                    dict(temperature=1.1, top_k=3000, top_p=0.9, min_p=0.01)],
+                         ids=["plain", "greedy", "top_k 50", "top_k 5000", "top_p", "min_p", "all"])
+def test_masks_across_the_ctas_of_a_row(gs, dtype, cols, params):
+    import torch
+    x = torch.stack(_across(dtype, cols))
+    _check(gs, x, _uniform(x.shape[0], 1), **params)
+
+
+@pytest.mark.parametrize("dtype,cols", [("f32", 70001), ("f16", 70001), ("bf16", 70001), ("f32", 200003), ("bf16", 262139)])
+@pytest.mark.parametrize("n", [1, 20, 700])
+def test_best_across_the_ctas_of_a_row(gs, dtype, cols, n):
+    import torch
+    _check_best(gs, torch.stack(_across(dtype, cols)), n)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("params", [{}, dict(temperature=0.0), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.05, temperature=1.5)],
+                         ids=["plain", "greedy", "top_k", "top_p", "min_p"])
+def test_batches_on_both_sides_of_the_size_rule(gs, dtype, params):
+    """Clusters take 20 rows, streaming CTAs 600 of them where nothing is cut by mass: the same bits."""
+    import torch
+    x, u = _peaked(20, 70001, dtype, 2), _uniform(20, 3)
+    tok, lp = _check(gs, x, u, **params)
+    big_tok, big_lp = gs.sample(x.repeat(30, 1), u.repeat(30), sync=True, **params)
+    assert torch.equal(big_tok, tok.repeat(30)) and torch.equal(big_lp, lp.repeat(30))
+    if not params:
+        small, big = gs.top_logprobs(x, 9, sync=True), gs.top_logprobs(x.repeat(30, 1), 9, sync=True)
+        _check_best(gs, x, 9)
+        for a, b in zip(small, big):
+            assert torch.equal(a.repeat(30, *[1] * (a.dim() - 1)), b)
