@@ -90,15 +90,19 @@ template <typename T, bool BEST> int launch_solo(fs_sorter* s, const SorterView&
 
 // A cluster a row, or one CTA that streams it.  While one wave of clusters
 // takes the batch, clusters: they read a row once and several CTAs share its
-// work (16 rows of 128256 bf16, n = 20: 11.7 us against 20.8; 96 rows: 19.2
-// against 21.4).  Beyond, a streaming CTA has no partners to wait for (148 rows:
-// 23.9 us against 28.4; 1024 rows: 102 against 118; 1024 x 128256 f32: 166
-// against 195), but not for rows of a single part (512 x 32000 bf16: 30.5 us against
-// 26.4).  Nor for nuclei: a row whose cut lies far down takes several times as
+// work (16 rows of 128256 bf16, n = 20: 10.4 us against 17.9; 96 rows: 16.0
+// against 18.6).  Beyond, a streaming CTA has no partners to wait for (148 rows:
+// 18.6 us against 24.7; 1024 rows: 92 against 111; 1024 x 128256 f32: 151
+// against 184), though it loses where its rows fill the SMs one and a bit times
+// (160 rows: 28.8 against 25.1; 200 x 100003 f16 without cuts: 26.8 against
+// 25.4); not for rows of a single part (512 x 32000 bf16: 26.8 us against
+// 21.7).  Nor for nuclei: a row whose cut lies far down takes several times as
 // long as the rest of the batch, and less so on several CTAs (256 x 131072 bf16
-// peaked rows, a sixth of them such: 73 us by clusters, 105 streaming; 512
-// x 131072 f32, a twentieth of them, 131 and 147.  Where all rows are such, streaming
-// gains: 256 x 128256 bf16 110 and 111 us, 512 x 128256 f32 299 and 238).
+// peaked rows, a sixth of them such: 66 us by clusters, 104 streaming; 512
+// x 131072 f32, a twentieth of them, 112 and 144.  Where all rows are such, clusters
+// lose in 32 bits: 256 x 128256 bf16 106 and 115 us, 512 x 128256 f32 279 and
+// 242).  Whether there are nuclei is told by top_p being passed: its numbers are
+// on the device, so a batch of ones takes clusters, too.
 template <typename T, bool BEST> int launch(fs_sorter* s, const SorterView& v, RowArgs& a) {
   const uint32_t ctas = row_ctas(row_vecs(a, RowElem<T>::N) * 16, a.rows, v.sm_count);
   const bool streams = !a.top_p && ctas > 1 && (uint64_t)ctas * a.rows > 3ull * v.sm_count;

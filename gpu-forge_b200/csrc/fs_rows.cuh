@@ -49,7 +49,7 @@ constexpr int ROW_BEST_MAX = 1024;
 constexpr int ROW_TOPS = 512;   // thread maxima that a cluster's warps publish
 // A nucleus is first looked for among about this many entries: few nuclei of a
 // model's rows that hold more than that end before thousands (256 x 131072 bf16:
-// 192 entries 74.6 us, 128 entries 73.2, 64 entries 70.2).
+// 192 entries 68.8 us, 128 entries 68.1, 64 entries 65.8).
 constexpr uint32_t ROW_NUCLEUS_GUESS = 64;
 // Bins linear in y: of the published maxima (1/6 octave of weight each, 42 in
 // all; entries with q > 0 have y < 41), and of all entries (1/42 octave).
@@ -1649,11 +1649,11 @@ template <typename T, int NT, bool MEM> struct Row {
 // A cut that does not end among the candidates (a nucleus beyond the guess,
 // a large top_k, many equal values) keeps the cluster to narrow it down.
 //
-// Measured (B200, device time): 1 x 32768 f32 9.6 us; 16 x 131072 bf16 of mixed
-// parameters 14 to 21 us; 256 x 131072 bf16, nuclei, 67 us (a sixth of the rows
+// Measured (B200, device time): 1 x 32768 f32 9.7 us; 16 x 131072 bf16 of mixed
+// parameters 14 to 21 us; 256 x 131072 bf16, nuclei, 66 us (a sixth of the rows
 // are narrowed down, and one of those among the last to start makes the tail); 200 x
-// 100003 f16 without cuts 29 us (1.4 TB/s); 64 x 131072 f32 with nuclei of tens
-// of thousands 55 us; 512 x 131072 f32 of mixed parameters 124 us (2.2 TB/s).
+// 100003 f16 without cuts 27 to 29 us (1.4 TB/s); 64 x 131072 f32 with nuclei of tens
+// of thousands 54 us; 512 x 131072 f32 of mixed parameters 114 us (2.4 TB/s).
 template <typename T, int NT, bool MEM>
 __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typename Row<T, NT, MEM>::Shared& sh, uint4* data) {
   RowFinish& f = *reinterpret_cast<RowFinish*>(data);
@@ -1761,9 +1761,9 @@ __device__ __forceinline__ void row_sample(const RowArgs& a, uint32_t row, typen
 // ---- the n best ---------------------------------------------------------------------
 // As a sampling row with top_k = n, whose ordered candidates are the answer.
 // Measured (B200, device time): n = 5 of 1 x 32768 f32 8.3 us, n = 20 of 128 x
-// 131072 bf16 19.9 us (1.7 TB/s), n = 8 of 1024 x 50021 f32 70 us (2.9 TB/s,
-// one streaming CTA a row; bound by issue: 16 instructions an entry in the two
-// passes together).
+// 131072 bf16 18.0 us (1.9 TB/s), n = 8 of 1024 x 50021 f32 68 us (3.0 TB/s,
+// one streaming CTA a row: two passes, of 16 instructions an entry together, with
+// 57% of the issue slots taken and 37% of DRAM's rate).
 template <typename T, int NT, bool MEM>
 __device__ __forceinline__ void row_best(const RowArgs& a, uint32_t row, typename Row<T, NT, MEM>::Shared& sh, uint4* data) {
   RowFinish& f = *reinterpret_cast<RowFinish*>(data);

@@ -164,7 +164,9 @@ class GpuSampler:
         logits: [rows, vocabulary] f32, f16 or bf16, rows any distance apart;
         uniform: f32 [rows], one number of [0, 1) per row.  temperature, top_p,
         min_p (f32 [rows] or a number) and top_k (int32 [rows] or a number)
-        filter as fs_sample_rows describes; None switches each off.  Equal
+        filter as fs_sample_rows describes; None switches each off.  A number
+        costs a launch that spreads it over the rows; a loop keeps tensors.
+        What comes back is detached: no gradient reaches the logits.  Equal
         inputs give equal tokens, whatever the batch around them; a row with
         nothing above -inf gives token -1."""
         t = self._torch
@@ -186,8 +188,9 @@ class GpuSampler:
     def top_logprobs(self, logits, n: int, *, indices=None, logprobs=None, lse=None, sync: bool = False):
         """(indices int32 [rows, n], logprobs f32 [rows, n], lse f32 [rows]):
         the n largest logits of every row in descending order (ties: lowest
-        index first), their log-softmax, and the rows' log-sum-exp.  Places
-        beyond a row's entries above -inf hold index -1, log-probability -inf."""
+        index first), their log-softmax, and the rows' log-sum-exp, detached
+        from the logits' graph.  Places beyond a row's entries above -inf hold
+        index -1, log-probability -inf."""
         t = self._torch
         code, rows, cols, stride = self._rows(logits)
         indices, ip = self._out(indices, "indices", (rows, n), t.int32)
